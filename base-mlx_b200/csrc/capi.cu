@@ -1,6 +1,7 @@
 // extern "C" boundary (include/qwen3_b200.h).  Each entry point converts
 // exceptions into a status code plus a thread-local message, mirroring the
 // Result<T, Error> convention of crates/base-mlx-core/src/error.rs:6-32.
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -11,6 +12,7 @@
 #include <string>
 #include <vector>
 
+#include "kv4.h"
 #include "model.h"
 
 namespace {
@@ -771,3 +773,207 @@ extern "C" int qw_quantized_matmul_argmax_static(const void* x, const void* w, c
     });
 }
 
+
+// ---------------------------------------------------------------------------
+// 4-bit KV cache operators.
+// ---------------------------------------------------------------------------
+namespace {
+
+// The GPU that holds the cache becomes current for the call (a launch on a
+// stream of another GPU then fails with an error).
+struct Kv4Device {
+    int prev = 0, dev = 0;
+    explicit Kv4Device(const void* p) {
+        cudaPointerAttributes at;
+        QW_CUDA(cudaGetDevice(&prev));
+        QW_CUDA(cudaPointerGetAttributes(&at, p));
+        need(at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged, "the cache is not device memory");
+        dev = at.device;
+        if (dev != prev) QW_CUDA(cudaSetDevice(dev));
+    }
+    ~Kv4Device() {
+        if (dev != prev) cudaSetDevice(prev);
+    }
+    int sms() const {
+        int n = 0;
+        QW_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+        return n;
+    }
+};
+
+qw::Kv4View kv4_view(const qw_kv4* c) {
+    need(c != nullptr, "cache");
+    void* const ptr[6] = {c->k_w, c->k_s, c->k_b, c->v_w, c->v_s, c->v_b};
+    for (void* p : ptr) need(p && (uintptr_t)p % 16 == 0, "the cache's arrays must be given and 16-byte aligned");
+    if (c->head_dim != 64 && c->head_dim != 128)
+        throw qw::Error(QW_ERR_UNSUPPORTED, "kv4: head_dim must be 64 or 128, got " + std::to_string(c->head_dim));
+    need(c->max_pos >= 16 && c->max_pos % 16 == 0, "kv4: max_pos must be a positive multiple of 16");
+    need(c->batch >= 1 && c->batch <= 65535, "kv4: batch must be 1..65535");
+    need(c->kv_heads >= 1 && c->kv_heads <= 4096, "kv4: kv_heads must be 1..4096");
+    qw::Kv4View v;
+    v.p[0] = {(uint32_t*)c->k_w, (bf16*)c->k_s, (bf16*)c->k_b};
+    v.p[1] = {(uint32_t*)c->v_w, (bf16*)c->v_s, (bf16*)c->v_b};
+    v.batch = c->batch;
+    v.heads = c->kv_heads;
+    v.max_pos = c->max_pos;
+    v.D = c->head_dim;
+    return v;
+}
+
+qw::Kv4Strides kv4_strides(const int64_t* s, int S, int heads, int D) {
+    if (s) return {s[0], s[1], s[2]};
+    return {(long long)S * heads * D, (long long)heads * D, (long long)D};
+}
+
+void kv4_rows_arg(int S) { need(S >= 1 && S <= (1 << 24), "kv4: S must be 1..2^24"); }
+
+void kv4_heads_arg(const qw::Kv4View& v, int S, int heads) {
+    kv4_rows_arg(S);
+    need(heads >= 1 && heads <= 65535 && heads % v.heads == 0, "kv4: heads must be a positive multiple of kv_heads");
+}
+
+bool overlaps(const void* a, size_t na, const void* b, size_t nb) {
+    return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+
+}  // namespace
+
+extern "C" int qw_kv4_append(const qw_kv4* cache, const void* k, const int64_t* k_strides, const void* v,
+                             const int64_t* v_strides, int S, const int32_t* seq_len, const int32_t* n_new,
+                             int32_t* err, void* stream) {
+    return guard([&] {
+        qw::Kv4StoreArgs a;
+        a.c = kv4_view(cache);
+        need(k && v && seq_len, "k/v/seq_len");
+        need((uintptr_t)k % 2 == 0 && (uintptr_t)v % 2 == 0, "k and v must be aligned to their elements");
+        kv4_rows_arg(S);
+        a.x[0] = (const bf16*)k;
+        a.x[1] = (const bf16*)v;
+        a.xs[0] = kv4_strides(k_strides, S, a.c.heads, a.c.D);
+        a.xs[1] = kv4_strides(v_strides, S, a.c.heads, a.c.D);
+        a.S = S;
+        a.seq_len = seq_len;
+        a.n_new = n_new;
+        a.err = err;
+        Kv4Device dev(cache->k_w);
+        QW_CUDA(qw::launch_kv4_append(a, (cudaStream_t)stream));
+    });
+}
+
+extern "C" int qw_kv4_read(const qw_kv4* cache, void* k_out, void* v_out, int S, const int32_t* seq_len,
+                           const int32_t* n_new, int32_t* err, void* stream) {
+    return guard([&] {
+        qw::Kv4ReadArgs a;
+        a.c = kv4_view(cache);
+        need(k_out || v_out, "k_out/v_out");
+        need((uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0, "k_out and v_out must be 16-byte aligned");
+        kv4_rows_arg(S);
+        a.y[0] = (bf16*)k_out;
+        a.y[1] = (bf16*)v_out;
+        a.S = S;
+        a.seq_len = seq_len;
+        a.n_new = n_new;
+        a.err = err;
+        Kv4Device dev(cache->k_w);
+        QW_CUDA(qw::launch_kv4_read(a, (cudaStream_t)stream));
+    });
+}
+
+extern "C" int qw_kv4_attention_scratch(const qw_kv4* cache, int S, int heads, size_t* bytes) {
+    return guard([&] {
+        const qw::Kv4View v = kv4_view(cache);
+        need(bytes != nullptr, "bytes");
+        kv4_heads_arg(v, S, heads);
+        Kv4Device dev(cache->k_w);
+        *bytes = qw::kv4_attn_scratch_bytes(v, S, heads, dev.sms());
+    });
+}
+
+extern "C" int qw_kv4_attention(const qw_kv4* cache, const void* q, const int64_t* q_strides, void* out,
+                                const int64_t* out_strides, int S, int heads, float scale, int causal,
+                                const int32_t* seq_len, const int32_t* n_new, float* lse, float* mass, void* scratch,
+                                size_t scratch_bytes, int32_t* err, void* stream) {
+    return guard([&] {
+        qw::Kv4AttnArgs a;
+        a.c = kv4_view(cache);
+        need(q && out && seq_len && scratch, "q/out/seq_len/scratch");
+        kv4_heads_arg(a.c, S, heads);
+        need(std::isfinite(scale), "kv4: scale must be finite");
+        a.q = (const bf16*)q;
+        a.qs = kv4_strides(q_strides, S, heads, a.c.D);
+        a.out = (bf16*)out;
+        a.os = kv4_strides(out_strides, S, heads, a.c.D);
+        for (const qw::Kv4Strides& s : {a.qs, a.os})
+            need(s.b % 8 == 0 && s.s % 8 == 0 && s.h % 8 == 0, "kv4: strides of q and out must be multiples of 8 elements");
+        need((uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)scratch % 16 == 0,
+             "kv4: q, out and scratch must be 16-byte aligned");
+        need((a.os.b != 0 || a.c.batch == 1) && (a.os.s != 0 || S == 1) && (a.os.h != 0 || heads == 1),
+             "kv4: out has a zero stride");
+        a.S = S;
+        a.Hq = heads;
+        a.causal = causal ? 1 : 0;
+        a.scale = scale;
+        a.seq_len = seq_len;
+        a.n_new = n_new;
+        a.lse = lse;
+        a.mass = mass;
+        a.err = err;
+        Kv4Device dev(cache->k_w);
+        const int sms = dev.sms();
+        const size_t want = qw::kv4_attn_scratch_bytes(a.c, S, heads, sms);
+        if (scratch_bytes < want)
+            throw qw::Error(QW_ERR_INVALID_ARG, "qw_kv4_attention: scratch has " + std::to_string(scratch_bytes) +
+                                                    " bytes, needs " + std::to_string(want));
+        QW_CUDA(qw::launch_kv4_attention(a, scratch, sms, (cudaStream_t)stream));
+    });
+}
+
+extern "C" int qw_kv4_evict_scratch(const qw_kv4* src, int keep, size_t* bytes) {
+    return guard([&] {
+        const qw::Kv4View v = kv4_view(src);
+        need(bytes && keep >= 1, "bytes/keep");
+        *bytes = qw::kv4_evict_scratch_bytes(v, keep);
+    });
+}
+
+extern "C" int qw_kv4_evict(const qw_kv4* src, const qw_kv4* dst, const float* mass_src, float* mass_dst,
+                            const int32_t* seq_len, int32_t* new_len, int keep, int recent, int32_t* index_out,
+                            void* scratch, size_t scratch_bytes, void* stream) {
+    return guard([&] {
+        qw::Kv4EvictArgs a;
+        a.src = kv4_view(src);
+        a.dst = kv4_view(dst);
+        need(mass_src && mass_dst && seq_len && new_len && scratch, "mass/seq_len/new_len/scratch");
+        need(a.src.batch == a.dst.batch && a.src.heads == a.dst.heads && a.src.D == a.dst.D,
+             "kv4: the caches differ in batch, kv_heads or head_dim");
+        need(keep >= 1 && keep <= a.dst.max_pos, "kv4: keep must be 1..max_pos of the destination");
+        need(recent >= 0 && recent <= keep, "kv4: recent must be 0..keep");
+        need((uintptr_t)scratch % 16 == 0, "kv4: scratch must be 16-byte aligned");
+        // in place (every array the same), or no two arrays overlapping
+        const size_t rows_s = (size_t)a.src.batch * a.src.heads * a.src.max_pos,
+                     rows_d = (size_t)a.dst.batch * a.dst.heads * a.dst.max_pos;
+        const void* ps[7] = {src->k_w, src->k_s, src->k_b, src->v_w, src->v_s, src->v_b, mass_src};
+        const void* pd[7] = {dst->k_w, dst->k_s, dst->k_b, dst->v_w, dst->v_s, dst->v_b, mass_dst};
+        const size_t wb = (size_t)a.src.D / 2, sb = (size_t)a.src.D / 32;
+        const size_t rb[7] = {wb, sb, sb, wb, sb, sb, sizeof(float)};
+        bool same = a.src.max_pos == a.dst.max_pos, apart = true;
+        for (int i = 0; i < 7; ++i) {
+            same = same && ps[i] == pd[i];
+            for (int j = 0; j < 7; ++j) apart = apart && !overlaps(ps[i], rows_s * rb[i], pd[j], rows_d * rb[j]);
+        }
+        need(same || apart, "kv4: the destination must be the source itself or not overlap it");
+        const size_t want = qw::kv4_evict_scratch_bytes(a.src, keep);
+        if (scratch_bytes < want)
+            throw qw::Error(QW_ERR_INVALID_ARG, "qw_kv4_evict: scratch has " + std::to_string(scratch_bytes) +
+                                                    " bytes, needs " + std::to_string(want));
+        a.mass_src = mass_src;
+        a.mass_dst = mass_dst;
+        a.seq_len = seq_len;
+        a.new_len = new_len;
+        a.keep = keep;
+        a.recent = recent;
+        a.index_out = index_out;
+        Kv4Device dev(src->k_w);
+        QW_CUDA(qw::launch_kv4_evict(a, scratch, (cudaStream_t)stream));
+    });
+}

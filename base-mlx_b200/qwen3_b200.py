@@ -10,7 +10,8 @@ flakerimi/base-mlx project root):
 * ``KvCache.slice_update`` -- ``mlx_ext::slice_update`` (``mlx_ext.rs:36-64``) on a cache tensor;
 * ``Qwen3.generate_greedy`` -- ``LoadedModel::generate_text`` with temperature 0 (``engine.rs:149-201``);
 * ``speculative_generate`` / ``check_compatible`` -- ``speculative.rs:40-286``;
-* ``quantized_matmul`` -- ``mlx_rs::ops::quantized_matmul(transpose=true, 64, 4)``.
+* ``quantized_matmul`` -- ``mlx_rs::ops::quantized_matmul(transpose=true, 64, 4)``;
+* ``Kv4`` and ``kv4_*`` -- operators of a 4-bit KV cache (no counterpart in the crate).
 
 Errors map onto the crate's ``Error`` enum (``error.rs:6-32``).  There is no
 CPU fallback: every compute call goes to the CUDA library and raises when no
@@ -97,11 +98,23 @@ class SpecStats(ctypes.Structure):
                 ("accept_ms_mean", ctypes.c_double)]
 
 
+class Kv4(ctypes.Structure):
+    """The device arrays of a 4-bit KV cache: Kv4(k_w, k_s, k_b, v_w, v_s, v_b,
+    batch, kv_heads, max_pos, head_dim), words uint32 [batch, kv_heads, max_pos,
+    head_dim / 8], scales and biases bf16 [batch, kv_heads, max_pos, head_dim / 64]."""
+    _fields_ = [("k_w", ctypes.c_void_p), ("k_s", ctypes.c_void_p), ("k_b", ctypes.c_void_p),
+                ("v_w", ctypes.c_void_p), ("v_s", ctypes.c_void_p), ("v_b", ctypes.c_void_p),
+                ("batch", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("max_pos", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32)]
+
+
 _lib = None
 P = ctypes.c_void_p
 I = ctypes.c_int
 U32P = ctypes.POINTER(ctypes.c_uint32)
 U16P = ctypes.POINTER(ctypes.c_uint16)
+I64P = ctypes.POINTER(ctypes.c_int64)
+KV4P = ctypes.POINTER(Kv4)
 
 # name -> argtypes; every function returns int
 SIGNATURES = {
@@ -141,6 +154,12 @@ SIGNATURES = {
                                  U32P, ctypes.POINTER(I), ctypes.POINTER(SpecStats)],
     "qw_quantized_matmul": [P, P, P, P, P, I, I, I, I, I, P],
     "qw_quantized_matmul_argmax_static": [P, P, P, P, P, P, I, I, I, I, I, P],
+    "qw_kv4_append": [KV4P, P, I64P, P, I64P, I, P, P, P, P],
+    "qw_kv4_read": [KV4P, P, P, I, P, P, P, P],
+    "qw_kv4_attention_scratch": [KV4P, I, I, ctypes.POINTER(ctypes.c_size_t)],
+    "qw_kv4_attention": [KV4P, P, I64P, P, I64P, I, I, ctypes.c_float, I, P, P, P, P, P, ctypes.c_size_t, P, P],
+    "qw_kv4_evict_scratch": [KV4P, I, ctypes.POINTER(ctypes.c_size_t)],
+    "qw_kv4_evict": [KV4P, KV4P, P, P, P, P, I, I, P, P, ctypes.c_size_t, P],
 }
 
 
@@ -520,3 +539,61 @@ def quantized_matmul_argmax_static(x_ptr: int, w_ptr: int, s_ptr: int, b_ptr: in
     device should come before any stream capture."""
     check(lib().qw_quantized_matmul_argmax_static(x_ptr, w_ptr, s_ptr, b_ptr, y_ptr or None, argmax_ptr, M, N, K,
                                                   group_size, bits, stream or None))
+
+
+def _strides(s):
+    return None if s is None else (ctypes.c_int64 * 3)(*s)
+
+
+def kv4_append(cache: Kv4, k_ptr: int, v_ptr: int, S: int, seq_len_ptr: int, n_new_ptr: int = 0, k_strides=None,
+               v_strides=None, err_ptr: int = 0, stream: int = 0) -> None:
+    """Quantize S new bf16 rows per sequence ([batch, S, kv_heads, head_dim],
+    strides {sequence, row, head} in elements) into positions seq_len[b] + i of
+    the cache; the lengths (device int32) are not advanced."""
+    check(lib().qw_kv4_append(ctypes.byref(cache), k_ptr, _strides(k_strides), v_ptr, _strides(v_strides), S,
+                              seq_len_ptr, n_new_ptr or None, err_ptr or None, stream or None))
+
+
+def kv4_read(cache: Kv4, k_ptr: int, v_ptr: int, S: int, seq_len_ptr: int = 0, n_new_ptr: int = 0, err_ptr: int = 0,
+             stream: int = 0) -> None:
+    """bf16 values of S rows per sequence from position seq_len[b] (0 without
+    seq_len) to contiguous [batch, S, kv_heads, head_dim]; either output may be 0."""
+    check(lib().qw_kv4_read(ctypes.byref(cache), k_ptr or None, v_ptr or None, S, seq_len_ptr or None,
+                            n_new_ptr or None, err_ptr or None, stream or None))
+
+
+def kv4_attention_scratch_bytes(cache: Kv4, S: int, heads: int) -> int:
+    """Size of the device scratch kv4_attention needs for S rows of `heads` query heads."""
+    n = ctypes.c_size_t()
+    check(lib().qw_kv4_attention_scratch(ctypes.byref(cache), S, heads, ctypes.byref(n)))
+    return n.value
+
+
+def kv4_attention(cache: Kv4, q_ptr: int, out_ptr: int, S: int, heads: int, scale: float, seq_len_ptr: int,
+                  scratch_ptr: int, scratch_bytes: int, n_new_ptr: int = 0, causal: bool = True, lse_ptr: int = 0,
+                  mass_ptr: int = 0, q_strides=None, out_strides=None, err_ptr: int = 0, stream: int = 0) -> None:
+    """Attention of S new rows per sequence (appended already, the last of the
+    cache) over the 4-bit cache; optional log-sum-exp per row (fp32 [batch, S,
+    heads]) and each key's attention weight added to mass (fp32 [batch,
+    kv_heads, max_pos])."""
+    check(lib().qw_kv4_attention(ctypes.byref(cache), q_ptr, _strides(q_strides), out_ptr, _strides(out_strides), S,
+                                 heads, scale, 1 if causal else 0, seq_len_ptr, n_new_ptr or None, lse_ptr or None,
+                                 mass_ptr or None, scratch_ptr, scratch_bytes, err_ptr or None, stream or None))
+
+
+def kv4_evict_scratch_bytes(src: Kv4, keep: int) -> int:
+    """Size of the device scratch kv4_evict needs."""
+    n = ctypes.c_size_t()
+    check(lib().qw_kv4_evict_scratch(ctypes.byref(src), keep, ctypes.byref(n)))
+    return n.value
+
+
+def kv4_evict(src: Kv4, dst: Kv4, mass_src_ptr: int, mass_dst_ptr: int, seq_len_ptr: int, new_len_ptr: int,
+              keep: int, recent: int, scratch_ptr: int, scratch_bytes: int, index_ptr: int = 0,
+              stream: int = 0) -> None:
+    """Cut sequences longer than `keep` to `keep` positions per kv head: the last
+    `recent` and the others of largest accumulated weight, moved to the front
+    of dst (src itself, or a cache apart from it) in their old order."""
+    check(lib().qw_kv4_evict(ctypes.byref(src), ctypes.byref(dst), mass_src_ptr, mass_dst_ptr, seq_len_ptr,
+                             new_len_ptr, keep, recent, index_ptr or None, scratch_ptr, scratch_bytes,
+                             stream or None))

@@ -17,6 +17,7 @@
  *   qw_sample_topp           LoadedModel::pick_next on one logits row (device)         engine.rs:195-263
  *   qw_spec_generate         speculative::generate                 speculative.rs:57-286
  *   qw_check_compatible      speculative::check_compatible         speculative.rs:40-54
+ *   qw_kv4_*                 operators of a 4-bit KV cache (no counterpart: KvCache holds bf16, model/qwen3.rs:116-162)
  *
  * Conventions
  *   - every function returns an int status: QW_OK (0) or a negative QW_ERR_*
@@ -28,8 +29,9 @@
  *     thread at a time (the crate serialises requests behind a Mutex,
  *     base-mlx-server/src/state.rs:18-27).
  *   - token ids are uint32; logits are bf16 bit patterns (uint16).
- *   - pointers named *_host are host memory; qw_quantized_matmul takes device
- *     pointers (it stands in for an op on MLX arrays that already live on the GPU).
+ *   - pointers named *_host are host memory; qw_quantized_matmul and the qw_kv4_*
+ *     operators take device pointers (they stand in for ops on MLX arrays that
+ *     already live on the GPU).
  *   - there is no CPU fallback: without a usable sm_100 GPU every compute call
  *     fails with QW_ERR_CUDA.
  */
@@ -311,6 +313,90 @@ QW_API int qw_quantized_matmul(const void* x, const void* w, const void* scales,
 QW_API int qw_quantized_matmul_argmax_static(const void* x, const void* w, const void* scales,
                                              const void* biases, void* y_or_null, int* argmax_dev, int M,
                                              int N, int K, int group_size, int bits, void* stream);
+
+/* ---- 4-bit KV cache ------------------------------------------------------- */
+
+/* Keys and values of `batch` sequences in the affine 4-bit format of the model
+ * weights (the arrays an MLX quantized KV cache holds at 64 / 4):
+ *   k_w, v_w            uint32 [batch][kv_heads][max_pos][head_dim / 8], element e at bits 4 (e % 8) of word e / 8
+ *   k_s, k_b, v_s, v_b  bf16   [batch][kv_heads][max_pos][head_dim / 64], value = scale * q + bias
+ * head_dim is 64 or 128, max_pos a multiple of 16, every pointer 16-byte
+ * aligned device memory of one GPU.  The struct is read during the call only.
+ *
+ * Common to the operators below (no reference counterpart: the reference
+ * caches bf16 rows):
+ *   - everything is asynchronous on `stream` (NULL: the default stream of the
+ *     GPU that holds the cache); a stream of another GPU is an error.  The
+ *     calling thread's current device may be another one and stays so.
+ *   - lengths live on the device (int32, one per sequence), so a captured step
+ *     can be replayed at every position; no call reads them on the host.
+ *   - seq_len_dev[b] is the number of positions cached before the step's S new
+ *     rows; n_new_dev[b] (NULL: S) says how many of the S rows sequence b has.
+ *     Rows that would lie past max_pos are left out, a sequence whose seq_len
+ *     is outside [0, max_pos] counts as empty and without rows; a call that
+ *     meets either sets bit 0 of *err_dev (int32, may be NULL).
+ *   - strides are in elements, {sequence, row, head}, of a tensor
+ *     [batch][S][heads][head_dim] with contiguous head_dim; NULL: contiguous.
+ *   - no call allocates; scratch is the caller's (16-byte aligned, no initial
+ *     contents), and calls that may overlap on the GPU need one each. */
+typedef struct qw_kv4 {
+    void *k_w, *k_s, *k_b;
+    void *v_w, *v_s, *v_b;
+    int32_t batch, kv_heads, max_pos, head_dim;
+} qw_kv4;
+
+/* Quantize S new bf16 K and V rows per sequence into positions seq_len[b] .. .
+ * Per 64 elements: bias = min, scale = bf16((max - min) / 15), q = the nearest
+ * integer to the exact (x - bias) / scale (ties to even) clamped to 0..15; a
+ * group holding a NaN or an infinity reads back as NaN.  The lengths are not
+ * advanced. */
+QW_API int qw_kv4_append(const qw_kv4* cache, const void* k, const int64_t* k_strides, const void* v,
+                         const int64_t* v_strides, int S, const int32_t* seq_len_dev, const int32_t* n_new_dev,
+                         int32_t* err_dev, void* stream);
+
+/* bf16 values of rows seq_len[b] .. (seq_len_dev NULL: 0 ..) to contiguous
+ * [batch][S][kv_heads][head_dim]; rows a sequence does not have are zero.
+ * k_out or v_out may be NULL. */
+QW_API int qw_kv4_read(const qw_kv4* cache, void* k_out, void* v_out, int S, const int32_t* seq_len_dev,
+                       const int32_t* n_new_dev, int32_t* err_dev, void* stream);
+
+/* Scratch of qw_kv4_attention for S rows of `heads` query heads on the cache's GPU. */
+QW_API int qw_kv4_attention_scratch(const qw_kv4* cache, int S, int heads, size_t* bytes);
+
+/* Attention of S new rows per sequence (already appended) over the cache:
+ * out[b][i][h] = softmax(scale * <q[b][i][h], k_j>) . v_j over the keys
+ * j < seq_len[b] + n_new[b] of kv head h / (heads / kv_heads), with causal != 0
+ * only j <= seq_len[b] + i.  q and out are bf16 (16-byte aligned, strides a
+ * multiple of 8 elements).  lse (fp32 [batch][S][heads], may be NULL) receives
+ * the natural logarithm of each row's sum of exponentials; a row without keys
+ * gives out = 0, lse = -inf.  mass (fp32 [batch][kv_heads][max_pos], may be
+ * NULL) has every key's probability, summed over the sequence's rows and the
+ * kv head's query heads, added to it; positions past the last key are left as
+ * they are. */
+QW_API int qw_kv4_attention(const qw_kv4* cache, const void* q, const int64_t* q_strides, void* out,
+                            const int64_t* out_strides, int S, int heads, float scale, int causal,
+                            const int32_t* seq_len_dev, const int32_t* n_new_dev, float* lse, float* mass,
+                            void* scratch, size_t scratch_bytes, int32_t* err_dev, void* stream);
+
+/* Scratch of qw_kv4_evict. */
+QW_API int qw_kv4_evict_scratch(const qw_kv4* src, int keep, size_t* bytes);
+
+/* Cut every sequence longer than `keep` to `keep` positions, per kv head: the
+ * last `recent` stay, and of the others the keep - recent with the largest
+ * accumulated weight mass_src (fp32 [batch][kv_heads][src max_pos]; equal
+ * weights: the lower position stays, NaN counts as the largest).  The kept
+ * rows go to positions 0.. of dst in their old order, their weights to
+ * mass_dst, new_len_dev[b] = min(seq_len[b], keep).  index_out (int32
+ * [batch][kv_heads][keep], may be NULL) receives the kept positions, -1 behind
+ * them.  dst is src itself (in place; then mass_dst = mass_src, and
+ * new_len_dev may be seq_len_dev) or a cache that does not overlap it, of the
+ * same batch, kv_heads and head_dim with max_pos >= keep; its rows past
+ * new_len are left as they are.  Keys keep the positions they were rotated
+ * with: rows appended later count seq_len from the new length, rotary
+ * positions go on from the old one. */
+QW_API int qw_kv4_evict(const qw_kv4* src, const qw_kv4* dst, const float* mass_src, float* mass_dst,
+                        const int32_t* seq_len_dev, int32_t* new_len_dev, int keep, int recent, int32_t* index_out,
+                        void* scratch, size_t scratch_bytes, void* stream);
 
 #ifdef __cplusplus
 }
