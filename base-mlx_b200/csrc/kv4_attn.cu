@@ -7,104 +7,474 @@
 //   s_j = scale <q, k_j>, lse = log sum_j exp(s_j), out = sum_j exp(s_j - lse) v_j,
 //   mass[b][kv head][j] += sum over the rows and the kv head's query heads of exp(s_j - lse).
 // A row that sees no key (a row past n_b, or an empty sequence) gives out = 0, lse = -inf.
-#include "kv4.h"
+//
+// A column is one (row, query head) of a kv head: column c = i G + head.  The
+// work of a call is the list of (sequence, kv head, column block) segments,
+// each of ceil(T_b / 32) tiles of 32 keys; the thread blocks take equal
+// contiguous shares of that list, whatever the lengths, so a ragged batch and
+// one long sequence both fill the GPU.  A segment inside one share is finished
+// there; one that spans shares leaves a partial (maximum, sum, output) per
+// share, which a second kernel joins.
+#include "kv4_tile.cuh"
+#include "smem_attr.h"
 
 namespace qw {
 namespace {
 
-// One warp per (sequence, row, query head); lane l holds the dimensions
-// [l * D / 32, (l + 1) * D / 32).  One pass over the keys with a running
-// maximum and sum in fp32.
-template <int D>
-__global__ void __launch_bounds__(128) kv4_attn_row_kernel(const Kv4AttnArgs a) {
-    constexpr int V = D / 32;
-    const int lane = threadIdx.x & 31;
-    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (item >= (long long)a.c.batch * a.S * a.Hq) return;
-    const int h = (int)(item % a.Hq), i = (int)(item / a.Hq % a.S), b = (int)(item / a.Hq / a.S);
-    const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, a.err, h == 0 && i == 0 && lane == 0);
-    const int vis = i >= rw.n ? 0 : (a.causal ? rw.off + i + 1 : rw.off + rw.n);
-    const int kvh = h / (a.Hq / a.c.heads);
-    const size_t row0 = ((size_t)b * a.c.heads + kvh) * a.c.max_pos;
-    const bf16* qp = a.q + (b * a.qs.b + i * a.qs.s + h * a.qs.h) + lane * V;
-    float q[V], o[V], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-        q[e] = bf2f(qp[e]) * a.scale;
-        o[e] = 0.f;
-    }
-    const int word = lane * V / 8, sh = 4 * (lane * V % 8), g = lane * V / 64;
-    for (int j = 0; j < vis; ++j) {
-        const size_t r = row0 + j;
-        const uint32_t kw = a.c.p[0].w[r * (D / 8) + word] >> sh, vw = a.c.p[1].w[r * (D / 8) + word] >> sh;
-        const float ks = bf2f(a.c.p[0].s[r * (D / 64) + g]), kb = bf2f(a.c.p[0].b[r * (D / 64) + g]);
-        const float vs = bf2f(a.c.p[1].s[r * (D / 64) + g]), vb = bf2f(a.c.p[1].b[r * (D / 64) + g]);
-        float s = 0.f;
-#pragma unroll
-        for (int e = 0; e < V; ++e) s = fmaf(q[e], fmaf(ks, (float)((kw >> (4 * e)) & 15u), kb), s);
-        s = warp_sum(s);
-        const float mn = fmaxf(m, s);
-        const float al = m == mn ? 1.f : expf(m - mn), p = s == mn ? 1.f : expf(s - mn);
-        l = fmaf(l, al, p);
-#pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = fmaf(o[e], al, p * fmaf(vs, (float)((vw >> (4 * e)) & 15u), vb));
-        m = mn;
-    }
-    bf16* op = a.out + (b * a.os.b + i * a.os.s + h * a.os.h) + lane * V;
-#pragma unroll
-    for (int e = 0; e < V; ++e) op[e] = f2bf(vis > 0 ? o[e] / l : 0.f);
-    if (a.lse && lane == 0) a.lse[((size_t)b * a.S + i) * a.Hq + h] = vis > 0 ? m + logf(l) : -INFINITY;
+using namespace kv4;
+
+constexpr int AW = 8, ANT = 32 * AW;  // warps and threads of a block
+constexpr int ASTAGES = 3;            // tiles of a warp's load ring
+
+// Scratch: [0] tiles per share, [1 + b] first tile of sequence b; then the
+// partials [2 shares][columns][D] and their (maximum, sum); then the lse of a
+// call that accumulates weights but returns none.
+struct Scratch {
+    long long* plan;
+    float* part;
+    float2* ml;
+    float* lse;
+    size_t bytes;
+};
+Scratch scratch_of(void* base, const Kv4View& c, int S, int Hq, int shares, int cb) {
+    Scratch s;
+    unsigned char* p = static_cast<unsigned char*>(base);
+    auto take = [&](size_t n) {
+        unsigned char* r = p;
+        p += (n + 255) & ~(size_t)255;
+        return r;
+    };
+    s.plan = reinterpret_cast<long long*>(take((size_t)(c.batch + 1) * 8));
+    s.part = reinterpret_cast<float*>(take((size_t)2 * shares * cb * c.D * 4));
+    s.ml = reinterpret_cast<float2*>(take((size_t)2 * shares * cb * 8));
+    s.lse = reinterpret_cast<float*>(take((size_t)c.batch * S * Hq * 4));
+    s.bytes = (size_t)(p - static_cast<unsigned char*>(base));
+    return s;
 }
 
-// One warp per (sequence, kv head, key): the key's probability summed over the
-// rows and query heads in a fixed order.
-template <int D>
-__global__ void __launch_bounds__(128) kv4_mass_row_kernel(const Kv4AttnArgs a) {
-    constexpr int V = D / 32;
-    const int lane = threadIdx.x & 31;
-    const int j = blockIdx.x * 4 + (threadIdx.x >> 5), kvh = blockIdx.y, b = blockIdx.z;
-    const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
-    if (j >= rw.off + rw.n) return;
-    const size_t r = ((size_t)b * a.c.heads + kvh) * a.c.max_pos + j;
-    const int word = lane * V / 8, sh = 4 * (lane * V % 8), g = lane * V / 64, G = a.Hq / a.c.heads;
-    const uint32_t kw = a.c.p[0].w[r * (D / 8) + word] >> sh;
-    const float ks = bf2f(a.c.p[0].s[r * (D / 64) + g]), kb = bf2f(a.c.p[0].b[r * (D / 64) + g]);
-    float k[V], acc = 0.f;
+QW_DEV long long block_sum(long long v, long long* red) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) k[e] = fmaf(ks, (float)((kw >> (4 * e)) & 15u), kb);
-    for (int i = a.causal ? max(0, j - rw.off) : 0; i < rw.n; ++i)
-        for (int h = kvh * G; h < (kvh + 1) * G; ++h) {
-            const bf16* qp = a.q + (b * a.qs.b + i * a.qs.s + h * a.qs.h) + lane * V;
-            float s = 0.f;
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0;
 #pragma unroll
-            for (int e = 0; e < V; ++e) s = fmaf(bf2f(qp[e]) * a.scale, k[e], s);
-            s = warp_sum(s);
-            acc += expf(s - a.lse[((size_t)b * a.S + i) * a.Hq + h]);
+    for (int w = 0; w < AW; ++w) v += red[w];
+    return v;
+}
+// Exclusive prefix over the block's threads.
+QW_DEV long long block_prefix(long long v, long long* red) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long t = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += t;
+    }
+    __syncthreads();
+    if (lane == 31) red[warp] = s;
+    __syncthreads();
+    s -= v;
+    for (int w = 0; w < warp; ++w) s += red[w];
+    return s;
+}
+
+QW_DEV int tiles_of(const Kv4Rows& r) { return (r.off + r.n + TK - 1) / TK; }
+
+struct Share {
+    long long per, begin, end;  // tiles of a share; this block's [begin, end)
+    int b;                      // sequence of tile `begin`
+    long long b0;               // its first tile
+};
+
+// This block's share; block 0 writes the plan for the joining kernel.
+QW_DEV Share take_share(const Kv4AttnArgs& a, int ncb, long long* plan) {
+    __shared__ long long red[AW], found[2];
+    const int B = a.c.batch, tid = threadIdx.x;
+    const long long per_tile = (long long)a.c.heads * ncb;
+    long long total = 0;
+    for (int b = tid; b < B; b += ANT)
+        total += per_tile * tiles_of(kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, a.err, blockIdx.x == 0));
+    total = block_sum(total, red);
+    Share s;
+    s.per = max(1ll, (total + gridDim.x - 1) / gridDim.x);
+    s.begin = min(total, s.per * blockIdx.x);
+    s.end = min(total, s.begin + s.per);
+    if (tid == 0) found[0] = B;
+    if (blockIdx.x == 0 && tid == 0) plan[0] = s.per;
+    long long base = 0;
+    for (int b0 = 0; b0 < B; b0 += ANT) {
+        const int b = b0 + tid;
+        const long long n = b < B ? per_tile * tiles_of(kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false)) : 0;
+        const long long at = base + block_prefix(n, red);
+        if (blockIdx.x == 0 && b < B) plan[1 + b] = at;
+        if (n > 0 && at <= s.begin && s.begin < at + n) {
+            found[0] = b;
+            found[1] = at;
         }
-    if (lane == 0) a.mass[r] += acc;
+        base += block_sum(n, red);
+        if (blockIdx.x != 0 && base > s.begin) break;
+    }
+    __syncthreads();
+    s.b = (int)found[0];
+    s.b0 = found[1];
+    return s;
+}
+
+template <int D, int NT>
+struct SplitSmem {
+    static constexpr int RING = AW * ASTAGES * Tile<D>::BYTES;
+    static constexpr int OLD = D + 2;  // output row of a warp's merge buffer, floats
+    static constexpr int MERGE = AW * 8 * NT * OLD * 4;
+    static constexpr int BYTES = (RING > MERGE ? RING : MERGE) + AW * 8 * NT * 8;
+};
+
+// The eight warps take a segment's tiles in turn, each with its own columns'
+// state and its own ring of tiles (cp.async, so no warp waits for another),
+// and are merged through shared memory at the end of the segment.
+template <int D, int NT>
+__global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(const Kv4AttnArgs a, int ncb, long long* plan,
+                                                                              float* part, float2* pml) {
+    using L = Tile<D>;
+    using SM = SplitSmem<D, NT>;
+    constexpr int CB = 8 * NT;
+    extern __shared__ __align__(128) unsigned char smem[];
+    float2* wml = reinterpret_cast<float2*>(smem + SM::BYTES - AW * CB * 8);  // [warp][column]
+    float* wo = reinterpret_cast<float*>(smem);                               // [warp][column][OLD]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int G = a.Hq / a.c.heads, C = G * a.S;
+    const Share sh = take_share(a, ncb, plan);
+    const uint32_t ring = smem_u32(smem) + warp * ASTAGES * L::BYTES;
+    const unsigned char* ringp = smem + warp * ASTAGES * L::BYTES;
+
+    long long u = sh.begin, b0 = sh.b0;
+    int b = sh.b;
+    while (u < sh.end) {
+        const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
+        const int T = rw.off + rw.n, nt = tiles_of(rw);
+        const long long nseq = (long long)nt * a.c.heads * ncb;
+        if (u >= b0 + nseq) {  // the next sequence (some are empty)
+            b0 += nseq;
+            ++b;
+            continue;
+        }
+        const int seg = (int)((u - b0) / nt), t0 = (int)((u - b0) % nt);
+        const int t1 = (int)min((long long)nt, t0 + (sh.end - u));
+        const int h = seg / ncb, cb = seg % ncb;
+        const Rows rows = head_rows<D>(a.c, (size_t)b * a.c.heads + h);
+
+        const int mine = max(0, (t1 - t0 - warp + AW - 1) / AW);  // tiles t0 + warp, t0 + warp + 8, ...
+        auto issue = [&](int k) {
+            if (k < mine)
+                load_tile<D, true>(ring + (k % ASTAGES) * L::BYTES, rows, (t0 + warp + k * AW) * TK, T, lane);
+            cp_async_commit();
+        };
+#pragma unroll
+        for (int k = 0; k < ASTAGES - 1; ++k) issue(k);
+
+        Cols<D, NT> cols;
+        State<D, NT> st;
+        st.init();
+        int vis[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int c = cb * CB + 8 * n + g, i = c / G;
+            const bf16* src = c < C && i < rw.n ? a.q + (b * a.qs.b + i * a.qs.s + (h * G + c % G) * a.qs.h) : nullptr;
+            load_cols<D, NT>(cols, n, src, a.scale, lane);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int ci = (cb * CB + 8 * n + 2 * t + e) / G;
+                vis[n][e] = a.causal ? min(T, rw.off + ci + 1) : T;
+            }
+        }
+        const int all = a.causal ? min(T, rw.off + cb * CB / G + 1) : T;  // keys that every column sees
+        for (int k = 0; k < mine; ++k) {
+            cp_async_wait<ASTAGES - 2>();
+            __syncwarp();
+            issue(k + ASTAGES - 1);  // into the stage that the warp left in the turn before
+            const int key0 = (t0 + warp + k * AW) * TK;
+            const unsigned char* tile = ringp + (k % ASTAGES) * L::BYTES;
+            if (key0 + TK <= all)
+                attend_tile<D, NT, false>(st, cols, tile, key0, T, vis, lane);
+            else
+                attend_tile<D, NT, true>(st, cols, tile, key0, T, vis, lane);
+            __syncwarp();
+        }
+        cp_async_wait<0>();
+        reduce_lanes(st);
+        if (g == 0)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) wml[warp * CB + 8 * n + 2 * t + e] = make_float2(st.m[n][e], st.l[n][e]);
+        __syncthreads();  // also: every warp has left its ring
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int col = 8 * n + 2 * t + e;
+                float M = wml[col].x;
+#pragma unroll
+                for (int w = 1; w < AW; ++w) M = fmaxf(M, wml[w * CB + col].x);
+                const float f = ex2(st.m[n][e] - M);
+                float* dst = wo + (warp * CB + col) * SM::OLD + 8 * g;
+#pragma unroll
+                for (int gr = 0; gr < D / 64; ++gr)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 v = out_pair(st, gr, i, n, e);
+                        *reinterpret_cast<float2*>(dst + 64 * gr + 2 * i) = make_float2(v.x * f, v.y * f);
+                    }
+            }
+        __syncthreads();
+        const bool whole = t0 == 0 && t1 == nt;
+        const long long slot = 2ll * blockIdx.x + (u == sh.begin ? 0 : 1);
+        for (int idx = tid; idx < CB * (D / 2); idx += ANT) {
+            const int col = idx / (D / 2), d = 2 * (idx % (D / 2)), c = cb * CB + col, i = c / G;
+            if (c >= C) break;
+            float M = wml[col].x, l = 0.f;
+#pragma unroll
+            for (int w = 1; w < AW; ++w) M = fmaxf(M, wml[w * CB + col].x);
+            float2 o = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < AW; ++w) {
+                const float2 ml = wml[w * CB + col];
+                l = fmaf(ml.y, ex2(ml.x - M), l);
+                const float2 v = *reinterpret_cast<const float2*>(wo + (w * CB + col) * SM::OLD + d);
+                o.x += v.x;
+                o.y += v.y;
+            }
+            if (whole) {
+                const bool has = i < rw.n && l != 0.f;
+                const float inv = has ? 1.f / l : 0.f;
+                bf16* dst = a.out + (b * a.os.b + i * a.os.s + (h * G + c % G) * a.os.h) + d;
+                *reinterpret_cast<uint32_t*>(dst) = has ? pack_bf16x2(o.x * inv, o.y * inv) : 0u;
+                if (d == 0 && a.lse)
+                    a.lse[((size_t)b * a.S + i) * a.Hq + h * G + c % G] = has ? (M + log2f(l)) * LN2 : -INFINITY;
+            } else {
+                *reinterpret_cast<float2*>(part + (slot * CB + col) * D + d) = o;
+                if (d == 0) pml[slot * CB + col] = make_float2(M, l);
+            }
+        }
+        __syncthreads();  // the merge buffer is the ring
+        u += t1 - t0;
+    }
+    pdl_launch_dependents();
+}
+
+// Joins the partials of segments that span shares, and writes the rows of empty
+// sequences.  One block per (column, sequence), one thread per dimension.
+template <int D>
+__global__ void __launch_bounds__(D) kv4_attn_join_kernel(const Kv4AttnArgs a, int cb_size, int ncb, const long long* plan,
+                                                          const float* part, const float2* pml) {
+    pdl_wait();
+    const int b = blockIdx.y, G = a.Hq / a.c.heads, d = threadIdx.x;
+    const int h = blockIdx.x % a.Hq, i = blockIdx.x / a.Hq;  // query head, row
+    const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
+    const int nt = tiles_of(rw);
+    bf16* dst = a.out + (b * a.os.b + i * a.os.s + h * a.os.h) + d;
+    float* lse = a.lse ? a.lse + ((size_t)b * a.S + i) * a.Hq + h : nullptr;
+    if (nt == 0 || i >= rw.n) {
+        *dst = f2bf(0.f);
+        if (lse && d == 0) *lse = -INFINITY;
+        return;
+    }
+    const int c = i * G + h % G, cb = c / cb_size, col = c % cb_size;
+    const long long per = plan[0], s0 = plan[1 + b] + ((long long)(h / G) * ncb + cb) * nt;
+    const long long first = s0 / per, last = (s0 + nt - 1) / per;
+    if (first == last) return;
+    auto slot = [&](long long k) { return (2 * k + (k * per >= s0 ? 0 : 1)) * cb_size + col; };
+    float M = M0;
+    for (long long k = first; k <= last; ++k) M = fmaxf(M, pml[slot(k)].x);
+    float o = 0.f, l = 0.f;
+#pragma unroll 4
+    for (long long k = first; k <= last; ++k) {
+        const float2 ml = pml[slot(k)];
+        const float f = ex2(ml.x - M);
+        l = fmaf(ml.y, f, l);
+        o = fmaf(part[slot(k) * D + d], f, o);
+    }
+    *dst = f2bf(l != 0.f ? o / l : 0.f);
+    if (lse && d == 0) *lse = l != 0.f ? (M + log2f(l)) * LN2 : -INFINITY;
+}
+
+// Attention weights: a warp keeps 32 keys and walks the columns, 64 at a time
+// prepared by the block.  A key's weight is summed by one lane quad in a fixed
+// order.
+constexpr int MC = 8;  // n-tiles of 8 columns prepared together
+template <int D>
+__global__ void __launch_bounds__(ANT, 2) kv4_mass_kernel(const Kv4AttnArgs a) {
+    constexpr int GR = D / 64;
+    __shared__ uint32_t sf[MC][GR * 4 * 2][32];  // n-tile, fragment register, lane
+    __shared__ float sc[MC][3 + GR][8];          // n-tile, {c, q per group, log2 of the sum, keys seen}, column
+    pdl_wait();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int h = blockIdx.y, b = blockIdx.z, G = a.Hq / a.c.heads;
+    const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
+    const int T = rw.off + rw.n;
+    const int key0 = (blockIdx.x * AW + warp) * TK, block0 = blockIdx.x * AW * TK;
+    if (block0 >= T) return;
+    const size_t bh = (size_t)b * a.c.heads + h;
+    // K words, scales and biases straight to registers (each is read once)
+    KeyBlock<D> kw[2];
+    float ks[4][GR], kz[4][GR];
+    const uint32_t* w = a.c.p[0].w + bh * a.c.max_pos * (D / 8);
+    const uint16_t* s = reinterpret_cast<const uint16_t*>(a.c.p[0].s) + bh * a.c.max_pos * GR;
+    const uint16_t* z = reinterpret_cast<const uint16_t*>(a.c.p[0].b) + bh * a.c.max_pos * GR;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int k = key0 + 8 * r + g;
+        const bool ok = k < T;
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr) {
+            uint2 u = make_uint2(0u, 0u);
+            if (ok) u = *reinterpret_cast<const uint2*>(w + (size_t)k * (D / 8) + 8 * gr + 2 * t);
+            kw[r >> 1].w[gr][r & 1][0] = u.x;
+            kw[r >> 1].w[gr][r & 1][1] = u.y;
+            ks[r][gr] = ok ? u16_to_f(s[(size_t)k * GR + gr]) : 0.f;
+            kz[r][gr] = ok ? u16_to_f(z[(size_t)k * GR + gr]) : 0.f;
+        }
+    }
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    // columns that see none of the block's keys come first when causal: skip them
+    const int c_first = a.causal ? max(0, block0 - rw.off) * G / 8 * 8 : 0;
+    const int c_end = rw.n * G;
+    for (int c0 = c_first; c0 < c_end; c0 += 8 * MC) {
+        __syncthreads();
+        if (c0 + 8 * warp < c_end) {  // n-tile `warp` of this round
+            const int c = c0 + 8 * warp + g, i = c / G;
+            Cols<D, 1> o;
+            load_cols<D, 1>(o, 0, c < c_end ? a.q + (b * a.qs.b + i * a.qs.s + (h * G + c % G) * a.qs.h) : nullptr, a.scale, lane);
+#pragma unroll
+            for (int gr = 0; gr < GR; ++gr)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    sf[warp][(gr * 4 + j) * 2][lane] = o.f[gr][j][0][0];
+                    sf[warp][(gr * 4 + j) * 2 + 1][lane] = o.f[gr][j][0][1];
+                }
+            if (g == 0)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    sc[warp][0][2 * t + e] = o.c[0][e];
+#pragma unroll
+                    for (int gr = 0; gr < GR; ++gr) sc[warp][1 + gr][2 * t + e] = o.q[gr][0][e];
+                }
+            if (t == 0) {
+                // log2 of the row's sum (+inf: a column past the end), and the keys it sees
+                sc[warp][1 + GR][g] = c < c_end ? a.lse[((size_t)b * a.S + i) * a.Hq + h * G + c % G] * LOG2E : INFINITY;
+                sc[warp][2 + GR][g] = __int_as_float(c < c_end ? (a.causal ? min(T, rw.off + i + 1) : T) : 0);
+            }
+        }
+        __syncthreads();
+        if (key0 >= T) continue;
+        const int nn = min(MC, (c_end - c0 + 7) / 8);
+        for (int n = 0; n < nn; ++n) {
+            Cols<D, 1> cols;
+            float lse2[2];
+            int vis[2];
+#pragma unroll
+            for (int gr = 0; gr < GR; ++gr)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    cols.f[gr][j][0][0] = sf[n][(gr * 4 + j) * 2][lane];
+                    cols.f[gr][j][0][1] = sf[n][(gr * 4 + j) * 2 + 1][lane];
+                }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                cols.c[0][e] = sc[n][0][2 * t + e];
+#pragma unroll
+                for (int gr = 0; gr < GR; ++gr) cols.q[gr][0][e] = sc[n][1 + gr][2 * t + e];
+                lse2[e] = sc[n][1 + GR][2 * t + e];
+                vis[e] = __float_as_int(sc[n][2 + GR][2 * t + e]);
+            }
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                float acc[GR][1][4];
+                key_dots<D, 1>(acc, kw[kb], cols);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 2 * kb + (e >> 1);
+                    float d = ks[r][0] * acc[0][0][e], u = fmaf(kz[r][0], cols.q[0][0][e & 1], -lse2[e & 1]);
+                    if (GR == 2) {
+                        d = fmaf(ks[r][GR - 1], acc[GR - 1][0][e], d);
+                        u = fmaf(kz[r][GR - 1], cols.q[GR - 1][0][e & 1], u);
+                    }
+                    const float p = ex2(fmaf(cols.c[0][e & 1], d, u));
+                    sum[r] += key0 + 8 * r + g < vis[e & 1] ? p : 0.f;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+        const int k = key0 + 8 * r + g;
+        if (t == 0 && k < T) a.mass[bh * a.c.max_pos + k] += sum[r];
+    }
+}
+
+template <typename K, typename... Args>
+cudaError_t launch(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+struct Shape {
+    int nt, cb, ncb, shares;
+};
+Shape shape_of(const Kv4View& c, int S, int Hq, int num_sms) {
+    const long long C = (long long)(Hq / c.heads) * S;
+    Shape s;
+    s.nt = C <= 8 ? 1 : 2;
+    s.cb = 8 * s.nt;
+    s.ncb = (int)((C + s.cb - 1) / s.cb);
+    s.shares = s.nt == 1 ? 2 * num_sms : num_sms;
+    return s;
+}
+
+template <int D, int NT>
+cudaError_t launch_split(const Kv4AttnArgs& a, const Shape& sp, const Scratch& sc, cudaStream_t st) {
+    constexpr int smem = SplitSmem<D, NT>::BYTES;
+    cudaError_t e = ensure_max_dyn_smem(kv4_attn_split_kernel<D, NT>, smem);
+    if (e != cudaSuccess) return e;
+    e = launch(kv4_attn_split_kernel<D, NT>, dim3(sp.shares), dim3(ANT), smem, st, false, a, sp.ncb, sc.plan, sc.part, sc.ml);
+    if (e != cudaSuccess) return e;
+    return launch(kv4_attn_join_kernel<D>, dim3((unsigned)(a.S * a.Hq), a.c.batch), dim3(D), 0, st, true, a, sp.cb, sp.ncb,
+                  (const long long*)sc.plan, (const float*)sc.part, (const float2*)sc.ml);
+}
+
+template <int D>
+cudaError_t launch_d(const Kv4AttnArgs& a, const Shape& sp, const Scratch& sc, cudaStream_t st) {
+    const cudaError_t e = sp.nt == 1 ? launch_split<D, 1>(a, sp, sc, st) : launch_split<D, 2>(a, sp, sc, st);
+    if (e != cudaSuccess || !a.mass) return e;
+    const dim3 grid((a.c.max_pos + AW * TK - 1) / (AW * TK), a.c.heads, a.c.batch);
+    return launch(kv4_mass_kernel<D>, grid, dim3(ANT), 0, st, true, a);
 }
 
 }  // namespace
 
-size_t kv4_attn_scratch_bytes(const Kv4View& c, int S, int Hq, int) { return (size_t)c.batch * S * Hq * sizeof(float); }
+size_t kv4_attn_scratch_bytes(const Kv4View& c, int S, int Hq, int num_sms) {
+    const Shape sp = shape_of(c, S, Hq, num_sms);
+    return scratch_of(nullptr, c, S, Hq, sp.shares, sp.cb).bytes;
+}
 
-cudaError_t launch_kv4_attention(const Kv4AttnArgs& in, void* scratch, int, cudaStream_t st) {
+cudaError_t launch_kv4_attention(const Kv4AttnArgs& in, void* scratch, int num_sms, cudaStream_t st) {
     Kv4AttnArgs a = in;
-    if (a.mass && !a.lse) a.lse = static_cast<float*>(scratch);
-    const long long items = (long long)a.c.batch * a.S * a.Hq;
-    const unsigned blocks = (unsigned)((items + 3) / 4);
-    if (a.c.D == 128)
-        kv4_attn_row_kernel<128><<<blocks, 128, 0, st>>>(a);
-    else
-        kv4_attn_row_kernel<64><<<blocks, 128, 0, st>>>(a);
-    if (a.mass) {
-        const dim3 grid((a.c.max_pos + 3) / 4, a.c.heads, a.c.batch);
-        if (a.c.D == 128)
-            kv4_mass_row_kernel<128><<<grid, 128, 0, st>>>(a);
-        else
-            kv4_mass_row_kernel<64><<<grid, 128, 0, st>>>(a);
-    }
-    return cudaGetLastError();
+    const Shape sp = shape_of(a.c, a.S, a.Hq, num_sms);
+    const Scratch sc = scratch_of(scratch, a.c, a.S, a.Hq, sp.shares, sp.cb);
+    if (a.mass && !a.lse) a.lse = sc.lse;
+    return a.c.D == 128 ? launch_d<128>(a, sp, sc, st) : launch_d<64>(a, sp, sc, st);
 }
 
 }  // namespace qw

@@ -1,0 +1,428 @@
+// Attention arithmetic on 32-key tiles of a 4-bit KV cache, shared by the
+// attention and the weight-accumulation kernels.
+//
+// A warp multiplies a tile's packed rows without dequantising them.  With
+// n the stored integers, group g of a key row stands for s_g n + b_g, so
+//   <q, k_j>       = sum_g s_jg <q_g, n_jg> + b_jg sum(q_g)
+//   sum_j p_j v_j  = sum_j (p_j s_jg) n_jg + sum_j p_j b_jg
+// and the tensor cores (mma m16n8k16, fp16 operands, fp32 sums) only see n and
+// q or n and p s.  A nibble left in the low bits of an fp16 is the subnormal
+// n 2^-24 (16 n 2^-24 for the odd ones): four ANDs and a shift unpack a word,
+// and the products are exact.  Keys (for the scores) and dimensions (for the
+// values) are the M index, 8 query columns per kv head the N index, so the few
+// rows of a decode step waste little of the tensor cores.
+//
+// Operand rounding:
+//   * q: bf16 times a power of two per column (largest magnitude at 2^14) is
+//     exact in fp16; elements 2^25 below the largest lose bits that are below
+//     2^-39 of it.
+//   * p s: fp16 (relative 2^-11; normal numbers down to 2^-25 of the largest
+//     p s) -- p and s times powers of two, p against the running maximum m, s
+//     against the largest value scale met so far (sref).  The output is bf16,
+//     whose own half step is eight times that.
+// Everything else (scores, maxima, sums, the bias part of the output) is fp32.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "kv4.h"
+
+namespace qw {
+namespace kv4 {
+
+constexpr int TK = 32;            // keys of a tile
+constexpr float M0 = -3.0e38f;    // running maximum before the first key
+constexpr float LAZY = 4.f;       // the maximum is raised when a score passes it by 2^LAZY
+constexpr float PSCALE = 2048.f;  // p s / sref <= 2^LAZY enters fp16 times this: at most 2^15
+constexpr float LN2 = 0.6931471805599453f, LOG2E = 1.4426950408889634f;
+
+// Shared memory of a tile: K words, V words (16-byte chunks at chunk_pos), then
+// scales and biases of K and of V.
+template <int D>
+struct Tile {
+    static constexpr int GR = D / 64, ROWB = D / 2, CPR = D / 32;  // groups, word bytes and 16-byte chunks of a row
+    static constexpr int VW = TK * ROWB, SB = 2 * TK * ROWB, SBB = TK * GR * 2;
+    static constexpr int BYTES = SB + 4 * SBB;
+    // Chunk c of key k.  The score reads (8 bytes per lane: 4 keys, 4 lanes each) and the value
+    // reads (4 bytes per lane: keys 0, 2, 4, 6 or 1, 3, 5, 7, 8 lanes each) both touch all 32 banks once.
+    static QW_DEV int chunk_pos(int k, int c) {
+        return D == 128 ? (k >> 1) * 8 + ((k ^ (k >> 2)) & 1) * 4 + (c ^ (k & 2))
+                        : (k >> 2) * 8 + (((k ^ (k >> 2)) & 1) | (k & 2)) * 2 + c;
+    }
+};
+
+QW_DEV void cp_async16_zfill(uint32_t dst, const void* src, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+
+// Global pointers of one (sequence, kv head).
+struct Rows {
+    const unsigned char* w[2];
+    const unsigned char *s[2], *b[2];
+};
+template <int D>
+QW_DEV Rows head_rows(const Kv4View& c, size_t bh) {
+    Rows r;
+    const size_t row = bh * c.max_pos;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        r.w[i] = reinterpret_cast<const unsigned char*>(c.p[i].w) + row * (D / 2);
+        r.s[i] = reinterpret_cast<const unsigned char*>(c.p[i].s) + row * (D / 32);
+        r.b[i] = reinterpret_cast<const unsigned char*>(c.p[i].b) + row * (D / 32);
+    }
+    return r;
+}
+
+// Keys [key0, key0 + 32) into the tile at shared address `dst`, by the lanes of
+// one warp; rows from T on arrive as zeros (scales and biases in pieces of 16
+// bytes, so up to 7 rows past T may hold what the cache has there).
+template <int D, bool V>
+QW_DEV void load_tile(uint32_t dst, const Rows& r, int key0, int T, int lane) {
+    using L = Tile<D>;
+    constexpr int CH = TK * L::CPR;
+#pragma unroll
+    for (int w = 0; w < (V ? 2 : 1); ++w)
+#pragma unroll
+        for (int i = 0; i < CH / 32; ++i) {
+            const int idx = lane + 32 * i, k = idx / L::CPR, c = idx % L::CPR;
+            const bool ok = key0 + k < T;
+            cp_async16_zfill(dst + w * L::VW + L::chunk_pos(k, c) * 16,
+                             r.w[w] + (ok ? (size_t)(key0 + k) * L::ROWB + c * 16 : 0), ok);
+        }
+    constexpr int SC = L::SBB / 16, KPC = TK / SC;  // 16-byte pieces of a scale array, keys of a piece
+    if (lane < (V ? 4 : 2) * SC) {
+        const int arr = lane / SC, c = lane % SC;
+        const unsigned char* base = arr & 1 ? r.b[arr >> 1] : r.s[arr >> 1];
+        const bool ok = key0 + c * KPC < T;
+        cp_async16_zfill(dst + L::SB + arr * L::SBB + c * 16, base + (ok ? (size_t)(key0 + c * KPC) * (2 * L::GR) : 0), ok);
+    }
+}
+
+// Query columns of a warp: 8 NT of them.
+template <int D, int NT>
+struct Cols {
+    static constexpr int GR = D / 64;
+    uint32_t f[GR][4][NT][2];                 // B fragments: column lane / 4
+    float c[NT][2], q[GR][NT][2];             // columns 2 (lane % 4) + {0, 1}: score = c <n s, f> + q b
+};
+
+// Column lane / 4 of n-tile n from bf16 row `src` (null: zeros); scale * log2(e) goes into c and q.
+template <int D, int NT>
+QW_DEV void load_cols(Cols<D, NT>& o, int n, const bf16* src, float scale, int lane) {
+    constexpr int GR = D / 64;
+    const int t = lane & 3;
+    float x[GR][16], sum[GR], mx = 0.f;
+#pragma unroll
+    for (int g = 0; g < GR; ++g) {
+        sum[g] = 0.f;
+        uint4 u[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+        if (src) {
+            u[0] = *reinterpret_cast<const uint4*>(src + 64 * g + 16 * t);
+            u[1] = *reinterpret_cast<const uint4*>(src + 64 * g + 16 * t + 8);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t X[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[g][8 * j + 2 * e] = bits_lo_f(X[e]);
+                x[g][8 * j + 2 * e + 1] = bits_hi_f(X[e]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            sum[g] += x[g][e];
+            mx = fmaxf(mx, fabsf(x[g][e]));
+        }
+        sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
+        sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
+    }
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    // 2^ex is the largest magnitude's power of two; columns below 2^-100 keep that scaling
+    const int ex = max((int)(__float_as_uint(mx) >> 23) - 127, -100);
+    const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
+    const float down = ldexpf(scale * LOG2E, ex - 14 + 24);
+#pragma unroll
+    for (int g = 0; g < GR; ++g)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                // k-steps of word j: nibbles (0, 4) and 16 x (1, 5), then (2, 6) and 16 x (3, 7)
+                const float* v = &x[g][8 * j + 2 * s];
+                const __half2 lo = __floats2half2_rn(v[0] * up, v[4] * up);
+                const __half2 hi = __floats2half2_rn(v[1] * up * 0.0625f, v[5] * up * 0.0625f);
+                o.f[g][2 * j + s][n][0] = *reinterpret_cast<const uint32_t*>(&lo);
+                o.f[g][2 * j + s][n][1] = *reinterpret_cast<const uint32_t*>(&hi);
+            }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int from = 8 * t + 4 * e;  // a lane of column 2 t + e
+        o.c[n][e] = __shfl_sync(0xffffffffu, down, from);
+#pragma unroll
+        for (int g = 0; g < GR; ++g) o.q[g][n][e] = __shfl_sync(0xffffffffu, sum[g], from) * (scale * LOG2E);
+    }
+}
+
+// A tile's K operand of one 16-key block: rows lane / 4 and lane / 4 + 8.
+template <int D>
+struct KeyBlock {
+    uint32_t w[D / 64][2][2];  // [group][row half][word 2 t + j]
+};
+template <int D>
+QW_DEV void read_keys(KeyBlock<D>& o, const unsigned char* tile, int kb, int lane) {
+    using L = Tile<D>;
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int gr = 0; gr < L::GR; ++gr)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const uint2 u = *reinterpret_cast<const uint2*>(tile + L::chunk_pos(16 * kb + 8 * r + g, 2 * gr + (t >> 1)) * 16 +
+                                                            (t & 1) * 8);
+            o.w[gr][r][0] = u.x;
+            o.w[gr][r][1] = u.y;
+        }
+}
+// acc[group][n][4] = integer dot products of the block's keys with the columns
+template <int D, int NT>
+QW_DEV void key_dots(float (&acc)[D / 64][NT][4], const KeyBlock<D>& k, const Cols<D, NT>& c) {
+#pragma unroll
+    for (int gr = 0; gr < D / 64; ++gr) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[gr][n][e] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const uint32_t a = k.w[gr][0][j] >> (8 * s), b = k.w[gr][1][j] >> (8 * s);
+                const uint32_t a0 = nib_even(a), a1 = nib_even(b), a2 = nib_odd(a), a3 = nib_odd(b);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    mma_f16(acc[gr][n], a0, a1, a2, a3, c.f[gr][2 * j + s][n][0], c.f[gr][2 * j + s][n][1], acc[gr][n]);
+            }
+    }
+}
+
+// Scale and bias pair(s) of key k in array `arr` (0 K, 1 V) of a tile.
+template <int D>
+QW_DEV void read_sb(const unsigned char* tile, int arr, int k, float (&s)[D / 64], float (&b)[D / 64]) {
+    using L = Tile<D>;
+    const unsigned char* p = tile + L::SB + 2 * arr * L::SBB + k * (2 * L::GR);
+    if (D == 128) {
+        const uint32_t us = *reinterpret_cast<const uint32_t*>(p), ub = *reinterpret_cast<const uint32_t*>(p + L::SBB);
+        s[0] = bits_lo_f(us);
+        s[L::GR - 1] = bits_hi_f(us);
+        b[0] = bits_lo_f(ub);
+        b[L::GR - 1] = bits_hi_f(ub);
+    } else {
+        s[0] = u16_to_f(*reinterpret_cast<const uint16_t*>(p));
+        b[0] = u16_to_f(*reinterpret_cast<const uint16_t*>(p + L::SBB));
+    }
+}
+
+QW_DEV float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+QW_DEV uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+// Running softmax and output of a warp's columns.  Lane (g, t) holds the
+// columns 2 t + {0, 1} of every n-tile; l and bs are the lane's share (its keys).
+template <int D, int NT>
+struct State {
+    static constexpr int GR = D / 64;
+    float o[D / 16][NT][4];  // [4 group + i]: rows g -> dimension 64 group + 8 g + 2 i, rows g + 8 -> the next (times 16)
+    float m[NT][2], l[NT][2], bs[GR][NT][2];
+    float sref, sinv;        // value-scale reference (a power of two) and PSCALE / sref
+    QW_DEV void init() {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                m[n][e] = M0;
+                l[n][e] = 0.f;
+#pragma unroll
+                for (int g = 0; g < GR; ++g) bs[g][n][e] = 0.f;
+            }
+        set_sref(0.f);
+    }
+    // sref: the power of two above s, at least 2^-99
+    QW_DEV void set_sref(float s) {
+        const uint32_t e = min(max(__float_as_uint(s) >> 23, 27u) + 1u, 254u);
+        sref = __uint_as_float(e << 23);
+        sinv = __uint_as_float((254u + 11u - e) << 23);
+    }
+};
+
+// One tile: keys [key0, key0 + 32) of which vis[n][e] (absolute) are visible to
+// column (n, e).  EDGE: some key of the tile is not visible to some column.
+template <int D, int NT, bool EDGE>
+QW_DEV void attend_tile(State<D, NT>& st, const Cols<D, NT>& cols, const unsigned char* tile, int key0, int T,
+                        const int (&vis)[NT][2], int lane) {
+    using L = Tile<D>;
+    constexpr int GR = L::GR;
+    const int g = lane >> 2, t = lane & 3;
+    float acc[2][GR][NT][4];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+        KeyBlock<D> k;
+        read_keys<D>(k, tile, kb, lane);
+        key_dots<D, NT>(acc[kb], k, cols);
+    }
+    float ks[4][GR], kz[4][GR];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) read_sb<D>(tile, 0, 8 * r + g, ks[r], kz[r]);
+    // x[kb][n][2 r + e]: score of key 16 kb + 8 r + g and column 2 t + e, less the column's base
+    float x[2][NT][4];
+    auto scores = [&](auto base) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 2 * kb + (e >> 1);
+                    float d = ks[r][0] * acc[kb][0][n][e], u = fmaf(kz[r][0], cols.q[0][n][e & 1], -base(n, e & 1));
+                    if (GR == 2) {
+                        d = fmaf(ks[r][GR - 1], acc[kb][GR - 1][n][e], d);
+                        u = fmaf(kz[r][GR - 1], cols.q[GR - 1][n][e & 1], u);
+                    }
+                    x[kb][n][e] = fmaf(cols.c[n][e & 1], d, u);
+                    if (EDGE && key0 + 8 * r + g >= vis[n][e & 1]) x[kb][n][e] = -INFINITY;
+                }
+    };
+    scores([&](int n, int e) { return st.m[n][e]; });
+    // largest value scale of the tile (lane = key)
+    float vs[4][GR], vz[4][GR], smax;
+    read_sb<D>(tile, 1, lane, vs[0], vz[0]);
+    smax = GR == 2 ? fmaxf(fabsf(vs[0][0]), fabsf(vs[0][GR - 1])) : fabsf(vs[0][0]);
+    if (EDGE && key0 + lane >= T) smax = 0.f;
+    float top = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, x[kb][n][e]);
+    if (__any_sync(0xffffffffu, top > LAZY || smax > st.sref)) {
+        // rare: raise the column maxima to the tile's, the scale reference to its largest scale
+        const float before = st.sref;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, o));
+        if (smax > st.sref) st.set_sref(smax);
+        const float rs = before == st.sref ? 1.f : before / st.sref;
+        scores([](int, int) { return 0.f; });
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float mx = fmaxf(fmaxf(x[0][n][e], x[0][n][2 + e]), fmaxf(x[1][n][e], x[1][n][2 + e]));
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                mx = fmaxf(mx, st.m[n][e]);
+                const float al = ex2(st.m[n][e] - mx);
+                st.m[n][e] = mx;
+                st.l[n][e] *= al;
+#pragma unroll
+                for (int gr = 0; gr < GR; ++gr) st.bs[gr][n][e] *= al;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    st.o[i][n][e] *= al * rs;
+                    st.o[i][n][2 + e] *= al * rs;
+                }
+            }
+        scores([&](int n, int e) { return st.m[n][e]; });
+    }
+    // probabilities, their sums, and p s in the B-operand layout (keys along k)
+    uint32_t pb[2][GR][NT][2];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) read_sb<D>(tile, 1, 8 * r + g, vs[r], vz[r]);
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float x0 = x[kb][n][2 * r], x1 = x[kb][n][2 * r + 1];
+                const float p0 = ex2(x0), p1 = ex2(x1);
+                const int kr = 2 * kb + r;
+                st.l[n][0] += p0;
+                st.l[n][1] += p1;
+#pragma unroll
+                for (int gr = 0; gr < GR; ++gr) {
+                    const float sc = vs[kr][gr] * st.sinv;
+                    float a0 = p0 * sc, a1 = p1 * sc;
+                    if (EDGE) {  // a hidden key's scale and bias may be anything
+                        a0 = x0 == -INFINITY ? 0.f : a0;
+                        a1 = x1 == -INFINITY ? 0.f : a1;
+                        st.bs[gr][n][0] = x0 == -INFINITY ? st.bs[gr][n][0] : fmaf(p0, vz[kr][gr], st.bs[gr][n][0]);
+                        st.bs[gr][n][1] = x1 == -INFINITY ? st.bs[gr][n][1] : fmaf(p1, vz[kr][gr], st.bs[gr][n][1]);
+                    } else {
+                        st.bs[gr][n][0] = fmaf(p0, vz[kr][gr], st.bs[gr][n][0]);
+                        st.bs[gr][n][1] = fmaf(p1, vz[kr][gr], st.bs[gr][n][1]);
+                    }
+                    const __half2 h = __floats2half2_rn(a0, a1);
+                    pb[kb][gr][n][r] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h));
+                }
+            }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr) {
+            uint32_t w[4];  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of the block
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int k = 16 * kb + 2 * t + (i & 1) + 8 * (i >> 1);
+                w[i] = *reinterpret_cast<const uint32_t*>(tile + L::VW + L::chunk_pos(k, 2 * gr + (g >> 2)) * 16 + (g & 3) * 4);
+            }
+            const uint32_t lo[2] = {prmt(w[0], w[1], 0x5410), prmt(w[0], w[1], 0x7632)};
+            const uint32_t hi[2] = {prmt(w[2], w[3], 0x5410), prmt(w[2], w[3], 0x7632)};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t u = lo[i >> 1] >> (8 * (i & 1)), v = hi[i >> 1] >> (8 * (i & 1));
+                const uint32_t a0 = nib_even(u), a1 = nib_odd(u), a2 = nib_even(v), a3 = nib_odd(v);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    mma_f16(st.o[4 * gr + i][n], a0, a1, a2, a3, pb[kb][gr][n][0], pb[kb][gr][n][1], st.o[4 * gr + i][n]);
+            }
+        }
+}
+
+// The state's share of the output, dimension pair 64 gr + 8 g + 2 i of columns 2 t + e:
+// what the tensor cores summed, in the values' units, plus the lanes' bias sums (reduced before).
+template <int D, int NT>
+QW_DEV float2 out_pair(const State<D, NT>& st, int gr, int i, int n, int e) {
+    constexpr float f = QW_NIB_SCALE / PSCALE;
+    return make_float2(fmaf(st.o[4 * gr + i][n][e] * f, st.sref, st.bs[gr][n][e]),
+                       fmaf(st.o[4 * gr + i][n][2 + e] * (f * 0.0625f), st.sref, st.bs[gr][n][e]));
+}
+// Sums over the lanes of a column (its keys).
+template <int D, int NT>
+QW_DEV void reduce_lanes(State<D, NT>& st) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                st.l[n][e] += __shfl_xor_sync(0xffffffffu, st.l[n][e], o);
+#pragma unroll
+                for (int gr = 0; gr < D / 64; ++gr) st.bs[gr][n][e] += __shfl_xor_sync(0xffffffffu, st.bs[gr][n][e], o);
+            }
+}
+
+}  // namespace kv4
+}  // namespace qw
