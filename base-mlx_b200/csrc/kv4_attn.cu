@@ -30,7 +30,7 @@ constexpr int ASTAGES = 3;            // tiles of a warp's load ring
 // partials [2 shares][columns][D] and their (maximum, sum); then the lse of a
 // call that accumulates weights but returns none.
 struct Scratch {
-    long long* plan;
+    int* plan;
     float* part;
     float2* ml;
     float* lse;
@@ -44,7 +44,7 @@ Scratch scratch_of(void* base, const Kv4View& c, int S, int Hq, int shares, int 
         p += (n + 255) & ~(size_t)255;
         return r;
     };
-    s.plan = reinterpret_cast<long long*>(take((size_t)(c.batch + 1) * 8));
+    s.plan = reinterpret_cast<int*>(take((size_t)(c.batch + 1) * 4));
     s.part = reinterpret_cast<float*>(take((size_t)2 * shares * cb * c.D * 4));
     s.ml = reinterpret_cast<float2*>(take((size_t)2 * shares * cb * 8));
     s.lse = reinterpret_cast<float*>(take((size_t)c.batch * S * Hq * 4));
@@ -52,9 +52,42 @@ Scratch scratch_of(void* base, const Kv4View& c, int S, int Hq, int shares, int 
     return s;
 }
 
-QW_DEV long long block_sum(long long v, long long* red) {
+QW_DEV int tiles_of(const Kv4Rows& r) { return (r.off + r.n + TK - 1) / TK; }
+
+// How the call's tiles fall on the shares: sequence b's tiles are [first, first + heads * ncb * nt).
+constexpr int WARP_SEQS = 128;  // up to here every warp works the plan out by itself
+
+// A warp's view of up to WARP_SEQS sequences: lane l holds sequences 4 l .. 4 l + 3.
+struct WarpPlan {
+    int n[4], at, total;  // tiles of the lane's sequences, first tile of its first one, all tiles
+    QW_DEV void make(const Kv4AttnArgs& a, int per_tile, bool report) {
+        const int lane = threadIdx.x & 31;
+        int s = 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        for (int i = 0; i < 4; ++i) {
+            const int b = 4 * lane + i;
+            n[i] = b < a.c.batch ? per_tile * tiles_of(kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, a.err, report)) : 0;
+            s += n[i];
+        }
+        at = s;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, at, o);
+            if (lane >= o) at += v;
+        }
+        total = __shfl_sync(0xffffffffu, at, 31);
+        at -= s;
+    }
+    QW_DEV int first(int b) const {  // first tile of sequence b
+        const int i = b & 3;
+        int v = at + (i > 0 ? n[0] : 0) + (i > 1 ? n[1] : 0) + (i > 2 ? n[2] : 0);
+        return __shfl_sync(0xffffffffu, v, b >> 2);
+    }
+};
+QW_DEV int share_size(int total, int shares) { return max(1, (total + shares - 1) / shares); }
+
+QW_DEV int block_sum(int v, int* red) {
+    v = __reduce_add_sync(0xffffffffu, v);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
@@ -64,12 +97,12 @@ QW_DEV long long block_sum(long long v, long long* red) {
     return v;
 }
 // Exclusive prefix over the block's threads.
-QW_DEV long long block_prefix(long long v, long long* red) {
+QW_DEV int block_prefix(int v, int* red) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long s = v;
+    int s = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long t = __shfl_up_sync(0xffffffffu, s, o);
+        const int t = __shfl_up_sync(0xffffffffu, s, o);
         if (lane >= o) s += t;
     }
     __syncthreads();
@@ -80,36 +113,53 @@ QW_DEV long long block_prefix(long long v, long long* red) {
     return s;
 }
 
-QW_DEV int tiles_of(const Kv4Rows& r) { return (r.off + r.n + TK - 1) / TK; }
-
 struct Share {
-    long long per, begin, end;  // tiles of a share; this block's [begin, end)
-    int b;                      // sequence of tile `begin`
-    long long b0;               // its first tile
+    int begin, end;  // this block's tiles
+    int b, b0;       // sequence of tile `begin` and its first tile
 };
 
-// This block's share; block 0 writes the plan for the joining kernel.
-QW_DEV Share take_share(const Kv4AttnArgs& a, int ncb, long long* plan) {
-    __shared__ long long red[AW], found[2];
-    const int B = a.c.batch, tid = threadIdx.x;
-    const long long per_tile = (long long)a.c.heads * ncb;
-    long long total = 0;
+// This block's share.  For many sequences block 0 leaves the plan to the joining kernel.
+QW_DEV Share take_share(const Kv4AttnArgs& a, int ncb, int* plan) {
+    const int B = a.c.batch, tid = threadIdx.x, per_tile = a.c.heads * ncb;
+    Share s;
+    if (B <= WARP_SEQS) {
+        WarpPlan p;
+        p.make(a, per_tile, blockIdx.x == 0 && tid < 32);
+        const int per = share_size(p.total, gridDim.x);
+        s.begin = min((long long)p.total, (long long)per * blockIdx.x);
+        s.end = min(p.total, s.begin + per);
+        s.b = B;
+        s.b0 = 0;
+        int at = p.at;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned hit = __ballot_sync(0xffffffffu, at <= s.begin && s.begin < at + p.n[i]);
+            if (hit) {
+                const int l = __ffs(hit) - 1;
+                s.b = 4 * l + i;
+                s.b0 = __shfl_sync(0xffffffffu, at, l);
+            }
+            at += p.n[i];
+        }
+        return s;
+    }
+    __shared__ int red[AW], found[2];
+    int total = 0;
     for (int b = tid; b < B; b += ANT)
         total += per_tile * tiles_of(kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, a.err, blockIdx.x == 0));
     total = block_sum(total, red);
-    Share s;
-    s.per = max(1ll, (total + gridDim.x - 1) / gridDim.x);
-    s.begin = min(total, s.per * blockIdx.x);
-    s.end = min(total, s.begin + s.per);
+    const int per = share_size(total, gridDim.x);
+    s.begin = min((long long)total, (long long)per * blockIdx.x);
+    s.end = min(total, s.begin + per);
     if (tid == 0) found[0] = B;
-    if (blockIdx.x == 0 && tid == 0) plan[0] = s.per;
-    long long base = 0;
+    if (blockIdx.x == 0 && tid == 0) plan[0] = per;
+    int base = 0;
     for (int b0 = 0; b0 < B; b0 += ANT) {
         const int b = b0 + tid;
-        const long long n = b < B ? per_tile * tiles_of(kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false)) : 0;
-        const long long at = base + block_prefix(n, red);
+        const int n = b < B ? per_tile * tiles_of(kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false)) : 0;
+        const int at = base + block_prefix(n, red);
         if (blockIdx.x == 0 && b < B) plan[1 + b] = at;
-        if (n > 0 && at <= s.begin && s.begin < at + n) {
+        if (at <= s.begin && s.begin < at + n) {
             found[0] = b;
             found[1] = at;
         }
@@ -117,7 +167,7 @@ QW_DEV Share take_share(const Kv4AttnArgs& a, int ncb, long long* plan) {
         if (blockIdx.x != 0 && base > s.begin) break;
     }
     __syncthreads();
-    s.b = (int)found[0];
+    s.b = found[0];
     s.b0 = found[1];
     return s;
 }
@@ -134,7 +184,7 @@ struct SplitSmem {
 // state and its own ring of tiles (cp.async, so no warp waits for another),
 // and are merged through shared memory at the end of the segment.
 template <int D, int NT>
-__global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(const Kv4AttnArgs a, int ncb, long long* plan,
+__global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(const Kv4AttnArgs a, int ncb, int* plan,
                                                                               float* part, float2* pml) {
     using L = Tile<D>;
     using SM = SplitSmem<D, NT>;
@@ -144,30 +194,30 @@ __global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(co
     float* wo = reinterpret_cast<float*>(smem);                               // [warp][column][OLD]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int G = a.Hq / a.c.heads, C = G * a.S;
+    pdl_launch_dependents();  // the joining kernel's blocks may settle in; they wait for this kernel's end
     const Share sh = take_share(a, ncb, plan);
     const uint32_t ring = smem_u32(smem) + warp * ASTAGES * L::BYTES;
     const unsigned char* ringp = smem + warp * ASTAGES * L::BYTES;
 
-    long long u = sh.begin, b0 = sh.b0;
-    int b = sh.b;
+    int u = sh.begin, b0 = sh.b0, b = sh.b;
     while (u < sh.end) {
         const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
         const int T = rw.off + rw.n, nt = tiles_of(rw);
-        const long long nseq = (long long)nt * a.c.heads * ncb;
+        const int nseq = nt * a.c.heads * ncb;
         if (u >= b0 + nseq) {  // the next sequence (some are empty)
             b0 += nseq;
             ++b;
             continue;
         }
-        const int seg = (int)((u - b0) / nt), t0 = (int)((u - b0) % nt);
-        const int t1 = (int)min((long long)nt, t0 + (sh.end - u));
+        const int seg = (u - b0) / nt, t0 = (u - b0) % nt;
+        const int t1 = min(nt, t0 + (sh.end - u));
         const int h = seg / ncb, cb = seg % ncb;
         const Rows rows = head_rows<D>(a.c, (size_t)b * a.c.heads + h);
 
         const int mine = max(0, (t1 - t0 - warp + AW - 1) / AW);  // tiles t0 + warp, t0 + warp + 8, ...
         auto issue = [&](int k) {
             if (k < mine)
-                load_tile<D, true>(ring + (k % ASTAGES) * L::BYTES, rows, (t0 + warp + k * AW) * TK, T, lane);
+                load_tile<D>(ring + (k % ASTAGES) * L::BYTES, rows, (t0 + warp + k * AW) * TK, T, lane);
             cp_async_commit();
         };
 #pragma unroll
@@ -218,18 +268,18 @@ __global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(co
 #pragma unroll
                 for (int w = 1; w < AW; ++w) M = fmaxf(M, wml[w * CB + col].x);
                 const float f = ex2(st.m[n][e] - M);
-                float* dst = wo + (warp * CB + col) * SM::OLD + 8 * g;
+                float* dst = wo + (warp * CB + col) * SM::OLD + 4 * g;
 #pragma unroll
                 for (int gr = 0; gr < D / 64; ++gr)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float2 v = out_pair(st, gr, i, n, e);
-                        *reinterpret_cast<float2*>(dst + 64 * gr + 2 * i) = make_float2(v.x * f, v.y * f);
+                        *reinterpret_cast<float2*>(dst + 64 * gr + 32 * (i >> 1) + 2 * (i & 1)) = make_float2(v.x * f, v.y * f);
                     }
             }
         __syncthreads();
         const bool whole = t0 == 0 && t1 == nt;
-        const long long slot = 2ll * blockIdx.x + (u == sh.begin ? 0 : 1);
+        const size_t slot = 2 * (size_t)blockIdx.x + (u == sh.begin ? 0 : 1);
         for (int idx = tid; idx < CB * (D / 2); idx += ANT) {
             const int col = idx / (D / 2), d = 2 * (idx % (D / 2)), c = cb * CB + col, i = c / G;
             if (c >= C) break;
@@ -260,19 +310,30 @@ __global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(co
         __syncthreads();  // the merge buffer is the ring
         u += t1 - t0;
     }
-    pdl_launch_dependents();
 }
 
 // Joins the partials of segments that span shares, and writes the rows of empty
-// sequences.  One block per (column, sequence), one thread per dimension.
+// sequences.  One block per (column, sequence), one thread per dimension; every
+// warp works out the segment's shares and their weights by itself.
 template <int D>
-__global__ void __launch_bounds__(D) kv4_attn_join_kernel(const Kv4AttnArgs a, int cb_size, int ncb, const long long* plan,
+__global__ void __launch_bounds__(D) kv4_attn_join_kernel(const Kv4AttnArgs a, int cb_size, int ncb, int shares, const int* plan,
                                                           const float* part, const float2* pml) {
-    pdl_wait();
-    const int b = blockIdx.y, G = a.Hq / a.c.heads, d = threadIdx.x;
+    const int b = blockIdx.y, G = a.Hq / a.c.heads, d = threadIdx.x, lane = d & 31;
     const int h = blockIdx.x % a.Hq, i = blockIdx.x / a.Hq;  // query head, row
     const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
     const int nt = tiles_of(rw);
+    int per, s0;
+    if (a.c.batch <= WARP_SEQS) {  // before the wait: the lengths are not this call's
+        WarpPlan p;
+        p.make(a, a.c.heads * ncb, false);
+        per = share_size(p.total, shares);
+        s0 = p.first(b);
+        pdl_wait();
+    } else {
+        pdl_wait();
+        per = plan[0];
+        s0 = plan[1 + b];
+    }
     bf16* dst = a.out + (b * a.os.b + i * a.os.s + h * a.os.h) + d;
     float* lse = a.lse ? a.lse + ((size_t)b * a.S + i) * a.Hq + h : nullptr;
     if (nt == 0 || i >= rw.n) {
@@ -281,19 +342,27 @@ __global__ void __launch_bounds__(D) kv4_attn_join_kernel(const Kv4AttnArgs a, i
         return;
     }
     const int c = i * G + h % G, cb = c / cb_size, col = c % cb_size;
-    const long long per = plan[0], s0 = plan[1 + b] + ((long long)(h / G) * ncb + cb) * nt;
-    const long long first = s0 / per, last = (s0 + nt - 1) / per;
+    s0 += ((h / G) * ncb + cb) * nt;
+    const int first = s0 / per, last = (s0 + nt - 1) / per;
     if (first == last) return;
-    auto slot = [&](long long k) { return (2 * k + (k * per >= s0 ? 0 : 1)) * cb_size + col; };
-    float M = M0;
-    for (long long k = first; k <= last; ++k) M = fmaxf(M, pml[slot(k)].x);
-    float o = 0.f, l = 0.f;
-#pragma unroll 4
-    for (long long k = first; k <= last; ++k) {
-        const float2 ml = pml[slot(k)];
-        const float f = ex2(ml.x - M);
-        l = fmaf(ml.y, f, l);
-        o = fmaf(part[slot(k) * D + d], f, o);
+    // the first share's partial of this segment is its second one if the share began before it
+    const size_t p0 = (2 * (size_t)first + (first * per >= s0 ? 0 : 1)) * cb_size + col;
+    auto slot = [&](int k) { return k == first ? p0 : 2 * (size_t)k * cb_size + col; };
+    float M = M0, o = 0.f, l = 0.f;
+    for (int k0 = first; k0 <= last; k0 += 32) {
+        const int n = min(32, last + 1 - k0);
+        const float2 ml = lane < n ? pml[slot(k0 + lane)] : make_float2(M0, 0.f);
+        const float m = fmaxf(M, warp_max(ml.x)), al = ex2(M - m), f = ex2(ml.x - m);
+        l = fmaf(l, al, warp_sum(ml.y * f));
+        o *= al;
+        M = m;
+        for (int j = 0; j < n; j += 8) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = j + e < n ? part[slot(k0 + j + e) * D + d] : 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o = fmaf(v[e], __shfl_sync(0xffffffffu, f, min(j + e, 31)), o);
+        }
     }
     *dst = f2bf(l != 0.f ? o / l : 0.f);
     if (lse && d == 0) *lse = l != 0.f ? (M + log2f(l)) * LN2 : -INFINITY;
@@ -329,7 +398,10 @@ __global__ void __launch_bounds__(ANT, 2) kv4_mass_kernel(const Kv4AttnArgs a) {
 #pragma unroll
         for (int gr = 0; gr < GR; ++gr) {
             uint2 u = make_uint2(0u, 0u);
-            if (ok) u = *reinterpret_cast<const uint2*>(w + (size_t)k * (D / 8) + 8 * gr + 2 * t);
+            if (ok) {
+                u.x = w[(size_t)k * (D / 8) + 8 * gr + t];
+                u.y = w[(size_t)k * (D / 8) + 8 * gr + 4 + t];
+            }
             kw[r >> 1].w[gr][r & 1][0] = u.x;
             kw[r >> 1].w[gr][r & 1][1] = u.y;
             ks[r][gr] = ok ? u16_to_f(s[(size_t)k * GR + gr]) : 0.f;
@@ -451,7 +523,7 @@ cudaError_t launch_split(const Kv4AttnArgs& a, const Shape& sp, const Scratch& s
     e = launch(kv4_attn_split_kernel<D, NT>, dim3(sp.shares), dim3(ANT), smem, st, false, a, sp.ncb, sc.plan, sc.part, sc.ml);
     if (e != cudaSuccess) return e;
     return launch(kv4_attn_join_kernel<D>, dim3((unsigned)(a.S * a.Hq), a.c.batch), dim3(D), 0, st, true, a, sp.cb, sp.ncb,
-                  (const long long*)sc.plan, (const float*)sc.part, (const float2*)sc.ml);
+                  sp.shares, (const int*)sc.plan, (const float*)sc.part, (const float2*)sc.ml);
 }
 
 template <int D>
@@ -472,6 +544,8 @@ size_t kv4_attn_scratch_bytes(const Kv4View& c, int S, int Hq, int num_sms) {
 cudaError_t launch_kv4_attention(const Kv4AttnArgs& in, void* scratch, int num_sms, cudaStream_t st) {
     Kv4AttnArgs a = in;
     const Shape sp = shape_of(a.c, a.S, a.Hq, num_sms);
+    // tiles are counted in 32 bits (180 GB of cache are less than 2^26 tiles of one column block)
+    if ((long long)a.c.batch * a.c.heads * sp.ncb * ((a.c.max_pos + TK - 1) / TK) > 0x7FFFFFFF) return cudaErrorInvalidValue;
     const Scratch sc = scratch_of(scratch, a.c, a.S, a.Hq, sp.shares, sp.cb);
     if (a.mass && !a.lse) a.lse = sc.lse;
     return a.c.D == 128 ? launch_d<128>(a, sp, sc, st) : launch_d<64>(a, sp, sc, st);

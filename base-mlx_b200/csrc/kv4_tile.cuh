@@ -42,14 +42,15 @@ struct Tile {
     static constexpr int GR = D / 64, ROWB = D / 2, CPR = D / 32;  // groups, word bytes and 16-byte chunks of a row
     static constexpr int VW = TK * ROWB, SB = 2 * TK * ROWB, SBB = TK * GR * 2;
     static constexpr int BYTES = SB + 4 * SBB;
-    // Chunk c of key k.  The score reads (8 bytes per lane: 4 keys, 4 lanes each) and the value
-    // reads (4 bytes per lane: keys 0, 2, 4, 6 or 1, 3, 5, 7, 8 lanes each) both touch all 32 banks once.
+    // Chunk c of key k: eight consecutive keys' chunks c, the rows of an ldmatrix, lie in eight bank groups.
     static QW_DEV int chunk_pos(int k, int c) {
-        return D == 128 ? (k >> 1) * 8 + ((k ^ (k >> 2)) & 1) * 4 + (c ^ (k & 2))
-                        : (k >> 2) * 8 + (((k ^ (k >> 2)) & 1) | (k & 2)) * 2 + c;
+        return D == 128 ? 4 * k + (c ^ ((k >> 1) & 3)) : 2 * k + (c ^ ((k >> 2) & 1));
     }
 };
 
+QW_DEV void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 QW_DEV void cp_async16_zfill(uint32_t dst, const void* src, bool ok) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
@@ -75,25 +76,36 @@ QW_DEV Rows head_rows(const Kv4View& c, size_t bh) {
 // Keys [key0, key0 + 32) into the tile at shared address `dst`, by the lanes of
 // one warp; rows from T on arrive as zeros (scales and biases in pieces of 16
 // bytes, so up to 7 rows past T may hold what the cache has there).
-template <int D, bool V>
+template <int D>
 QW_DEV void load_tile(uint32_t dst, const Rows& r, int key0, int T, int lane) {
     using L = Tile<D>;
-    constexpr int CH = TK * L::CPR;
-#pragma unroll
-    for (int w = 0; w < (V ? 2 : 1); ++w)
-#pragma unroll
-        for (int i = 0; i < CH / 32; ++i) {
-            const int idx = lane + 32 * i, k = idx / L::CPR, c = idx % L::CPR;
-            const bool ok = key0 + k < T;
-            cp_async16_zfill(dst + w * L::VW + L::chunk_pos(k, c) * 16,
-                             r.w[w] + (ok ? (size_t)(key0 + k) * L::ROWB + c * 16 : 0), ok);
-        }
+    constexpr int CH = TK * L::CPR;              // 16-byte chunks of the tile's words
     constexpr int SC = L::SBB / 16, KPC = TK / SC;  // 16-byte pieces of a scale array, keys of a piece
-    if (lane < (V ? 4 : 2) * SC) {
-        const int arr = lane / SC, c = lane % SC;
-        const unsigned char* base = arr & 1 ? r.b[arr >> 1] : r.s[arr >> 1];
-        const bool ok = key0 + c * KPC < T;
-        cp_async16_zfill(dst + L::SB + arr * L::SBB + c * 16, base + (ok ? (size_t)(key0 + c * KPC) * (2 * L::GR) : 0), ok);
+    // a row group of 32 chunks further on is a fixed distance away on both sides
+    const uint32_t d = dst + L::chunk_pos(lane / L::CPR, lane % L::CPR) * 16;
+    const unsigned char* s[2] = {r.w[0] + (size_t)key0 * L::ROWB + lane * 16, r.w[1] + (size_t)key0 * L::ROWB + lane * 16};
+    const int arr = lane / SC, piece = lane % SC;
+    const unsigned char* sb = (arr & 2 ? (arr & 1 ? r.b[1] : r.s[1]) : (arr & 1 ? r.b[0] : r.s[0])) +
+                              (size_t)key0 * (2 * L::GR) + piece * 16;
+    const uint32_t sd = dst + L::SB + lane * 16;
+    if (key0 + TK <= T) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int i = 0; i < CH / 32; ++i) cp_async16(d + w * L::VW + i * 512, s[w] + i * 512);
+        if (lane < 4 * SC) cp_async16(sd, sb);
+    } else {
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int i = 0; i < CH / 32; ++i) {
+                const bool ok = key0 + (lane + 32 * i) / L::CPR < T;
+                cp_async16_zfill(d + w * L::VW + i * 512, ok ? s[w] + i * 512 : r.w[w], ok);
+            }
+        if (lane < 4 * SC) {
+            const bool ok = key0 + piece * KPC < T;
+            cp_async16_zfill(sd, ok ? sb : r.s[0], ok);
+        }
     }
 }
 
@@ -101,7 +113,7 @@ QW_DEV void load_tile(uint32_t dst, const Rows& r, int key0, int T, int lane) {
 template <int D, int NT>
 struct Cols {
     static constexpr int GR = D / 64;
-    uint32_t f[GR][4][NT][2];                 // B fragments: column lane / 4
+    uint32_t f[GR][4][NT][2];                 // B fragments: column lane / 4; [2 j + half] of word 4 j + lane % 4
     float c[NT][2], q[GR][NT][2];             // columns 2 (lane % 4) + {0, 1}: score = c <n s, f> + q b
 };
 
@@ -116,8 +128,8 @@ QW_DEV void load_cols(Cols<D, NT>& o, int n, const bf16* src, float scale, int l
         sum[g] = 0.f;
         uint4 u[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
         if (src) {
-            u[0] = *reinterpret_cast<const uint4*>(src + 64 * g + 16 * t);
-            u[1] = *reinterpret_cast<const uint4*>(src + 64 * g + 16 * t + 8);
+            u[0] = *reinterpret_cast<const uint4*>(src + 64 * g + 8 * t);
+            u[1] = *reinterpret_cast<const uint4*>(src + 64 * g + 32 + 8 * t);
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -164,24 +176,41 @@ QW_DEV void load_cols(Cols<D, NT>& o, int n, const bf16* src, float scale, int l
     }
 }
 
-// A tile's K operand of one 16-key block: rows lane / 4 and lane / 4 + 8.
+// Four 8 x 8 matrices of 16-bit halves; lane l gives the row address of matrix l / 8, row l % 8.
+QW_DEV void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+QW_DEV void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+// K operand of one 16-key block: rows g and g + 8 (g = lane / 4), words 4 j + t of every group.
 template <int D>
 struct KeyBlock {
-    uint32_t w[D / 64][2][2];  // [group][row half][word 2 t + j]
+    uint32_t w[D / 64][2][2];  // [group][row half][j]
 };
 template <int D>
-QW_DEV void read_keys(KeyBlock<D>& o, const unsigned char* tile, int kb, int lane) {
+QW_DEV void read_keys(KeyBlock<D>& o, uint32_t tile, int kb, int lane) {
     using L = Tile<D>;
-    const int g = lane >> 2, t = lane & 3;
+    uint32_t r[4];
+    if (D == 128) {  // a matrix = 8 keys x chunk (one word of each per lane); chunk = 2 group + j
 #pragma unroll
-    for (int gr = 0; gr < L::GR; ++gr)
+        for (int h = 0; h < 2; ++h) {
+            ldmatrix4(r, tile + L::chunk_pos(lane & 7, lane >> 3) * 16 + (16 * kb + 8 * h) * L::ROWB);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const uint2 u = *reinterpret_cast<const uint2*>(tile + L::chunk_pos(16 * kb + 8 * r + g, 2 * gr + (t >> 1)) * 16 +
-                                                            (t & 1) * 8);
-            o.w[gr][r][0] = u.x;
-            o.w[gr][r][1] = u.y;
+            for (int c = 0; c < 4; ++c) o.w[(c >> 1) % L::GR][h][c & 1] = r[c];
         }
+    } else {  // matrices: keys 0-7 chunks 0, 1, keys 8-15 chunks 0, 1
+        ldmatrix4(r, tile + L::chunk_pos((lane & 7) + 8 * (lane >> 4), (lane >> 3) & 1) * 16 + 16 * kb * L::ROWB);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o.w[0][c >> 1][c & 1] = r[c];
+    }
 }
 // acc[group][n][4] = integer dot products of the block's keys with the columns
 template <int D, int NT>
@@ -238,7 +267,7 @@ QW_DEV uint32_t transpose8x8(uint32_t v) {
 template <int D, int NT>
 struct State {
     static constexpr int GR = D / 64;
-    float o[D / 16][NT][4];  // [4 group + i]: rows g -> dimension 64 group + 8 g + 2 i, rows g + 8 -> the next (times 16)
+    float o[D / 16][NT][4];  // [4 group + i]: rows g -> dimension 64 group + 32 (i / 2) + 4 g + 2 (i % 2), rows g + 8 -> the next (times 16)
     float m[NT][2], l[NT][2], bs[GR][NT][2];
     float sref, sinv;        // value-scale reference (a power of two) and PSCALE / sref
     QW_DEV void init() {
@@ -272,14 +301,15 @@ struct State {
 template <int D, int NT, bool EDGE>
 QW_DEV void attend_tile(State<D, NT>& st, const Cols<D, NT>& cols, const unsigned char* tile, int key0, int T,
                         const int (&vis)[NT][2], int lane) {
+    const uint32_t tile_s = smem_u32(tile);
     using L = Tile<D>;
     constexpr int GR = L::GR;
-    const int g = lane >> 2, t = lane & 3;
+    const int g = lane >> 2;
     float acc[2][GR][NT][4];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
         KeyBlock<D> k;
-        read_keys<D>(k, tile, kb, lane);
+        read_keys<D>(k, tile_s, kb, lane);
         key_dots<D, NT>(acc[kb], k, cols);
     }
     float ks[4][GR], kz[4][GR];
@@ -378,21 +408,17 @@ QW_DEV void attend_tile(State<D, NT>& st, const Cols<D, NT>& cols, const unsigne
                     pb[kb][gr][n][r] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h));
                 }
             }
+    // Transposed 8 x 8 matrices of the packed rows put halfword h of two neighbouring keys, four
+    // dimensions each, into one register: h = 8 m + g, dimensions 4 h + {0, 1, 2, 3}.
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int gr = 0; gr < GR; ++gr) {
-            uint32_t w[4];  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of the block
+            uint32_t w[4];  // [m & 1][keys 0-7, 8-15 of the block]
+            ldmatrix4_trans(w, tile_s + L::VW + L::chunk_pos((lane & 7) + (lane & 8), 2 * gr + (lane >> 4)) * 16 + 16 * kb * L::ROWB);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int k = 16 * kb + 2 * t + (i & 1) + 8 * (i >> 1);
-                w[i] = *reinterpret_cast<const uint32_t*>(tile + L::VW + L::chunk_pos(k, 2 * gr + (g >> 2)) * 16 + (g & 3) * 4);
-            }
-            const uint32_t lo[2] = {prmt(w[0], w[1], 0x5410), prmt(w[0], w[1], 0x7632)};
-            const uint32_t hi[2] = {prmt(w[2], w[3], 0x5410), prmt(w[2], w[3], 0x7632)};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t u = lo[i >> 1] >> (8 * (i & 1)), v = hi[i >> 1] >> (8 * (i & 1));
+                const uint32_t u = w[2 * (i >> 1)] >> (8 * (i & 1)), v = w[2 * (i >> 1) + 1] >> (8 * (i & 1));
                 const uint32_t a0 = nib_even(u), a1 = nib_odd(u), a2 = nib_even(v), a3 = nib_odd(v);
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
@@ -401,7 +427,7 @@ QW_DEV void attend_tile(State<D, NT>& st, const Cols<D, NT>& cols, const unsigne
         }
 }
 
-// The state's share of the output, dimension pair 64 gr + 8 g + 2 i of columns 2 t + e:
+// The state's share of the output, dimensions 64 gr + 32 (i / 2) + 4 g + 2 (i % 2) + {0, 1} of columns 2 t + e:
 // what the tensor cores summed, in the values' units, plus the lanes' bias sums (reduced before).
 template <int D, int NT>
 QW_DEV float2 out_pair(const State<D, NT>& st, int gr, int i, int n, int e) {
