@@ -13,7 +13,7 @@
 // each of ceil(T_b / 32) tiles of 32 keys; the thread blocks take equal
 // contiguous shares of that list, whatever the lengths, so a ragged batch and
 // one long sequence both fill the GPU.  A segment inside one share is finished
-// there; one that spans shares leaves a partial (maximum, sum, output) per
+// there; one that spans shares leaves a partial (base exponent, sum, output) per
 // share, which a second kernel joins.
 #include "kv4_tile.cuh"
 #include "smem_attr.h"
@@ -27,7 +27,7 @@ constexpr int AW = 8, ANT = 32 * AW;  // warps and threads of a block
 constexpr int ASTAGES = 3;            // tiles of a warp's load ring
 
 // Scratch: [0] tiles per share, [1 + b] first tile of sequence b; then the
-// partials [2 shares][columns][D] and their (maximum, sum); then the lse of a
+// partials [2 shares][columns][D] and their (base exponent, sum); then the lse of a
 // call that accumulates weights but returns none.
 struct Scratch {
     int* plan;
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(co
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) wml[warp * CB + 8 * n + 2 * t + e] = make_float2(st.m[n][e], st.l[n][e]);
+                for (int e = 0; e < 2; ++e) wml[warp * CB + 8 * n + 2 * t + e] = make_float2(-st.nm[n][e], st.l[n][e]);
         __syncthreads();  // also: every warp has left its ring
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -267,14 +267,14 @@ __global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(co
                 float M = wml[col].x;
 #pragma unroll
                 for (int w = 1; w < AW; ++w) M = fmaxf(M, wml[w * CB + col].x);
-                const float f = ex2(st.m[n][e] - M);
+                const float f = half_pow(-st.nm[n][e] - M);
                 float* dst = wo + (warp * CB + col) * SM::OLD + 4 * g;
 #pragma unroll
                 for (int gr = 0; gr < D / 64; ++gr)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float2 v = out_pair(st, gr, i, n, e);
-                        *reinterpret_cast<float2*>(dst + 64 * gr + 32 * (i >> 1) + 2 * (i & 1)) = make_float2(v.x * f, v.y * f);
+                        *reinterpret_cast<float2*>(dst + 64 * gr + 32 * (i >> 1) + 2 * (i & 1)) = make_float2(v.x * f * f, v.y * f * f);
                     }
             }
         __syncthreads();
@@ -290,7 +290,8 @@ __global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(co
 #pragma unroll
             for (int w = 0; w < AW; ++w) {
                 const float2 ml = wml[w * CB + col];
-                l = fmaf(ml.y, ex2(ml.x - M), l);
+                const float f = half_pow(ml.x - M);
+                l = fmaf(ml.y * f, f, l);
                 const float2 v = *reinterpret_cast<const float2*>(wo + (w * CB + col) * SM::OLD + d);
                 o.x += v.x;
                 o.y += v.y;
@@ -352,16 +353,19 @@ __global__ void __launch_bounds__(D) kv4_attn_join_kernel(const Kv4AttnArgs a, i
     for (int k0 = first; k0 <= last; k0 += 32) {
         const int n = min(32, last + 1 - k0);
         const float2 ml = lane < n ? pml[slot(k0 + lane)] : make_float2(M0, 0.f);
-        const float m = fmaxf(M, warp_max(ml.x)), al = ex2(M - m), f = ex2(ml.x - m);
-        l = fmaf(l, al, warp_sum(ml.y * f));
-        o *= al;
+        const float m = fmaxf(M, warp_max(ml.x)), al = half_pow(M - m), f = half_pow(ml.x - m);
+        l = fmaf(l * al, al, warp_sum(ml.y * f * f));
+        o = o * al * al;
         M = m;
         for (int j = 0; j < n; j += 8) {
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = j + e < n ? part[slot(k0 + j + e) * D + d] : 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o = fmaf(v[e], __shfl_sync(0xffffffffu, f, min(j + e, 31)), o);
+            for (int e = 0; e < 8; ++e) {
+                const float fe = __shfl_sync(0xffffffffu, f, min(j + e, 31));
+                o = fmaf(v[e] * fe, fe, o);
+            }
         }
     }
     *dst = f2bf(l != 0.f ? o / l : 0.f);
@@ -376,7 +380,8 @@ template <int D>
 __global__ void __launch_bounds__(ANT, 2) kv4_mass_kernel(const Kv4AttnArgs a) {
     constexpr int GR = D / 64;
     __shared__ uint32_t sf[MC][GR * 4 * 2][32];  // n-tile, fragment register, lane
-    __shared__ float sc[MC][3 + GR][8];          // n-tile, {c, q per group, log2 of the sum, keys seen}, column
+    __shared__ float sc[MC][3][8];               // n-tile, {c, log2 of the sum, keys seen}, column
+    __shared__ uint32_t sq[MC][32];              // n-tile, bias operand, lane
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int h = blockIdx.y, b = blockIdx.z, G = a.Hq / a.c.heads;
@@ -387,7 +392,8 @@ __global__ void __launch_bounds__(ANT, 2) kv4_mass_kernel(const Kv4AttnArgs a) {
     const size_t bh = (size_t)b * a.c.heads + h;
     // K words, scales and biases straight to registers (each is read once)
     KeyBlock<D> kw[2];
-    float ks[4][GR], kz[4][GR];
+    float ks[4][GR];
+    uint32_t kz[4];
     const uint32_t* w = a.c.p[0].w + bh * a.c.max_pos * (D / 8);
     const uint16_t* s = reinterpret_cast<const uint16_t*>(a.c.p[0].s) + bh * a.c.max_pos * GR;
     const uint16_t* z = reinterpret_cast<const uint16_t*>(a.c.p[0].b) + bh * a.c.max_pos * GR;
@@ -405,8 +411,8 @@ __global__ void __launch_bounds__(ANT, 2) kv4_mass_kernel(const Kv4AttnArgs a) {
             kw[r >> 1].w[gr][r & 1][0] = u.x;
             kw[r >> 1].w[gr][r & 1][1] = u.y;
             ks[r][gr] = ok ? u16_to_f(s[(size_t)k * GR + gr]) : 0.f;
-            kz[r][gr] = ok ? u16_to_f(z[(size_t)k * GR + gr]) : 0.f;
         }
+        kz[r] = !ok ? 0u : GR == 2 ? *reinterpret_cast<const uint32_t*>(z + (size_t)k * GR) : (uint32_t)z[(size_t)k * GR];
     }
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     // columns that see none of the block's keys come first when causal: skip them
@@ -427,15 +433,12 @@ __global__ void __launch_bounds__(ANT, 2) kv4_mass_kernel(const Kv4AttnArgs a) {
                 }
             if (g == 0)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    sc[warp][0][2 * t + e] = o.c[0][e];
-#pragma unroll
-                    for (int gr = 0; gr < GR; ++gr) sc[warp][1 + gr][2 * t + e] = o.q[gr][0][e];
-                }
+                for (int e = 0; e < 2; ++e) sc[warp][0][2 * t + e] = o.c[0][e];
+            sq[warp][lane] = o.qb[0];
             if (t == 0) {
                 // log2 of the row's sum (+inf: a column past the end), and the keys it sees
-                sc[warp][1 + GR][g] = c < c_end ? a.lse[((size_t)b * a.S + i) * a.Hq + h * G + c % G] * LOG2E : INFINITY;
-                sc[warp][2 + GR][g] = __int_as_float(c < c_end ? (a.causal ? min(T, rw.off + i + 1) : T) : 0);
+                sc[warp][1][g] = c < c_end ? a.lse[((size_t)b * a.S + i) * a.Hq + h * G + c % G] * LOG2E : INFINITY;
+                sc[warp][2][g] = __int_as_float(c < c_end ? (a.causal ? min(T, rw.off + i + 1) : T) : 0);
             }
         }
         __syncthreads();
@@ -443,8 +446,9 @@ __global__ void __launch_bounds__(ANT, 2) kv4_mass_kernel(const Kv4AttnArgs a) {
         const int nn = min(MC, (c_end - c0 + 7) / 8);
         for (int n = 0; n < nn; ++n) {
             Cols<D, 1> cols;
-            float lse2[2];
+            float base[4];
             int vis[2];
+            cols.qb[0] = sq[n][lane];
 #pragma unroll
             for (int gr = 0; gr < GR; ++gr)
 #pragma unroll
@@ -455,24 +459,20 @@ __global__ void __launch_bounds__(ANT, 2) kv4_mass_kernel(const Kv4AttnArgs a) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 cols.c[0][e] = sc[n][0][2 * t + e];
-#pragma unroll
-                for (int gr = 0; gr < GR; ++gr) cols.q[gr][0][e] = sc[n][1 + gr][2 * t + e];
-                lse2[e] = sc[n][1 + GR][2 * t + e];
-                vis[e] = __float_as_int(sc[n][2 + GR][2 * t + e]);
+                base[e] = base[2 + e] = -sc[n][1][2 * t + e];
+                vis[e] = __float_as_int(sc[n][2][2 * t + e]);
             }
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
-                float acc[GR][1][4];
+                float acc[GR][1][4], x[4];
                 key_dots<D, 1>(acc, kw[kb], cols);
+                mma_bf16_k8(x, kz[2 * kb], kz[2 * kb + 1], cols.qb[0], base);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int r = 2 * kb + (e >> 1);
-                    float d = ks[r][0] * acc[0][0][e], u = fmaf(kz[r][0], cols.q[0][0][e & 1], -lse2[e & 1]);
-                    if (GR == 2) {
-                        d = fmaf(ks[r][GR - 1], acc[GR - 1][0][e], d);
-                        u = fmaf(kz[r][GR - 1], cols.q[GR - 1][0][e & 1], u);
-                    }
-                    const float p = ex2(fmaf(cols.c[0][e & 1], d, u));
+                    float d = ks[r][0] * acc[0][0][e];
+                    if (GR == 2) d = fmaf(ks[r][GR - 1], acc[GR - 1][0][e], d);
+                    const float p = ex2(fmaf(cols.c[0][e & 1], d, x[e]));
                     sum[r] += key0 + 8 * r + g < vis[e & 1] ? p : 0.f;
                 }
             }

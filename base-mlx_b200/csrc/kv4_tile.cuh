@@ -17,9 +17,8 @@
 //     exact in fp16; elements 2^25 below the largest lose bits that are below
 //     2^-39 of it.
 //   * p s: fp16 (relative 2^-11; normal numbers down to 2^-25 of the largest
-//     p s) -- p and s times powers of two, p against the running maximum m, s
-//     against the largest value scale met so far (sref).  The output is bf16,
-//     whose own half step is eight times that.
+//     p s) -- taken times a power of two that keeps the largest near 2^11, see
+//     State.  The output is bf16, whose own half step is eight times that.
 // Everything else (scores, maxima, sums, the bias part of the output) is fp32.
 #pragma once
 #include <cuda_fp16.h>
@@ -32,7 +31,7 @@ namespace kv4 {
 constexpr int TK = 32;            // keys of a tile
 constexpr float M0 = -3.0e38f;    // running maximum before the first key
 constexpr float LAZY = 4.f;       // the maximum is raised when a score passes it by 2^LAZY
-constexpr float PSCALE = 2048.f;  // p s / sref <= 2^LAZY enters fp16 times this: at most 2^15
+constexpr int LOG2_PSCALE = 11;   // p s / sref <= 2^LAZY enters fp16 times 2^11: at most 2^15
 constexpr float LN2 = 0.6931471805599453f, LOG2E = 1.4426950408889634f;
 
 // Shared memory of a tile: K words, V words (16-byte chunks at chunk_pos), then
@@ -114,7 +113,8 @@ template <int D, int NT>
 struct Cols {
     static constexpr int GR = D / 64;
     uint32_t f[GR][4][NT][2];                 // B fragments: column lane / 4; [2 j + half] of word 4 j + lane % 4
-    float c[NT][2], q[GR][NT][2];             // columns 2 (lane % 4) + {0, 1}: score = c <n s, f> + q b
+    float c[NT][2];                           // columns 2 (lane % 4) + {0, 1}: score = c sum_g s_g <n_g, f_g> + sum_g b_g q_g
+    uint32_t qb[NT];                          // the q_g as a B operand of three bf16 terms (24 bits): k = 2 term + group
 };
 
 // Column lane / 4 of n-tile n from bf16 row `src` (null: zeros); scale * log2(e) goes into c and q.
@@ -168,12 +168,22 @@ QW_DEV void load_cols(Cols<D, NT>& o, int n, const bf16* src, float scale, int l
                 o.f[g][2 * j + s][n][1] = *reinterpret_cast<const uint32_t*>(&hi);
             }
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        const int from = 8 * t + 4 * e;  // a lane of column 2 t + e
-        o.c[n][e] = __shfl_sync(0xffffffffu, down, from);
+    for (int e = 0; e < 2; ++e) o.c[n][e] = __shfl_sync(0xffffffffu, down, 8 * t + 4 * e);  // a lane of column 2 t + e
+    uint32_t qb = 0;
 #pragma unroll
-        for (int g = 0; g < GR; ++g) o.q[g][n][e] = __shfl_sync(0xffffffffu, sum[g], from) * (scale * LOG2E);
+    for (int g = 0; g < GR; ++g) {
+        const float v = sum[g] * (scale * LOG2E), hi = bfr(v), mid = bfr(v - hi), lo = v - hi - mid;
+        qb |= (uint32_t)f_to_bf16bits(t == 0 ? hi : t == 1 ? mid : t == 2 ? lo : 0.f) << (16 * g);
     }
+    o.qb[n] = qb;
+}
+
+// D[16x8] (fp32) = A[16x8] (bf16) * B[8x8] (bf16) + C: a0 row g, a1 row g + 8, b column g, k = 2 t + {0, 1}.
+QW_DEV void mma_bf16_k8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b, const float (&c)[4]) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%8,%9,%10};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(b), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
 // Four 8 x 8 matrices of 16-bit halves; lane l gives the row address of matrix l / 8, row l % 8.
@@ -234,21 +244,17 @@ QW_DEV void key_dots(float (&acc)[D / 64][NT][4], const KeyBlock<D>& k, const Co
     }
 }
 
-// Scale and bias pair(s) of key k in array `arr` (0 K, 1 V) of a tile.
+// The bf16 of every group of key k, packed; array 0 K scales, 1 K biases, 2 V scales, 3 V biases.
 template <int D>
-QW_DEV void read_sb(const unsigned char* tile, int arr, int k, float (&s)[D / 64], float (&b)[D / 64]) {
+QW_DEV uint32_t read_packed(const unsigned char* tile, int arr, int k) {
     using L = Tile<D>;
-    const unsigned char* p = tile + L::SB + 2 * arr * L::SBB + k * (2 * L::GR);
-    if (D == 128) {
-        const uint32_t us = *reinterpret_cast<const uint32_t*>(p), ub = *reinterpret_cast<const uint32_t*>(p + L::SBB);
-        s[0] = bits_lo_f(us);
-        s[L::GR - 1] = bits_hi_f(us);
-        b[0] = bits_lo_f(ub);
-        b[L::GR - 1] = bits_hi_f(ub);
-    } else {
-        s[0] = u16_to_f(*reinterpret_cast<const uint16_t*>(p));
-        b[0] = u16_to_f(*reinterpret_cast<const uint16_t*>(p + L::SBB));
-    }
+    const unsigned char* p = tile + L::SB + arr * L::SBB + k * (2 * L::GR);
+    return D == 128 ? *reinterpret_cast<const uint32_t*>(p) : (uint32_t)*reinterpret_cast<const uint16_t*>(p);
+}
+template <int GR>
+QW_DEV void unpack(uint32_t u, float (&v)[GR]) {
+    v[0] = bits_lo_f(u);
+    if (GR == 2) v[GR - 1] = bits_hi_f(u);
 }
 
 QW_DEV float ex2(float x) {
@@ -256,6 +262,8 @@ QW_DEV float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// 2^(d / 2), applied twice where a base changes by d: bases may lie more than 2^126 apart
+QW_DEV float half_pow(float d) { return ex2(0.5f * d); }
 QW_DEV uint32_t transpose8x8(uint32_t v) {
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -263,13 +271,18 @@ QW_DEV uint32_t transpose8x8(uint32_t v) {
 }
 
 // Running softmax and output of a warp's columns.  Lane (g, t) holds the
-// columns 2 t + {0, 1} of every n-tile; l and bs are the lane's share (its keys).
+// columns 2 t + {0, 1} of every n-tile; l and bs are the lane's share (its
+// keys).  o, l and bs are relative to 2^-nm = 2^m sref / PSCALE with m the
+// column's running maximum and sref a power of two above the largest value
+// scale met so far, so exp2(x + nm) s <= 2^LAZY PSCALE enters fp16.
 template <int D, int NT>
 struct State {
     static constexpr int GR = D / 64;
-    float o[D / 16][NT][4];  // [4 group + i]: rows g -> dimension 64 group + 32 (i / 2) + 4 g + 2 (i % 2), rows g + 8 -> the next (times 16)
-    float m[NT][2], l[NT][2], bs[GR][NT][2];
-    float sref, sinv;        // value-scale reference (a power of two) and PSCALE / sref
+    // [4 group + i]: rows g -> dimension 64 group + 32 (i / 2) + 4 g + 2 (i % 2), rows g + 8 -> the next (times 16)
+    float o[D / 16][NT][4];
+    float nm[NT][4];         // {column 0, 1, 0, 1}: the C operand of a score tile
+    float l[NT][2], bs[GR][NT][2];
+    float sref, lim;         // lim: exponent above which a score + nm calls for a new maximum
     QW_DEV void init() {
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
@@ -281,19 +294,20 @@ struct State {
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                m[n][e] = M0;
+                nm[n][e] = nm[n][2 + e] = -M0;
                 l[n][e] = 0.f;
 #pragma unroll
                 for (int g = 0; g < GR; ++g) bs[g][n][e] = 0.f;
             }
         set_sref(0.f);
     }
-    // sref: the power of two above s, at least 2^-99
+    // sref: the power of two above s, at least 2^-79
     QW_DEV void set_sref(float s) {
-        const uint32_t e = min(max(__float_as_uint(s) >> 23, 27u) + 1u, 254u);
+        const uint32_t e = min(max(__float_as_uint(s) >> 23, 47u) + 1u, 254u);
         sref = __uint_as_float(e << 23);
-        sinv = __uint_as_float((254u + 11u - e) << 23);
+        lim = LAZY + shift();
     }
+    QW_DEV float shift() const { return (float)(LOG2_PSCALE + 127 - (int)(__float_as_uint(sref) >> 23)); }  // log2(PSCALE / sref)
 };
 
 // One tile: keys [key0, key0 + 32) of which vis[n][e] (absolute) are visible to
@@ -312,32 +326,35 @@ QW_DEV void attend_tile(State<D, NT>& st, const Cols<D, NT>& cols, const unsigne
         read_keys<D>(k, tile_s, kb, lane);
         key_dots<D, NT>(acc[kb], k, cols);
     }
-    float ks[4][GR], kz[4][GR];
+    float ks[4][GR];
+    uint32_t kz[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) read_sb<D>(tile, 0, 8 * r + g, ks[r], kz[r]);
-    // x[kb][n][2 r + e]: score of key 16 kb + 8 r + g and column 2 t + e, less the column's base
+    for (int r = 0; r < 4; ++r) {
+        unpack<GR>(read_packed<D>(tile, 0, 8 * r + g), ks[r]);
+        kz[r] = read_packed<D>(tile, 1, 8 * r + g);
+    }
+    // x[kb][n][2 r + e]: score of key 16 kb + 8 r + g and column 2 t + e, plus the column's base
     float x[2][NT][4];
-    auto scores = [&](auto base) {
+    auto scores = [&](const float (&base)[NT][4]) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n) {
+                mma_bf16_k8(x[kb][n], kz[2 * kb], kz[2 * kb + 1], cols.qb[n], base[n]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int r = 2 * kb + (e >> 1);
-                    float d = ks[r][0] * acc[kb][0][n][e], u = fmaf(kz[r][0], cols.q[0][n][e & 1], -base(n, e & 1));
-                    if (GR == 2) {
-                        d = fmaf(ks[r][GR - 1], acc[kb][GR - 1][n][e], d);
-                        u = fmaf(kz[r][GR - 1], cols.q[GR - 1][n][e & 1], u);
-                    }
-                    x[kb][n][e] = fmaf(cols.c[n][e & 1], d, u);
+                    float d = ks[r][0] * acc[kb][0][n][e];
+                    if (GR == 2) d = fmaf(ks[r][GR - 1], acc[kb][GR - 1][n][e], d);
+                    x[kb][n][e] = fmaf(cols.c[n][e & 1], d, x[kb][n][e]);
                     if (EDGE && key0 + 8 * r + g >= vis[n][e & 1]) x[kb][n][e] = -INFINITY;
                 }
+            }
     };
-    scores([&](int n, int e) { return st.m[n][e]; });
+    scores(st.nm);
     // largest value scale of the tile (lane = key)
     float vs[4][GR], vz[4][GR], smax;
-    read_sb<D>(tile, 1, lane, vs[0], vz[0]);
+    unpack<GR>(read_packed<D>(tile, 2, lane), vs[0]);
     smax = GR == 2 ? fmaxf(fabsf(vs[0][0]), fabsf(vs[0][GR - 1])) : fabsf(vs[0][0]);
     if (EDGE && key0 + lane >= T) smax = 0.f;
     float top = -INFINITY;
@@ -347,14 +364,15 @@ QW_DEV void attend_tile(State<D, NT>& st, const Cols<D, NT>& cols, const unsigne
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) top = fmaxf(top, x[kb][n][e]);
-    if (__any_sync(0xffffffffu, top > LAZY || smax > st.sref)) {
+    if (__any_sync(0xffffffffu, top > st.lim || smax > st.sref)) {
         // rare: raise the column maxima to the tile's, the scale reference to its largest scale
-        const float before = st.sref;
+        const float before = st.shift();
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, o));
         if (smax > st.sref) st.set_sref(smax);
-        const float rs = before == st.sref ? 1.f : before / st.sref;
-        scores([](int, int) { return 0.f; });
+        const float now = st.shift();
+        const float zero[NT][4] = {};
+        scores(zero);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -362,24 +380,32 @@ QW_DEV void attend_tile(State<D, NT>& st, const Cols<D, NT>& cols, const unsigne
                 float mx = fmaxf(fmaxf(x[0][n][e], x[0][n][2 + e]), fmaxf(x[1][n][e], x[1][n][2 + e]));
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                mx = fmaxf(mx, st.m[n][e]);
-                const float al = ex2(st.m[n][e] - mx);
-                st.m[n][e] = mx;
-                st.l[n][e] *= al;
+                const float old = st.nm[n][e];
+                if (old == -M0) {
+                    if (mx == -INFINITY) continue;  // still no key for this column
+                } else {
+                    mx = fmaxf(mx, before - old);   // the old maximum
+                }
+                const float nm = now - mx, al = old == -M0 ? 0.f : half_pow(nm - old);
+                st.nm[n][e] = st.nm[n][2 + e] = nm;
+                st.l[n][e] = st.l[n][e] * al * al;
 #pragma unroll
-                for (int gr = 0; gr < GR; ++gr) st.bs[gr][n][e] *= al;
+                for (int gr = 0; gr < GR; ++gr) st.bs[gr][n][e] = st.bs[gr][n][e] * al * al;
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) {
-                    st.o[i][n][e] *= al * rs;
-                    st.o[i][n][2 + e] *= al * rs;
+                    st.o[i][n][e] = st.o[i][n][e] * al * al;
+                    st.o[i][n][2 + e] = st.o[i][n][2 + e] * al * al;
                 }
             }
-        scores([&](int n, int e) { return st.m[n][e]; });
+        scores(st.nm);
     }
     // probabilities, their sums, and p s in the B-operand layout (keys along k)
     uint32_t pb[2][GR][NT][2];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) read_sb<D>(tile, 1, 8 * r + g, vs[r], vz[r]);
+    for (int r = 0; r < 4; ++r) {
+        unpack<GR>(read_packed<D>(tile, 2, 8 * r + g), vs[r]);
+        unpack<GR>(read_packed<D>(tile, 3, 8 * r + g), vz[r]);
+    }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -393,8 +419,7 @@ QW_DEV void attend_tile(State<D, NT>& st, const Cols<D, NT>& cols, const unsigne
                 st.l[n][1] += p1;
 #pragma unroll
                 for (int gr = 0; gr < GR; ++gr) {
-                    const float sc = vs[kr][gr] * st.sinv;
-                    float a0 = p0 * sc, a1 = p1 * sc;
+                    float a0 = p0 * vs[kr][gr], a1 = p1 * vs[kr][gr];
                     if (EDGE) {  // a hidden key's scale and bias may be anything
                         a0 = x0 == -INFINITY ? 0.f : a0;
                         a1 = x1 == -INFINITY ? 0.f : a1;
@@ -427,13 +452,12 @@ QW_DEV void attend_tile(State<D, NT>& st, const Cols<D, NT>& cols, const unsigne
         }
 }
 
-// The state's share of the output, dimensions 64 gr + 32 (i / 2) + 4 g + 2 (i % 2) + {0, 1} of columns 2 t + e:
-// what the tensor cores summed, in the values' units, plus the lanes' bias sums (reduced before).
+// The state's share of the output (times the sum's base), dimensions 64 gr + 32 (i / 2) + 4 g +
+// 2 (i % 2) + {0, 1} of columns 2 t + e: what the tensor cores summed plus the bias sums (lanes reduced before).
 template <int D, int NT>
 QW_DEV float2 out_pair(const State<D, NT>& st, int gr, int i, int n, int e) {
-    constexpr float f = QW_NIB_SCALE / PSCALE;
-    return make_float2(fmaf(st.o[4 * gr + i][n][e] * f, st.sref, st.bs[gr][n][e]),
-                       fmaf(st.o[4 * gr + i][n][2 + e] * (f * 0.0625f), st.sref, st.bs[gr][n][e]));
+    return make_float2(fmaf(st.o[4 * gr + i][n][e], QW_NIB_SCALE, st.bs[gr][n][e]),
+                       fmaf(st.o[4 * gr + i][n][2 + e], QW_NIB_SCALE_ODD, st.bs[gr][n][e]));
 }
 // Sums over the lanes of a column (its keys).
 template <int D, int NT>
