@@ -5,16 +5,25 @@
 // position wins a tie).  The kept rows move to the front in position order,
 // with their weights; n <= keep keeps every row.
 //
-//   1. select: weights become unsigned keys of the same order; a radix select
-//      (four 8-bit histogram passes) finds the threshold key and how many of
-//      the keys equal to it stay; one ordered pass writes the kept positions.
+//   1. select: weights become unsigned keys of the same order.  A cluster of
+//      thread blocks takes a (sequence, head), each block a slice of its
+//      positions; three histogram passes (11, 11 and 10 bits, summed over the
+//      cluster through distributed shared memory) find the threshold key and
+//      how many of its equals stay, one prefix over the threads' consecutive
+//      positions writes the kept ones in order.
 //   2. move: dst row r = src row index[r].
+#include <algorithm>
+
 #include "kv4.h"
+#include "smem_attr.h"
 
 namespace qw {
 namespace {
 
 constexpr int SEL_NT = 1024;
+constexpr int BINS = 2048;
+constexpr int SEL_MAX_CLUSTER = 8;
+constexpr int SEL_KEYS = 40960;  // keys of a slice held in shared memory; longer slices are read again per pass
 
 // Unsigned key of the same order as the float; -0 equals +0, NaN is above everything.
 QW_DEV uint32_t order_key(float v) {
@@ -25,6 +34,19 @@ QW_DEV uint32_t order_key(float v) {
 }
 
 QW_DEV int clamp_len(const Kv4EvictArgs& a, int b) { return max(0, min(a.seq_len[b], a.src.max_pos)); }
+
+QW_DEV void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
+// The int at `p` of the cluster's block `rank`.
+QW_DEV int cluster_load(const int* p, int rank) {
+    uint32_t addr;
+    int v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
 
 // Exclusive prefix of `v` over the block (SEL_NT threads) and the block total.
 QW_DEV int block_scan(int v, int* red, int& total) {
@@ -53,96 +75,182 @@ QW_DEV int block_scan(int v, int* red, int& total) {
 }
 
 // index[b][h][0..new length): the kept positions in increasing order.
-__global__ void __launch_bounds__(SEL_NT) kv4_select_kernel(const Kv4EvictArgs a, int* index, int* count) {
-    __shared__ int hist[256];
-    __shared__ int red[32];
-    __shared__ int pick[2];
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+__global__ void __launch_bounds__(SEL_NT) kv4_select_kernel(const Kv4EvictArgs a, int cluster, int slice_keys, int* index,
+                                                            int* count) {
+    extern __shared__ __align__(16) int sel_smem[];
+    int* hist = sel_smem;                                                // [3][BINS]
+    uint32_t* sk = reinterpret_cast<uint32_t*>(sel_smem + 3 * BINS);     // [slice_keys]
+    __shared__ int red[32], pick[2], tally[2];
+    const int rank = blockIdx.x % cluster, h = blockIdx.x / cluster, b = blockIdx.y, tid = threadIdx.x;
+    pdl_launch_dependents();
     const int n = clamp_len(a, b);
     const size_t bh = (size_t)b * a.src.heads + h;
     int* idx = index + bh * a.keep;
-    if (tid == 0 && h == 0) count[b] = min(n, a.keep);
-    if (n <= a.keep) {
-        for (int r = tid; r < a.keep; r += SEL_NT) {
-            idx[r] = r < n ? r : -1;
-            if (a.index_out) a.index_out[bh * a.keep + r] = r < n ? r : -1;
+    int* out = a.index_out ? a.index_out + bh * a.keep : nullptr;
+    if (tid == 0 && h == 0 && rank == 0) count[b] = min(n, a.keep);
+    if (n <= a.keep) {  // the whole cluster takes this branch
+        for (int r = rank * SEL_NT + tid; r < a.keep; r += cluster * SEL_NT) {
+            const int v = r < n ? r : -1;
+            idx[r] = v;
+            if (out) out[r] = v;
         }
         return;
     }
     const float* mass = a.mass_src + bh * a.src.max_pos;
     const int old = n - a.recent, want = a.keep - a.recent;
-    // threshold key and how many of its equals stay
+    const int slice = (n + cluster - 1) / cluster, j0 = min(n, rank * slice), j1 = min(n, j0 + slice);
+    const int jo = max(j0, min(j1, old));  // [j0, jo): may be dropped; [jo, j1): recent
+    const bool held = slice <= slice_keys;
+    for (int i = tid; i < 3 * BINS; i += SEL_NT) hist[i] = 0;
+    __syncthreads();
+    auto key = [&](int j) { return held ? sk[j - j0] : order_key(mass[j]); };
     uint32_t prefix = 0;
     int left = want;
     if (want > 0) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
-            __syncthreads();
-            for (int j = tid; j < old; j += SEL_NT) {
-                const uint32_t k = order_key(mass[j]);
-                if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
+#pragma unroll
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+            const uint32_t mask = pass == 2 ? 1023u : 2047u;
+            int* hp = hist + pass * BINS;
+            for (int j = j0 + tid; j < jo; j += SEL_NT) {
+                uint32_t k;
+                if (pass == 0) {
+                    k = order_key(mass[j]);
+                    if (held) sk[j - j0] = k;
+                } else {
+                    k = key(j);
+                    // every higher digit has to agree
+                    if ((k >> (pass == 1 ? 21 : 10)) != (prefix >> (pass == 1 ? 21 : 10))) continue;
+                }
+                atomicAdd(&hp[(k >> shift) & mask], 1);
             }
-            __syncthreads();
-            if (tid == 0) {
-                int acc = 0, d = 255;
-                while (d > 0 && acc + hist[d] < left) acc += hist[d--];
-                pick[0] = d;
-                pick[1] = left - acc;
+            if (cluster > 1)
+                cluster_sync();
+            else
+                __syncthreads();
+            // thread t counts the bins 2 (1023 - t) + {1, 0}: prefixes run from the largest digit down
+            const int d1 = 2 * (SEL_NT - 1 - tid) + 1;
+            int c1 = 0, c0 = 0;
+            if (cluster > 1) {
+                for (int r = 0; r < cluster; ++r) {
+                    c1 += cluster_load(&hp[d1], r);
+                    c0 += cluster_load(&hp[d1 - 1], r);
+                }
+            } else {
+                c1 = hp[d1];
+                c0 = hp[d1 - 1];
+            }
+            int total;
+            const int above = block_scan(c1 + c0, red, total);
+            if (above < left && left <= above + c1 + c0) {
+                const bool hi = left <= above + c1;
+                pick[0] = hi ? d1 : d1 - 1;
+                pick[1] = left - above - (hi ? 0 : c1);
             }
             __syncthreads();
             prefix |= (uint32_t)pick[0] << shift;
             left = pick[1];
         }
     }
-    int base = 0, ties = 0;
-    for (int j0 = 0; j0 < n; j0 += SEL_NT) {
-        const int j = j0 + tid;
-        int above = 0, equal = 0;
-        if (j < n) {
-            if (j >= old) {
-                above = 1;
-            } else if (want > 0) {
-                const uint32_t k = order_key(mass[j]);
-                above = k > prefix;
-                equal = k == prefix;
-            }
+    // consecutive positions per thread, in order
+    const int kpt = (slice + SEL_NT - 1) / SEL_NT, t0 = min(j1, j0 + tid * kpt), t1 = min(j1, t0 + kpt);
+    int above = 0, equal = 0;
+    for (int j = t0; j < t1; ++j) {
+        if (j >= jo) {
+            ++above;
+        } else if (want > 0) {
+            const uint32_t k = key(j);
+            above += k > prefix;
+            equal += k == prefix;
         }
-        int tot_eq, tot;
-        const int eq_before = ties + block_scan(equal, red, tot_eq);
-        const int keep = above | (equal && eq_before < left);
-        const int at = base + block_scan(keep, red, tot);
+    }
+    int tot_above, tot_equal;
+    int a_before = block_scan(above, red, tot_above), e_before = block_scan(equal, red, tot_equal);
+    if (cluster > 1) {
+        if (tid == 0) {
+            tally[0] = tot_above;
+            tally[1] = tot_equal;
+        }
+        cluster_sync();
+        for (int r = 0; r < rank; ++r) {
+            a_before += cluster_load(&tally[0], r);
+            e_before += cluster_load(&tally[1], r);
+        }
+        cluster_sync();  // a block's tally is read until here
+    }
+    int at = a_before + min(e_before, left);
+    for (int j = t0; j < t1; ++j) {
+        bool keep = j >= jo;
+        if (!keep && want > 0) {
+            const uint32_t k = key(j);
+            keep = k > prefix || (k == prefix && e_before < left);
+            e_before += k == prefix;
+        }
         if (keep) {
             idx[at] = j;
-            if (a.index_out) a.index_out[bh * a.keep + at] = j;
+            if (out) out[at] = j;
+            ++at;
         }
-        ties += tot_eq;
-        base += tot;
     }
 }
 
-// Out of place: one thread per (kept row, 16-byte piece of its words).
+// Out of place.  Words: one thread per 16-byte piece of MR kept rows, all loads
+// before the first store; the rest (blockIdx.y's last part): one thread per row.
+constexpr int MR = 4;
 template <int D>
 __global__ void __launch_bounds__(256) kv4_move_kernel(const Kv4EvictArgs a, const int* index, const int* count) {
-    constexpr int P = D / 32;  // 16-byte pieces of a packed row
-    const int h = blockIdx.y, b = blockIdx.z;
+    constexpr int P = D / 32, RB = 256 / P, GR = D / 64;
+    const int part = blockIdx.y / a.src.heads, h = blockIdx.y % a.src.heads, b = blockIdx.z, tid = threadIdx.x;
     const size_t bh = (size_t)b * a.src.heads + h;
-    const int r = blockIdx.x * (256 / P) + threadIdx.x / P, e = threadIdx.x % P;
-    if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) a.new_len[b] = count[b];
-    if (r >= count[b]) return;
-    const int j = index[bh * a.keep + r];
-    const size_t sr = bh * a.src.max_pos + j, dr = bh * a.dst.max_pos + r;
+    pdl_wait();
+    const int n = count[b];
+    const int* idx = index + bh * a.keep;
+    const size_t s0 = bh * a.src.max_pos, d0 = bh * a.dst.max_pos;
+    const int first = blockIdx.x * MR * RB;
+    if (part < 2) {
+        const int e = tid % P;
+        const uint4* sw = reinterpret_cast<const uint4*>(a.src.p[part].w) + s0 * P + e;
+        uint4* dw = reinterpret_cast<uint4*>(a.dst.p[part].w) + d0 * P + e;
+        int j[MR];
+        uint4 v[MR];
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-        reinterpret_cast<uint4*>(a.dst.p[w].w)[dr * P + e] = reinterpret_cast<const uint4*>(a.src.p[w].w)[sr * P + e];
-        if (e == 0) {
-#pragma unroll
-            for (int g = 0; g < D / 64; ++g) {
-                a.dst.p[w].s[dr * (D / 64) + g] = a.src.p[w].s[sr * (D / 64) + g];
-                a.dst.p[w].b[dr * (D / 64) + g] = a.src.p[w].b[sr * (D / 64) + g];
-            }
+        for (int i = 0; i < MR; ++i) {
+            const int r = first + i * RB + tid / P;
+            j[i] = r < n ? idx[r] : -1;
         }
+#pragma unroll
+        for (int i = 0; i < MR; ++i)
+            if (j[i] >= 0) v[i] = __ldcs(sw + (size_t)j[i] * P);
+#pragma unroll
+        for (int i = 0; i < MR; ++i)
+            if (j[i] >= 0) dw[(size_t)(first + i * RB + tid / P) * P] = v[i];
+        return;
     }
-    if (e == 0) a.mass_dst[dr] = a.mass_src[sr];
+    if (blockIdx.x == 0 && h == 0 && tid == 0) a.new_len[b] = n;
+    for (int r = first + tid; r < min(n, first + MR * RB); r += 256) {
+        const size_t sr = s0 + idx[r], dr = d0 + r;
+        const float m = a.mass_src[sr];
+        if (GR == 2) {
+            uint32_t v[4];
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                v[2 * w] = reinterpret_cast<const uint32_t*>(a.src.p[w].s)[sr];
+                v[2 * w + 1] = reinterpret_cast<const uint32_t*>(a.src.p[w].b)[sr];
+            }
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                reinterpret_cast<uint32_t*>(a.dst.p[w].s)[dr] = v[2 * w];
+                reinterpret_cast<uint32_t*>(a.dst.p[w].b)[dr] = v[2 * w + 1];
+            }
+        } else {
+            const bf16 v0 = a.src.p[0].s[sr], v1 = a.src.p[0].b[sr], v2 = a.src.p[1].s[sr], v3 = a.src.p[1].b[sr];
+            a.dst.p[0].s[dr] = v0;
+            a.dst.p[0].b[dr] = v1;
+            a.dst.p[1].s[dr] = v2;
+            a.dst.p[1].b[dr] = v3;
+        }
+        a.mass_dst[dr] = m;
+    }
 }
 
 // In place: one CTA per (sequence, head, K words | V words | the rest) walks the
@@ -153,6 +261,7 @@ __global__ void __launch_bounds__(1024) kv4_move_inplace_kernel(const Kv4EvictAr
     constexpr int P = D / 32;
     const int part = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const size_t bh = (size_t)b * a.src.heads + h;
+    pdl_wait();
     const int n = count[b];
     const int* idx = index + bh * a.keep;
     const size_t row0 = bh * a.src.max_pos;
@@ -200,6 +309,30 @@ __global__ void __launch_bounds__(1024) kv4_move_inplace_kernel(const Kv4EvictAr
     }
 }
 
+template <typename K, typename... Args>
+cudaError_t launch(K kernel, dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t st, bool pdl, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (pdl) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = cluster;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 }  // namespace
 
 size_t kv4_evict_scratch_bytes(const Kv4View& src, int keep) {
@@ -209,23 +342,28 @@ size_t kv4_evict_scratch_bytes(const Kv4View& src, int keep) {
 cudaError_t launch_kv4_evict(const Kv4EvictArgs& a, void* scratch, cudaStream_t st) {
     int* index = static_cast<int*>(scratch);
     int* count = index + (size_t)a.src.batch * a.src.heads * a.keep;
-    const int D = a.src.D;
-    kv4_select_kernel<<<dim3(a.src.heads, a.src.batch), SEL_NT, 0, st>>>(a, index, count);
+    // blocks of a head: slices of about 1024 positions, as long as one round of blocks holds them all
+    int cluster = 1;
+    while (cluster < SEL_MAX_CLUSTER && a.src.max_pos > 1024 * cluster &&
+           (long long)a.src.batch * a.src.heads * cluster * 2 <= 2 * 148)
+        cluster *= 2;
+    const int keys = std::min(SEL_KEYS, (a.src.max_pos + cluster - 1) / cluster);
+    const int smem = (3 * BINS + keys) * (int)sizeof(int);
+    cudaError_t e = ensure_max_dyn_smem(kv4_select_kernel, (3 * BINS + SEL_KEYS) * (int)sizeof(int));
+    if (e != cudaSuccess) return e;
+    e = launch(kv4_select_kernel, dim3(a.src.heads * cluster, a.src.batch), dim3(SEL_NT), smem, cluster, st, false, a, cluster,
+               keys, index, count);
+    if (e != cudaSuccess) return e;
+    const bool wide = a.src.D == 128;
     if (a.dst.p[0].w == a.src.p[0].w) {
         const dim3 grid(3, a.src.heads, a.src.batch);
-        if (D == 128)
-            kv4_move_inplace_kernel<128><<<grid, 1024, 0, st>>>(a, index, count);
-        else
-            kv4_move_inplace_kernel<64><<<grid, 1024, 0, st>>>(a, index, count);
-    } else {
-        const int rows = 256 / (D / 32);
-        const dim3 grid((a.keep + rows - 1) / rows, a.src.heads, a.src.batch);
-        if (D == 128)
-            kv4_move_kernel<128><<<grid, 256, 0, st>>>(a, index, count);
-        else
-            kv4_move_kernel<64><<<grid, 256, 0, st>>>(a, index, count);
+        return wide ? launch(kv4_move_inplace_kernel<128>, grid, dim3(1024), 0, 1, st, true, a, (const int*)index, (const int*)count)
+                    : launch(kv4_move_inplace_kernel<64>, grid, dim3(1024), 0, 1, st, true, a, (const int*)index, (const int*)count);
     }
-    return cudaGetLastError();
+    const int rows = MR * 256 / (a.src.D / 32);
+    const dim3 grid((a.keep + rows - 1) / rows, 3 * a.src.heads, a.src.batch);
+    return wide ? launch(kv4_move_kernel<128>, grid, dim3(256), 0, 1, st, true, a, (const int*)index, (const int*)count)
+                : launch(kv4_move_kernel<64>, grid, dim3(256), 0, 1, st, true, a, (const int*)index, (const int*)count);
 }
 
 }  // namespace qw

@@ -36,96 +36,149 @@ QW_DEV float group_scale(float hi, float lo) {
     return bfr(s);
 }
 
-QW_DEV uint32_t quantize(float x, float bias, float scale, float inv) {
-    float t = __fmul_rn(__fsub_rn(x, bias), inv);
-    float r = rintf(t);
+// clamp(round_half_even((x - bias) / scale), 0, 15)
+QW_DEV float quantize(float x, float bias, float scale, float inv) {
+    const float t = __fmul_rn(__fsub_rn(x, bias), inv);
+    float r = __fsub_rn(__fadd_rn(t, 12582912.f), 12582912.f);  // 1.5 2^23: rounds to an integer
     if (!(fabsf(t - r) < 0.49999f))  // also taken for an overflowed quotient
         r = (float)rint(((double)x - (double)bias) / (double)scale);
-    return (uint32_t)fminf(fmaxf(r, 0.f), 15.f);
+    return fminf(fmaxf(r, 0.f), 15.f);
 }
 
-// CTA = one (sequence, K or V, head) and NT / TPR consecutive new rows.
-template <int D, bool VEC>
+// Block = one (sequence, K or V, head) and R * NT / TPR consecutive new rows,
+// each thread one word of R of them.  Every input is loaded before the first
+// is used and before the lengths arrive: the blocks are short, so the kernel
+// is bound by the latency of its loads, not by their bytes.
+template <int D, bool VEC, int R>
 __global__ void __launch_bounds__(NT) kv4_append_kernel(const Kv4StoreArgs a) {
-    constexpr int T = TPR<D>;
+    constexpr int T = TPR<D>, RB = NT / T;
     const int which = blockIdx.y / a.c.heads, h = blockIdx.y % a.c.heads, b = blockIdx.z;
-    const int i = blockIdx.x * (NT / T) + threadIdx.x / T, e = threadIdx.x % T;
+    const int i0 = blockIdx.x * (R * RB) + threadIdx.x / T, e = threadIdx.x % T;
+    const bf16* src = a.x[which] + (b * a.xs[which].b + h * a.xs[which].h) + e * 8;
+    uint4 u[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i = i0 + r * RB;
+        u[r] = make_uint4(0u, 0u, 0u, 0u);
+        if (i < a.S) {
+            const bf16* p = src + i * a.xs[which].s;
+            if (VEC) {
+                u[r] = __ldcs(reinterpret_cast<const uint4*>(p));
+            } else {
+                const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+                u[r] = make_uint4(q[0] | ((uint32_t)q[1] << 16), q[2] | ((uint32_t)q[3] << 16),
+                                  q[4] | ((uint32_t)q[5] << 16), q[6] | ((uint32_t)q[7] << 16));
+            }
+        }
+    }
     const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, a.err,
                                 blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0);
-    const bool live = i < rw.n;
-    float x[8];
-    if (live) {
-        const bf16* src = a.x[which] + (b * a.xs[which].b + i * a.xs[which].s + h * a.xs[which].h) + e * 8;
-        if (VEC) {
-            const uint4 u = *reinterpret_cast<const uint4*>(src);
-            const uint32_t X[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[2 * j] = bits_lo_f(X[j]);
-                x[2 * j + 1] = bits_hi_f(X[j]);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = bf2f(src[j]);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = 0.f;
-    }
-    float hi = x[0], lo = x[0];
-#pragma unroll
-    for (int j = 1; j < 8; ++j) {
-        hi = max_nan(hi, x[j]);
-        lo = fminf(lo, x[j]);
-    }
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    }
-    if (!live) return;
-    const bool bad = !(hi <= 3.4e38f) || !(lo >= -3.4e38f);
-    float scale = 0.f;
-    uint32_t word = 0;
-    if (!bad) {
-        scale = group_scale(hi, lo);
-        if (scale != 0.f) {
-            const float inv = __fdiv_rn(1.0f, scale);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) word |= quantize(x[j], lo, scale, inv) << (4 * j);
-        }
-    }
     const Kv4Part& p = a.c.p[which];
-    const size_t row = ((size_t)b * a.c.heads + h) * a.c.max_pos + (size_t)(rw.off + i);
-    p.w[row * T + e] = word;
-    if (e % 8 == 0) {
-        uint16_t* s = reinterpret_cast<uint16_t*>(p.s) + row * (D / 64) + e / 8;
-        uint16_t* z = reinterpret_cast<uint16_t*>(p.b) + row * (D / 64) + e / 8;
-        *s = bad ? (uint16_t)0x7FC0 : f_to_bf16bits(scale);
-        *z = bad ? (uint16_t)0x7FC0 : f_to_bf16bits(lo);
+    const size_t row0 = ((size_t)b * a.c.heads + h) * a.c.max_pos + (size_t)rw.off;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const uint32_t X[4] = {u[r].x, u[r].y, u[r].z, u[r].w};
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[2 * j] = bits_lo_f(X[j]);
+            x[2 * j + 1] = bits_hi_f(X[j]);
+        }
+        float hi = x[0], lo = x[0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) {
+            hi = max_nan(hi, x[j]);
+            lo = fminf(lo, x[j]);
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+            hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        }
+        const int i = i0 + r * RB;
+        if (i >= rw.n) continue;
+        const bool bad = !(hi <= 3.4e38f) || !(lo >= -3.4e38f);
+        float scale = 0.f;
+        uint32_t word = 0;
+        if (!bad) {
+            scale = group_scale(hi, lo);
+            if (scale != 0.f) {
+                const float inv = __fdiv_rn(1.0f, scale);
+                // q + 2^23 is 0x4B000000 + q; the constant part of the sum comes off at the end
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    word += __float_as_uint(__fadd_rn(quantize(x[j], lo, scale, inv), 8388608.f)) << (4 * j);
+                word -= 0x4B000000u * 0x11111111u;
+            }
+        }
+        const size_t row = row0 + i;
+        p.w[row * T + e] = word;
+        if (e % 8 == 0) {
+            reinterpret_cast<uint16_t*>(p.s)[row * (D / 64) + e / 8] = bad ? (uint16_t)0x7FC0 : f_to_bf16bits(scale);
+            reinterpret_cast<uint16_t*>(p.b)[row * (D / 64) + e / 8] = bad ? (uint16_t)0x7FC0 : f_to_bf16bits(lo);
+        }
     }
 }
 
-template <int D>
+// The same split for reading back.
+template <int D, int R>
 __global__ void __launch_bounds__(NT) kv4_read_kernel(const Kv4ReadArgs a) {
-    constexpr int T = TPR<D>;
+    constexpr int T = TPR<D>, RB = NT / T;
     const int which = blockIdx.y / a.c.heads, h = blockIdx.y % a.c.heads, b = blockIdx.z;
-    const int i = blockIdx.x * (NT / T) + threadIdx.x / T, e = threadIdx.x % T;
+    const int i0 = blockIdx.x * (R * RB) + threadIdx.x / T, e = threadIdx.x % T;
     const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, a.err,
                                 blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0);
-    if (i >= a.S || a.y[which] == nullptr) return;
-    uint32_t o[4] = {0u, 0u, 0u, 0u};
-    if (i < rw.n) {
-        const Kv4Part& p = a.c.p[which];
-        const size_t row = ((size_t)b * a.c.heads + h) * a.c.max_pos + (size_t)(rw.off + i);
-        const uint32_t w = p.w[row * T + e];
-        const float s = bf2f(p.s[row * (D / 64) + e / 8]), z = bf2f(p.b[row * (D / 64) + e / 8]);
+    if (a.y[which] == nullptr) return;
+    const Kv4Part& p = a.c.p[which];
+    const size_t row0 = ((size_t)b * a.c.heads + h) * a.c.max_pos + (size_t)rw.off;
+    uint32_t w[R];
+    float s[R], z[R];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            o[j] = pack_bf16x2(fmaf(s, (float)((w >> (8 * j)) & 15u), z), fmaf(s, (float)((w >> (8 * j + 4)) & 15u), z));
+    for (int r = 0; r < R; ++r) {
+        const int i = i0 + r * RB;
+        w[r] = 0u;
+        s[r] = z[r] = 0.f;
+        if (i < rw.n) {
+            const size_t row = row0 + i;
+            w[r] = p.w[row * T + e];
+            s[r] = bf2f(p.s[row * (D / 64) + e / 8]);
+            z[r] = bf2f(p.b[row * (D / 64) + e / 8]);
+        }
     }
-    bf16* dst = a.y[which] + (((size_t)b * a.S + i) * a.c.heads + h) * D + e * 8;
-    *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+    bf16* dst = a.y[which] + ((size_t)b * a.S * a.c.heads + h) * D + e * 8;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i = i0 + r * RB;
+        if (i >= a.S) continue;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)  // 2^23 + q, less 2^23
+            v[j] = fmaf(s[r], __fsub_rn(__uint_as_float(0x4B000000u | ((w[r] >> (4 * j)) & 15u)), 8388608.f), z[r]);
+        __stcs(reinterpret_cast<uint4*>(dst + (size_t)i * a.c.heads * D),
+               make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])));
+    }
+}
+
+// Rows of a thread: four once one each would make more than two rounds of
+// blocks on the GPU (8 of these blocks fit an SM).
+int rows_per_thread(const Kv4View& c, int S) {
+    const int rb = NT / (c.D / 8);
+    return (long long)((S + rb - 1) / rb) * 2 * c.heads * c.batch > 2 * 8 * 148 ? 4 : 1;
+}
+
+template <int D, int R>
+cudaError_t append_t(const Kv4StoreArgs& a, bool vec, cudaStream_t st) {
+    const int rows = R * NT / TPR<D>;
+    const dim3 grid((a.S + rows - 1) / rows, 2 * a.c.heads, a.c.batch);
+    vec ? kv4_append_kernel<D, true, R><<<grid, NT, 0, st>>>(a) : kv4_append_kernel<D, false, R><<<grid, NT, 0, st>>>(a);
+    return cudaGetLastError();
+}
+template <int D, int R>
+cudaError_t read_t(const Kv4ReadArgs& a, cudaStream_t st) {
+    const int rows = R * NT / TPR<D>;
+    const dim3 grid((a.S + rows - 1) / rows, 2 * a.c.heads, a.c.batch);
+    kv4_read_kernel<D, R><<<grid, NT, 0, st>>>(a);
+    return cudaGetLastError();
 }
 
 }  // namespace
@@ -134,23 +187,15 @@ cudaError_t launch_kv4_append(const Kv4StoreArgs& a, cudaStream_t st) {
     bool vec = true;
     for (int w = 0; w < 2; ++w)
         vec = vec && (uintptr_t)a.x[w] % 16 == 0 && a.xs[w].b % 8 == 0 && a.xs[w].s % 8 == 0 && a.xs[w].h % 8 == 0;
-    const int rows = NT / (a.c.D / 8);
-    const dim3 grid((a.S + rows - 1) / rows, 2 * a.c.heads, a.c.batch);
-    if (a.c.D == 128)
-        vec ? kv4_append_kernel<128, true><<<grid, NT, 0, st>>>(a) : kv4_append_kernel<128, false><<<grid, NT, 0, st>>>(a);
-    else
-        vec ? kv4_append_kernel<64, true><<<grid, NT, 0, st>>>(a) : kv4_append_kernel<64, false><<<grid, NT, 0, st>>>(a);
-    return cudaGetLastError();
+    const bool four = rows_per_thread(a.c, a.S) == 4;
+    if (a.c.D == 128) return four ? append_t<128, 4>(a, vec, st) : append_t<128, 1>(a, vec, st);
+    return four ? append_t<64, 4>(a, vec, st) : append_t<64, 1>(a, vec, st);
 }
 
 cudaError_t launch_kv4_read(const Kv4ReadArgs& a, cudaStream_t st) {
-    const int rows = NT / (a.c.D / 8);
-    const dim3 grid((a.S + rows - 1) / rows, 2 * a.c.heads, a.c.batch);
-    if (a.c.D == 128)
-        kv4_read_kernel<128><<<grid, NT, 0, st>>>(a);
-    else
-        kv4_read_kernel<64><<<grid, NT, 0, st>>>(a);
-    return cudaGetLastError();
+    const bool four = rows_per_thread(a.c, a.S) == 4;
+    if (a.c.D == 128) return four ? read_t<128, 4>(a, st) : read_t<128, 1>(a, st);
+    return four ? read_t<64, 4>(a, st) : read_t<64, 1>(a, st);
 }
 
 }  // namespace qw
