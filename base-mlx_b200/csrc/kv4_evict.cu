@@ -39,49 +39,49 @@ QW_DEV void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
-// The int at `p` of the cluster's block `rank`.
-QW_DEV int cluster_load(const int* p, int rank) {
+// The pair of ints at `p` in the cluster's block `rank`.
+QW_DEV uint32_t cluster_addr(const int* p, int rank) {
     uint32_t addr;
-    int v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(rank));
+    return addr;
+}
+QW_DEV int2 cluster_load2(const int* p, int rank) {
+    int2 v;
+    asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(cluster_addr(p, rank)) : "memory");
     return v;
 }
 
-// Exclusive prefix of `v` over the block (SEL_NT threads) and the block total.
-QW_DEV int block_scan(int v, int* red, int& total) {
+// Exclusive prefixes of v and w over the block (SEL_NT threads) and the block totals.
+QW_DEV void block_scan2(int& v, int& w, int2* red, int2& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int s = v;
+    int s = v, r = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int t = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += t;
-    }
-    __syncthreads();
-    if (lane == 31) red[warp] = s;
-    __syncthreads();
-    if (warp == 0) {
-        int t = red[lane];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, t, o);
-            if (lane >= o) t += u;
+        const int t = __shfl_up_sync(0xffffffffu, s, o), u = __shfl_up_sync(0xffffffffu, r, o);
+        if (lane >= o) {
+            s += t;
+            r += u;
         }
-        red[lane] = t;
     }
+    if (lane == 31) red[warp] = make_int2(s, r);
     __syncthreads();
-    total = red[31];
-    return s - v + (warp ? red[warp - 1] : 0);
+    const int2 p = red[lane];  // every warp: the warps before it, and all
+    total = make_int2(__reduce_add_sync(0xffffffffu, p.x), __reduce_add_sync(0xffffffffu, p.y));
+    v = s - v + __reduce_add_sync(0xffffffffu, lane < warp ? p.x : 0);
+    w = r - w + __reduce_add_sync(0xffffffffu, lane < warp ? p.y : 0);
 }
 
 // index[b][h][0..new length): the kept positions in increasing order.
-__global__ void __launch_bounds__(SEL_NT) kv4_select_kernel(const Kv4EvictArgs a, int cluster, int slice_keys, int* index,
+// (two blocks per SM: at most 32 registers a thread)
+__global__ void __launch_bounds__(SEL_NT, 2) kv4_select_kernel(const Kv4EvictArgs a, int cluster, int slice_keys, int* index,
                                                             int* count) {
     extern __shared__ __align__(16) int sel_smem[];
     int* hist = sel_smem;                                                // [3][BINS]
     uint32_t* sk = reinterpret_cast<uint32_t*>(sel_smem + 3 * BINS);     // [slice_keys]
-    __shared__ int red[32], pick[2], tally[2];
-    const int rank = blockIdx.x % cluster, h = blockIdx.x / cluster, b = blockIdx.y, tid = threadIdx.x;
+    __shared__ int2 red[32], tally;
+    __shared__ int wsum[3][32], pick[3][2];
+    const int rank = blockIdx.x % cluster, h = blockIdx.x / cluster, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31,
+              warp = tid >> 5;
     pdl_launch_dependents();
     const int n = clamp_len(a, b);
     const size_t bh = (size_t)b * a.src.heads + h;
@@ -128,28 +128,44 @@ __global__ void __launch_bounds__(SEL_NT) kv4_select_kernel(const Kv4EvictArgs a
                 cluster_sync();
             else
                 __syncthreads();
-            // thread t counts the bins 2 (1023 - t) + {1, 0}: prefixes run from the largest digit down
-            const int d1 = 2 * (SEL_NT - 1 - tid) + 1;
+            // warp w counts the 64 bins from 64 (31 - w) on, lane l the pair 2 (31 - l) of them:
+            // both in order from the largest digit down
+            const int d0 = 64 * (31 - warp) + 2 * (31 - lane);
             int c1 = 0, c0 = 0;
             if (cluster > 1) {
-                for (int r = 0; r < cluster; ++r) {
-                    c1 += cluster_load(&hp[d1], r);
-                    c0 += cluster_load(&hp[d1 - 1], r);
+                int2 c[SEL_MAX_CLUSTER];
+#pragma unroll
+                for (int r = 0; r < SEL_MAX_CLUSTER; ++r) c[r] = r < cluster ? cluster_load2(&hp[d0], r) : make_int2(0, 0);
+#pragma unroll
+                for (int r = 0; r < SEL_MAX_CLUSTER; ++r) {
+                    c0 += c[r].x;
+                    c1 += c[r].y;
                 }
             } else {
-                c1 = hp[d1];
-                c0 = hp[d1 - 1];
+                c0 = hp[d0];
+                c1 = hp[d0 + 1];
             }
-            int total;
-            const int above = block_scan(c1 + c0, red, total);
-            if (above < left && left <= above + c1 + c0) {
-                const bool hi = left <= above + c1;
-                pick[0] = hi ? d1 : d1 - 1;
-                pick[1] = left - above - (hi ? 0 : c1);
+            const int mine = __reduce_add_sync(0xffffffffu, c0 + c1);
+            if (lane == 0) wsum[pass][warp] = mine;
+            __syncthreads();
+            const int before = __reduce_add_sync(0xffffffffu, lane < warp ? wsum[pass][lane] : 0);
+            if (before < left && left <= before + mine) {  // this warp's bins hold the threshold
+                int s = c0 + c1;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, s, o);
+                    if (lane >= o) s += v;
+                }
+                const int above = before + s - c0 - c1;
+                if (above < left && left <= above + c0 + c1) {
+                    const bool hi = left <= above + c1;
+                    pick[pass][0] = hi ? d0 + 1 : d0;
+                    pick[pass][1] = left - above - (hi ? 0 : c1);
+                }
             }
             __syncthreads();
-            prefix |= (uint32_t)pick[0] << shift;
-            left = pick[1];
+            prefix |= (uint32_t)pick[pass][0] << shift;
+            left = pick[pass][1];
         }
     }
     // consecutive positions per thread, in order
@@ -164,17 +180,19 @@ __global__ void __launch_bounds__(SEL_NT) kv4_select_kernel(const Kv4EvictArgs a
             equal += k == prefix;
         }
     }
-    int tot_above, tot_equal;
-    int a_before = block_scan(above, red, tot_above), e_before = block_scan(equal, red, tot_equal);
+    int a_before = above, e_before = equal;
+    int2 total;
+    block_scan2(a_before, e_before, red, total);
     if (cluster > 1) {
-        if (tid == 0) {
-            tally[0] = tot_above;
-            tally[1] = tot_equal;
-        }
+        if (tid == 0) tally = total;
         cluster_sync();
-        for (int r = 0; r < rank; ++r) {
-            a_before += cluster_load(&tally[0], r);
-            e_before += cluster_load(&tally[1], r);
+        int2 c[SEL_MAX_CLUSTER];
+#pragma unroll
+        for (int r = 0; r < SEL_MAX_CLUSTER; ++r) c[r] = r < rank ? cluster_load2(&tally.x, r) : make_int2(0, 0);
+#pragma unroll
+        for (int r = 0; r < SEL_MAX_CLUSTER; ++r) {
+            a_before += c[r].x;
+            e_before += c[r].y;
         }
         cluster_sync();  // a block's tally is read until here
     }

@@ -6,9 +6,9 @@
 // A group that holds a NaN or an infinity gets scale = bias = NaN, so all of
 // it reads back as NaN.
 //
-// Every q is the rounding of the exact quotient: the fp32 quotient (error below
-// 3e-6 for values up to 16) decides unless it lies within 1e-5 of a half, and
-// the few that do are redone in fp64.
+// Every q is the rounding of the exact quotient, ties to even.  Ties are common
+// (about one element in 500: x, bias and scale are 8-bit numbers), so they are
+// settled without a branch, from the exact remainder.
 #include "kv4.h"
 
 namespace qw {
@@ -28,21 +28,48 @@ QW_DEV float max_nan(float a, float b) {
 // bf16((hi - lo) / 15) of the exact difference, rounded through fp32
 QW_DEV float group_scale(float hi, float lo) {
     const float d = __fsub_rn(hi, lo);
-    float s = __fdiv_rn(d, 15.0f);
-    // next to a midpoint of two bf16 values (or past the fp32 range) the fp32 steps may decide wrongly
+    float s = __fmul_rn(d, 1.0f / 15.0f);
+    // next to a midpoint of two bf16 values, past the fp32 range or below bf16's normal numbers the
+    // fp32 steps (off by less than 3 units) may decide wrongly
     const uint32_t low = __float_as_uint(s) & 0xFFFFu;
-    if (!(d <= 3.0e38f) || (low >= 0x7FF8u && low <= 0x8008u))
+    if (!(d <= 3.0e38f) || (low >= 0x7FF8u && low <= 0x8008u) || s < 1.2e-38f)
         s = __double2float_rn(((double)hi - (double)lo) / 15.0);
     return bfr(s);
 }
 
-// clamp(round_half_even((x - bias) / scale), 0, 15)
-QW_DEV float quantize(float x, float bias, float scale, float inv) {
-    const float t = __fmul_rn(__fsub_rn(x, bias), inv);
-    float r = __fsub_rn(__fadd_rn(t, 12582912.f), 12582912.f);  // 1.5 2^23: rounds to an integer
-    if (!(fabsf(t - r) < 0.49999f))  // also taken for an overflowed quotient
-        r = (float)rint(((double)x - (double)bias) / (double)scale);
-    return fminf(fmaxf(r, 0.f), 15.f);
+// Word of the eight values' clamp(round_half_even((x - bias) / scale), 0, 15).
+// quantize8_any decides every element in fp64; quantize8 gives the same word
+// in fp32 where every x - bias is exact in it.
+__device__ __noinline__ uint32_t quantize8_any(uint4 u, float bias, float scale) {
+    const uint32_t X[4] = {u.x, u.y, u.z, u.w};
+    uint32_t word = 0;
+    for (int j = 0; j < 8; ++j) {
+        const float x = j & 1 ? bits_hi_f(X[j >> 1]) : bits_lo_f(X[j >> 1]);
+        const double r = rint(((double)x - (double)bias) / (double)scale);
+        word |= (uint32_t)fmin(fmax(r, 0.0), 15.0) << (4 * j);
+    }
+    return word;
+}
+QW_DEV uint32_t quantize8(const float (&x)[8], float bias, float scale) {
+    // 1.5 2^23 + t rounds t (within 4e-6 of the quotient) to an integer r, the nearest or, next to a
+    // half, its neighbour; r is in the low bits of 0x4B400000 + r.  The remainder (x - bias) - r scale
+    // is exact, so comparing it with scale / 2 (as bit patterns; a tie counts against an odd r) tells
+    // whether r has to move towards it.  A scale that is a normal bf16 is within 2^-9 of
+    // (max - min) / 15: 0 <= t < 15.1, and r needs no clamp.
+    constexpr float MAGIC = 12582912.f;
+    float inv;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(scale));
+    const int half = __float_as_int(0.5f * scale);
+    uint32_t word = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float d = __fsub_rn(x[j], bias), m = __fadd_rn(__fmul_rn(d, inv), MAGIC);
+        const int rem = __float_as_int(fmaf(-__fsub_rn(m, MAGIC), scale, d));
+        int r = __float_as_int(m);
+        if ((rem & 0x7FFFFFFF) + (r & 1) > half) r += (rem >> 31) | 1;
+        word += (uint32_t)r << (4 * j);
+    }
+    return word - 0x4B400000u * 0x11111111u;
 }
 
 // Block = one (sequence, K or V, head) and R * NT / TPR consecutive new rows,
@@ -103,12 +130,13 @@ __global__ void __launch_bounds__(NT) kv4_append_kernel(const Kv4StoreArgs a) {
         if (!bad) {
             scale = group_scale(hi, lo);
             if (scale != 0.f) {
-                const float inv = __fdiv_rn(1.0f, scale);
-                // q + 2^23 is 0x4B000000 + q; the constant part of the sum comes off at the end
+                // x - lo is exact in fp32 when no magnitude lies 2^16 below the width (or is 0: also exact,
+                // but not worth telling apart); the rest, and subnormal scales, go the long way
+                float least = lo == 0.f ? INFINITY : fabsf(lo);
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    word += __float_as_uint(__fadd_rn(quantize(x[j], lo, scale, inv), 8388608.f)) << (4 * j);
-                word -= 0x4B000000u * 0x11111111u;
+                for (int j = 0; j < 8; ++j) least = fminf(least, fabsf(x[j]));
+                const bool exact = least * 65536.f >= hi - lo && scale >= 1.2e-38f;
+                word = exact ? quantize8(x, lo, scale) : quantize8_any(u[r], lo, scale);
             }
         }
         const size_t row = row0 + i;
