@@ -15,6 +15,7 @@
 // one long sequence both fill the GPU.  A segment inside one share is finished
 // there; one that spans shares leaves a partial (base exponent, sum, output) per
 // share, which a second kernel joins.
+#include "kv4_tc.h"
 #include "kv4_tile.cuh"
 #include "smem_attr.h"
 
@@ -28,7 +29,7 @@ constexpr int ASTAGES = 3;            // tiles of a warp's load ring
 
 // Scratch: [0] tiles per share, [1 + b] first tile of sequence b; then the
 // partials [2 shares][columns][D] and their (base exponent, sum); then the lse of a
-// call that accumulates weights but returns none.
+// call that accumulates weights but returns none.  (The tcgen05 form has no plan.)
 struct Scratch {
     int* plan;
     float* part;
@@ -36,7 +37,7 @@ struct Scratch {
     float* lse;
     size_t bytes;
 };
-Scratch scratch_of(void* base, const Kv4View& c, int S, int Hq, int shares, int cb) {
+Scratch scratch_of(void* base, const Kv4View& c, int S, int Hq, size_t part_rows) {
     Scratch s;
     unsigned char* p = static_cast<unsigned char*>(base);
     auto take = [&](size_t n) {
@@ -45,8 +46,8 @@ Scratch scratch_of(void* base, const Kv4View& c, int S, int Hq, int shares, int 
         return r;
     };
     s.plan = reinterpret_cast<int*>(take((size_t)(c.batch + 1) * 4));
-    s.part = reinterpret_cast<float*>(take((size_t)2 * shares * cb * c.D * 4));
-    s.ml = reinterpret_cast<float2*>(take((size_t)2 * shares * cb * 8));
+    s.part = reinterpret_cast<float*>(take(part_rows * c.D * 4));
+    s.ml = reinterpret_cast<float2*>(take(part_rows * 8));
     s.lse = reinterpret_cast<float*>(take((size_t)c.batch * S * Hq * 4));
     s.bytes = (size_t)(p - static_cast<unsigned char*>(base));
     return s;
@@ -502,16 +503,29 @@ cudaError_t launch(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t st
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// Form of a call: from TC_COLUMNS columns per kv head the tcgen05 kernel, below it the split kernel
+// with column blocks of 8 (two blocks of threads per SM) or 16.
+constexpr int TC_COLUMNS = 64;
 struct Shape {
+    bool tc;
+    TcShape t;
     int nt, cb, ncb, shares;
+    size_t part_rows;
 };
 Shape shape_of(const Kv4View& c, int S, int Hq, int num_sms) {
     const long long C = (long long)(Hq / c.heads) * S;
-    Shape s;
+    Shape s = {};
+    s.tc = C >= TC_COLUMNS;
+    if (s.tc) {
+        s.t = kv4_tc_shape(c, S, Hq, num_sms);
+        s.part_rows = s.t.part_rows;
+        return s;
+    }
     s.nt = C <= 8 ? 1 : 2;
     s.cb = 8 * s.nt;
     s.ncb = (int)((C + s.cb - 1) / s.cb);
     s.shares = s.nt == 1 ? 2 * num_sms : num_sms;
+    s.part_rows = (size_t)2 * s.shares * s.cb;
     return s;
 }
 
@@ -528,7 +542,9 @@ cudaError_t launch_split(const Kv4AttnArgs& a, const Shape& sp, const Scratch& s
 
 template <int D>
 cudaError_t launch_d(const Kv4AttnArgs& a, const Shape& sp, const Scratch& sc, cudaStream_t st) {
-    const cudaError_t e = sp.nt == 1 ? launch_split<D, 1>(a, sp, sc, st) : launch_split<D, 2>(a, sp, sc, st);
+    const cudaError_t e = sp.tc      ? launch_kv4_attn_tc(a, sp.t, sc.part, sc.ml, st)
+                          : sp.nt == 1 ? launch_split<D, 1>(a, sp, sc, st)
+                                       : launch_split<D, 2>(a, sp, sc, st);
     if (e != cudaSuccess || !a.mass) return e;
     const dim3 grid((a.c.max_pos + AW * TK - 1) / (AW * TK), a.c.heads, a.c.batch);
     return launch(kv4_mass_kernel<D>, grid, dim3(ANT), 0, st, true, a);
@@ -538,15 +554,15 @@ cudaError_t launch_d(const Kv4AttnArgs& a, const Shape& sp, const Scratch& sc, c
 
 size_t kv4_attn_scratch_bytes(const Kv4View& c, int S, int Hq, int num_sms) {
     const Shape sp = shape_of(c, S, Hq, num_sms);
-    return scratch_of(nullptr, c, S, Hq, sp.shares, sp.cb).bytes;
+    return scratch_of(nullptr, c, S, Hq, sp.part_rows).bytes;
 }
 
 cudaError_t launch_kv4_attention(const Kv4AttnArgs& in, void* scratch, int num_sms, cudaStream_t st) {
     Kv4AttnArgs a = in;
     const Shape sp = shape_of(a.c, a.S, a.Hq, num_sms);
     // tiles are counted in 32 bits (180 GB of cache are less than 2^26 tiles of one column block)
-    if ((long long)a.c.batch * a.c.heads * sp.ncb * ((a.c.max_pos + TK - 1) / TK) > 0x7FFFFFFF) return cudaErrorInvalidValue;
-    const Scratch sc = scratch_of(scratch, a.c, a.S, a.Hq, sp.shares, sp.cb);
+    if (!sp.tc && (long long)a.c.batch * a.c.heads * sp.ncb * ((a.c.max_pos + TK - 1) / TK) > 0x7FFFFFFF) return cudaErrorInvalidValue;
+    const Scratch sc = scratch_of(scratch, a.c, a.S, a.Hq, sp.part_rows);
     if (a.mass && !a.lse) a.lse = sc.lse;
     return a.c.D == 128 ? launch_d<128>(a, sp, sc, st) : launch_d<64>(a, sp, sc, st);
 }
