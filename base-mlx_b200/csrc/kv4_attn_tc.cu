@@ -1,8 +1,8 @@
 // Attention over the 4-bit KV cache for many rows per kv head (prompt chunks),
 // on the tcgen05 tensor cores.
 //
-// A thread block takes 128 columns (row, query head) of one (sequence, kv head)
-// and walks the keys they see in tiles of 64:
+// A thread block takes NB = 1 or 2 blocks of 128 columns (row, query head) of one
+// (sequence, kv head) and walks the keys they see in tiles of 64:
 //   S_g = Q_g N_g^T   per 64-element group g: Q (fp16, scaled per column as in
 //                     kv4_tile.cuh) against the packed integers, which enter as
 //                     fp16 subnormals (n 2^-24, the odd nibbles 16 n 2^-24
@@ -15,11 +15,11 @@
 // maximum moves only when a score passes it by 2^4 (P <= 2^15), and then O is
 // rescaled in TMEM.
 //
-// Roles (288 threads, two blocks per SM: one block's softmax overlaps the
-// other's products): warps 0-3 one column per thread; warps 4-7 copy packed
-// rows (cp.async ring) and expand them; one lane of warp 8 issues the products.
-// Every wait is bounded: a lost arrival sets QW_DERR_TIMEOUT and the block
-// still frees its TMEM and ends.
+// Roles: warps 0 .. 4 NB - 1 one column per thread (with NB = 2 one column
+// block's softmax overlaps the other's products); four warps copy packed rows
+// (cp.async ring) and expand them, once for all column blocks; one lane of the
+// last warp issues the products.  Every wait is bounded: a lost arrival sets
+// QW_DERR_TIMEOUT and the block still frees its TMEM and ends.
 #include "kv4_tc.h"
 #include "kv4_tile.cuh"
 #include "smem_attr.h"
@@ -29,28 +29,30 @@ namespace {
 
 using namespace kv4;
 
-constexpr int CM = 128;      // columns of a block
+constexpr int CM = 128;      // columns of a column block
 constexpr int KT = 64;       // keys of a tile
-constexpr int NT_TC = 288;
 constexpr int STAGES = 3;    // packed tiles in flight
+constexpr int TABS = 4;      // score tables: a tile's is read until the products of the next tile but one are issued
+template <int NB>
+constexpr int THREADS = 128 * NB + 160;
 constexpr float BASE = 11.f;          // P = 2^(x - max + 11)
 constexpr float RAISE = BASE + 4.f;   // a larger exponent raises the maximum
 constexpr float UNSET = -3.0e38f;
 constexpr unsigned long long TIMEOUT_NS = 2000000000ull;
 
 // Shared memory, from a 1 KB aligned base.
-template <int D>
+template <int D, int NB>
 struct Plan {
-    static constexpr int GR = D / 64;
-    static constexpr int Q = 1024;                    // [GR][128 rows][128 B], swizzled
-    static constexpr int K = Q + GR * CM * 128;       // [GR][64 keys][128 B], swizzled
-    static constexpr int V = K + GR * KT * 128;       // the same, read along the keys
-    static constexpr int TAB = V + GR * KT * 128;     // [2][K scale, K bias][GR][64] fp32
-    static constexpr int PACK = TAB + 2 * 2 * GR * KT * 4;
+    static constexpr int GR = D / 64, OPB = GR * KT * 128;
+    static constexpr int Q = 1024;                    // [NB][GR][128 rows][128 B], swizzled
+    static constexpr int K = Q + NB * GR * CM * 128;  // [2][GR][64 keys][128 B], swizzled
+    static constexpr int V = K + 2 * OPB;             // the same, read along the keys
+    static constexpr int TAB = V + 2 * OPB;           // [TABS][K scale, K bias][GR][64] fp32
+    static constexpr int PACK = TAB + TABS * 2 * GR * KT * 4;
     static constexpr int PW = KT * D / 2, PS = KT * GR * 2, PACKB = 2 * PW + 4 * PS;
     static constexpr int BYTES = PACK + STAGES * PACKB + 1024;
-    static constexpr uint32_t TMEM = D == 128 ? 256 : 128;
-    static constexpr uint32_t TO = GR * KT;           // TMEM columns: S_0, (S_1), O; P over S_0
+    // TMEM columns of a column block: S_0, (S_1), O; P over S_0
+    static constexpr uint32_t TO = GR * KT, TB = GR * KT + D, TMEM = NB * TB;
 };
 
 QW_DEV unsigned long long now_ns() {
@@ -125,18 +127,43 @@ QW_DEV uint32_t as_u(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h);
 // 16-byte chunk c of a swizzled operand row.  A word fills one chunk, its elements in the order 0, 4, 1, 5, 2, 6, 3, 7.
 QW_DEV uint32_t chunk_at(int row, int c) { return (uint32_t)row * 128 + (uint32_t)((c ^ (row & 7)) << 4); }
 
-template <int D>
-__global__ void __launch_bounds__(NT_TC, 2) kv4_attn_tc_kernel(const Kv4AttnArgs a, int ncb, int nsplit, float* part, float2* pml) {
-    using P = Plan<D>;
-    constexpr int GR = P::GR;
+QW_DEV unsigned long long pack2(float lo, float hi) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+QW_DEV void unpack2(unsigned long long v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+QW_DEV unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+QW_DEV unsigned long long mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+QW_DEV unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+template <int D, int NB>
+__global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4AttnArgs a, int ncb, int nsplit, float* part, float2* pml) {
+    using P = Plan<D, NB>;
+    constexpr int GR = P::GR, CB = CM * NB, PW0 = 4 * NB;  // columns of the block, first producer warp
     extern __shared__ unsigned char tc_raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>(((uintptr_t)tc_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t* k_full = reinterpret_cast<uint64_t*>(sm);  // [2] K operand and table of tile i (i & 1)
-    uint64_t* v_full = k_full + 2;
-    uint64_t* s_full = v_full + 1;                        // products Q N done
-    uint64_t* p_full = s_full + 1;
-    uint64_t* pv_done = p_full + 1;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 1);
+    // barriers: tile i uses [i & 1] of the paired ones; those per column block count tiles
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(sm);  // K operand and table written
+    uint64_t* k_free = k_full + 2;                        // products Q N of every column block done
+    uint64_t* v_full = k_free + 2;
+    uint64_t* v_free = v_full + 2;
+    uint64_t* s_full = v_free + 2;                        // per column block: scores in TMEM
+    uint64_t* p_full = s_full + 2;
+    uint64_t* pv_done = p_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2);
     float* vmax = reinterpret_cast<float*>(tmem_slot + 2);  // [4] producers' warps
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -148,33 +175,36 @@ __global__ void __launch_bounds__(NT_TC, 2) kv4_attn_tc_kernel(const Kv4AttnArgs
     const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, a.err, tid == 0 && cb == 0 && sp == 0 && h == 0);
     const int T = rw.off + rw.n;
     // rows of the block's columns, keys they see, this split's tiles
-    const int i_first = cb * CM / G, i_last = min(rw.n, (min(C, (cb + 1) * CM) - 1) / G + 1) - 1;
+    const int i_first = cb * CB / G, i_last = min(rw.n, (min(C, (cb + 1) * CB) - 1) / G + 1) - 1;
     const int keys = i_last < i_first ? 0 : a.causal ? min(T, rw.off + i_last + 1) : T;
     const int nt = (keys + KT - 1) / KT, t0 = (int)((long long)nt * sp / nsplit), t1 = (int)((long long)nt * (sp + 1) / nsplit);
     const int all = a.causal ? min(T, rw.off + i_first + 1) : T;  // keys that every column sees
     const size_t seg = ((size_t)b * a.c.heads + h) * ncb + cb;
 
-    const int col = tid & 127, c = cb * CM + col, i_row = c / G, head = h * G + c % G;
+    const int col = min(tid, CB - 1), c = cb * CB + col, i_row = c / G, head = h * G + c % G;
     const bool row = c < C && i_row < rw.n;
     bf16* out = a.out + (b * a.os.b + (long long)i_row * a.os.s + (long long)head * a.os.h);
     const size_t lse_at = ((size_t)b * a.S + i_row) * a.Hq + head;
     if (t0 == t1) {  // nothing to see: zeros (a split's empty share is skipped by the joining kernel)
-        if (nsplit == 1 && tid < 128 && c < C) {
+        if (nsplit == 1 && tid < CB && c < C) {
             for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(out + d) = make_uint4(0u, 0u, 0u, 0u);
             if (a.lse) a.lse[lse_at] = -INFINITY;
         }
         return;
     }
     if (tid == 0) {
-        mbar_init(k_full, 128);
-        mbar_init(k_full + 1, 128);
-        mbar_init(v_full, 128);
-        mbar_init(s_full, 1);
-        mbar_init(p_full, 128);
-        mbar_init(pv_done, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(k_full + i, 128);
+            mbar_init(k_free + i, 1);
+            mbar_init(v_full + i, 128);
+            mbar_init(v_free + i, 1);
+            mbar_init(s_full + i, 2);
+            mbar_init(p_full + i, 128);
+            mbar_init(pv_done + i, 1);
+        }
         fence_mbar_init();
     }
-    if (warp == 8) {
+    if (warp == PW0 + 4) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(P::TMEM)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -182,7 +212,7 @@ __global__ void __launch_bounds__(NT_TC, 2) kv4_attn_tc_kernel(const Kv4AttnArgs
 
     const Rows rows = head_rows<D>(a.c, (size_t)b * a.c.heads + h);
     const int key_end = min(T, t1 * KT);  // this block's keys end here
-    const int pt = tid - 128;             // producer thread
+    const int pt = tid - CB;              // producer thread
     auto fetch = [&](int i) {  // tile t0 + i into stage i % STAGES, 16-byte pieces; zeros past the last key
         if (t0 + i < t1) {
             const int key0 = (t0 + i) * KT;
@@ -207,7 +237,7 @@ __global__ void __launch_bounds__(NT_TC, 2) kv4_attn_tc_kernel(const Kv4AttnArgs
     };
 
     float cc = 0.f, q0 = 0.f, q1 = 0.f;  // the column's score constants (softmax threads)
-    if (warp < 4) {
+    if (warp < PW0) {
         // Q operand: column `col`, elements of a chunk in the order of an expanded word
         const bf16* src = a.q + (b * a.qs.b + (long long)i_row * a.qs.s + (long long)head * a.qs.h);
         float mx = 0.f, sum[GR];
@@ -245,11 +275,11 @@ __global__ void __launch_bounds__(NT_TC, 2) kv4_attn_tc_kernel(const Kv4AttnArgs
                     x[2 * e] = bits_lo_f(X[e]) * up;
                     x[2 * e + 1] = bits_hi_f(X[e]) * up;
                 }
-                *reinterpret_cast<uint4*>(sm + P::Q + g * CM * 128 + chunk_at(col, k)) =
+                *reinterpret_cast<uint4*>(sm + P::Q + ((col >> 7) * GR + g) * CM * 128 + chunk_at(col & 127, k)) =
                     make_uint4(h2(x[0], x[4]), h2(x[1] * 0.0625f, x[5] * 0.0625f), h2(x[2], x[6]), h2(x[3] * 0.0625f, x[7] * 0.0625f));
             }
         fence_proxy_async_smem();
-    } else if (warp < 8) {
+    } else if (warp < PW0 + 4) {
 #pragma unroll
         for (int i = 0; i < STAGES - 1; ++i) fetch(i);
         // largest |value| that the block's V rows can stand for: max(|b|, |b + 15 s|) (a NaN counts as nothing here)
@@ -266,7 +296,7 @@ __global__ void __launch_bounds__(NT_TC, 2) kv4_attn_tc_kernel(const Kv4AttnArgs
             mx = fmaxf(mx, m);
         }
         mx = warp_max(mx);
-        if (lane == 0) vmax[warp - 4] = mx;
+        if (lane == 0) vmax[warp - PW0] = mx;
     }
     fence_before();
     __syncthreads();
@@ -278,17 +308,19 @@ __global__ void __launch_bounds__(NT_TC, 2) kv4_attn_tc_kernel(const Kv4AttnArgs
     const int n_tiles = t1 - t0;
     bool ok = true;
 
-    if (warp < 4) {
+    if (warp < PW0) {
         // ---- softmax: one column per thread ------------------------------------------------------
-        const uint32_t tm = tmem + ((uint32_t)(32 * warp) << 16);
+        const int blk = warp >> 2;
+        const uint32_t tm = tmem + blk * P::TB + ((uint32_t)(32 * (warp & 3)) << 16);
         const int vis = row ? (a.causal ? min(T, rw.off + i_row + 1) : T) : 0;
+        const unsigned long long c2 = pack2(cc, cc), q02 = pack2(q0, q0), q12 = pack2(q1, q1);
         float nm = 0.f, l = 0.f, thr = UNSET;  // BASE - maximum; up to thr the maximum stays
         for (int i = 0; i < n_tiles; ++i) {
             const int key0 = (t0 + i) * KT;
-            if (ok && !wait_ns(k_full + (i & 1), (i >> 1) & 1)) ok = false;
-            if (ok && !wait_ns(s_full, i & 1)) ok = false;
+            if (ok && !wait_ns(s_full + blk, i & 1)) ok = false;
             fence_after();
-            const float* tab = reinterpret_cast<const float*>(sm + P::TAB) + (i & 1) * 2 * GR * KT;
+            const float* tab = reinterpret_cast<const float*>(sm + P::TAB) + (i % TABS) * 2 * GR * KT;
+            const unsigned long long nm2 = pack2(nm, nm);
             float x[KT];
 #pragma unroll
             for (int k = 0; k < KT; k += 16) {
@@ -298,23 +330,20 @@ __global__ void __launch_bounds__(NT_TC, 2) kv4_attn_tc_kernel(const Kv4AttnArgs
                 wait_ld();
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) {
-                    const float4 s0 = *reinterpret_cast<const float4*>(tab + k + e), z0 = *reinterpret_cast<const float4*>(tab + GR * KT + k + e);
-                    const float s0v[4] = {s0.x, s0.y, s0.z, s0.w}, z0v[4] = {z0.x, z0.y, z0.z, z0.w};
-                    float4 s1, z1;
+                    const ulonglong2 s0 = *reinterpret_cast<const ulonglong2*>(tab + k + e),
+                                     z0 = *reinterpret_cast<const ulonglong2*>(tab + GR * KT + k + e);
+                    unsigned long long d[2] = {mul2(s0.x, pack2(a0[e], a0[e + 1])), mul2(s0.y, pack2(a0[e + 2], a0[e + 3]))};
+                    unsigned long long u[2] = {fma2(z0.x, q02, nm2), fma2(z0.y, q02, nm2)};
                     if (GR == 2) {
-                        s1 = *reinterpret_cast<const float4*>(tab + KT + k + e);
-                        z1 = *reinterpret_cast<const float4*>(tab + 3 * KT + k + e);
+                        const ulonglong2 s1 = *reinterpret_cast<const ulonglong2*>(tab + KT + k + e),
+                                         z1 = *reinterpret_cast<const ulonglong2*>(tab + 3 * KT + k + e);
+                        d[0] = fma2(s1.x, pack2(a1[e], a1[e + 1]), d[0]);
+                        d[1] = fma2(s1.y, pack2(a1[e + 2], a1[e + 3]), d[1]);
+                        u[0] = fma2(z1.x, q12, u[0]);
+                        u[1] = fma2(z1.y, q12, u[1]);
                     }
-                    const float s1v[4] = {s1.x, s1.y, s1.z, s1.w}, z1v[4] = {z1.x, z1.y, z1.z, z1.w};
-#pragma unroll
-                    for (int f = 0; f < 4; ++f) {
-                        float d = s0v[f] * a0[e + f], u = fmaf(z0v[f], q0, nm);
-                        if (GR == 2) {
-                            d = fmaf(s1v[f], a1[e + f], d);
-                            u = fmaf(z1v[f], q1, u);
-                        }
-                        x[k + e + f] = fmaf(cc, d, u);
-                    }
+                    unpack2(fma2(c2, d[0], u[0]), x[k + e], x[k + e + 1]);
+                    unpack2(fma2(c2, d[1], u[1]), x[k + e + 2], x[k + e + 3]);
                 }
             }
             if (key0 + KT > all)
@@ -349,31 +378,32 @@ __global__ void __launch_bounds__(NT_TC, 2) kv4_attn_tc_kernel(const Kv4AttnArgs
                     l *= al;
                 }
             }
-            float l0 = 0.f, l1 = 0.f;
+            unsigned long long l2[2] = {0ull, 0ull};
 #pragma unroll
             for (int k = 0; k < KT; k += 32) {
                 uint32_t r[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const float p0 = ex2(x[k + 2 * e]), p1 = ex2(x[k + 2 * e + 1]);
-                    l0 += p0;
-                    l1 += p1;
+                    l2[e & 1] = add2(l2[e & 1], pack2(p0, p1));
                     r[e] = h2(p0, p1);
                 }
                 st16(tm + k / 2, r);
             }
+            float l0, l1;
+            unpack2(add2(l2[0], l2[1]), l0, l1);
             l += l0 + l1;
             wait_st();
             fence_before();
-            arrive(p_full);
+            arrive(p_full + blk);
         }
-        if (ok && !wait_ns(pv_done, (n_tiles - 1) & 1)) ok = false;
+        if (ok && !wait_ns(pv_done + blk, (n_tiles - 1) & 1)) ok = false;
         fence_after();
         // ---- output ---------------------------------------------------------------------------------
         const bool has = row && l != 0.f;
         const float f = nsplit == 1 ? (has ? 1.f / l : 0.f) : 1.f;
         const float e0 = __uint_as_float((uint32_t)(127 - 13) << 23), e1 = __uint_as_float((uint32_t)(127 + ev) << 23);
-        const size_t slot = (seg * nsplit + sp) * CM + col;
+        const size_t slot = (seg * nsplit + sp) * CB + col;
 #pragma unroll 1
         for (int d = 0; d < D; d += 16) {
             float o[16];
@@ -403,7 +433,7 @@ __global__ void __launch_bounds__(NT_TC, 2) kv4_attn_tc_kernel(const Kv4AttnArgs
                 pml[slot] = make_float2(l != 0.f ? -nm : M0, l);
             }
         }
-    } else if (warp < 8) {
+    } else if (warp < PW0 + 4) {
         // ---- producers: packed rows -> operands ----------------------------------------------------
         const int key = pt & 63, g = D == 128 ? pt >> 6 : 0, half = D == 128 ? 0 : pt >> 6;  // D = 64: half a row each
         constexpr int WPT = D == 128 ? 8 : 4;  // words per thread
@@ -436,14 +466,14 @@ __global__ void __launch_bounds__(NT_TC, 2) kv4_attn_tc_kernel(const Kv4AttnArgs
                 kz = vs + vz + INFINITY - INFINITY;
                 vs = vz = 0.f;
             }
-            if (ok && i > 0 && !wait_ns(s_full, (i - 1) & 1)) ok = false;  // K is free
-            unsigned char* kd = sm + P::K + g * KT * 128;
+            if (ok && i > 1 && !wait_ns(k_free + (i & 1), ((i - 2) >> 1) & 1)) ok = false;
+            unsigned char* kd = sm + P::K + (i & 1) * P::OPB + g * KT * 128;
 #pragma unroll
             for (int j = 0; j < WPT; ++j)
                 *reinterpret_cast<uint4*>(kd + chunk_at(key, half * 4 + j)) =
                     make_uint4(nib_even(w[j]), nib_odd(w[j]), nib_even(w[j] >> 8), nib_odd(w[j] >> 8));
             if (half == 0) {
-                float* tab = reinterpret_cast<float*>(sm + P::TAB) + (i & 1) * 2 * GR * KT + g * KT + key;
+                float* tab = reinterpret_cast<float*>(sm + P::TAB) + (i % TABS) * 2 * GR * KT + g * KT + key;
                 tab[0] = ks;
                 tab[GR * KT] = kz;
             }
@@ -461,8 +491,8 @@ __global__ void __launch_bounds__(NT_TC, 2) kv4_attn_tc_kernel(const Kv4AttnArgs
                 }
             }
             const __half2 s2 = __float2half2_rn(vs * dn), z2 = __float2half2_rn(vz * dn);
-            if (ok && i > 0 && !wait_ns(pv_done, (i - 1) & 1)) ok = false;  // V is free
-            unsigned char* vd = sm + P::V + g * KT * 128;
+            if (ok && i > 1 && !wait_ns(v_free + (i & 1), ((i - 2) >> 1) & 1)) ok = false;
+            unsigned char* vd = sm + P::V + (i & 1) * P::OPB + g * KT * 128;
 #pragma unroll
             for (int j = 0; j < WPT; ++j) {
                 uint32_t o[4];
@@ -472,41 +502,57 @@ __global__ void __launch_bounds__(NT_TC, 2) kv4_attn_tc_kernel(const Kv4AttnArgs
                 *reinterpret_cast<uint4*>(vd + chunk_at(key, half * 4 + j)) = make_uint4(o[0], o[1], o[2], o[3]);
             }
             fence_proxy_async_smem();
-            arrive(v_full);
+            arrive(v_full + (i & 1));
         }
         cp_async_wait<0>();
     } else if (lane == 0) {
         // ---- products ------------------------------------------------------------------------------------
         const uint32_t qb = smem_u32(sm + P::Q), kb = smem_u32(sm + P::K), vb = smem_u32(sm + P::V);
-        for (int i = 0; i < n_tiles && ok; ++i) {
-            // S_0 also holds the P of the tile before
-            if (!wait_ns(k_full + (i & 1), (i >> 1) & 1) || (i > 0 && !wait_ns(pv_done, (i - 1) & 1))) {
-                ok = false;
-                break;
-            }
-            fence_after();
+        auto scores = [&](int blk, int i) {  // S of tile i; the arrival passes on what the producers wrote
 #pragma unroll
             for (int g = 0; g < GR; ++g)
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    mma_ss(tmem + g * KT, desc(qb + g * CM * 128 + 32 * k, 16), desc(kb + g * KT * 128 + 32 * k, 16), idesc(KT, false),
-                           k != 0 ? 1u : 0u);
-            commit(s_full);
-            if (!wait_ns(v_full, i & 1) || !wait_ns(p_full, i & 1)) {
-                ok = false;
-                break;
-            }
+                    mma_ss(tmem + blk * P::TB + g * KT, desc(qb + (blk * GR + g) * CM * 128 + 32 * k, 16),
+                           desc(kb + (i & 1) * P::OPB + g * KT * 128 + 32 * k, 16), idesc(KT, false), k != 0 ? 1u : 0u);
+            commit(s_full + blk);
+            arrive(s_full + blk);
+            if (blk == NB - 1) commit(k_free + (i & 1));
+        };
+        if (!wait_ns(k_full, 0)) ok = false;
+        if (ok) {
             fence_after();
 #pragma unroll
-            for (int k = 0; k < KT / 16; ++k)
-                mma_ts(tmem + P::TO, tmem + 8 * k, desc(vb + 16 * 128 * k, KT * 128), idesc(D, true), (i | k) != 0 ? 1u : 0u);
-            commit(pv_done);
+            for (int blk = 0; blk < NB; ++blk) scores(blk, 0);
+        }
+        for (int i = 0; i < n_tiles && ok; ++i) {
+            if (!wait_ns(v_full + (i & 1), (i >> 1) & 1)) ok = false;
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk) {
+                if (ok && !wait_ns(p_full + blk, i & 1)) ok = false;
+                if (!ok) break;
+                fence_after();
+#pragma unroll
+                for (int k = 0; k < KT / 16; ++k)
+                    mma_ts(tmem + blk * P::TB + P::TO, tmem + blk * P::TB + 8 * k, desc(vb + (i & 1) * P::OPB + 16 * 128 * k, KT * 128),
+                           idesc(D, true), (i | k) != 0 ? 1u : 0u);
+                commit(pv_done + blk);
+                if (blk == NB - 1) commit(v_free + (i & 1));
+                if (i + 1 < n_tiles) {  // S_0 holds P until its product is done
+                    if ((blk == 0 && !wait_ns(k_full + ((i + 1) & 1), ((i + 1) >> 1) & 1)) || !wait_ns(pv_done + blk, i & 1)) {
+                        ok = false;
+                        break;
+                    }
+                    fence_after();
+                    scores(blk, i + 1);
+                }
+            }
         }
     }
     if (!ok && a.err) atomicOr(a.err, (int)QW_DERR_TIMEOUT);
     fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == PW0 + 4) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P::TMEM) : "memory");
     }
@@ -514,26 +560,26 @@ __global__ void __launch_bounds__(NT_TC, 2) kv4_attn_tc_kernel(const Kv4AttnArgs
 
 // Joins the splits' partials.  One block per (column, sequence), one thread per dimension.
 template <int D>
-__global__ void __launch_bounds__(D) kv4_attn_tc_join_kernel(const Kv4AttnArgs a, int ncb, int nsplit, const float* part, const float2* pml) {
+__global__ void __launch_bounds__(D) kv4_attn_tc_join_kernel(const Kv4AttnArgs a, int cb_size, int ncb, int nsplit, const float* part, const float2* pml) {
     const int b = blockIdx.y, G = a.Hq / a.c.heads, d = threadIdx.x, h = blockIdx.x % a.Hq, i = blockIdx.x / a.Hq;
     const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
-    const int c = i * G + h % G, cb = c / CM, C = G * a.S;
-    const int i_last = min(rw.n, (min(C, (cb + 1) * CM) - 1) / G + 1) - 1;
+    const int c = i * G + h % G, cb = c / cb_size, C = G * a.S;
+    const int i_last = min(rw.n, (min(C, (cb + 1) * cb_size) - 1) / G + 1) - 1;
     const int T = rw.off + rw.n, nt = ((a.causal ? min(T, rw.off + i_last + 1) : T) + KT - 1) / KT;
     bf16* dst = a.out + (b * a.os.b + (long long)i * a.os.s + (long long)h * a.os.h) + d;
     float* lse = a.lse ? a.lse + ((size_t)b * a.S + i) * a.Hq + h : nullptr;
     pdl_wait();
     float M = M0, o = 0.f, l = 0.f;
     if (i < rw.n) {
-        const size_t s0 = ((((size_t)b * a.c.heads + h / G) * ncb + cb) * nsplit) * CM + c % CM;
+        const size_t s0 = ((((size_t)b * a.c.heads + h / G) * ncb + cb) * nsplit) * cb_size + c % cb_size;
         for (int s = 0; s < nsplit; ++s)
-            if ((long long)nt * s / nsplit != (long long)nt * (s + 1) / nsplit) M = fmaxf(M, pml[s0 + (size_t)s * CM].x);
+            if ((long long)nt * s / nsplit != (long long)nt * (s + 1) / nsplit) M = fmaxf(M, pml[s0 + (size_t)s * cb_size].x);
         for (int s = 0; s < nsplit; ++s)
             if ((long long)nt * s / nsplit != (long long)nt * (s + 1) / nsplit) {
-                const float2 ml = pml[s0 + (size_t)s * CM];
+                const float2 ml = pml[s0 + (size_t)s * cb_size];
                 const float f = half_pow(ml.x - M);
                 l = fmaf(ml.y * f, f, l);
-                o = fmaf(part[(s0 + (size_t)s * CM) * D + d] * f, f, o);
+                o = fmaf(part[(s0 + (size_t)s * cb_size) * D + d] * f, f, o);
             }
     }
     *dst = f2bf(l != 0.f ? o / l : 0.f);
@@ -555,16 +601,17 @@ cudaError_t launch(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t st
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <int D>
+template <int D, int NB>
 cudaError_t launch_tc(const Kv4AttnArgs& a, const TcShape& sp, float* part, float2* ml, cudaStream_t st) {
-    cudaError_t e = ensure_max_dyn_smem(kv4_attn_tc_kernel<D>, Plan<D>::BYTES);
+    constexpr int smem = Plan<D, NB>::BYTES;
+    cudaError_t e = ensure_max_dyn_smem(kv4_attn_tc_kernel<D, NB>, smem);
     if (e != cudaSuccess) return e;
     const long long blocks = (long long)sp.ncb * sp.nsplit * a.c.heads * a.c.batch;
     if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
-    e = launch(kv4_attn_tc_kernel<D>, dim3((unsigned)blocks), dim3(NT_TC), Plan<D>::BYTES, st, false, a, sp.ncb, sp.nsplit, part, ml);
+    e = launch(kv4_attn_tc_kernel<D, NB>, dim3((unsigned)blocks), dim3(THREADS<NB>), smem, st, false, a, sp.ncb, sp.nsplit, part, ml);
     if (e != cudaSuccess || sp.nsplit == 1) return e;
-    return launch(kv4_attn_tc_join_kernel<D>, dim3((unsigned)(a.S * a.Hq), a.c.batch), dim3(D), 0, st, true, a, sp.ncb, sp.nsplit,
-                  (const float*)part, (const float2*)ml);
+    return launch(kv4_attn_tc_join_kernel<D>, dim3((unsigned)(a.S * a.Hq), a.c.batch), dim3(D), 0, st, true, a, CM * NB, sp.ncb,
+                  sp.nsplit, (const float*)part, (const float2*)ml);
 }
 
 }  // namespace
@@ -572,25 +619,27 @@ cudaError_t launch_tc(const Kv4AttnArgs& a, const TcShape& sp, float* part, floa
 TcShape kv4_tc_shape(const Kv4View& c, int S, int Hq, int num_sms) {
     const long long C = (long long)(Hq / c.heads) * S;
     TcShape s;
-    s.ncb = (int)((C + CM - 1) / CM);
-    // splits of the keys: fill rounds of two blocks per SM, at least four tiles each if the cache were
-    // full; a split costs a partial's write and read, counted as a fiftieth of a round
-    const long long segs = (long long)s.ncb * c.heads * c.batch, slots = 2ll * num_sms;
+    s.nb = C > CM ? 2 : 1;
+    s.ncb = (int)((C + CM * s.nb - 1) / (CM * s.nb));
+    // splits of the keys: fill rounds of one block per SM, at least four tiles each if the cache were
+    // full; a split costs a partial's write and read, counted as a tenth of a round
+    const long long segs = (long long)s.ncb * c.heads * c.batch;
     s.nsplit = 1;
     float best = 1e30f;
     for (int n = 1; n <= 64 && (n == 1 || n * 4 * KT <= c.max_pos); ++n) {
-        const float t = (float)((segs * n + slots - 1) / slots) / n * (1.f + 0.02f * (n - 1));
+        const float t = (float)((segs * n + num_sms - 1) / num_sms) / n * (1.f + 0.1f * (n - 1));
         if (t < best) {
             best = t;
             s.nsplit = n;
         }
     }
-    s.part_rows = s.nsplit > 1 ? (size_t)segs * s.nsplit * CM : 0;
+    s.part_rows = s.nsplit > 1 ? (size_t)segs * s.nsplit * CM * s.nb : 0;
     return s;
 }
 
 cudaError_t launch_kv4_attn_tc(const Kv4AttnArgs& a, const TcShape& s, float* part, float2* ml, cudaStream_t st) {
-    return a.c.D == 128 ? launch_tc<128>(a, s, part, ml, st) : launch_tc<64>(a, s, part, ml, st);
+    if (a.c.D == 128) return s.nb == 2 ? launch_tc<128, 2>(a, s, part, ml, st) : launch_tc<128, 1>(a, s, part, ml, st);
+    return s.nb == 2 ? launch_tc<64, 2>(a, s, part, ml, st) : launch_tc<64, 1>(a, s, part, ml, st);
 }
 
 }  // namespace qw

@@ -6,7 +6,7 @@
 namespace qw {
 
 struct TcShape {
-    int ncb, nsplit;   // blocks of 128 columns, splits of the keys
+    int nb, ncb, nsplit;  // 128-column blocks per thread block, blocks of nb * 128 columns, splits of the keys
     size_t part_rows;  // partial rows (D floats and a float2 each) the splits leave
 };
 TcShape kv4_tc_shape(const Kv4View& c, int S, int Hq, int num_sms);
