@@ -2,24 +2,32 @@
 // on the tcgen05 tensor cores.
 //
 // A thread block takes NB = 1 or 2 blocks of 128 columns (row, query head) of one
-// (sequence, kv head) and walks the keys they see in tiles of 64:
-//   S_g = Q_g N_g^T   per 64-element group g: Q (fp16, scaled per column as in
-//                     kv4_tile.cuh) against the packed integers, which enter as
-//                     fp16 subnormals (n 2^-24, the odd nibbles 16 n 2^-24
-//                     against q / 16): exact products, fp32 sums in TMEM
-//   x = c sum_g s_g S_g + sum_g b_g q_g - m      fp32, one thread per column
-//   P = 2^x           fp16 in TMEM, over S_0's columns
-//   O += P V          V dequantised to fp16 in shared memory, fp32 sums in TMEM
-// V is taken times 2^-E with E the exponent of the block's largest value (found
-// first, from scales and biases alone), so any bf16 range fits fp16; the running
-// maximum moves only when a score passes it by 2^4 (P <= 2^15), and then O is
-// rescaled in TMEM.
+// (sequence, kv head) and walks the keys they see in tiles of 128.  A key's
+// element in group g is s_g (n - 8) + c_g with c_g = b_g + 8 s_g:
+//   S  = Q K'^T + Q* C*^T    K' = s (n - 8): an 8-bit by a 3-bit number, exact in
+//                            fp16; Q exact in fp16 (scaled per column as in
+//                            kv4_tile.cuh); Q* and C* hold the group sums of q and
+//                            the c_g in pieces of 11 bits, one more k-step of 16
+//   x  = c S - m             fp32, two threads per column
+//   P  = 2^x                 fp16 in TMEM, over the first half of S
+//   O += P V                 V dequantised to fp16, fp32 sums in TMEM
+// So scores are exact up to fp32 sums, and the softmax threads need no per-key
+// numbers.  (With the integers themselves as operand and a sum per group, the
+// per-key scales cost four shared-memory words per score, and their reads were
+// the bound: 309 us for 1024 rows of 32 heads on 8192 keys.)  K and V are taken
+// times powers of two that put the block's largest value (found first, from
+// scales and biases alone) where fp16 holds it; the running maximum moves only
+// when a score passes it by 2^4 (P <= 2^15), and then O is rescaled in TMEM.
 //
-// Roles: warps 0 .. 4 NB - 1 one column per thread (with NB = 2 one column
-// block's softmax overlaps the other's products); four warps copy packed rows
-// (cp.async ring) and expand them, once for all column blocks; one lane of the
-// last warp issues the products.  Every wait is bounded: a lost arrival sets
-// QW_DERR_TIMEOUT and the block still frees its TMEM and ends.
+// Roles: one lane of the last warp issues the products; all other warps, two
+// threads per column with half a tile's keys each, do the softmax and between two
+// softmaxes expand a share of packed rows (the values of the next tile, the keys
+// of the one after), which they loaded into registers a tile earlier.  With NB =
+// 2 one column block's softmax runs beside the other's products.  (Three warps of
+// their own for the expansion took 11 400 cycles a tile: alone on their issue
+// slots they run at the pace of instruction fetch and of single dependent
+// chains.)  Every wait is bounded: a lost arrival sets QW_DERR_TIMEOUT and the
+// block still frees its TMEM and ends.
 #include "kv4_tc.h"
 #include "kv4_tile.cuh"
 #include "smem_attr.h"
@@ -30,11 +38,9 @@ namespace {
 using namespace kv4;
 
 constexpr int CM = 128;      // columns of a column block
-constexpr int KT = 64;       // keys of a tile
-constexpr int STAGES = 3;    // packed tiles in flight
-constexpr int TABS = 4;      // score tables: a tile's is read until the products of the next tile but one are issued
+constexpr int KT = 128;      // keys of a tile
 template <int NB>
-constexpr int THREADS = 128 * NB + 160;
+constexpr int THREADS = 256 * NB + 32;
 constexpr float BASE = 11.f;          // P = 2^(x - max + 11)
 constexpr float RAISE = BASE + 4.f;   // a larger exponent raises the maximum
 constexpr float UNSET = -3.0e38f;
@@ -43,16 +49,14 @@ constexpr unsigned long long TIMEOUT_NS = 2000000000ull;
 // Shared memory, from a 1 KB aligned base.
 template <int D, int NB>
 struct Plan {
-    static constexpr int GR = D / 64, OPB = GR * KT * 128;
-    static constexpr int Q = 1024;                    // [NB][GR][128 rows][128 B], swizzled
-    static constexpr int K = Q + NB * GR * CM * 128;  // [2][GR][64 keys][128 B], swizzled
-    static constexpr int V = K + 2 * OPB;             // the same, read along the keys
-    static constexpr int TAB = V + 2 * OPB;           // [TABS][K scale, K bias][GR][64] fp32
-    static constexpr int PACK = TAB + TABS * 2 * GR * KT * 4;
-    static constexpr int PW = KT * D / 2, PS = KT * GR * 2, PACKB = 2 * PW + 4 * PS;
-    static constexpr int BYTES = PACK + STAGES * PACKB + 1024;
-    // TMEM columns of a column block: S_0, (S_1), O; P over S_0
-    static constexpr uint32_t TO = GR * KT, TB = GR * KT + D, TMEM = NB * TB;
+    static constexpr int GR = D / 64;
+    static constexpr int QB = GR * CM * 128 + CM * 32, KB = GR * KT * 128 + KT * 32, VB = GR * KT * 128;
+    static constexpr int Q = 5120;           // after the barriers and two exchange arrays: [NB]{[GR][128 rows][128 B] swizzled; Q*}
+    static constexpr int K = Q + NB * QB;    // [2]{[GR][128 keys][128 B] swizzled; C*}
+    static constexpr int V = K + 2 * KB;     // [2][GR][128 keys][128 B], swizzled, read along the keys
+    static constexpr int BYTES = V + 2 * VB + 1024;
+    // TMEM columns of a column block: S (P over its first half), O
+    static constexpr uint32_t TO = KT, TB = KT + D, TMEM = NB * TB <= 256 ? 256 : 512;
 };
 
 QW_DEV unsigned long long now_ns() {
@@ -72,8 +76,14 @@ QW_DEV void arrive(uint64_t* bar) {
 }
 QW_DEV void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 QW_DEV void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-QW_DEV void commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+// The product warp runs as a whole, so that its control flow and descriptors stay in uniform
+// registers; `lead` picks the one lane that issues.
+QW_DEV void commit(uint64_t* bar, uint32_t lead) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+        "r"(lead)
+        : "memory");
 }
 // 128-byte-swizzled operand rows of 64 fp16: descriptor version 1, 1 KB between 8-row groups; along_keys:
 // the matrix' k runs over the rows and its 64-element blocks lie `lead` bytes apart.
@@ -81,20 +91,27 @@ QW_DEV uint64_t desc(uint32_t addr, uint32_t lead) {
     return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) |
            (2ull << 61);
 }
+// The 16-wide extra operand: 8 rows x 16 bytes make a block of 128 bytes, [row / 8][k / 8][row % 8][16 B], no swizzle.
+QW_DEV uint64_t desc16(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(128u >> 4) << 16) | ((uint64_t)(256u >> 4) << 32) | (1ull << 46);
+}
+QW_DEV uint32_t at16(int row, int khalf) { return (uint32_t)(row >> 3) * 256 + khalf * 128 + (row & 7) * 16; }
 // kind::f16, fp32 sums, fp16 operands, A along k, B along k or (bit 16) along n; M = 128.
 __host__ __device__ constexpr uint32_t idesc(int n, bool b_along_n) {
     return (1u << 4) | (b_along_n ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(CM >> 4) << 24);
 }
-QW_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+QW_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate, uint32_t lead) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate),
+        "r"(lead)
         : "memory");
 }
-QW_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+QW_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate, uint32_t lead) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate),
+        "r"(lead)
         : "memory");
 }
 QW_DEV void ld16(uint32_t addr, float (&v)[16]) {
@@ -138,11 +155,6 @@ QW_DEV unsigned long long fma2(unsigned long long a, unsigned long long b, unsig
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
-QW_DEV unsigned long long mul2(unsigned long long a, unsigned long long b) {
-    unsigned long long r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 QW_DEV unsigned long long add2(unsigned long long a, unsigned long long b) {
     unsigned long long r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -152,11 +164,11 @@ QW_DEV unsigned long long add2(unsigned long long a, unsigned long long b) {
 template <int D, int NB>
 __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4AttnArgs a, int ncb, int nsplit, float* part, float2* pml) {
     using P = Plan<D, NB>;
-    constexpr int GR = P::GR, CB = CM * NB, PW0 = 4 * NB;  // columns of the block, first producer warp
+    constexpr int GR = P::GR, CB = CM * NB, PW0 = 8 * NB;  // columns of the block, first producer warp
     extern __shared__ unsigned char tc_raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>(((uintptr_t)tc_raw + 1023) & ~(uintptr_t)1023);
     // barriers: tile i uses [i & 1] of the paired ones; those per column block count tiles
-    uint64_t* k_full = reinterpret_cast<uint64_t*>(sm);  // K operand and table written
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(sm);  // K operand written
     uint64_t* k_free = k_full + 2;                        // products Q N of every column block done
     uint64_t* v_full = k_free + 2;
     uint64_t* v_free = v_full + 2;
@@ -164,7 +176,8 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
     uint64_t* p_full = s_full + 2;
     uint64_t* pv_done = p_full + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2);
-    float* vmax = reinterpret_cast<float*>(tmem_slot + 2);  // [4] producers' warps
+    float* kvmax = reinterpret_cast<float*>(tmem_slot + 2);  // [8 NB][2] of the warps: largest |K|, |V|
+    float* xch = reinterpret_cast<float*>(sm + 1024);       // [round][half][CB]: largest scores; in the end the halves' sums
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     // heaviest column blocks first
@@ -181,12 +194,13 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
     const int all = a.causal ? min(T, rw.off + i_first + 1) : T;  // keys that every column sees
     const size_t seg = ((size_t)b * a.c.heads + h) * ncb + cb;
 
-    const int col = min(tid, CB - 1), c = cb * CB + col, i_row = c / G, head = h * G + c % G;
+    const int half = (warp >> 2) & 1;  // softmax threads: half of a tile's keys
+    const int col = min((warp >> 3) * CM + (tid & 127), CB - 1), c = cb * CB + col, i_row = c / G, head = h * G + c % G;
     const bool row = c < C && i_row < rw.n;
     bf16* out = a.out + (b * a.os.b + (long long)i_row * a.os.s + (long long)head * a.os.h);
     const size_t lse_at = ((size_t)b * a.S + i_row) * a.Hq + head;
     if (t0 == t1) {  // nothing to see: zeros (a split's empty share is skipped by the joining kernel)
-        if (nsplit == 1 && tid < CB && c < C) {
+        if (nsplit == 1 && warp < PW0 && half == 0 && c < C) {
             for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(out + d) = make_uint4(0u, 0u, 0u, 0u);
             if (a.lse) a.lse[lse_at] = -INFINITY;
         }
@@ -194,17 +208,17 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
     }
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(k_full + i, 128);
+            mbar_init(k_full + i, 256 * NB);
             mbar_init(k_free + i, 1);
-            mbar_init(v_full + i, 128);
+            mbar_init(v_full + i, 256 * NB);
             mbar_init(v_free + i, 1);
-            mbar_init(s_full + i, 2);
-            mbar_init(p_full + i, 128);
+            mbar_init(s_full + i, 1);
+            mbar_init(p_full + i, 256);
             mbar_init(pv_done + i, 1);
         }
         fence_mbar_init();
     }
-    if (warp == PW0 + 4) {
+    if (warp == PW0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(P::TMEM)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -212,33 +226,9 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
 
     const Rows rows = head_rows<D>(a.c, (size_t)b * a.c.heads + h);
     const int key_end = min(T, t1 * KT);  // this block's keys end here
-    const int pt = tid - CB;              // producer thread
-    auto fetch = [&](int i) {  // tile t0 + i into stage i % STAGES, 16-byte pieces; zeros past the last key
-        if (t0 + i < t1) {
-            const int key0 = (t0 + i) * KT;
-            const uint32_t dst = smem_u32(sm + P::PACK + (i % STAGES) * P::PACKB);
-#pragma unroll
-            for (int w = 0; w < 2; ++w)
-#pragma unroll
-                for (int j = 0; j < P::PW / 16; j += 128) {
-                    const int piece = j + pt;
-                    const bool ok = key0 + piece / (D / 32) < T;
-                    cp_async16_zfill(dst + w * P::PW + piece * 16, ok ? rows.w[w] + (size_t)key0 * (D / 2) + piece * 16 : rows.w[w], ok);
-                }
-            constexpr int SP = P::PS / 16, KPP = KT / SP;  // pieces of a scale array, keys of a piece
-            if (pt < 4 * SP) {
-                const int arr = pt / SP, piece = pt % SP;
-                const unsigned char* base = arr & 2 ? (arr & 1 ? rows.b[1] : rows.s[1]) : (arr & 1 ? rows.b[0] : rows.s[0]);
-                const bool ok = key0 + piece * KPP < T;
-                cp_async16_zfill(dst + 2 * P::PW + pt * 16, ok ? base + (size_t)key0 * (2 * GR) + piece * 16 : base, ok);
-            }
-        }
-        cp_async_commit();
-    };
-
-    float cc = 0.f, q0 = 0.f, q1 = 0.f;  // the column's score constants (softmax threads)
+    float cc = 0.f;  // score of a column = cc * S (softmax threads; K's power of two comes in below)
     if (warp < PW0) {
-        // Q operand: column `col`, elements of a chunk in the order of an expanded word
+        // Q operand: column `col`, the thread's half of its chunks, elements in the order of an expanded word
         const bf16* src = a.q + (b * a.qs.b + (long long)i_row * a.qs.s + (long long)head * a.qs.h);
         float mx = 0.f, sum[GR];
 #pragma unroll
@@ -259,144 +249,295 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
         }
         const int ex = max((int)(__float_as_uint(mx) >> 23) - 127, -100);
         const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
-        cc = ldexpf(a.scale * LOG2E, ex - 14 + 24);
-        q0 = sum[0] * (a.scale * LOG2E);
-        q1 = sum[GR - 1] * (a.scale * LOG2E);
-#pragma unroll
-        for (int g = 0; g < GR; ++g)
+        cc = ldexpf(a.scale * LOG2E, ex - 14);
+        unsigned char* qo = sm + P::Q + (col >> 7) * P::QB;
 #pragma unroll 4
-            for (int k = 0; k < 8; ++k) {
-                uint4 u = make_uint4(0u, 0u, 0u, 0u);
-                if (row) u = *reinterpret_cast<const uint4*>(src + 64 * g + 8 * k);
-                const uint32_t X[4] = {u.x, u.y, u.z, u.w};
-                float x[8];
+        for (int j = 0; j < 4 * GR; ++j) {
+            const int g = (half * 4 * GR + j) / 8, k = (half * 4 * GR + j) % 8;
+            uint4 u = make_uint4(0u, 0u, 0u, 0u);
+            if (row) u = *reinterpret_cast<const uint4*>(src + 64 * g + 8 * k);
+            const uint32_t X[4] = {u.x, u.y, u.z, u.w};
+            float x[8];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[2 * e] = bits_lo_f(X[e]) * up;
-                    x[2 * e + 1] = bits_hi_f(X[e]) * up;
-                }
-                *reinterpret_cast<uint4*>(sm + P::Q + ((col >> 7) * GR + g) * CM * 128 + chunk_at(col & 127, k)) =
-                    make_uint4(h2(x[0], x[4]), h2(x[1] * 0.0625f, x[5] * 0.0625f), h2(x[2], x[6]), h2(x[3] * 0.0625f, x[7] * 0.0625f));
+            for (int e = 0; e < 4; ++e) {
+                x[2 * e] = bits_lo_f(X[e]) * up;
+                x[2 * e + 1] = bits_hi_f(X[e]) * up;
             }
-        fence_proxy_async_smem();
-    } else if (warp < PW0 + 4) {
-#pragma unroll
-        for (int i = 0; i < STAGES - 1; ++i) fetch(i);
-        // largest |value| that the block's V rows can stand for: max(|b|, |b + 15 s|) (a NaN counts as nothing here)
-        float mx = 0.f;
-        const uint32_t* s = reinterpret_cast<const uint32_t*>(rows.s[1]);
-        const uint32_t* z = reinterpret_cast<const uint32_t*>(rows.b[1]);
-        constexpr int KW = 2 / GR;  // keys of a 32-bit word of scales (rows end at a multiple of 16)
-#pragma unroll 8
-        for (int w = t0 * KT / KW + pt; w < (key_end + KW - 1) / KW; w += 128) {
-            const uint32_t us = s[w], uz = z[w];
-            const float z0 = bits_lo_f(uz), z1 = bits_hi_f(uz);
-            float m = fmaxf(fabsf(z0), fabsf(fmaf(15.f, bits_lo_f(us), z0)));
-            if (GR == 2 || w * KW + 1 < key_end) m = fmaxf(m, fmaxf(fabsf(z1), fabsf(fmaf(15.f, bits_hi_f(us), z1))));
-            mx = fmaxf(mx, m);
+            *reinterpret_cast<uint4*>(qo + g * CM * 128 + chunk_at(col & 127, k)) =
+                make_uint4(h2(x[0], x[4]), h2(x[1], x[5]), h2(x[2], x[6]), h2(x[3], x[7]));
         }
-        mx = warp_max(mx);
-        if (lane == 0) vmax[warp - PW0] = mx;
+        // Q*: a group's sum times 2^-6 in three fp16 terms, k = 5 g + {0..4}: hi, hi, mid, mid, lo
+        // (against the two terms of 2^6 c: hi, lo, hi, lo, hi)
+        if (half == 0) {
+            __half t[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) t[e] = __float2half_rn(0.f);
+#pragma unroll
+            for (int g = 0; g < GR; ++g) {
+                const float v = sum[g] * up * 0.015625f;
+                const __half hi = __float2half_rn(v), mid = __float2half_rn(v - __half2float(hi));
+                t[5 * g] = t[5 * g + 1] = hi;
+                t[5 * g + 2] = t[5 * g + 3] = mid;
+                t[5 * g + 4] = __float2half_rn(v - __half2float(hi) - __half2float(mid));
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                uint32_t r[4];
+#pragma unroll
+                for (int f = 0; f < 4; ++f) r[f] = as_u(__halves2half2(t[8 * e + 2 * f], t[8 * e + 2 * f + 1]));
+                *reinterpret_cast<uint4*>(qo + GR * CM * 128 + at16(col & 127, e)) = make_uint4(r[0], r[1], r[2], r[3]);
+            }
+        }
+        // largest magnitudes that the block's rows can stand for: max(|b|, |b + 15 s|) (a NaN counts as nothing here)
+        constexpr int KW = 2 / GR;  // keys of a 32-bit word of scales (rows end at a multiple of 16)
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+            float mx = 0.f;
+            const uint32_t* s = reinterpret_cast<const uint32_t*>(rows.s[v]);
+            const uint32_t* z = reinterpret_cast<const uint32_t*>(rows.b[v]);
+#pragma unroll 8
+            for (int w = t0 * KT / KW + tid; w < (key_end + KW - 1) / KW; w += 256 * NB) {
+                const uint32_t us = s[w], uz = z[w];
+                const float z0 = bits_lo_f(uz), z1 = bits_hi_f(uz);
+                float m = fmaxf(fabsf(z0), fabsf(fmaf(15.f, bits_lo_f(us), z0)));
+                if (GR == 2 || w * KW + 1 < key_end) m = fmaxf(m, fmaxf(fabsf(z1), fabsf(fmaf(15.f, bits_hi_f(us), z1))));
+                mx = fmaxf(mx, m);
+            }
+            mx = warp_max(mx);
+            if (lane == 0) kvmax[2 * warp + v] = mx;
+        }
     }
     fence_before();
     __syncthreads();
     fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-    // V enters as value 2^(13 - ev): below 2^14
-    const float vm = fmaxf(fmaxf(vmax[0], vmax[1]), fmaxf(vmax[2], vmax[3]));
-    const int ev = max((int)(__float_as_uint(fminf(vm, 3.0e38f)) >> 23) - 127, -100);
+    // exponents of the largest values: K enters times 2^(7 - ek), V times 2^(13 - ev)
+    auto exponent = [&](int v) {
+        float m = 0.f;
+#pragma unroll
+        for (int w = 0; w < PW0; ++w) m = fmaxf(m, kvmax[2 * w + v]);
+        return max((int)(__float_as_uint(fminf(m, 3.0e38f)) >> 23) - 127, -100);
+    };
+    const int ek = exponent(0), ev = exponent(1);
     const int n_tiles = t1 - t0;
     bool ok = true;
 
     if (warp < PW0) {
-        // ---- softmax: one column per thread ------------------------------------------------------
-        const int blk = warp >> 2;
+        // ---- softmax: two threads per column, half of a tile's keys each ----------------------------------
+        constexpr int KH = 32;  // keys of a thread and round
+        const int blk = warp >> 3;
         const uint32_t tm = tmem + blk * P::TB + ((uint32_t)(32 * (warp & 3)) << 16);
         const int vis = row ? (a.causal ? min(T, rw.off + i_row + 1) : T) : 0;
-        const unsigned long long c2 = pack2(cc, cc), q02 = pack2(q0, q0), q12 = pack2(q1, q1);
-        float nm = 0.f, l = 0.f, thr = UNSET;  // BASE - maximum; up to thr the maximum stays
-        for (int i = 0; i < n_tiles; ++i) {
-            const int key0 = (t0 + i) * KT;
-            if (ok && !wait_ns(s_full + blk, i & 1)) ok = false;
-            fence_after();
-            const float* tab = reinterpret_cast<const float*>(sm + P::TAB) + (i % TABS) * 2 * GR * KT;
-            const unsigned long long nm2 = pack2(nm, nm);
-            float x[KT];
+        cc = ldexpf(cc, ek - 7);
+        const unsigned long long c2 = pack2(cc, cc);
+
+        // ---- expansion of this thread's share of a tile --------------------------------------------------
+        // A thread takes 16-byte pieces (4 words of a row), thread after thread: piece p of a tile is words
+        // 4 (p % CPR) .. of key p / CPR.  With two groups the second one's words go out in another order
+        // (e ^ 2): the eight lanes of a store phase (two keys, all pieces) hit eight different chunk columns.
+        constexpr int CPR = D / 32, PIECES = KT * CPR, NTH = 256 * NB, PER = PIECES >= NTH ? PIECES / NTH : 1;
+        const bool has_piece = tid < PIECES;  // D = 64 and two column blocks: half of the threads
+        const float kup = __uint_as_float((uint32_t)(127 + 7 - ek) << 23), vup = __uint_as_float((uint32_t)(127 + 13 - ev) << 23);
+        // A NaN in V: where every column sees the key its value is simply NaN; in a tile that some column sees in
+        // part only, the value is left out and the key's score made NaN, which reaches just the rows that see it.
+        auto partial = [&](int i) { return (t0 + i + 1) * KT > all; };
+        struct Share {
+            uint4 w[PER];
+            uint16_t s[PER], z[PER];  // scale and bias of the piece's group
+        } ks, vs;
+        uint32_t cs = 0, cz = 0;  // threads 0 .. 127: scales and biases of one key of the tile, every group
+        auto packed = [&](const unsigned char* base, int key) {
+            return GR == 2 ? *reinterpret_cast<const uint32_t*>(base + (size_t)key * 4) : (uint32_t)*reinterpret_cast<const uint16_t*>(base + (size_t)key * 2);
+        };
+        auto load = [&](Share& x, int which, int i) {  // zeros past the last key
+            const int k0 = (t0 + i) * KT;
+            const uint4* src = reinterpret_cast<const uint4*>(rows.w[which] + (size_t)k0 * (D / 2));
+            const uint16_t* s = reinterpret_cast<const uint16_t*>(rows.s[which]) + (size_t)k0 * GR;
+            const uint16_t* z = reinterpret_cast<const uint16_t*>(rows.b[which]) + (size_t)k0 * GR;
 #pragma unroll
-            for (int k = 0; k < KT; k += 16) {
-                float a0[16], a1[16];
-                ld16(tm + k, a0);
-                if (GR == 2) ld16(tm + KT + k, a1);
-                wait_ld();
+            for (int j = 0; j < PER; ++j) {
+                const int p = tid + NTH * j, at = p / CPR * GR + ((p % CPR) >> 1);
+                const bool in = has_piece && k0 + p / CPR < T;
+                x.w[j] = in ? src[p] : make_uint4(0u, 0u, 0u, 0u);
+                x.s[j] = in ? s[at] : (uint16_t)0;
+                if (which) x.z[j] = in ? z[at] : (uint16_t)0;
+            }
+        };
+        auto load_k = [&](int i) {
+            if (i >= n_tiles) return;
+            load(ks, 0, i);
+            const int key = (t0 + i) * KT + tid;
+            cs = tid < KT && key < T ? packed(rows.s[0], key) : 0u;
+            cz = tid < KT && key < T ? packed(rows.b[0], key) : 0u;
+        };
+        auto load_v = [&](int i) {
+            if (i < n_tiles) load(vs, 1, i);
+        };
+        auto expand = [&](const uint4& w, int p, unsigned char* dst, auto&& value) {
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+            const int key = p / CPR, q = p % CPR, g = q >> 1;
 #pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    const ulonglong2 s0 = *reinterpret_cast<const ulonglong2*>(tab + k + e),
-                                     z0 = *reinterpret_cast<const ulonglong2*>(tab + GR * KT + k + e);
-                    unsigned long long d[2] = {mul2(s0.x, pack2(a0[e], a0[e + 1])), mul2(s0.y, pack2(a0[e + 2], a0[e + 3]))};
-                    unsigned long long u[2] = {fma2(z0.x, q02, nm2), fma2(z0.y, q02, nm2)};
-                    if (GR == 2) {
-                        const ulonglong2 s1 = *reinterpret_cast<const ulonglong2*>(tab + KT + k + e),
-                                         z1 = *reinterpret_cast<const ulonglong2*>(tab + 3 * KT + k + e);
-                        d[0] = fma2(s1.x, pack2(a1[e], a1[e + 1]), d[0]);
-                        d[1] = fma2(s1.y, pack2(a1[e + 2], a1[e + 3]), d[1]);
-                        u[0] = fma2(z1.x, q12, u[0]);
-                        u[1] = fma2(z1.y, q12, u[1]);
-                    }
-                    unpack2(fma2(c2, d[0], u[0]), x[k + e], x[k + e + 1]);
-                    unpack2(fma2(c2, d[1], u[1]), x[k + e + 2], x[k + e + 3]);
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t v = g ? u[e ^ 2] : u[e];
+                uint32_t o[4];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) o[n] = value(((v >> (4 * n)) & 0x000F000Fu) | 0x64006400u);  // (1024 + n_j, 1024 + n_{j+4})
+                *reinterpret_cast<uint4*>(dst + g * KT * 128 + chunk_at(key, 4 * (q & 1) + (g ? e ^ 2 : e))) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+        };
+        auto store_k = [&](int i) {  // tile i's K operand from ks, cs, cz
+            if (i >= n_tiles) return;
+            if (ok && i > 1 && !wait_ns(k_free + (i & 1), ((i - 2) >> 1) & 1)) ok = false;
+            unsigned char* dst = sm + P::K + (i & 1) * P::KB;
+            const __half2 k1032 = __float2half2_rn(1032.f);
+            if (has_piece)
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    const __half2 s2 = __float2half2_rn(u16_to_f(ks.s[j]) * kup);
+                    expand(ks.w[j], tid + NTH * j, dst, [&](uint32_t n) { return as_u(__hmul2(__hsub2(as_h2(n), k1032), s2)); });
+                }
+            if (tid < KT) {
+                // C*: 2^6 c in two fp16 terms, k = 5 g + {0..4}: hi, lo, hi, lo, hi
+                bool nan = false;
+                const int key = (t0 + i) * KT + tid;
+                if (partial(i) && key < T) {
+                    const uint32_t s = packed(rows.s[1], key), z = packed(rows.b[1], key);
+                    nan = !(fabsf(bits_lo_f(s)) + fabsf(bits_lo_f(z)) < INFINITY) || !(fabsf(bits_hi_f(s)) + fabsf(bits_hi_f(z)) < INFINITY);
+                }
+                __half c[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) c[e] = __float2half_rn(0.f);
+#pragma unroll
+                for (int g = 0; g < GR; ++g) {
+                    float x = fmaf(8.f, g ? bits_hi_f(cs) : bits_lo_f(cs), g ? bits_hi_f(cz) : bits_lo_f(cz)) * kup * 64.f;
+                    if (nan) x = __int_as_float(0x7FC00000);
+                    const __half hi = __float2half_rn(x), lo = __float2half_rn(x - __half2float(hi));
+                    c[5 * g] = c[5 * g + 2] = c[5 * g + 4] = hi;
+                    c[5 * g + 1] = c[5 * g + 3] = lo;
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t r[4];
+#pragma unroll
+                    for (int f = 0; f < 4; ++f) r[f] = as_u(__halves2half2(c[8 * e + 2 * f], c[8 * e + 2 * f + 1]));
+                    *reinterpret_cast<uint4*>(dst + GR * KT * 128 + at16(tid, e)) = make_uint4(r[0], r[1], r[2], r[3]);
                 }
             }
-            if (key0 + KT > all)
+            fence_proxy_async_smem();
+            arrive(k_full + (i & 1));
+        };
+        auto store_v = [&](int i) {
+            if (i >= n_tiles) return;
+            if (ok && i > 1 && !wait_ns(v_free + (i & 1), ((i - 2) >> 1) & 1)) ok = false;
+            unsigned char* dst = sm + P::V + (i & 1) * P::VB;
+            const __half2 k1024 = __float2half2_rn(1024.f);
+            if (has_piece)
 #pragma unroll
-                for (int k = 0; k < KT; ++k)
-                    if (key0 + k >= vis) x[k] = -INFINITY;
-            float top = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < KT; ++k) top = fmaxf(top, x[k]);
-            if (__any_sync(0xffffffffu, top > thr)) {
-                // raise the maximum of the columns that ask for it, and rescale what they have summed
-                float al = 1.f;
-                if (top > thr) {
-                    const float up = BASE - top;
-                    al = thr == UNSET ? 0.f : ex2(up);  // the column's first key: nothing summed so far
-                    nm += up;
-                    thr = RAISE;
-#pragma unroll
-                    for (int k = 0; k < KT; ++k) x[k] += up;
+                for (int j = 0; j < PER; ++j) {
+                    float s = u16_to_f(vs.s[j]), z = u16_to_f(vs.z[j]);
+                    if (partial(i) && !(fabsf(s) + fabsf(z) < INFINITY)) s = z = 0.f;
+                    const __half2 s2 = __float2half2_rn(s * vup), z2 = __float2half2_rn(z * vup);
+                    expand(vs.w[j], tid + NTH * j, dst, [&](uint32_t n) { return as_u(__hfma2(__hsub2(as_h2(n), k1024), s2, z2)); });
                 }
-                if (i > 0) {  // P V of the tile before is complete: the products of this one came after it
+            fence_proxy_async_smem();
+            arrive(v_full + (i & 1));
+        };
+        fence_proxy_async_smem();  // the Q operand (published with the first tile's)
+        load_k(0);
+        load_v(0);
+        store_k(0);
+        load_k(1);
+        store_v(0);
+        load_v(1);
+        store_k(1);
+        load_k(2);
+
+        float nm = 0.f, l = 0.f, thr = UNSET;  // BASE - maximum; up to thr the maximum stays
+        for (int i = 0; i < n_tiles; ++i) {
+            if (ok && !wait_ns(s_full + blk, i & 1)) ok = false;
+            fence_after();
+            // Two rounds of 64 keys, 32 of them this thread's.  P of a round lies over columns of S that this
+            // round or the one before has read; the two warps of the column meet after each read.
 #pragma unroll 1
-                    for (int d = 0; d < D; d += 16) {
+            for (int m = 0; m < 2; ++m) {
+                const int k0 = 64 * m + 32 * half, key0 = (t0 + i) * KT + k0;
+                const unsigned long long nm2 = pack2(nm, nm);
+                float x[KH];
+                ld16(tm + k0, *reinterpret_cast<float(*)[16]>(&x[0]));
+                ld16(tm + k0 + 16, *reinterpret_cast<float(*)[16]>(&x[16]));
+                wait_ld();
+#pragma unroll
+                for (int k = 0; k < KH; k += 2) unpack2(fma2(c2, pack2(x[k], x[k + 1]), nm2), x[k], x[k + 1]);
+                if (key0 + KH > all)
+#pragma unroll
+                    for (int k = 0; k < KH; ++k)
+                        if (key0 + k >= vis) x[k] = -INFINITY;
+                float top = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < KH; ++k) top = fmaxf(top, x[k]);
+                xch[(2 * m + half) * CB + col] = top;
+                asm volatile("bar.sync %0, 64;" ::"r"(2 + blk * 4 + (warp & 3)) : "memory");
+                top = fmaxf(top, xch[(2 * m + (half ^ 1)) * CB + col]);
+                if (__any_sync(0xffffffffu, top > thr)) {
+                    // raise the maximum of the columns that ask for it, and rescale what they have summed
+                    float al = 1.f;
+                    if (top > thr) {
+                        const float up = BASE - top;
+                        al = thr == UNSET ? 0.f : ex2(up);  // the column's first key: nothing summed so far
+                        nm += up;
+                        thr = RAISE;
+#pragma unroll
+                        for (int k = 0; k < KH; ++k) x[k] += up;
+                    }
+                    if (i > 0)  // P V of the tile before is complete: the products of this one came after it
+#pragma unroll 1
+                        for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 16) {
+                            float o[16];
+                            uint32_t r[16];
+                            ld16(tm + P::TO + d, o);
+                            wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(o[e] * al);
+                            st16(tm + P::TO + d, r);
+                        }
+                    if (m > 0) {  // this tile's first round
                         float o[16];
                         uint32_t r[16];
-                        ld16(tm + P::TO + d, o);
+                        ld16(tm + half * (KH / 2), o);
                         wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(o[e] * al);
-                        st16(tm + P::TO + d, r);
+                        for (int e = 0; e < 16; ++e) {
+                            const float2 f = __half22float2(as_h2(__float_as_uint(o[e])));
+                            r[e] = h2(f.x * al, f.y * al);
+                        }
+                        st16(tm + half * (KH / 2), r);
                     }
                     l *= al;
                 }
-            }
-            unsigned long long l2[2] = {0ull, 0ull};
-#pragma unroll
-            for (int k = 0; k < KT; k += 32) {
+                unsigned long long l2[2] = {0ull, 0ull};
                 uint32_t r[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const float p0 = ex2(x[k + 2 * e]), p1 = ex2(x[k + 2 * e + 1]);
+                    const float p0 = ex2(x[2 * e]), p1 = ex2(x[2 * e + 1]);
                     l2[e & 1] = add2(l2[e & 1], pack2(p0, p1));
                     r[e] = h2(p0, p1);
                 }
-                st16(tm + k / 2, r);
+                st16(tm + k0 / 2, r);
+                float l0, l1;
+                unpack2(add2(l2[0], l2[1]), l0, l1);
+                l += l0 + l1;
             }
-            float l0, l1;
-            unpack2(add2(l2[0], l2[1]), l0, l1);
-            l += l0 + l1;
             wait_st();
             fence_before();
             arrive(p_full + blk);
+            store_v(i + 1);
+            load_v(i + 2);
+            store_k(i + 2);
+            load_k(i + 3);
         }
+        xch[half * CB + col] = l;
+        asm volatile("bar.sync %0, 64;" ::"r"(2 + blk * 4 + (warp & 3)) : "memory");
+        l = xch[col] + xch[CB + col];
         if (ok && !wait_ns(pv_done + blk, (n_tiles - 1) & 1)) ok = false;
         fence_after();
         // ---- output ---------------------------------------------------------------------------------
@@ -405,7 +546,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
         const float e0 = __uint_as_float((uint32_t)(127 - 13) << 23), e1 = __uint_as_float((uint32_t)(127 + ev) << 23);
         const size_t slot = (seg * nsplit + sp) * CB + col;
 #pragma unroll 1
-        for (int d = 0; d < D; d += 16) {
+        for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 16) {
             float o[16];
             ld16(tm + P::TO + d, o);
             wait_ld();
@@ -426,98 +567,30 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
                 }
             }
         }
-        if (ok && c < C) {
+        if (ok && c < C && half == 0) {
             if (nsplit == 1) {
                 if (a.lse) a.lse[lse_at] = has ? (log2f(l) - nm) * LN2 : -INFINITY;
             } else {
                 pml[slot] = make_float2(l != 0.f ? -nm : M0, l);
             }
         }
-    } else if (warp < PW0 + 4) {
-        // ---- producers: packed rows -> operands ----------------------------------------------------
-        const int key = pt & 63, g = D == 128 ? pt >> 6 : 0, half = D == 128 ? 0 : pt >> 6;  // D = 64: half a row each
-        constexpr int WPT = D == 128 ? 8 : 4;  // words per thread
-        const __half2 k1024 = __float2half2_rn(1024.f);
-        const float dn = __uint_as_float((uint32_t)(127 + 13 - max(ev, -100)) << 23);
-        for (int i = 0; i < n_tiles; ++i) {
-            cp_async_wait<STAGES - 2>();
-            asm volatile("bar.sync 1, 128;" ::: "memory");  // every producer's pieces have landed, and all have left the stage to be refilled
-            fetch(i + STAGES - 1);
-            const unsigned char* pk = sm + P::PACK + (i % STAGES) * P::PACKB;
-            const int kpos = (t0 + i) * KT + key;
-            const bool valid = kpos < T;  // rows past the last key may hold anything in their scales
-            uint32_t w[WPT];
-            {
-                const uint4* p = reinterpret_cast<const uint4*>(pk + key * (D / 2) + g * 32 + half * 16);
-#pragma unroll
-                for (int j = 0; j < WPT / 4; ++j) {
-                    const uint4 u = p[j];
-                    w[4 * j] = u.x;
-                    w[4 * j + 1] = u.y;
-                    w[4 * j + 2] = u.z;
-                    w[4 * j + 3] = u.w;
-                }
-            }
-            const uint16_t* sc = reinterpret_cast<const uint16_t*>(pk + 2 * P::PW) + key * GR + g;
-            float ks = valid ? u16_to_f(sc[0]) : 0.f, kz = valid ? u16_to_f(sc[P::PS / 2]) : 0.f;
-            float vs = valid ? u16_to_f(sc[P::PS]) : 0.f, vz = valid ? u16_to_f(sc[3 * P::PS / 2]) : 0.f;
-            if (!(fabsf(vs) < INFINITY) || !(fabsf(vz) < INFINITY)) {
-                // a NaN in V reaches the rows that see the key through its score, and no other row
-                kz = vs + vz + INFINITY - INFINITY;
-                vs = vz = 0.f;
-            }
-            if (ok && i > 1 && !wait_ns(k_free + (i & 1), ((i - 2) >> 1) & 1)) ok = false;
-            unsigned char* kd = sm + P::K + (i & 1) * P::OPB + g * KT * 128;
-#pragma unroll
-            for (int j = 0; j < WPT; ++j)
-                *reinterpret_cast<uint4*>(kd + chunk_at(key, half * 4 + j)) =
-                    make_uint4(nib_even(w[j]), nib_odd(w[j]), nib_even(w[j] >> 8), nib_odd(w[j] >> 8));
-            if (half == 0) {
-                float* tab = reinterpret_cast<float*>(sm + P::TAB) + (i % TABS) * 2 * GR * KT + g * KT + key;
-                tab[0] = ks;
-                tab[GR * KT] = kz;
-            }
-            fence_proxy_async_smem();
-            arrive(k_full + (i & 1));
-            {
-                const uint4* p = reinterpret_cast<const uint4*>(pk + P::PW + key * (D / 2) + g * 32 + half * 16);
-#pragma unroll
-                for (int j = 0; j < WPT / 4; ++j) {
-                    const uint4 u = p[j];
-                    w[4 * j] = u.x;
-                    w[4 * j + 1] = u.y;
-                    w[4 * j + 2] = u.z;
-                    w[4 * j + 3] = u.w;
-                }
-            }
-            const __half2 s2 = __float2half2_rn(vs * dn), z2 = __float2half2_rn(vz * dn);
-            if (ok && i > 1 && !wait_ns(v_free + (i & 1), ((i - 2) >> 1) & 1)) ok = false;
-            unsigned char* vd = sm + P::V + (i & 1) * P::OPB + g * KT * 128;
-#pragma unroll
-            for (int j = 0; j < WPT; ++j) {
-                uint32_t o[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    o[e] = as_u(__hfma2(__hsub2(as_h2(((w[j] >> (4 * e)) & 0x000F000Fu) | 0x64006400u), k1024), s2, z2));
-                *reinterpret_cast<uint4*>(vd + chunk_at(key, half * 4 + j)) = make_uint4(o[0], o[1], o[2], o[3]);
-            }
-            fence_proxy_async_smem();
-            arrive(v_full + (i & 1));
-        }
-        cp_async_wait<0>();
-    } else if (lane == 0) {
+    } else {
         // ---- products ------------------------------------------------------------------------------------
-        const uint32_t qb = smem_u32(sm + P::Q), kb = smem_u32(sm + P::K), vb = smem_u32(sm + P::V);
-        auto scores = [&](int blk, int i) {  // S of tile i; the arrival passes on what the producers wrote
+        const uint32_t lead = lane == 0 ? 1u : 0u;
+        const uint32_t qa = smem_u32(sm + P::Q), ka = smem_u32(sm + P::K);
+        const uint64_t qd = desc(qa, 16), kd = desc(ka, 16), vd = desc(smem_u32(sm + P::V), KT * 128);
+        const uint64_t qx = desc16(qa + GR * CM * 128), kx = desc16(ka + GR * KT * 128);
+        // descriptor of an operand `bytes` further on (shared addresses stay below the field's end)
+        auto at = [](uint64_t d, uint32_t bytes) { return d + (bytes >> 4); };
+        auto scores = [&](int blk, int i) {  // S of tile i
+            const uint32_t qo = blk * P::QB, ko = (i & 1) * P::KB, d = tmem + blk * P::TB;
 #pragma unroll
-            for (int g = 0; g < GR; ++g)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    mma_ss(tmem + blk * P::TB + g * KT, desc(qb + (blk * GR + g) * CM * 128 + 32 * k, 16),
-                           desc(kb + (i & 1) * P::OPB + g * KT * 128 + 32 * k, 16), idesc(KT, false), k != 0 ? 1u : 0u);
-            commit(s_full + blk);
-            arrive(s_full + blk);
-            if (blk == NB - 1) commit(k_free + (i & 1));
+            for (int k = 0; k < D / 16; ++k)
+                mma_ss(d, at(qd, qo + (k >> 2) * CM * 128 + 32 * (k & 3)), at(kd, ko + (k >> 2) * KT * 128 + 32 * (k & 3)), idesc(KT, false),
+                       k != 0 ? 1u : 0u, lead);
+            mma_ss(d, at(qx, qo), at(kx, ko), idesc(KT, false), 1u, lead);
+            commit(s_full + blk, lead);
+            if (blk == NB - 1) commit(k_free + (i & 1), lead);
         };
         if (!wait_ns(k_full, 0)) ok = false;
         if (ok) {
@@ -527,6 +600,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
         }
         for (int i = 0; i < n_tiles && ok; ++i) {
             if (!wait_ns(v_full + (i & 1), (i >> 1) & 1)) ok = false;
+            const uint32_t vo = (i & 1) * P::VB;
 #pragma unroll
             for (int blk = 0; blk < NB; ++blk) {
                 if (ok && !wait_ns(p_full + blk, i & 1)) ok = false;
@@ -534,11 +608,11 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
                 fence_after();
 #pragma unroll
                 for (int k = 0; k < KT / 16; ++k)
-                    mma_ts(tmem + blk * P::TB + P::TO, tmem + blk * P::TB + 8 * k, desc(vb + (i & 1) * P::OPB + 16 * 128 * k, KT * 128),
-                           idesc(D, true), (i | k) != 0 ? 1u : 0u);
-                commit(pv_done + blk);
-                if (blk == NB - 1) commit(v_free + (i & 1));
-                if (i + 1 < n_tiles) {  // S_0 holds P until its product is done
+                    mma_ts(tmem + blk * P::TB + P::TO, tmem + blk * P::TB + 8 * k, at(vd, vo + 16 * 128 * k), idesc(D, true),
+                           (i | k) != 0 ? 1u : 0u, lead);
+                commit(pv_done + blk, lead);
+                if (blk == NB - 1) commit(v_free + (i & 1), lead);
+                if (i + 1 < n_tiles) {  // S holds P until its product is done
                     if ((blk == 0 && !wait_ns(k_full + ((i + 1) & 1), ((i + 1) >> 1) & 1)) || !wait_ns(pv_done + blk, i & 1)) {
                         ok = false;
                         break;
@@ -548,11 +622,12 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
                 }
             }
         }
+        ok = __all_sync(0xffffffffu, ok);
     }
     if (!ok && a.err) atomicOr(a.err, (int)QW_DERR_TIMEOUT);
     fence_before();
     __syncthreads();
-    if (warp == PW0 + 4) {
+    if (warp == PW0) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P::TMEM) : "memory");
     }
@@ -621,12 +696,12 @@ TcShape kv4_tc_shape(const Kv4View& c, int S, int Hq, int num_sms) {
     TcShape s;
     s.nb = C > CM ? 2 : 1;
     s.ncb = (int)((C + CM * s.nb - 1) / (CM * s.nb));
-    // splits of the keys: fill rounds of one block per SM, at least four tiles each if the cache were
+    // splits of the keys: fill rounds of one block per SM, at least two tiles each if the cache were
     // full; a split costs a partial's write and read, counted as a tenth of a round
     const long long segs = (long long)s.ncb * c.heads * c.batch;
     s.nsplit = 1;
     float best = 1e30f;
-    for (int n = 1; n <= 64 && (n == 1 || n * 4 * KT <= c.max_pos); ++n) {
+    for (int n = 1; n <= 64 && (n == 1 || n * 2 * KT <= c.max_pos); ++n) {
         const float t = (float)((segs * n + num_sms - 1) / num_sms) / n * (1.f + 0.1f * (n - 1));
         if (t < best) {
             best = t;
