@@ -44,7 +44,6 @@ constexpr int THREADS = 256 * NB + 32;
 constexpr float BASE = 11.f;          // P = 2^(x - max + 11)
 constexpr float RAISE = BASE + 4.f;   // a larger exponent raises the maximum
 constexpr float UNSET = -3.0e38f;
-constexpr unsigned long long TIMEOUT_NS = 2000000000ull;
 
 // Shared memory, from a 1 KB aligned base.
 template <int D, int NB>
@@ -59,30 +58,19 @@ struct Plan {
     static constexpr uint32_t TO = KT, TB = KT + D, TMEM = NB * TB <= 256 ? 256 : 512;
 };
 
-QW_DEV unsigned long long now_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-QW_DEV bool wait_ns(uint64_t* bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const unsigned long long t0 = now_ns();
-    while (!mbar_try_wait(bar, parity))
-        if (now_ns() - t0 > TIMEOUT_NS) return false;
-    return true;
-}
+// Bounded wait: every poll suspends for a while, 2^22 of them are far beyond any tile's time.
+QW_DEV bool wait_bar(uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity); }
 QW_DEV void arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 QW_DEV void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 QW_DEV void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // The product warp runs as a whole, so that its control flow and descriptors stay in uniform
-// registers; `lead` picks the one lane that issues.
-QW_DEV void commit(uint64_t* bar, uint32_t lead) {
+// registers; one elected lane issues.
+QW_DEV void commit(uint64_t* bar) {
     asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
-        "r"(lead)
+        "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar))
         : "memory");
 }
 // 128-byte-swizzled operand rows of 64 fp16: descriptor version 1, 1 KB between 8-row groups; along_keys:
@@ -100,18 +88,16 @@ QW_DEV uint32_t at16(int row, int khalf) { return (uint32_t)(row >> 3) * 256 + k
 __host__ __device__ constexpr uint32_t idesc(int n, bool b_along_n) {
     return (1u << 4) | (b_along_n ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(CM >> 4) << 24);
 }
-QW_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate, uint32_t lead) {
+QW_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate),
-        "r"(lead)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate)
         : "memory");
 }
-QW_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate, uint32_t lead) {
+QW_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate),
-        "r"(lead)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate)
         : "memory");
 }
 QW_DEV void ld16(uint32_t addr, float (&v)[16]) {
@@ -349,18 +335,29 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
         auto packed = [&](const unsigned char* base, int key) {
             return GR == 2 ? *reinterpret_cast<const uint32_t*>(base + (size_t)key * 4) : (uint32_t)*reinterpret_cast<const uint16_t*>(base + (size_t)key * 2);
         };
+        // A block-wide base and a 32-bit offset of the thread's own each.
+        const uint32_t po = (uint32_t)tid, so = (uint32_t)(tid / CPR * GR + ((tid % CPR) >> 1));
+        constexpr uint32_t PSTEP = NTH, SSTEP = NTH / CPR * GR;
         auto load = [&](Share& x, int which, int i) {  // zeros past the last key
             const int k0 = (t0 + i) * KT;
             const uint4* src = reinterpret_cast<const uint4*>(rows.w[which] + (size_t)k0 * (D / 2));
             const uint16_t* s = reinterpret_cast<const uint16_t*>(rows.s[which]) + (size_t)k0 * GR;
             const uint16_t* z = reinterpret_cast<const uint16_t*>(rows.b[which]) + (size_t)k0 * GR;
+            if (k0 + KT <= T && (PIECES >= NTH || has_piece)) {
 #pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const int p = tid + NTH * j, at = p / CPR * GR + ((p % CPR) >> 1);
-                const bool in = has_piece && k0 + p / CPR < T;
-                x.w[j] = in ? src[p] : make_uint4(0u, 0u, 0u, 0u);
-                x.s[j] = in ? s[at] : (uint16_t)0;
-                if (which) x.z[j] = in ? z[at] : (uint16_t)0;
+                for (uint32_t j = 0; j < PER; ++j) {
+                    x.w[j] = src[po + PSTEP * j];
+                    x.s[j] = s[so + SSTEP * j];
+                    if (which) x.z[j] = z[so + SSTEP * j];
+                }
+                return;
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < PER; ++j) {
+                const bool in = has_piece && k0 + (tid + NTH * (int)j) / CPR < T;
+                x.w[j] = in ? src[po + PSTEP * j] : make_uint4(0u, 0u, 0u, 0u);
+                x.s[j] = in ? s[so + SSTEP * j] : (uint16_t)0;
+                if (which) x.z[j] = in ? z[so + SSTEP * j] : (uint16_t)0;
             }
         };
         auto load_k = [&](int i) {
@@ -387,7 +384,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
         };
         auto store_k = [&](int i) {  // tile i's K operand from ks, cs, cz
             if (i >= n_tiles) return;
-            if (ok && i > 1 && !wait_ns(k_free + (i & 1), ((i - 2) >> 1) & 1)) ok = false;
+            if (ok && i > 1 && !wait_bar(k_free + (i & 1), ((i - 2) >> 1) & 1)) ok = false;
             unsigned char* dst = sm + P::K + (i & 1) * P::KB;
             const __half2 k1032 = __float2half2_rn(1032.f);
             if (has_piece)
@@ -423,12 +420,10 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
                     *reinterpret_cast<uint4*>(dst + GR * KT * 128 + at16(tid, e)) = make_uint4(r[0], r[1], r[2], r[3]);
                 }
             }
-            fence_proxy_async_smem();
-            arrive(k_full + (i & 1));
         };
         auto store_v = [&](int i) {
             if (i >= n_tiles) return;
-            if (ok && i > 1 && !wait_ns(v_free + (i & 1), ((i - 2) >> 1) & 1)) ok = false;
+            if (ok && i > 1 && !wait_bar(v_free + (i & 1), ((i - 2) >> 1) & 1)) ok = false;
             unsigned char* dst = sm + P::V + (i & 1) * P::VB;
             const __half2 k1024 = __float2half2_rn(1024.f);
             if (has_piece)
@@ -439,22 +434,27 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
                     const __half2 s2 = __float2half2_rn(s * vup), z2 = __float2half2_rn(z * vup);
                     expand(vs.w[j], tid + NTH * j, dst, [&](uint32_t n) { return as_u(__hfma2(__hsub2(as_h2(n), k1024), s2, z2)); });
                 }
-            fence_proxy_async_smem();
-            arrive(v_full + (i & 1));
         };
-        fence_proxy_async_smem();  // the Q operand (published with the first tile's)
+        // Stores first, then one fence, then the loads: a fence waits for the thread's loads in flight.
+        auto publish = [&](int ik, int iv) {
+            fence_proxy_async_smem();
+            if (iv < n_tiles) arrive(v_full + (iv & 1));
+            if (ik < n_tiles) arrive(k_full + (ik & 1));
+        };
         load_k(0);
         load_v(0);
         store_k(0);
-        load_k(1);
         store_v(0);
+        publish(0, 0);  // and the Q operand
+        load_k(1);
         load_v(1);
         store_k(1);
+        publish(1, n_tiles);
         load_k(2);
 
         float nm = 0.f, l = 0.f, thr = UNSET;  // BASE - maximum; up to thr the maximum stays
         for (int i = 0; i < n_tiles; ++i) {
-            if (ok && !wait_ns(s_full + blk, i & 1)) ok = false;
+            if (ok && !wait_bar(s_full + blk, i & 1)) ok = false;
             fence_after();
             // Two rounds of 64 keys, 32 of them this thread's.  P of a round lies over columns of S that this
             // round or the one before has read; the two warps of the column meet after each read.
@@ -531,14 +531,15 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
             fence_before();
             arrive(p_full + blk);
             store_v(i + 1);
-            load_v(i + 2);
             store_k(i + 2);
+            publish(i + 2, i + 1);
+            load_v(i + 2);
             load_k(i + 3);
         }
         xch[half * CB + col] = l;
         asm volatile("bar.sync %0, 64;" ::"r"(2 + blk * 4 + (warp & 3)) : "memory");
         l = xch[col] + xch[CB + col];
-        if (ok && !wait_ns(pv_done + blk, (n_tiles - 1) & 1)) ok = false;
+        if (ok && !wait_bar(pv_done + blk, (n_tiles - 1) & 1)) ok = false;
         fence_after();
         // ---- output ---------------------------------------------------------------------------------
         const bool has = row && l != 0.f;
@@ -576,7 +577,6 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
         }
     } else {
         // ---- products ------------------------------------------------------------------------------------
-        const uint32_t lead = lane == 0 ? 1u : 0u;
         const uint32_t qa = smem_u32(sm + P::Q), ka = smem_u32(sm + P::K);
         const uint64_t qd = desc(qa, 16), kd = desc(ka, 16), vd = desc(smem_u32(sm + P::V), KT * 128);
         const uint64_t qx = desc16(qa + GR * CM * 128), kx = desc16(ka + GR * KT * 128);
@@ -587,33 +587,33 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
                 mma_ss(d, at(qd, qo + (k >> 2) * CM * 128 + 32 * (k & 3)), at(kd, ko + (k >> 2) * KT * 128 + 32 * (k & 3)), idesc(KT, false),
-                       k != 0 ? 1u : 0u, lead);
-            mma_ss(d, at(qx, qo), at(kx, ko), idesc(KT, false), 1u, lead);
-            commit(s_full + blk, lead);
-            if (blk == NB - 1) commit(k_free + (i & 1), lead);
+                       k != 0 ? 1u : 0u);
+            mma_ss(d, at(qx, qo), at(kx, ko), idesc(KT, false), 1u);
+            commit(s_full + blk);
+            if (blk == NB - 1) commit(k_free + (i & 1));
         };
-        if (!wait_ns(k_full, 0)) ok = false;
+        if (!wait_bar(k_full, 0)) ok = false;
         if (ok) {
             fence_after();
 #pragma unroll
             for (int blk = 0; blk < NB; ++blk) scores(blk, 0);
         }
         for (int i = 0; i < n_tiles && ok; ++i) {
-            if (!wait_ns(v_full + (i & 1), (i >> 1) & 1)) ok = false;
+            if (!wait_bar(v_full + (i & 1), (i >> 1) & 1)) ok = false;
             const uint32_t vo = (i & 1) * P::VB;
 #pragma unroll
             for (int blk = 0; blk < NB; ++blk) {
-                if (ok && !wait_ns(p_full + blk, i & 1)) ok = false;
+                if (ok && !wait_bar(p_full + blk, i & 1)) ok = false;
                 if (!ok) break;
                 fence_after();
 #pragma unroll
                 for (int k = 0; k < KT / 16; ++k)
                     mma_ts(tmem + blk * P::TB + P::TO, tmem + blk * P::TB + 8 * k, at(vd, vo + 16 * 128 * k), idesc(D, true),
-                           (i | k) != 0 ? 1u : 0u, lead);
-                commit(pv_done + blk, lead);
-                if (blk == NB - 1) commit(v_free + (i & 1), lead);
+                           (i | k) != 0 ? 1u : 0u);
+                commit(pv_done + blk);
+                if (blk == NB - 1) commit(v_free + (i & 1));
                 if (i + 1 < n_tiles) {  // S holds P until its product is done
-                    if ((blk == 0 && !wait_ns(k_full + ((i + 1) & 1), ((i + 1) >> 1) & 1)) || !wait_ns(pv_done + blk, i & 1)) {
+                    if ((blk == 0 && !wait_bar(k_full + ((i + 1) & 1), ((i + 1) >> 1) & 1)) || !wait_bar(pv_done + blk, i & 1)) {
                         ok = false;
                         break;
                     }
