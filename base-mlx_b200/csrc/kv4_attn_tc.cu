@@ -17,7 +17,7 @@
 // the bound: 309 us for 1024 rows of 32 heads on 8192 keys.)  K and V are taken
 // times powers of two that put the block's largest value (found first, from
 // scales and biases alone) where fp16 holds it; the running maximum moves only
-// when a score passes it by 2^4 (P <= 2^15), and then O is rescaled in TMEM.
+// when a score passes it by 2^8 (P <= 2^15), and then O is rescaled in TMEM.
 //
 // Roles: one lane of the last warp issues the products; all other warps, two
 // threads per column with half a tile's keys each, do the softmax and between two
@@ -41,8 +41,8 @@ constexpr int CM = 128;      // columns of a column block
 constexpr int KT = 128;      // keys of a tile
 template <int NB>
 constexpr int THREADS = 256 * NB + 32;
-constexpr float BASE = 11.f;          // P = 2^(x - max + 11)
-constexpr float RAISE = BASE + 4.f;   // a larger exponent raises the maximum
+constexpr float BASE = 7.f;           // P = 2^(x - max + 7): normal fp16 numbers down to 2^-21 of the largest
+constexpr float RAISE = BASE + 8.f;   // a larger exponent raises the maximum
 constexpr float UNSET = -3.0e38f;
 
 // Shared memory, from a 1 KB aligned base.
@@ -130,6 +130,11 @@ QW_DEV uint32_t as_u(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h);
 // 16-byte chunk c of a swizzled operand row.  A word fills one chunk, its elements in the order 0, 4, 1, 5, 2, 6, 3, 7.
 QW_DEV uint32_t chunk_at(int row, int c) { return (uint32_t)row * 128 + (uint32_t)((c ^ (row & 7)) << 4); }
 
+QW_DEV float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 QW_DEV unsigned long long pack2(float lo, float hi) {
     unsigned long long r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
@@ -474,7 +479,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
                         if (key0 + k >= vis) x[k] = -INFINITY;
                 float top = -INFINITY;
 #pragma unroll
-                for (int k = 0; k < KH; ++k) top = fmaxf(top, x[k]);
+                for (int k = 0; k < KH; k += 2) top = max3(top, x[k], x[k + 1]);
                 xch[(2 * m + half) * CB + col] = top;
                 asm volatile("bar.sync %0, 64;" ::"r"(2 + blk * 4 + (warp & 3)) : "memory");
                 top = fmaxf(top, xch[(2 * m + (half ^ 1)) * CB + col]);
