@@ -14,7 +14,9 @@
 // contiguous shares of that list, whatever the lengths, so a ragged batch and
 // one long sequence both fill the GPU.  A segment inside one share is finished
 // there; one that spans shares leaves a partial (base exponent, sum, output) per
-// share, which a second kernel joins.
+// share, which a second kernel joins.  Caches so short that a cluster of blocks
+// holds a segment in a few tiles per warp skip the list and join in the cluster.
+#include "kv4_join.cuh"
 #include "kv4_tc.h"
 #include "kv4_tile.cuh"
 #include "smem_attr.h"
@@ -26,6 +28,20 @@ using namespace kv4;
 
 constexpr int AW = 8, ANT = 32 * AW;  // warps and threads of a block
 constexpr int ASTAGES = 3;            // tiles of a warp's load ring
+constexpr int MAX_CLUSTER = 8;
+
+QW_DEV void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
+// The pair of floats at `p` in the cluster's block `rank`.
+QW_DEV float2 cluster_load2(const float* p, int rank) {
+    uint32_t addr;
+    float2 v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
 
 // Scratch: [0] tiles per share, [1 + b] first tile of sequence b; then the
 // partials [2 shares][columns][D] and their (base exponent, sum); then the lse of a
@@ -175,91 +191,74 @@ QW_DEV Share take_share(const Kv4AttnArgs& a, int ncb, int* plan) {
 
 template <int D, int NT>
 struct SplitSmem {
+    static constexpr int CB = 8 * NT;
     static constexpr int RING = AW * ASTAGES * Tile<D>::BYTES;
     static constexpr int OLD = D + 2;  // output row of a warp's merge buffer, floats
-    static constexpr int MERGE = AW * 8 * NT * OLD * 4;
-    static constexpr int BYTES = (RING > MERGE ? RING : MERGE) + AW * 8 * NT * 8;
+    static constexpr int MERGE = AW * CB * OLD * 4, BLOCK = CB * (D * 4 + 8);  // + the block's own sums (cluster form)
+    static constexpr int BYTES = (RING > MERGE + BLOCK ? RING : MERGE + BLOCK) + AW * CB * 8;
 };
 
-// The eight warps take a segment's tiles in turn, each with its own columns'
-// state and its own ring of tiles (cp.async, so no warp waits for another),
-// and are merged through shared memory at the end of the segment.
+// This warp's tiles first, first + step, ... below t1 of column block cb of (b, h):
+// every warp has its own columns' state and its own ring of
+// tiles (cp.async, so no warp waits for another).  Leaves (base exponent, sum) of every warp and column in
+// wml and the warps' outputs, relative to the block's base, in wo.
 template <int D, int NT>
-__global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(const Kv4AttnArgs a, int ncb, int* plan,
-                                                                              float* part, float2* pml) {
+QW_DEV void run_tiles(const Kv4AttnArgs& a, const Kv4Rows& rw, int b, int h, int cb, int first, int step, int t1, unsigned char* smem) {
     using L = Tile<D>;
     using SM = SplitSmem<D, NT>;
-    constexpr int CB = 8 * NT;
-    extern __shared__ __align__(128) unsigned char smem[];
+    constexpr int CB = SM::CB;
     float2* wml = reinterpret_cast<float2*>(smem + SM::BYTES - AW * CB * 8);  // [warp][column]
     float* wo = reinterpret_cast<float*>(smem);                               // [warp][column][OLD]
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int G = a.Hq / a.c.heads, C = G * a.S;
-    pdl_launch_dependents();  // the joining kernel's blocks may settle in; they wait for this kernel's end
-    const Share sh = take_share(a, ncb, plan);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int G = a.Hq / a.c.heads, C = G * a.S, T = rw.off + rw.n;
     const uint32_t ring = smem_u32(smem) + warp * ASTAGES * L::BYTES;
     const unsigned char* ringp = smem + warp * ASTAGES * L::BYTES;
+    const Rows rows = head_rows<D>(a.c, (size_t)b * a.c.heads + h);
+    const int mine = max(0, (t1 - first + step - 1) / step);
+    auto issue = [&](int k) {
+        if (k < mine) load_tile<D>(ring + (k % ASTAGES) * L::BYTES, rows, (first + k * step) * TK, T, lane);
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int k = 0; k < ASTAGES - 1; ++k) issue(k);
 
-    int u = sh.begin, b0 = sh.b0, b = sh.b;
-    while (u < sh.end) {
-        const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
-        const int T = rw.off + rw.n, nt = tiles_of(rw);
-        const int nseq = nt * a.c.heads * ncb;
-        if (u >= b0 + nseq) {  // the next sequence (some are empty)
-            b0 += nseq;
-            ++b;
-            continue;
+    Cols<D, NT> cols;
+    State<D, NT> st;
+    st.init();
+    int vis[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int c = cb * CB + 8 * n + g, i = c / G;
+        const bf16* src = mine > 0 && c < C && i < rw.n ? a.q + (b * a.qs.b + i * a.qs.s + (h * G + c % G) * a.qs.h) : nullptr;
+        load_cols<D, NT>(cols, n, src, a.scale, lane);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int ci = (cb * CB + 8 * n + 2 * t + e) / G;
+            vis[n][e] = a.causal ? min(T, rw.off + ci + 1) : T;
         }
-        const int seg = (u - b0) / nt, t0 = (u - b0) % nt;
-        const int t1 = min(nt, t0 + (sh.end - u));
-        const int h = seg / ncb, cb = seg % ncb;
-        const Rows rows = head_rows<D>(a.c, (size_t)b * a.c.heads + h);
-
-        const int mine = max(0, (t1 - t0 - warp + AW - 1) / AW);  // tiles t0 + warp, t0 + warp + 8, ...
-        auto issue = [&](int k) {
-            if (k < mine)
-                load_tile<D>(ring + (k % ASTAGES) * L::BYTES, rows, (t0 + warp + k * AW) * TK, T, lane);
-            cp_async_commit();
-        };
+    }
+    const int all = a.causal ? min(T, rw.off + cb * CB / G + 1) : T;  // keys that every column sees
+    for (int k = 0; k < mine; ++k) {
+        cp_async_wait<ASTAGES - 2>();
+        __syncwarp();
+        issue(k + ASTAGES - 1);  // into the stage that the warp left in the turn before
+        const int key0 = (first + k * step) * TK;
+        const unsigned char* tile = ringp + (k % ASTAGES) * L::BYTES;
+        if (key0 + TK <= all)
+            attend_tile<D, NT, false>(st, cols, tile, key0, T, vis, lane);
+        else
+            attend_tile<D, NT, true>(st, cols, tile, key0, T, vis, lane);
+        __syncwarp();
+    }
+    cp_async_wait<0>();
+    if (mine > 0) reduce_lanes(st);
+    if (g == 0)
 #pragma unroll
-        for (int k = 0; k < ASTAGES - 1; ++k) issue(k);
-
-        Cols<D, NT> cols;
-        State<D, NT> st;
-        st.init();
-        int vis[NT][2];
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int c = cb * CB + 8 * n + g, i = c / G;
-            const bf16* src = c < C && i < rw.n ? a.q + (b * a.qs.b + i * a.qs.s + (h * G + c % G) * a.qs.h) : nullptr;
-            load_cols<D, NT>(cols, n, src, a.scale, lane);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int ci = (cb * CB + 8 * n + 2 * t + e) / G;
-                vis[n][e] = a.causal ? min(T, rw.off + ci + 1) : T;
-            }
-        }
-        const int all = a.causal ? min(T, rw.off + cb * CB / G + 1) : T;  // keys that every column sees
-        for (int k = 0; k < mine; ++k) {
-            cp_async_wait<ASTAGES - 2>();
-            __syncwarp();
-            issue(k + ASTAGES - 1);  // into the stage that the warp left in the turn before
-            const int key0 = (t0 + warp + k * AW) * TK;
-            const unsigned char* tile = ringp + (k % ASTAGES) * L::BYTES;
-            if (key0 + TK <= all)
-                attend_tile<D, NT, false>(st, cols, tile, key0, T, vis, lane);
-            else
-                attend_tile<D, NT, true>(st, cols, tile, key0, T, vis, lane);
-            __syncwarp();
-        }
-        cp_async_wait<0>();
-        reduce_lanes(st);
-        if (g == 0)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) wml[warp * CB + 8 * n + 2 * t + e] = make_float2(-st.nm[n][e], st.l[n][e]);
-        __syncthreads();  // also: every warp has left its ring
+            for (int e = 0; e < 2; ++e) wml[warp * CB + 8 * n + 2 * t + e] = make_float2(-st.nm[n][e], st.l[n][e]);
+    __syncthreads();  // also: every warp has left its ring
+    if (mine > 0)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -278,32 +277,73 @@ __global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(co
                         *reinterpret_cast<float2*>(dst + 64 * gr + 32 * (i >> 1) + 2 * (i & 1)) = make_float2(v.x * f * f, v.y * f * f);
                     }
             }
-        __syncthreads();
+    __syncthreads();
+}
+
+// Sum over the block's warps of column col, dimensions d, d + 1 (warps whose base is M0 have written nothing).
+template <int D, int NT>
+QW_DEV float2 warps_sum(const unsigned char* smem, int col, int d, float& M, float& l) {
+    using SM = SplitSmem<D, NT>;
+    const float2* wml = reinterpret_cast<const float2*>(smem + SM::BYTES - AW * SM::CB * 8);
+    const float* wo = reinterpret_cast<const float*>(smem);
+    M = wml[col].x;
+#pragma unroll
+    for (int w = 1; w < AW; ++w) M = fmaxf(M, wml[w * SM::CB + col].x);
+    l = 0.f;
+    float2 o = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < AW; ++w) {
+        const float2 ml = wml[w * SM::CB + col];
+        if (ml.x == M0) continue;
+        const float f = half_pow(ml.x - M);
+        l = fmaf(ml.y * f, f, l);
+        const float2 v = *reinterpret_cast<const float2*>(wo + (w * SM::CB + col) * SM::OLD + d);
+        o.x += v.x;
+        o.y += v.y;
+    }
+    return o;
+}
+
+// Output of column c, dimensions d, d + 1, from its sums.
+QW_DEV void write_out(const Kv4AttnArgs& a, const Kv4Rows& rw, int b, int h, int c, int d, float2 o, float M, float l) {
+    const int G = a.Hq / a.c.heads, i = c / G;
+    const bool has = i < rw.n && l != 0.f;
+    const float inv = has ? 1.f / l : 0.f;
+    bf16* dst = a.out + (b * a.os.b + i * a.os.s + (h * G + c % G) * a.os.h) + d;
+    *reinterpret_cast<uint32_t*>(dst) = has ? pack_bf16x2(o.x * inv, o.y * inv) : 0u;
+    if (d == 0 && a.lse) a.lse[((size_t)b * a.S + i) * a.Hq + h * G + c % G] = has ? (M + log2f(l)) * LN2 : -INFINITY;
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(const Kv4AttnArgs a, int ncb, int* plan, float* part, float2* pml) {
+    constexpr int CB = 8 * NT;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int tid = threadIdx.x, C = a.Hq / a.c.heads * a.S;
+    pdl_launch_dependents();  // the joining kernel's blocks may settle in; they wait for this kernel's end
+    const Share sh = take_share(a, ncb, plan);
+    int u = sh.begin, b0 = sh.b0, b = sh.b;
+    while (u < sh.end) {
+        const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
+        const int nt = tiles_of(rw);
+        const int nseq = nt * a.c.heads * ncb;
+        if (u >= b0 + nseq) {  // the next sequence (some are empty)
+            b0 += nseq;
+            ++b;
+            continue;
+        }
+        const int seg = (u - b0) / nt, t0 = (u - b0) % nt;
+        const int t1 = min(nt, t0 + (sh.end - u));
+        const int h = seg / ncb, cb = seg % ncb;
+        run_tiles<D, NT>(a, rw, b, h, cb, t0 + (tid >> 5), AW, t1, smem);
         const bool whole = t0 == 0 && t1 == nt;
         const size_t slot = 2 * (size_t)blockIdx.x + (u == sh.begin ? 0 : 1);
         for (int idx = tid; idx < CB * (D / 2); idx += ANT) {
-            const int col = idx / (D / 2), d = 2 * (idx % (D / 2)), c = cb * CB + col, i = c / G;
+            const int col = idx / (D / 2), d = 2 * (idx % (D / 2)), c = cb * CB + col;
             if (c >= C) break;
-            float M = wml[col].x, l = 0.f;
-#pragma unroll
-            for (int w = 1; w < AW; ++w) M = fmaxf(M, wml[w * CB + col].x);
-            float2 o = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < AW; ++w) {
-                const float2 ml = wml[w * CB + col];
-                const float f = half_pow(ml.x - M);
-                l = fmaf(ml.y * f, f, l);
-                const float2 v = *reinterpret_cast<const float2*>(wo + (w * CB + col) * SM::OLD + d);
-                o.x += v.x;
-                o.y += v.y;
-            }
+            float M, l;
+            const float2 o = warps_sum<D, NT>(smem, col, d, M, l);
             if (whole) {
-                const bool has = i < rw.n && l != 0.f;
-                const float inv = has ? 1.f / l : 0.f;
-                bf16* dst = a.out + (b * a.os.b + i * a.os.s + (h * G + c % G) * a.os.h) + d;
-                *reinterpret_cast<uint32_t*>(dst) = has ? pack_bf16x2(o.x * inv, o.y * inv) : 0u;
-                if (d == 0 && a.lse)
-                    a.lse[((size_t)b * a.S + i) * a.Hq + h * G + c % G] = has ? (M + log2f(l)) * LN2 : -INFINITY;
+                write_out(a, rw, b, h, c, d, o, M, l);
             } else {
                 *reinterpret_cast<float2*>(part + (slot * CB + col) * D + d) = o;
                 if (d == 0) pml[slot * CB + col] = make_float2(M, l);
@@ -314,13 +354,69 @@ __global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(co
     }
 }
 
+// Short caches: a cluster of `cluster` blocks takes a whole segment, tile k by block k % cluster, and joins
+// through distributed shared memory -- one launch and no partials in memory.
+template <int D, int NT>
+__global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_cluster_kernel(const Kv4AttnArgs a, int ncb, int cluster) {
+    using SM = SplitSmem<D, NT>;
+    constexpr int CB = SM::CB;
+    extern __shared__ __align__(128) unsigned char smem[];
+    float* bo = reinterpret_cast<float*>(smem + SM::MERGE);       // [column][D] of this block
+    float2* bml = reinterpret_cast<float2*>(bo + CB * D);         // [column]
+    pdl_launch_dependents();
+    const int tid = threadIdx.x, C = a.Hq / a.c.heads * a.S;
+    const int rank = blockIdx.x % cluster, seg = blockIdx.x / cluster;
+    const int cb = seg % ncb, h = seg / ncb % a.c.heads, b = seg / ncb / a.c.heads;
+    const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, a.err, rank == 0 && h == 0 && cb == 0 && tid == 0);
+    run_tiles<D, NT>(a, rw, b, h, cb, (tid >> 5) * cluster + rank, AW * cluster, tiles_of(rw), smem);
+    for (int idx = tid; idx < CB * (D / 2); idx += ANT) {
+        const int col = idx / (D / 2), d = 2 * (idx % (D / 2)), c = cb * CB + col;
+        if (c >= C) break;
+        float M, l;
+        const float2 o = warps_sum<D, NT>(smem, col, d, M, l);
+        if (cluster == 1) {
+            write_out(a, rw, b, h, c, d, o, M, l);
+        } else {
+            *reinterpret_cast<float2*>(bo + col * D + d) = o;
+            if (d == 0) bml[col] = make_float2(M, l);
+        }
+    }
+    if (cluster == 1) return;
+    cluster_sync();
+    for (int idx = rank * ANT + tid; idx < CB * (D / 2); idx += cluster * ANT) {
+        const int col = idx / (D / 2), d = 2 * (idx % (D / 2)), c = cb * CB + col;
+        if (c >= C) break;
+        float2 ml[MAX_CLUSTER], v[MAX_CLUSTER];
+#pragma unroll
+        for (int r = 0; r < MAX_CLUSTER; ++r) {
+            ml[r] = r < cluster ? cluster_load2(&bml[col].x, r) : make_float2(M0, 0.f);
+            v[r] = r < cluster ? cluster_load2(&bo[col * D + d], r) : make_float2(0.f, 0.f);
+        }
+        float M = M0, l = 0.f;
+#pragma unroll
+        for (int r = 0; r < MAX_CLUSTER; ++r) M = fmaxf(M, ml[r].x);
+        float2 o = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int r = 0; r < MAX_CLUSTER; ++r) {
+            const float f = half_pow(ml[r].x - M);
+            l = fmaf(ml[r].y * f, f, l);
+            o.x = fmaf(v[r].x * f, f, o.x);
+            o.y = fmaf(v[r].y * f, f, o.y);
+        }
+        write_out(a, rw, b, h, c, d, o, M, l);
+    }
+    cluster_sync();  // the blocks' sums are read until here
+}
+
 // Joins the partials of segments that span shares, and writes the rows of empty
-// sequences.  One block per (column, sequence), one thread per dimension; every
-// warp works out the segment's shares and their weights by itself.
+// sequences.  One block per (column, sequence); every warp works out the
+// segment's shares by itself.
+constexpr int JOIN_WARPS = 8;
 template <int D>
-__global__ void __launch_bounds__(D) kv4_attn_join_kernel(const Kv4AttnArgs a, int cb_size, int ncb, int shares, const int* plan,
-                                                          const float* part, const float2* pml) {
-    const int b = blockIdx.y, G = a.Hq / a.c.heads, d = threadIdx.x, lane = d & 31;
+__global__ void __launch_bounds__(32 * JOIN_WARPS) kv4_attn_join_kernel(const Kv4AttnArgs a, int cb_size, int ncb, int shares, const int* plan,
+                                                                        const float* part, const float2* pml) {
+    __shared__ float sh[JOIN_WARPS * (D + 2)];
+    const int b = blockIdx.y, G = a.Hq / a.c.heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int h = blockIdx.x % a.Hq, i = blockIdx.x / a.Hq;  // query head, row
     const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
     const int nt = tiles_of(rw);
@@ -336,11 +432,11 @@ __global__ void __launch_bounds__(D) kv4_attn_join_kernel(const Kv4AttnArgs a, i
         per = plan[0];
         s0 = plan[1 + b];
     }
-    bf16* dst = a.out + (b * a.os.b + i * a.os.s + h * a.os.h) + d;
+    bf16* dst = a.out + (b * a.os.b + i * a.os.s + h * a.os.h);
     float* lse = a.lse ? a.lse + ((size_t)b * a.S + i) * a.Hq + h : nullptr;
     if (nt == 0 || i >= rw.n) {
-        *dst = f2bf(0.f);
-        if (lse && d == 0) *lse = -INFINITY;
+        if (warp == 0 && lane < D / 8) *reinterpret_cast<uint4*>(dst + 8 * lane) = make_uint4(0u, 0u, 0u, 0u);
+        if (lse && threadIdx.x == 0) *lse = -INFINITY;
         return;
     }
     const int c = i * G + h % G, cb = c / cb_size, col = c % cb_size;
@@ -348,29 +444,8 @@ __global__ void __launch_bounds__(D) kv4_attn_join_kernel(const Kv4AttnArgs a, i
     const int first = s0 / per, last = (s0 + nt - 1) / per;
     if (first == last) return;
     // the first share's partial of this segment is its second one if the share began before it
-    const size_t p0 = (2 * (size_t)first + (first * per >= s0 ? 0 : 1)) * cb_size + col;
-    auto slot = [&](int k) { return k == first ? p0 : 2 * (size_t)k * cb_size + col; };
-    float M = M0, o = 0.f, l = 0.f;
-    for (int k0 = first; k0 <= last; k0 += 32) {
-        const int n = min(32, last + 1 - k0);
-        const float2 ml = lane < n ? pml[slot(k0 + lane)] : make_float2(M0, 0.f);
-        const float m = fmaxf(M, warp_max(ml.x)), al = half_pow(M - m), f = half_pow(ml.x - m);
-        l = fmaf(l * al, al, warp_sum(ml.y * f * f));
-        o = o * al * al;
-        M = m;
-        for (int j = 0; j < n; j += 8) {
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = j + e < n ? part[slot(k0 + j + e) * D + d] : 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float fe = __shfl_sync(0xffffffffu, f, min(j + e, 31));
-                o = fmaf(v[e] * fe, fe, o);
-            }
-        }
-    }
-    *dst = f2bf(l != 0.f ? o / l : 0.f);
-    if (lse && d == 0) *lse = l != 0.f ? (M + log2f(l)) * LN2 : -INFINITY;
+    auto slot = [&](int k) { return (2ll * (first + k) + (k == 0 && first * per < s0 ? 1 : 0)) * cb_size + col; };
+    join_row<D, JOIN_WARPS>(last - first + 1, warp, slot, part, pml, sh, dst, lse);
 }
 
 // Attention weights: a warp keeps 32 keys and walks the columns, 64 at a time
@@ -489,27 +564,38 @@ __global__ void __launch_bounds__(ANT, 2) kv4_mass_kernel(const Kv4AttnArgs a) {
 }
 
 template <typename K, typename... Args>
-cudaError_t launch(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl, Args... args) {
+cudaError_t launch(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl, int cluster, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (pdl) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = cluster;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
     cfg.attrs = attr;
-    cfg.numAttrs = pdl ? 1 : 0;
+    cfg.numAttrs = n;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 // Form of a call: from TC_COLUMNS columns per kv head the tcgen05 kernel, below it the split kernel
 // with column blocks of 8 (two blocks of threads per SM) or 16.
 constexpr int TC_COLUMNS = 64;
+constexpr int CLUSTER_TILES = 4;
 struct Shape {
     bool tc;
     TcShape t;
     int nt, cb, ncb, shares;
+    int cluster;  // blocks of a segment in the cluster form, 0: shares
     size_t part_rows;
 };
 Shape shape_of(const Kv4View& c, int S, int Hq, int num_sms) {
@@ -525,6 +611,16 @@ Shape shape_of(const Kv4View& c, int S, int Hq, int num_sms) {
     s.cb = 8 * s.nt;
     s.ncb = (int)((C + s.cb - 1) / s.cb);
     s.shares = s.nt == 1 ? 2 * num_sms : num_sms;
+    // The cluster form, when the longest sequence the cache can hold is at most CLUSTER_TILES tiles a warp (what a
+    // ragged batch loses to its longest sequence then costs less than the joining kernel) and its blocks fit at once.
+    const long long segs = (long long)c.batch * c.heads * s.ncb;
+    const int most = (c.max_pos + TK - 1) / TK;
+    int cl = 1;
+    while (cl < MAX_CLUSTER && segs * 2 * cl <= s.shares && most > AW * cl) cl *= 2;
+    if (most <= CLUSTER_TILES * AW * cl && segs * cl <= 0x7FFFFFFF) {
+        s.cluster = cl;
+        return s;
+    }
     s.part_rows = (size_t)2 * s.shares * s.cb;
     return s;
 }
@@ -532,11 +628,17 @@ Shape shape_of(const Kv4View& c, int S, int Hq, int num_sms) {
 template <int D, int NT>
 cudaError_t launch_split(const Kv4AttnArgs& a, const Shape& sp, const Scratch& sc, cudaStream_t st) {
     constexpr int smem = SplitSmem<D, NT>::BYTES;
+    if (sp.cluster) {
+        const cudaError_t e = ensure_max_dyn_smem(kv4_attn_cluster_kernel<D, NT>, smem);
+        if (e != cudaSuccess) return e;
+        const unsigned blocks = (unsigned)(sp.cluster * sp.ncb * a.c.heads) * (unsigned)a.c.batch;
+        return launch(kv4_attn_cluster_kernel<D, NT>, dim3(blocks), dim3(ANT), smem, st, false, sp.cluster, a, sp.ncb, sp.cluster);
+    }
     cudaError_t e = ensure_max_dyn_smem(kv4_attn_split_kernel<D, NT>, smem);
     if (e != cudaSuccess) return e;
-    e = launch(kv4_attn_split_kernel<D, NT>, dim3(sp.shares), dim3(ANT), smem, st, false, a, sp.ncb, sc.plan, sc.part, sc.ml);
+    e = launch(kv4_attn_split_kernel<D, NT>, dim3(sp.shares), dim3(ANT), smem, st, false, 1, a, sp.ncb, sc.plan, sc.part, sc.ml);
     if (e != cudaSuccess) return e;
-    return launch(kv4_attn_join_kernel<D>, dim3((unsigned)(a.S * a.Hq), a.c.batch), dim3(D), 0, st, true, a, sp.cb, sp.ncb,
+    return launch(kv4_attn_join_kernel<D>, dim3((unsigned)(a.S * a.Hq), a.c.batch), dim3(32 * JOIN_WARPS), 0, st, true, 1, a, sp.cb, sp.ncb,
                   sp.shares, (const int*)sc.plan, (const float*)sc.part, (const float2*)sc.ml);
 }
 
@@ -547,7 +649,7 @@ cudaError_t launch_d(const Kv4AttnArgs& a, const Shape& sp, const Scratch& sc, c
                                        : launch_split<D, 2>(a, sp, sc, st);
     if (e != cudaSuccess || !a.mass) return e;
     const dim3 grid((a.c.max_pos + AW * TK - 1) / (AW * TK), a.c.heads, a.c.batch);
-    return launch(kv4_mass_kernel<D>, grid, dim3(ANT), 0, st, true, a);
+    return launch(kv4_mass_kernel<D>, grid, dim3(ANT), 0, st, true, 1, a);
 }
 
 }  // namespace
@@ -561,7 +663,7 @@ cudaError_t launch_kv4_attention(const Kv4AttnArgs& in, void* scratch, int num_s
     Kv4AttnArgs a = in;
     const Shape sp = shape_of(a.c, a.S, a.Hq, num_sms);
     // tiles are counted in 32 bits (180 GB of cache are less than 2^26 tiles of one column block)
-    if (!sp.tc && (long long)a.c.batch * a.c.heads * sp.ncb * ((a.c.max_pos + TK - 1) / TK) > 0x7FFFFFFF) return cudaErrorInvalidValue;
+    if (!sp.tc && !sp.cluster && (long long)a.c.batch * a.c.heads * sp.ncb * ((a.c.max_pos + TK - 1) / TK) > 0x7FFFFFFF) return cudaErrorInvalidValue;
     const Scratch sc = scratch_of(scratch, a.c, a.S, a.Hq, sp.part_rows);
     if (a.mass && !a.lse) a.lse = sc.lse;
     return a.c.D == 128 ? launch_d<128>(a, sp, sc, st) : launch_d<64>(a, sp, sc, st);

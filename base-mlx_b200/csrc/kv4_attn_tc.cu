@@ -28,6 +28,7 @@
 // slots they run at the pace of instruction fetch and of single dependent
 // chains.)  Every wait is bounded: a lost arrival sets QW_DERR_TIMEOUT and the
 // block still frees its TMEM and ends.
+#include "kv4_join.cuh"
 #include "kv4_tc.h"
 #include "kv4_tile.cuh"
 #include "smem_attr.h"
@@ -638,32 +639,32 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
     }
 }
 
-// Joins the splits' partials.  One block per (column, sequence), one thread per dimension.
+// Joins the splits' partials.  One warp per row, the rows of a sequence in order.
+constexpr int JOIN_WARPS = 4;
 template <int D>
-__global__ void __launch_bounds__(D) kv4_attn_tc_join_kernel(const Kv4AttnArgs a, int cb_size, int ncb, int nsplit, const float* part, const float2* pml) {
-    const int b = blockIdx.y, G = a.Hq / a.c.heads, d = threadIdx.x, h = blockIdx.x % a.Hq, i = blockIdx.x / a.Hq;
+__global__ void __launch_bounds__(32 * JOIN_WARPS) kv4_attn_tc_join_kernel(const Kv4AttnArgs a, int cb_size, int ncb, int nsplit,
+                                                                           const float* part, const float2* pml) {
+    const int b = blockIdx.y, G = a.Hq / a.c.heads, lane = threadIdx.x & 31;
+    const int item = blockIdx.x * JOIN_WARPS + (threadIdx.x >> 5), h = item % a.Hq, i = item / a.Hq;
     const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
+    if (i >= a.S) return;
     const int c = i * G + h % G, cb = c / cb_size, C = G * a.S;
     const int i_last = min(rw.n, (min(C, (cb + 1) * cb_size) - 1) / G + 1) - 1;
     const int T = rw.off + rw.n, nt = ((a.causal ? min(T, rw.off + i_last + 1) : T) + KT - 1) / KT;
-    bf16* dst = a.out + (b * a.os.b + (long long)i * a.os.s + (long long)h * a.os.h) + d;
+    bf16* dst = a.out + (b * a.os.b + (long long)i * a.os.s + (long long)h * a.os.h);
     float* lse = a.lse ? a.lse + ((size_t)b * a.S + i) * a.Hq + h : nullptr;
+    const size_t s0 = ((((size_t)b * a.c.heads + h / G) * ncb + cb) * nsplit) * cb_size + c % cb_size;
     pdl_wait();
-    float M = M0, o = 0.f, l = 0.f;
-    if (i < rw.n) {
-        const size_t s0 = ((((size_t)b * a.c.heads + h / G) * ncb + cb) * nsplit) * cb_size + c % cb_size;
-        for (int s = 0; s < nsplit; ++s)
-            if ((long long)nt * s / nsplit != (long long)nt * (s + 1) / nsplit) M = fmaxf(M, pml[s0 + (size_t)s * cb_size].x);
-        for (int s = 0; s < nsplit; ++s)
-            if ((long long)nt * s / nsplit != (long long)nt * (s + 1) / nsplit) {
-                const float2 ml = pml[s0 + (size_t)s * cb_size];
-                const float f = half_pow(ml.x - M);
-                l = fmaf(ml.y * f, f, l);
-                o = fmaf(part[(s0 + (size_t)s * cb_size) * D + d] * f, f, o);
-            }
+    if (i >= rw.n) {
+        if (lane < D / 8) *reinterpret_cast<uint4*>(dst + 8 * lane) = make_uint4(0u, 0u, 0u, 0u);
+        if (lse && lane == 0) *lse = -INFINITY;
+        return;
     }
-    *dst = f2bf(l != 0.f ? o / l : 0.f);
-    if (lse && d == 0) *lse = l != 0.f ? (M + log2f(l)) * LN2 : -INFINITY;
+    // a split without tiles has left nothing
+    auto slot = [&](int k) {
+        return (long long)nt * k / nsplit == (long long)nt * (k + 1) / nsplit ? -1ll : (long long)(s0 + (size_t)k * cb_size);
+    };
+    join_row<D, 1>(nsplit, 0, slot, part, pml, nullptr, dst, lse);
 }
 
 template <typename K, typename... Args>
@@ -690,7 +691,7 @@ cudaError_t launch_tc(const Kv4AttnArgs& a, const TcShape& sp, float* part, floa
     if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
     e = launch(kv4_attn_tc_kernel<D, NB>, dim3((unsigned)blocks), dim3(THREADS<NB>), smem, st, false, a, sp.ncb, sp.nsplit, part, ml);
     if (e != cudaSuccess || sp.nsplit == 1) return e;
-    return launch(kv4_attn_tc_join_kernel<D>, dim3((unsigned)(a.S * a.Hq), a.c.batch), dim3(D), 0, st, true, a, CM * NB, sp.ncb,
+    return launch(kv4_attn_tc_join_kernel<D>, dim3((unsigned)((a.S * (long long)a.Hq + JOIN_WARPS - 1) / JOIN_WARPS), a.c.batch), dim3(32 * JOIN_WARPS), 0, st, true, a, CM * NB, sp.ncb,
                   sp.nsplit, (const float*)part, (const float2*)ml);
 }
 
