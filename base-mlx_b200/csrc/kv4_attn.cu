@@ -256,7 +256,7 @@ QW_DEV void run_tiles(const Kv4AttnArgs& a, const Kv4Rows& rw, int b, int h, int
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) wml[warp * CB + 8 * n + 2 * t + e] = make_float2(-st.nm[n][e], st.l[n][e]);
+            for (int e = 0; e < 2; ++e) wml[warp * CB + 8 * n + 2 * t + e] = make_float2(st.base(n, e), st.l[n][e]);
     __syncthreads();  // also: every warp has left its ring
     if (mine > 0)
 #pragma unroll
@@ -267,7 +267,7 @@ QW_DEV void run_tiles(const Kv4AttnArgs& a, const Kv4Rows& rw, int b, int h, int
                 float M = wml[col].x;
 #pragma unroll
                 for (int w = 1; w < AW; ++w) M = fmaxf(M, wml[w * CB + col].x);
-                const float f = half_pow(-st.nm[n][e] - M);
+                const float f = half_pow(st.base(n, e) - M);
                 float* dst = wo + (warp * CB + col) * SM::OLD + 4 * g;
 #pragma unroll
                 for (int gr = 0; gr < D / 64; ++gr)

@@ -29,7 +29,7 @@ namespace qw {
 namespace kv4 {
 
 constexpr int TK = 32;            // keys of a tile
-constexpr float M0 = -3.0e38f;    // running maximum before the first key
+constexpr float M0 = -3.0e38f;    // base exponent of a column before its first key
 constexpr float LAZY = 4.f;       // the maximum is raised when a score passes it by 2^LAZY
 constexpr int LOG2_PSCALE = 11;   // p s / sref <= 2^LAZY enters fp16 times 2^11: at most 2^15
 constexpr float LN2 = 0.6931471805599453f, LOG2E = 1.4426950408889634f;
@@ -280,9 +280,10 @@ struct State {
     static constexpr int GR = D / 64;
     // [4 group + i]: rows g -> dimension 64 group + 32 (i / 2) + 4 g + 2 (i % 2), rows g + 8 -> the next (times 16)
     float o[D / 16][NT][4];
-    float nm[NT][4];         // {column 0, 1, 0, 1}: the C operand of a score tile
+    float nm[NT][4];         // {column 0, 1, 0, 1}: the C operand of a score tile; 0 before the first key
+    float thr[NT][2];        // largest exponent that leaves the base as it is; M0 before the first key
     float l[NT][2], bs[GR][NT][2];
-    float sref, lim;         // lim: exponent above which a score + nm calls for a new maximum
+    float sref;
     QW_DEV void init() {
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
@@ -294,7 +295,8 @@ struct State {
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                nm[n][e] = nm[n][2 + e] = -M0;
+                nm[n][e] = nm[n][2 + e] = 0.f;
+                thr[n][e] = M0;
                 l[n][e] = 0.f;
 #pragma unroll
                 for (int g = 0; g < GR; ++g) bs[g][n][e] = 0.f;
@@ -305,9 +307,10 @@ struct State {
     QW_DEV void set_sref(float s) {
         const uint32_t e = min(max(__float_as_uint(s) >> 23, 47u) + 1u, 254u);
         sref = __uint_as_float(e << 23);
-        lim = LAZY + shift();
     }
     QW_DEV float shift() const { return (float)(LOG2_PSCALE + 127 - (int)(__float_as_uint(sref) >> 23)); }  // log2(PSCALE / sref)
+    // the base exponent of column (n, e), M0 before the first key
+    QW_DEV float base(int n, int e) const { return thr[n][e] == M0 ? M0 : -nm[n][e]; }
 };
 
 // One tile: keys [key0, key0 + 32) of which vis[n][e] (absolute) are visible to
@@ -333,61 +336,62 @@ QW_DEV void attend_tile(State<D, NT>& st, const Cols<D, NT>& cols, const unsigne
         unpack<GR>(read_packed<D>(tile, 0, 8 * r + g), ks[r]);
         kz[r] = read_packed<D>(tile, 1, 8 * r + g);
     }
-    // x[kb][n][2 r + e]: score of key 16 kb + 8 r + g and column 2 t + e, plus the column's base
+    // x[kb][n][2 r + e]: score of key 16 kb + 8 r + g and column 2 t + e, less the column's base
     float x[2][NT][4];
-    auto scores = [&](const float (&base)[NT][4]) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+    for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                mma_bf16_k8(x[kb][n], kz[2 * kb], kz[2 * kb + 1], cols.qb[n], base[n]);
+        for (int n = 0; n < NT; ++n) {
+            mma_bf16_k8(x[kb][n], kz[2 * kb], kz[2 * kb + 1], cols.qb[n], st.nm[n]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = 2 * kb + (e >> 1);
-                    float d = ks[r][0] * acc[kb][0][n][e];
-                    if (GR == 2) d = fmaf(ks[r][GR - 1], acc[kb][GR - 1][n][e], d);
-                    x[kb][n][e] = fmaf(cols.c[n][e & 1], d, x[kb][n][e]);
-                    if (EDGE && key0 + 8 * r + g >= vis[n][e & 1]) x[kb][n][e] = -INFINITY;
-                }
+            for (int e = 0; e < 4; ++e) {
+                const int r = 2 * kb + (e >> 1);
+                float d = ks[r][0] * acc[kb][0][n][e];
+                if (GR == 2) d = fmaf(ks[r][GR - 1], acc[kb][GR - 1][n][e], d);
+                x[kb][n][e] = fmaf(cols.c[n][e & 1], d, x[kb][n][e]);
+                if (EDGE && key0 + 8 * r + g >= vis[n][e & 1]) x[kb][n][e] = -INFINITY;
             }
-    };
-    scores(st.nm);
+        }
     // largest value scale of the tile (lane = key)
     float vs[4][GR], vz[4][GR], smax;
     unpack<GR>(read_packed<D>(tile, 2, lane), vs[0]);
     smax = GR == 2 ? fmaxf(fabsf(vs[0][0]), fabsf(vs[0][GR - 1])) : fabsf(vs[0][0]);
     if (EDGE && key0 + lane >= T) smax = 0.f;
-    float top = -INFINITY;
+    bool raise = smax > st.sref;
+    float top[NT][2];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) top = fmaxf(top, x[kb][n][e]);
-    if (__any_sync(0xffffffffu, top > st.lim || smax > st.sref)) {
+        for (int e = 0; e < 2; ++e) {
+            top[n][e] = fmaxf(fmaxf(x[0][n][e], x[0][n][2 + e]), fmaxf(x[1][n][e], x[1][n][2 + e]));
+            raise = raise || top[n][e] > st.thr[n][e];
+        }
+    if (__any_sync(0xffffffffu, raise)) {
         // rare: raise the column maxima to the tile's, the scale reference to its largest scale
         const float before = st.shift();
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, o));
         if (smax > st.sref) st.set_sref(smax);
         const float now = st.shift();
-        const float zero[NT][4] = {};
-        scores(zero);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                float mx = fmaxf(fmaxf(x[0][n][e], x[0][n][2 + e]), fmaxf(x[1][n][e], x[1][n][2 + e]));
+                float mx = top[n][e];
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                const float old = st.nm[n][e];
-                if (old == -M0) {
-                    if (mx == -INFINITY) continue;  // still no key for this column
-                } else {
-                    mx = fmaxf(mx, before - old);   // the old maximum
+                const bool seen = st.thr[n][e] != M0;
+                if (seen) mx = fmaxf(mx, before);        // the old maximum's exponent
+                if (!seen && mx == -INFINITY) continue;  // still no key for this column
+                const float by = now - mx, al = seen ? half_pow(by) : 0.f;
+                st.nm[n][e] += by;
+                st.nm[n][2 + e] += by;
+                st.thr[n][e] = now + LAZY;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+                    x[kb][n][e] += by;
+                    x[kb][n][2 + e] += by;
                 }
-                const float nm = now - mx, al = old == -M0 ? 0.f : half_pow(nm - old);
-                st.nm[n][e] = st.nm[n][2 + e] = nm;
                 st.l[n][e] = st.l[n][e] * al * al;
 #pragma unroll
                 for (int gr = 0; gr < GR; ++gr) st.bs[gr][n][e] = st.bs[gr][n][e] * al * al;
@@ -397,7 +401,6 @@ QW_DEV void attend_tile(State<D, NT>& st, const Cols<D, NT>& cols, const unsigne
                     st.o[i][n][2 + e] = st.o[i][n][2 + e] * al * al;
                 }
             }
-        scores(st.nm);
     }
     // probabilities, their sums, and p s in the B-operand layout (keys along k)
     uint32_t pb[2][GR][NT][2];
