@@ -616,7 +616,8 @@ Shape shape_of(const Kv4View& c, int S, int Hq, int num_sms) {
     const long long segs = (long long)c.batch * c.heads * s.ncb;
     const int most = (c.max_pos + TK - 1) / TK;
     int cl = 1;
-    while (cl < MAX_CLUSTER && segs * 2 * cl <= s.shares && most > AW * cl) cl *= 2;
+    // (clusters of 8 are counted on three quarters of the SMs: what is left of a GPC holds none)
+    while (cl < MAX_CLUSTER && segs * 2 * cl * (cl == 4 ? 4 : 3) <= 3ll * s.shares && most > AW * cl) cl *= 2;
     if (most <= CLUSTER_TILES * AW * cl && segs * cl <= 0x7FFFFFFF) {
         s.cluster = cl;
         return s;
