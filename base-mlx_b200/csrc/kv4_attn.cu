@@ -16,6 +16,8 @@
 // there; one that spans shares leaves a partial (base exponent, sum, output) per
 // share, which a second kernel joins.  Caches so short that a cluster of blocks
 // holds a segment in a few tiles per warp skip the list and join in the cluster.
+#include <algorithm>
+
 #include "kv4_join.cuh"
 #include "kv4_tc.h"
 #include "kv4_tile.cuh"
@@ -198,19 +200,31 @@ struct SplitSmem {
     static constexpr int BYTES = (RING > MERGE + BLOCK ? RING : MERGE + BLOCK) + AW * CB * 8;
 };
 
+// The warp's columns of a column block (rows that a sequence turns out not to have are read and not used).
+template <int D, int NT>
+QW_DEV void fetch_cols(const Kv4AttnArgs& a, int b, int h, int cb, RawCol<D> (&raw)[NT]) {
+    const int lane = threadIdx.x & 31, G = a.Hq / a.c.heads;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int c = cb * 8 * NT + 8 * n + (lane >> 2);
+        fetch_col<D>(raw[n], c < G * a.S ? a.q + (b * a.qs.b + (c / G) * a.qs.s + (h * G + c % G) * a.qs.h) : nullptr, lane);
+    }
+}
+
 // This warp's tiles first, first + step, ... below t1 of column block cb of (b, h):
 // every warp has its own columns' state and its own ring of
 // tiles (cp.async, so no warp waits for another).  Leaves (base exponent, sum) of every warp and column in
 // wml and the warps' outputs, relative to the block's base, in wo.
 template <int D, int NT>
-QW_DEV void run_tiles(const Kv4AttnArgs& a, const Kv4Rows& rw, int b, int h, int cb, int first, int step, int t1, unsigned char* smem) {
+QW_DEV void run_tiles(const Kv4AttnArgs& a, const Kv4Rows& rw, int b, int h, int cb, const RawCol<D> (&raw)[NT], int first, int step, int t1,
+                      unsigned char* smem) {
     using L = Tile<D>;
     using SM = SplitSmem<D, NT>;
     constexpr int CB = SM::CB;
     float2* wml = reinterpret_cast<float2*>(smem + SM::BYTES - AW * CB * 8);  // [warp][column]
     float* wo = reinterpret_cast<float*>(smem);                               // [warp][column][OLD]
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int G = a.Hq / a.c.heads, C = G * a.S, T = rw.off + rw.n;
+    const int G = a.Hq / a.c.heads, T = rw.off + rw.n;
     const uint32_t ring = smem_u32(smem) + warp * ASTAGES * L::BYTES;
     const unsigned char* ringp = smem + warp * ASTAGES * L::BYTES;
     const Rows rows = head_rows<D>(a.c, (size_t)b * a.c.heads + h);
@@ -228,9 +242,7 @@ QW_DEV void run_tiles(const Kv4AttnArgs& a, const Kv4Rows& rw, int b, int h, int
     int vis[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int c = cb * CB + 8 * n + g, i = c / G;
-        const bf16* src = mine > 0 && c < C && i < rw.n ? a.q + (b * a.qs.b + i * a.qs.s + (h * G + c % G) * a.qs.h) : nullptr;
-        load_cols<D, NT>(cols, n, src, a.scale, lane);
+        load_cols<D, NT>(cols, n, raw[n], a.scale, lane);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int ci = (cb * CB + 8 * n + 2 * t + e) / G;
@@ -334,7 +346,9 @@ __global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(co
         const int seg = (u - b0) / nt, t0 = (u - b0) % nt;
         const int t1 = min(nt, t0 + (sh.end - u));
         const int h = seg / ncb, cb = seg % ncb;
-        run_tiles<D, NT>(a, rw, b, h, cb, t0 + (tid >> 5), AW, t1, smem);
+        RawCol<D> raw[NT];
+        fetch_cols<D, NT>(a, b, h, cb, raw);
+        run_tiles<D, NT>(a, rw, b, h, cb, raw, t0 + (tid >> 5), AW, t1, smem);
         const bool whole = t0 == 0 && t1 == nt;
         const size_t slot = 2 * (size_t)blockIdx.x + (u == sh.begin ? 0 : 1);
         for (int idx = tid; idx < CB * (D / 2); idx += ANT) {
@@ -367,8 +381,10 @@ __global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_cluster_kernel(
     const int tid = threadIdx.x, C = a.Hq / a.c.heads * a.S;
     const int rank = blockIdx.x % cluster, seg = blockIdx.x / cluster;
     const int cb = seg % ncb, h = seg / ncb % a.c.heads, b = seg / ncb / a.c.heads;
+    RawCol<D> raw[NT];
+    fetch_cols<D, NT>(a, b, h, cb, raw);  // before the length arrives
     const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, a.err, rank == 0 && h == 0 && cb == 0 && tid == 0);
-    run_tiles<D, NT>(a, rw, b, h, cb, (tid >> 5) * cluster + rank, AW * cluster, tiles_of(rw), smem);
+    run_tiles<D, NT>(a, rw, b, h, cb, raw, (tid >> 5) * cluster + rank, AW * cluster, tiles_of(rw), smem);
     for (int idx = tid; idx < CB * (D / 2); idx += ANT) {
         const int col = idx / (D / 2), d = 2 * (idx % (D / 2)), c = cb * CB + col;
         if (c >= C) break;
@@ -448,82 +464,175 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) kv4_attn_join_kernel(const Kv
     join_row<D, JOIN_WARPS>(last - first + 1, warp, slot, part, pml, sh, dst, lse);
 }
 
-// Attention weights: a warp keeps 32 keys and walks the columns, 64 at a time
-// prepared by the block.  A key's weight is summed by one lane quad in a fixed
-// order.
-constexpr int MC = 8;  // n-tiles of 8 columns prepared together
-template <int D>
-__global__ void __launch_bounds__(ANT, 2) kv4_mass_kernel(const Kv4AttnArgs a) {
+// ---- attention weights ------------------------------------------------------
+// A key's weight is summed by one lane quad in a fixed order, over the scores recomputed from the K rows and
+// the rows' log-sum-exp.
+
+// K rows of keys key0 + 8 r + g (r < 2 KB) straight from memory, in the layout of read_keys; zeros from T on.
+template <int D, int KB>
+struct MassKeys {
+    KeyBlock<D> w[KB];
+    uint32_t s[2 * KB], z[2 * KB];
+};
+template <int D, int KB>
+QW_DEV void fetch_keys(MassKeys<D, KB>& o, const Kv4View& c, size_t bh, int key0, int T, int lane) {
     constexpr int GR = D / 64;
-    __shared__ uint32_t sf[MC][GR * 4 * 2][32];  // n-tile, fragment register, lane
-    __shared__ float sc[MC][3][8];               // n-tile, {c, log2 of the sum, keys seen}, column
-    __shared__ uint32_t sq[MC][32];              // n-tile, bias operand, lane
-    pdl_wait();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int h = blockIdx.y, b = blockIdx.z, G = a.Hq / a.c.heads;
-    const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
-    const int T = rw.off + rw.n;
-    const int key0 = (blockIdx.x * AW + warp) * TK, block0 = blockIdx.x * AW * TK;
-    if (block0 >= T) return;
-    const size_t bh = (size_t)b * a.c.heads + h;
-    // K words, scales and biases straight to registers (each is read once)
-    KeyBlock<D> kw[2];
-    float ks[4][GR];
-    uint32_t kz[4];
-    const uint32_t* w = a.c.p[0].w + bh * a.c.max_pos * (D / 8);
-    const uint16_t* s = reinterpret_cast<const uint16_t*>(a.c.p[0].s) + bh * a.c.max_pos * GR;
-    const uint16_t* z = reinterpret_cast<const uint16_t*>(a.c.p[0].b) + bh * a.c.max_pos * GR;
+    const int g = lane >> 2, t = lane & 3;
+    const uint32_t* w = c.p[0].w + bh * c.max_pos * (D / 8);
+    const unsigned char* s = reinterpret_cast<const unsigned char*>(c.p[0].s) + bh * c.max_pos * (2 * GR);
+    const unsigned char* z = reinterpret_cast<const unsigned char*>(c.p[0].b) + bh * c.max_pos * (2 * GR);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+    for (int r = 0; r < 2 * KB; ++r) {
         const int k = key0 + 8 * r + g;
         const bool ok = k < T;
 #pragma unroll
-        for (int gr = 0; gr < GR; ++gr) {
-            uint2 u = make_uint2(0u, 0u);
-            if (ok) {
-                u.x = w[(size_t)k * (D / 8) + 8 * gr + t];
-                u.y = w[(size_t)k * (D / 8) + 8 * gr + 4 + t];
-            }
-            kw[r >> 1].w[gr][r & 1][0] = u.x;
-            kw[r >> 1].w[gr][r & 1][1] = u.y;
-            ks[r][gr] = ok ? u16_to_f(s[(size_t)k * GR + gr]) : 0.f;
-        }
-        kz[r] = !ok ? 0u : GR == 2 ? *reinterpret_cast<const uint32_t*>(z + (size_t)k * GR) : (uint32_t)z[(size_t)k * GR];
+        for (int gr = 0; gr < GR; ++gr)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) o.w[r >> 1].w[gr][r & 1][j] = ok ? w[(size_t)k * (D / 8) + 8 * gr + 4 * j + t] : 0u;
+        const size_t at = (size_t)k * (2 * GR);
+        o.s[r] = !ok ? 0u : GR == 2 ? *reinterpret_cast<const uint32_t*>(s + at) : (uint32_t)*reinterpret_cast<const uint16_t*>(s + at);
+        o.z[r] = !ok ? 0u : GR == 2 ? *reinterpret_cast<const uint32_t*>(z + at) : (uint32_t)*reinterpret_cast<const uint16_t*>(z + at);
     }
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    // columns that see none of the block's keys come first when causal: skip them
-    const int c_first = a.causal ? max(0, block0 - rw.off) * G / 8 * 8 : 0;
-    const int c_end = rw.n * G;
-    for (int c0 = c_first; c0 < c_end; c0 += 8 * MC) {
-        __syncthreads();
-        if (c0 + 8 * warp < c_end) {  // n-tile `warp` of this round
-            const int c = c0 + 8 * warp + g, i = c / G;
-            Cols<D, 1> o;
-            load_cols<D, 1>(o, 0, c < c_end ? a.q + (b * a.qs.b + i * a.qs.s + (h * G + c % G) * a.qs.h) : nullptr, a.scale, lane);
+}
+// Adds the probabilities of the keys in the columns of n-tile n to sum[r]; base = -log2 of the rows' sums
+// (-inf: no column), vis the keys a column sees.
+template <int D, int KB, int NT>
+QW_DEV void add_weights(float (&sum)[2 * KB], const MassKeys<D, KB>& k, const Cols<D, NT>& cols, const float (&base)[NT][4],
+                        const int (&vis)[NT][2], int key0, int lane) {
+    constexpr int GR = D / 64;
+    const int g = lane >> 2;
 #pragma unroll
-            for (int gr = 0; gr < GR; ++gr)
+    for (int kb = 0; kb < KB; ++kb) {
+        float acc[GR][NT][4];
+        key_dots<D, NT>(acc, k.w[kb], cols);
+        float ks[2][GR];
+        unpack<GR>(k.s[2 * kb], ks[0]);
+        unpack<GR>(k.s[2 * kb + 1], ks[1]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    sf[warp][(gr * 4 + j) * 2][lane] = o.f[gr][j][0][0];
-                    sf[warp][(gr * 4 + j) * 2 + 1][lane] = o.f[gr][j][0][1];
-                }
-            if (g == 0)
+        for (int n = 0; n < NT; ++n) {
+            float x[4];
+            mma_bf16_k8(x, k.z[2 * kb], k.z[2 * kb + 1], cols.qb[n], base[n]);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) sc[warp][0][2 * t + e] = o.c[0][e];
-            sq[warp][lane] = o.qb[0];
-            if (t == 0) {
-                // log2 of the row's sum (+inf: a column past the end), and the keys it sees
-                sc[warp][1][g] = c < c_end ? a.lse[((size_t)b * a.S + i) * a.Hq + h * G + c % G] * LOG2E : INFINITY;
-                sc[warp][2][g] = __int_as_float(c < c_end ? (a.causal ? min(T, rw.off + i + 1) : T) : 0);
+            for (int e = 0; e < 4; ++e) {
+                float d = ks[e >> 1][0] * acc[0][n][e];
+                if (GR == 2) d = fmaf(ks[e >> 1][GR - 1], acc[GR - 1][n][e], d);
+                const float p = ex2(fmaf(cols.c[n][e & 1], d, x[e]));
+                const int r = 2 * kb + (e >> 1);
+                sum[r] += key0 + 8 * r + g < vis[n][e & 1] ? p : 0.f;
             }
+        }
+    }
+}
+// Sum over the lane quad of a key; lane t of the quad adds row r = t (and t + 4 ...) to mass.
+template <int KB>
+QW_DEV void store_weights(float (&sum)[2 * KB], float* mass, int key0, int T, int lane) {
+#pragma unroll
+    for (int r = 0; r < 2 * KB; ++r) {
+        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+    }
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int r = 0; r < 2 * KB; ++r)
+        if (t == r && key0 + 8 * r + g < T) mass[key0 + 8 * r + g] += sum[r];
+}
+
+// Up to 16 columns: a warp keeps them in registers and walks tiles of 32 keys, the next tile's rows in flight.
+template <int D, int NT>
+__global__ void __launch_bounds__(ANT, 2) kv4_mass_few_kernel(const Kv4AttnArgs a) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3;
+    const int h = blockIdx.y, b = blockIdx.z, G = a.Hq / a.c.heads, C = G * a.S;
+    RawCol<D> raw[NT];
+    fetch_cols<D, NT>(a, b, h, 0, raw);
+    const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
+    const int T = rw.off + rw.n, nt = tiles_of(rw), step = gridDim.x * AW;
+    const size_t bh = (size_t)b * a.c.heads + h;
+    int k = blockIdx.x * AW + warp;
+    MassKeys<D, 2> cur;
+    fetch_keys<D, 2>(cur, a.c, bh, k * TK, T, lane);
+    Cols<D, NT> cols;
+    float base[NT][4];
+    int vis[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) load_cols<D, NT>(cols, n, raw[n], a.scale, lane);
+    pdl_wait();  // the rows' log-sum-exp are the attention kernel's
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int c = 8 * n + 2 * t + e, i = c / G;
+            const bool has = c < C && i < rw.n;
+            base[n][e] = base[n][2 + e] = has ? -a.lse[((size_t)b * a.S + i) * a.Hq + h * G + c % G] * LOG2E : -INFINITY;
+            vis[n][e] = has ? (a.causal ? min(T, rw.off + i + 1) : T) : 0;
+        }
+    for (; k < nt; k += step) {
+        MassKeys<D, 2> next;
+        fetch_keys<D, 2>(next, a.c, bh, (k + step) * TK, T, lane);
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        add_weights<D, 2, NT>(sum, cur, cols, base, vis, k * TK, lane);
+        store_weights<2>(sum, a.mass + bh * a.c.max_pos, k * TK, T, lane);
+        cur = next;
+    }
+}
+
+// More columns: a warp keeps 16 keys (eight warps of 16: with 32 a chunk of 512 rows on 4096 keys left half of the
+// GPU without a second block per SM) and the block walks the columns, 64 at a time, one n-tile prepared by each warp
+// while the queries of the next 64 are in flight.
+constexpr int MC = 8;
+template <int D>
+__global__ void __launch_bounds__(ANT, 2) kv4_mass_kernel(const Kv4AttnArgs a) {
+    constexpr int GR = D / 64, MK = 16;
+    __shared__ uint32_t sf[MC][GR * 4 * 2][32];  // n-tile, fragment register, lane
+    __shared__ float sc[MC][3][8];               // n-tile, {c, -log2 of the sum, keys seen}, column
+    __shared__ uint32_t sq[MC][32];              // n-tile, bias operand, lane
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int h = blockIdx.y, b = blockIdx.z, G = a.Hq / a.c.heads;
+    const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
+    const int T = rw.off + rw.n;
+    const int block0 = blockIdx.x * AW * MK, key0 = block0 + warp * MK;
+    if (block0 >= T) return;
+    const size_t bh = (size_t)b * a.c.heads + h;
+    MassKeys<D, 1> keys;
+    fetch_keys<D, 1>(keys, a.c, bh, key0, T, lane);
+    float sum[2] = {0.f, 0.f};
+    // columns that see none of the block's keys come first when causal: skip them
+    const int c_first = a.causal ? max(0, block0 - rw.off) * G / 8 * 8 : 0, c_end = rw.n * G;
+    RawCol<D> raw;
+    auto fetch = [&](int c0) {
+        const int c = c0 + 8 * warp + g;
+        fetch_col<D>(raw, c < c_end ? a.q + (b * a.qs.b + (c / G) * a.qs.s + (h * G + c % G) * a.qs.h) : nullptr, lane);
+    };
+    fetch(c_first);
+    pdl_wait();  // the rows' log-sum-exp are the attention kernel's
+    for (int c0 = c_first; c0 < c_end; c0 += 8 * MC) {
+        const int cw = c0 + 8 * warp + g, iw = cw / G;
+        const float lse = t == 0 && cw < c_end ? a.lse[((size_t)b * a.S + iw) * a.Hq + h * G + cw % G] : INFINITY;
+        Cols<D, 1> o;
+        load_cols<D, 1>(o, 0, raw, a.scale, lane);
+        fetch(c0 + 8 * MC);
+        __syncthreads();
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                sf[warp][(gr * 4 + j) * 2][lane] = o.f[gr][j][0][0];
+                sf[warp][(gr * 4 + j) * 2 + 1][lane] = o.f[gr][j][0][1];
+            }
+        if (g == 0)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) sc[warp][0][2 * t + e] = o.c[0][e];
+        sq[warp][lane] = o.qb[0];
+        if (t == 0) {
+            sc[warp][1][g] = -lse * LOG2E;
+            sc[warp][2][g] = __int_as_float(cw < c_end ? (a.causal ? min(T, rw.off + iw + 1) : T) : 0);
         }
         __syncthreads();
         if (key0 >= T) continue;
         const int nn = min(MC, (c_end - c0 + 7) / 8);
         for (int n = 0; n < nn; ++n) {
             Cols<D, 1> cols;
-            float base[4];
-            int vis[2];
+            float base[1][4];
+            int vis[1][2];
             cols.qb[0] = sq[n][lane];
 #pragma unroll
             for (int gr = 0; gr < GR; ++gr)
@@ -535,32 +644,13 @@ __global__ void __launch_bounds__(ANT, 2) kv4_mass_kernel(const Kv4AttnArgs a) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 cols.c[0][e] = sc[n][0][2 * t + e];
-                base[e] = base[2 + e] = -sc[n][1][2 * t + e];
-                vis[e] = __float_as_int(sc[n][2][2 * t + e]);
+                base[0][e] = base[0][2 + e] = sc[n][1][2 * t + e];
+                vis[0][e] = __float_as_int(sc[n][2][2 * t + e]);
             }
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                float acc[GR][1][4], x[4];
-                key_dots<D, 1>(acc, kw[kb], cols);
-                mma_bf16_k8(x, kz[2 * kb], kz[2 * kb + 1], cols.qb[0], base);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = 2 * kb + (e >> 1);
-                    float d = ks[r][0] * acc[0][0][e];
-                    if (GR == 2) d = fmaf(ks[r][GR - 1], acc[GR - 1][0][e], d);
-                    const float p = ex2(fmaf(cols.c[0][e & 1], d, x[e]));
-                    sum[r] += key0 + 8 * r + g < vis[e & 1] ? p : 0.f;
-                }
-            }
+            add_weights<D, 1, 1>(sum, keys, cols, base, vis, key0, lane);
         }
     }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
-        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-        const int k = key0 + 8 * r + g;
-        if (t == 0 && k < T) a.mass[bh * a.c.max_pos + k] += sum[r];
-    }
+    store_weights<1>(sum, a.mass + bh * a.c.max_pos, key0, T, lane);
 }
 
 template <typename K, typename... Args>
@@ -644,12 +734,21 @@ cudaError_t launch_split(const Kv4AttnArgs& a, const Shape& sp, const Scratch& s
 }
 
 template <int D>
-cudaError_t launch_d(const Kv4AttnArgs& a, const Shape& sp, const Scratch& sc, cudaStream_t st) {
+cudaError_t launch_d(const Kv4AttnArgs& a, const Shape& sp, const Scratch& sc, int num_sms, cudaStream_t st) {
     const cudaError_t e = sp.tc      ? launch_kv4_attn_tc(a, sp.t, sc.part, sc.ml, st)
                           : sp.nt == 1 ? launch_split<D, 1>(a, sp, sc, st)
                                        : launch_split<D, 2>(a, sp, sc, st);
     if (e != cudaSuccess || !a.mass) return e;
-    const dim3 grid((a.c.max_pos + AW * TK - 1) / (AW * TK), a.c.heads, a.c.batch);
+    const long long C = (long long)(a.Hq / a.c.heads) * a.S;
+    if (C <= 16) {
+        // about two rounds of blocks, and no more than the cache can hold tiles for
+        const int most = (a.c.max_pos + AW * TK - 1) / (AW * TK);
+        const int x = (int)std::max(1ll, std::min<long long>(most, (4ll * num_sms + a.c.heads * a.c.batch - 1) / (a.c.heads * a.c.batch)));
+        const dim3 grid(x, a.c.heads, a.c.batch);
+        return C <= 8 ? launch(kv4_mass_few_kernel<D, 1>, grid, dim3(ANT), 0, st, true, 1, a)
+                      : launch(kv4_mass_few_kernel<D, 2>, grid, dim3(ANT), 0, st, true, 1, a);
+    }
+    const dim3 grid((a.c.max_pos + AW * 16 - 1) / (AW * 16), a.c.heads, a.c.batch);
     return launch(kv4_mass_kernel<D>, grid, dim3(ANT), 0, st, true, 1, a);
 }
 
@@ -667,7 +766,7 @@ cudaError_t launch_kv4_attention(const Kv4AttnArgs& in, void* scratch, int num_s
     if (!sp.tc && !sp.cluster && (long long)a.c.batch * a.c.heads * sp.ncb * ((a.c.max_pos + TK - 1) / TK) > 0x7FFFFFFF) return cudaErrorInvalidValue;
     const Scratch sc = scratch_of(scratch, a.c, a.S, a.Hq, sp.part_rows);
     if (a.mass && !a.lse) a.lse = sc.lse;
-    return a.c.D == 128 ? launch_d<128>(a, sp, sc, st) : launch_d<64>(a, sp, sc, st);
+    return a.c.D == 128 ? launch_d<128>(a, sp, sc, num_sms, st) : launch_d<64>(a, sp, sc, num_sms, st);
 }
 
 }  // namespace qw

@@ -117,23 +117,32 @@ struct Cols {
     uint32_t qb[NT];                          // the q_g as a B operand of three bf16 terms (24 bits): k = 2 term + group
 };
 
-// Column lane / 4 of n-tile n from bf16 row `src` (null: zeros); scale * log2(e) goes into c and q.
+// A lane's part of column lane / 4: words t and t + 4 of every group (t = lane % 4); null: zeros.
+template <int D>
+struct RawCol {
+    uint4 u[D / 64][2];
+};
+template <int D>
+QW_DEV void fetch_col(RawCol<D>& o, const bf16* src, int lane) {
+    const int t = lane & 3;
+#pragma unroll
+    for (int g = 0; g < D / 64; ++g)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            o.u[g][j] = src ? *reinterpret_cast<const uint4*>(src + 64 * g + 32 * j + 8 * t) : make_uint4(0u, 0u, 0u, 0u);
+}
+// Column lane / 4 of n-tile n from its bf16 row; scale * log2(e) goes into c and q.
 template <int D, int NT>
-QW_DEV void load_cols(Cols<D, NT>& o, int n, const bf16* src, float scale, int lane) {
+QW_DEV void load_cols(Cols<D, NT>& o, int n, const RawCol<D>& raw, float scale, int lane) {
     constexpr int GR = D / 64;
     const int t = lane & 3;
     float x[GR][16], sum[GR], mx = 0.f;
 #pragma unroll
     for (int g = 0; g < GR; ++g) {
         sum[g] = 0.f;
-        uint4 u[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-        if (src) {
-            u[0] = *reinterpret_cast<const uint4*>(src + 64 * g + 8 * t);
-            u[1] = *reinterpret_cast<const uint4*>(src + 64 * g + 32 + 8 * t);
-        }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const uint32_t X[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
+            const uint32_t X[4] = {raw.u[g][j].x, raw.u[g][j].y, raw.u[g][j].z, raw.u[g][j].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 x[g][8 * j + 2 * e] = bits_lo_f(X[e]);
