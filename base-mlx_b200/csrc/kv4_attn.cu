@@ -36,12 +36,19 @@ QW_DEV void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
-// The pair of floats at `p` in the cluster's block `rank`.
+// The pair (four) of floats at `p` in the cluster's block `rank`.
 QW_DEV float2 cluster_load2(const float* p, int rank) {
     uint32_t addr;
     float2 v;
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(rank));
     asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+QW_DEV float4 cluster_load4(const float* p, int rank) {
+    uint32_t addr;
+    float4 v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
 }
 
@@ -79,13 +86,15 @@ constexpr int WARP_SEQS = 128;  // up to here every warp works the plan out by i
 // A warp's view of up to WARP_SEQS sequences: lane l holds sequences 4 l .. 4 l + 3.
 struct WarpPlan {
     int n[4], at, total;  // tiles of the lane's sequences, first tile of its first one, all tiles
+    Kv4Rows rows[4];
     QW_DEV void make(const Kv4AttnArgs& a, int per_tile, bool report) {
         const int lane = threadIdx.x & 31;
         int s = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int b = 4 * lane + i;
-            n[i] = b < a.c.batch ? per_tile * tiles_of(kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, a.err, report)) : 0;
+            rows[i] = b < a.c.batch ? kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, a.err, report) : Kv4Rows{0, 0};
+            n[i] = per_tile * tiles_of(rows[i]);
             s += n[i];
         }
         at = s;
@@ -135,6 +144,7 @@ QW_DEV int block_prefix(int v, int* red) {
 struct Share {
     int begin, end;  // this block's tiles
     int b, b0;       // sequence of tile `begin` and its first tile
+    Kv4Rows rw;      // its rows
 };
 
 // This block's share.  For many sequences block 0 leaves the plan to the joining kernel.
@@ -149,6 +159,7 @@ QW_DEV Share take_share(const Kv4AttnArgs& a, int ncb, int* plan) {
         s.end = min(p.total, s.begin + per);
         s.b = B;
         s.b0 = 0;
+        s.rw = {0, 0};
         int at = p.at;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -157,6 +168,8 @@ QW_DEV Share take_share(const Kv4AttnArgs& a, int ncb, int* plan) {
                 const int l = __ffs(hit) - 1;
                 s.b = 4 * l + i;
                 s.b0 = __shfl_sync(0xffffffffu, at, l);
+                s.rw.off = __shfl_sync(0xffffffffu, p.rows[i].off, l);
+                s.rw.n = __shfl_sync(0xffffffffu, p.rows[i].n, l);
             }
             at += p.n[i];
         }
@@ -188,6 +201,7 @@ QW_DEV Share take_share(const Kv4AttnArgs& a, int ncb, int* plan) {
     __syncthreads();
     s.b = found[0];
     s.b0 = found[1];
+    s.rw = s.b < B ? kv4_rows(a.seq_len, a.n_new, s.b, a.S, a.c.max_pos, nullptr, false) : Kv4Rows{0, 0};
     return s;
 }
 
@@ -195,7 +209,7 @@ template <int D, int NT>
 struct SplitSmem {
     static constexpr int CB = 8 * NT;
     static constexpr int RING = AW * ASTAGES * Tile<D>::BYTES;
-    static constexpr int OLD = D + 2;  // output row of a warp's merge buffer, floats
+    static constexpr int OLD = D + 4;  // output row of a warp's merge buffer, floats
     static constexpr int MERGE = AW * CB * OLD * 4, BLOCK = CB * (D * 4 + 8);  // + the block's own sums (cluster form)
     static constexpr int BYTES = (RING > MERGE + BLOCK ? RING : MERGE + BLOCK) + AW * CB * 8;
 };
@@ -268,7 +282,7 @@ QW_DEV void run_tiles(const Kv4AttnArgs& a, const Kv4Rows& rw, int b, int h, int
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) wml[warp * CB + 8 * n + 2 * t + e] = make_float2(st.base(n, e), st.l[n][e]);
+            for (int e = 0; e < 2; ++e) wml[warp * CB + 8 * n + 2 * t + e].x = st.base(n, e);
     __syncthreads();  // also: every warp has left its ring
     if (mine > 0)
 #pragma unroll
@@ -280,6 +294,7 @@ QW_DEV void run_tiles(const Kv4AttnArgs& a, const Kv4Rows& rw, int b, int h, int
 #pragma unroll
                 for (int w = 1; w < AW; ++w) M = fmaxf(M, wml[w * CB + col].x);
                 const float f = half_pow(st.base(n, e) - M);
+                if (g == 0) wml[warp * CB + col].y = st.l[n][e] * f * f;
                 float* dst = wo + (warp * CB + col) * SM::OLD + 4 * g;
 #pragma unroll
                 for (int gr = 0; gr < D / 64; ++gr)
@@ -292,37 +307,46 @@ QW_DEV void run_tiles(const Kv4AttnArgs& a, const Kv4Rows& rw, int b, int h, int
     __syncthreads();
 }
 
-// Sum over the block's warps of column col, dimensions d, d + 1 (warps whose base is M0 have written nothing).
+// Sum over the block's first `warps` warps (those that had tiles) of column col, dimensions d .. d + 3,
+// relative to the block's base M.
 template <int D, int NT>
-QW_DEV float2 warps_sum(const unsigned char* smem, int col, int d, float& M, float& l) {
+QW_DEV float4 warps_sum(const unsigned char* smem, int warps, int col, int d, float& M, float& l) {
     using SM = SplitSmem<D, NT>;
     const float2* wml = reinterpret_cast<const float2*>(smem + SM::BYTES - AW * SM::CB * 8);
     const float* wo = reinterpret_cast<const float*>(smem);
-    M = wml[col].x;
-#pragma unroll
-    for (int w = 1; w < AW; ++w) M = fmaxf(M, wml[w * SM::CB + col].x);
+    M = M0;
     l = 0.f;
-    float2 o = make_float2(0.f, 0.f);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < AW; ++w) {
-        const float2 ml = wml[w * SM::CB + col];
-        if (ml.x == M0) continue;
-        const float f = half_pow(ml.x - M);
-        l = fmaf(ml.y * f, f, l);
-        const float2 v = *reinterpret_cast<const float2*>(wo + (w * SM::CB + col) * SM::OLD + d);
-        o.x += v.x;
-        o.y += v.y;
+    for (int w0 = 0; w0 < AW; w0 += 4) {
+        float2 ml[4];
+        float4 v[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            ml[w] = w0 + w < warps ? wml[(w0 + w) * SM::CB + col] : make_float2(M0, 0.f);
+            v[w] = w0 + w < warps ? *reinterpret_cast<const float4*>(wo + ((w0 + w) * SM::CB + col) * SM::OLD + d)
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            M = fmaxf(M, ml[w].x);
+            l += ml[w].y;
+            o.x += v[w].x;
+            o.y += v[w].y;
+            o.z += v[w].z;
+            o.w += v[w].w;
+        }
     }
     return o;
 }
 
-// Output of column c, dimensions d, d + 1, from its sums.
-QW_DEV void write_out(const Kv4AttnArgs& a, const Kv4Rows& rw, int b, int h, int c, int d, float2 o, float M, float l) {
+// Output of column c, dimensions d .. d + 3, from its sums.
+QW_DEV void write_out(const Kv4AttnArgs& a, const Kv4Rows& rw, int b, int h, int c, int d, float4 o, float M, float l) {
     const int G = a.Hq / a.c.heads, i = c / G;
     const bool has = i < rw.n && l != 0.f;
     const float inv = has ? 1.f / l : 0.f;
     bf16* dst = a.out + (b * a.os.b + i * a.os.s + (h * G + c % G) * a.os.h) + d;
-    *reinterpret_cast<uint32_t*>(dst) = has ? pack_bf16x2(o.x * inv, o.y * inv) : 0u;
+    *reinterpret_cast<uint2*>(dst) = has ? make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv)) : make_uint2(0u, 0u);
     if (d == 0 && a.lse) a.lse[((size_t)b * a.S + i) * a.Hq + h * G + c % G] = has ? (M + log2f(l)) * LN2 : -INFINITY;
 }
 
@@ -331,35 +355,39 @@ __global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(co
     constexpr int CB = 8 * NT;
     extern __shared__ __align__(128) unsigned char smem[];
     const int tid = threadIdx.x, C = a.Hq / a.c.heads * a.S;
-    pdl_launch_dependents();  // the joining kernel's blocks may settle in; they wait for this kernel's end
+    pdl_wait();
+    // the dependent kernel's blocks may settle in: they wait for this kernel's end before they touch what it
+    // writes, and read the lengths and the cache, which only earlier kernels write, while it runs
+    pdl_launch_dependents();
     const Share sh = take_share(a, ncb, plan);
     int u = sh.begin, b0 = sh.b0, b = sh.b;
+    Kv4Rows rw = sh.rw;
     while (u < sh.end) {
-        const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
         const int nt = tiles_of(rw);
         const int nseq = nt * a.c.heads * ncb;
         if (u >= b0 + nseq) {  // the next sequence (some are empty)
             b0 += nseq;
             ++b;
+            rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
             continue;
         }
-        const int seg = (u - b0) / nt, t0 = (u - b0) % nt;
+        const int seg = (u - b0) / nt, t0 = u - b0 - seg * nt;
         const int t1 = min(nt, t0 + (sh.end - u));
-        const int h = seg / ncb, cb = seg % ncb;
+        const int h = ncb == 1 ? seg : seg / ncb, cb = seg - h * ncb;
         RawCol<D> raw[NT];
         fetch_cols<D, NT>(a, b, h, cb, raw);
         run_tiles<D, NT>(a, rw, b, h, cb, raw, t0 + (tid >> 5), AW, t1, smem);
         const bool whole = t0 == 0 && t1 == nt;
         const size_t slot = 2 * (size_t)blockIdx.x + (u == sh.begin ? 0 : 1);
-        for (int idx = tid; idx < CB * (D / 2); idx += ANT) {
-            const int col = idx / (D / 2), d = 2 * (idx % (D / 2)), c = cb * CB + col;
+        for (int idx = tid; idx < CB * (D / 4); idx += ANT) {
+            const int col = idx / (D / 4), d = 4 * (idx % (D / 4)), c = cb * CB + col;
             if (c >= C) break;
             float M, l;
-            const float2 o = warps_sum<D, NT>(smem, col, d, M, l);
+            const float4 o = warps_sum<D, NT>(smem, min(AW, t1 - t0), col, d, M, l);
             if (whole) {
                 write_out(a, rw, b, h, c, d, o, M, l);
             } else {
-                *reinterpret_cast<float2*>(part + (slot * CB + col) * D + d) = o;
+                *reinterpret_cast<float4*>(part + (slot * CB + col) * D + d) = o;
                 if (d == 0) pml[slot * CB + col] = make_float2(M, l);
             }
         }
@@ -377,6 +405,7 @@ __global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_cluster_kernel(
     extern __shared__ __align__(128) unsigned char smem[];
     float* bo = reinterpret_cast<float*>(smem + SM::MERGE);       // [column][D] of this block
     float2* bml = reinterpret_cast<float2*>(bo + CB * D);         // [column]
+    pdl_wait();
     pdl_launch_dependents();
     const int tid = threadIdx.x, C = a.Hq / a.c.heads * a.S;
     const int rank = blockIdx.x % cluster, seg = blockIdx.x / cluster;
@@ -385,39 +414,43 @@ __global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_cluster_kernel(
     fetch_cols<D, NT>(a, b, h, cb, raw);  // before the length arrives
     const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, a.err, rank == 0 && h == 0 && cb == 0 && tid == 0);
     run_tiles<D, NT>(a, rw, b, h, cb, raw, (tid >> 5) * cluster + rank, AW * cluster, tiles_of(rw), smem);
-    for (int idx = tid; idx < CB * (D / 2); idx += ANT) {
-        const int col = idx / (D / 2), d = 2 * (idx % (D / 2)), c = cb * CB + col;
+    const int nt = tiles_of(rw);
+    for (int idx = tid; idx < CB * (D / 4); idx += ANT) {
+        const int col = idx / (D / 4), d = 4 * (idx % (D / 4)), c = cb * CB + col;
         if (c >= C) break;
-        float M, l;
-        const float2 o = warps_sum<D, NT>(smem, col, d, M, l);
+        float M, l;  // warp w has tiles when w * cluster + rank < nt
+        const float4 o = warps_sum<D, NT>(smem, max(0, min(AW, (nt - rank + cluster - 1) / cluster)), col, d, M, l);
         if (cluster == 1) {
             write_out(a, rw, b, h, c, d, o, M, l);
         } else {
-            *reinterpret_cast<float2*>(bo + col * D + d) = o;
+            *reinterpret_cast<float4*>(bo + col * D + d) = o;
             if (d == 0) bml[col] = make_float2(M, l);
         }
     }
     if (cluster == 1) return;
     cluster_sync();
-    for (int idx = rank * ANT + tid; idx < CB * (D / 2); idx += cluster * ANT) {
-        const int col = idx / (D / 2), d = 2 * (idx % (D / 2)), c = cb * CB + col;
+    for (int idx = rank * ANT + tid; idx < CB * (D / 4); idx += cluster * ANT) {
+        const int col = idx / (D / 4), d = 4 * (idx % (D / 4)), c = cb * CB + col;
         if (c >= C) break;
-        float2 ml[MAX_CLUSTER], v[MAX_CLUSTER];
+        float2 ml[MAX_CLUSTER];
+        float4 v[MAX_CLUSTER];
 #pragma unroll
         for (int r = 0; r < MAX_CLUSTER; ++r) {
             ml[r] = r < cluster ? cluster_load2(&bml[col].x, r) : make_float2(M0, 0.f);
-            v[r] = r < cluster ? cluster_load2(&bo[col * D + d], r) : make_float2(0.f, 0.f);
+            v[r] = r < cluster ? cluster_load4(&bo[col * D + d], r) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
         float M = M0, l = 0.f;
 #pragma unroll
         for (int r = 0; r < MAX_CLUSTER; ++r) M = fmaxf(M, ml[r].x);
-        float2 o = make_float2(0.f, 0.f);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int r = 0; r < MAX_CLUSTER; ++r) {
             const float f = half_pow(ml[r].x - M);
             l = fmaf(ml[r].y * f, f, l);
             o.x = fmaf(v[r].x * f, f, o.x);
             o.y = fmaf(v[r].y * f, f, o.y);
+            o.z = fmaf(v[r].z * f, f, o.z);
+            o.w = fmaf(v[r].w * f, f, o.w);
         }
         write_out(a, rw, b, h, c, d, o, M, l);
     }
@@ -590,7 +623,10 @@ __global__ void __launch_bounds__(ANT, 2) kv4_mass_kernel(const Kv4AttnArgs a) {
     const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
     const int T = rw.off + rw.n;
     const int block0 = blockIdx.x * AW * MK, key0 = block0 + warp * MK;
-    if (block0 >= T) return;
+    if (block0 >= T) {
+        pdl_wait();
+        return;
+    }
     const size_t bh = (size_t)b * a.c.heads + h;
     MassKeys<D, 1> keys;
     fetch_keys<D, 1>(keys, a.c, bh, key0, T, lane);
@@ -723,11 +759,11 @@ cudaError_t launch_split(const Kv4AttnArgs& a, const Shape& sp, const Scratch& s
         const cudaError_t e = ensure_max_dyn_smem(kv4_attn_cluster_kernel<D, NT>, smem);
         if (e != cudaSuccess) return e;
         const unsigned blocks = (unsigned)(sp.cluster * sp.ncb * a.c.heads) * (unsigned)a.c.batch;
-        return launch(kv4_attn_cluster_kernel<D, NT>, dim3(blocks), dim3(ANT), smem, st, false, sp.cluster, a, sp.ncb, sp.cluster);
+        return launch(kv4_attn_cluster_kernel<D, NT>, dim3(blocks), dim3(ANT), smem, st, true, sp.cluster, a, sp.ncb, sp.cluster);
     }
     cudaError_t e = ensure_max_dyn_smem(kv4_attn_split_kernel<D, NT>, smem);
     if (e != cudaSuccess) return e;
-    e = launch(kv4_attn_split_kernel<D, NT>, dim3(sp.shares), dim3(ANT), smem, st, false, 1, a, sp.ncb, sc.plan, sc.part, sc.ml);
+    e = launch(kv4_attn_split_kernel<D, NT>, dim3(sp.shares), dim3(ANT), smem, st, true, 1, a, sp.ncb, sc.plan, sc.part, sc.ml);
     if (e != cudaSuccess) return e;
     return launch(kv4_attn_join_kernel<D>, dim3((unsigned)(a.S * a.Hq), a.c.batch), dim3(32 * JOIN_WARPS), 0, st, true, 1, a, sp.cb, sp.ncb,
                   sp.shares, (const int*)sc.plan, (const float*)sc.part, (const float2*)sc.ml);

@@ -171,6 +171,8 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
     float* kvmax = reinterpret_cast<float*>(tmem_slot + 2);  // [8 NB][2] of the warps: largest |K|, |V|
     float* xch = reinterpret_cast<float*>(sm + 1024);       // [round][half][CB]: largest scores; in the end the halves' sums
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_wait();
+    pdl_launch_dependents();
 
     // heaviest column blocks first
     const int per_cb = nsplit * a.c.heads * a.c.batch;
@@ -647,7 +649,10 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) kv4_attn_tc_join_kernel(const
     const int b = blockIdx.y, G = a.Hq / a.c.heads, lane = threadIdx.x & 31;
     const int item = blockIdx.x * JOIN_WARPS + (threadIdx.x >> 5), h = item % a.Hq, i = item / a.Hq;
     const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
-    if (i >= a.S) return;
+    if (i >= a.S) {
+        pdl_wait();
+        return;
+    }
     const int c = i * G + h % G, cb = c / cb_size, C = G * a.S;
     const int i_last = min(rw.n, (min(C, (cb + 1) * cb_size) - 1) / G + 1) - 1;
     const int T = rw.off + rw.n, nt = ((a.causal ? min(T, rw.off + i_last + 1) : T) + KT - 1) / KT;
@@ -689,7 +694,7 @@ cudaError_t launch_tc(const Kv4AttnArgs& a, const TcShape& sp, float* part, floa
     if (e != cudaSuccess) return e;
     const long long blocks = (long long)sp.ncb * sp.nsplit * a.c.heads * a.c.batch;
     if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
-    e = launch(kv4_attn_tc_kernel<D, NB>, dim3((unsigned)blocks), dim3(THREADS<NB>), smem, st, false, a, sp.ncb, sp.nsplit, part, ml);
+    e = launch(kv4_attn_tc_kernel<D, NB>, dim3((unsigned)blocks), dim3(THREADS<NB>), smem, st, true, a, sp.ncb, sp.nsplit, part, ml);
     if (e != cudaSuccess || sp.nsplit == 1) return e;
     return launch(kv4_attn_tc_join_kernel<D>, dim3((unsigned)((a.S * (long long)a.Hq + JOIN_WARPS - 1) / JOIN_WARPS), a.c.batch), dim3(32 * JOIN_WARPS), 0, st, true, a, CM * NB, sp.ncb,
                   sp.nsplit, (const float*)part, (const float2*)ml);

@@ -82,6 +82,7 @@ __global__ void __launch_bounds__(SEL_NT, 2) kv4_select_kernel(const Kv4EvictArg
     __shared__ int wsum[3][32], pick[3][2];
     const int rank = blockIdx.x % cluster, h = blockIdx.x / cluster, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31,
               warp = tid >> 5;
+    pdl_wait();
     pdl_launch_dependents();
     const int n = clamp_len(a, b);
     const size_t bh = (size_t)b * a.src.heads + h;
@@ -221,6 +222,7 @@ __global__ void __launch_bounds__(256) kv4_move_kernel(const Kv4EvictArgs a, con
     const int part = blockIdx.y / a.src.heads, h = blockIdx.y % a.src.heads, b = blockIdx.z, tid = threadIdx.x;
     const size_t bh = (size_t)b * a.src.heads + h;
     pdl_wait();
+    pdl_launch_dependents();
     const int n = count[b];
     const int* idx = index + bh * a.keep;
     const size_t s0 = bh * a.src.max_pos, d0 = bh * a.dst.max_pos;
@@ -280,6 +282,7 @@ __global__ void __launch_bounds__(1024) kv4_move_inplace_kernel(const Kv4EvictAr
     const int part = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const size_t bh = (size_t)b * a.src.heads + h;
     pdl_wait();
+    pdl_launch_dependents();
     const int n = count[b];
     const int* idx = index + bh * a.keep;
     const size_t row0 = bh * a.src.max_pos;
@@ -369,7 +372,7 @@ cudaError_t launch_kv4_evict(const Kv4EvictArgs& a, void* scratch, cudaStream_t 
     const int smem = (3 * BINS + keys) * (int)sizeof(int);
     cudaError_t e = ensure_max_dyn_smem(kv4_select_kernel, (3 * BINS + SEL_KEYS) * (int)sizeof(int));
     if (e != cudaSuccess) return e;
-    e = launch(kv4_select_kernel, dim3(a.src.heads * cluster, a.src.batch), dim3(SEL_NT), smem, cluster, st, false, a, cluster,
+    e = launch(kv4_select_kernel, dim3(a.src.heads * cluster, a.src.batch), dim3(SEL_NT), smem, cluster, st, true, a, cluster,
                keys, index, count);
     if (e != cudaSuccess) return e;
     const bool wide = a.src.D == 128;

@@ -79,6 +79,8 @@ QW_DEV uint32_t quantize8(const float (&x)[8], float bias, float scale) {
 template <int D, bool VEC, int R>
 __global__ void __launch_bounds__(NT) kv4_append_kernel(const Kv4StoreArgs a) {
     constexpr int T = TPR<D>, RB = NT / T;
+    pdl_wait();
+    pdl_launch_dependents();
     const int which = blockIdx.y / a.c.heads, h = blockIdx.y % a.c.heads, b = blockIdx.z;
     const int i0 = blockIdx.x * (R * RB) + threadIdx.x / T, e = threadIdx.x % T;
     const bf16* src = a.x[which] + (b * a.xs[which].b + h * a.xs[which].h) + e * 8;
@@ -152,6 +154,8 @@ __global__ void __launch_bounds__(NT) kv4_append_kernel(const Kv4StoreArgs a) {
 template <int D, int R>
 __global__ void __launch_bounds__(NT) kv4_read_kernel(const Kv4ReadArgs a) {
     constexpr int T = TPR<D>, RB = NT / T;
+    pdl_wait();
+    pdl_launch_dependents();
     const int which = blockIdx.y / a.c.heads, h = blockIdx.y % a.c.heads, b = blockIdx.z;
     const int i0 = blockIdx.x * (R * RB) + threadIdx.x / T, e = threadIdx.x % T;
     const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, a.err,
@@ -194,19 +198,33 @@ int rows_per_thread(const Kv4View& c, int S) {
     return (long long)((S + rb - 1) / rb) * 2 * c.heads * c.batch > 2 * 8 * 148 ? 4 : 1;
 }
 
+// Programmatic launch, as the library's other kernels: the blocks start while the kernel before drains and wait
+// for it before they touch memory.
+template <typename K, typename A>
+cudaError_t launch(K kernel, dim3 grid, cudaStream_t st, const A& a) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(NT);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
 template <int D, int R>
 cudaError_t append_t(const Kv4StoreArgs& a, bool vec, cudaStream_t st) {
     const int rows = R * NT / TPR<D>;
     const dim3 grid((a.S + rows - 1) / rows, 2 * a.c.heads, a.c.batch);
-    vec ? kv4_append_kernel<D, true, R><<<grid, NT, 0, st>>>(a) : kv4_append_kernel<D, false, R><<<grid, NT, 0, st>>>(a);
-    return cudaGetLastError();
+    return vec ? launch(kv4_append_kernel<D, true, R>, grid, st, a) : launch(kv4_append_kernel<D, false, R>, grid, st, a);
 }
 template <int D, int R>
 cudaError_t read_t(const Kv4ReadArgs& a, cudaStream_t st) {
     const int rows = R * NT / TPR<D>;
     const dim3 grid((a.S + rows - 1) / rows, 2 * a.c.heads, a.c.batch);
-    kv4_read_kernel<D, R><<<grid, NT, 0, st>>>(a);
-    return cudaGetLastError();
+    return launch(kv4_read_kernel<D, R>, grid, st, a);
 }
 
 }  // namespace
