@@ -241,11 +241,15 @@ QW_DEV void run_tiles(const Kv4AttnArgs& a, const Kv4Rows& rw, int b, int h, int
     const int G = a.Hq / a.c.heads, T = rw.off + rw.n;
     const uint32_t ring = smem_u32(smem) + warp * ASTAGES * L::BYTES;
     const unsigned char* ringp = smem + warp * ASTAGES * L::BYTES;
-    const Rows rows = head_rows<D>(a.c, (size_t)b * a.c.heads + h);
     const int mine = max(0, (t1 - first + step - 1) / step);
+    TileLoader<D> loader;
+    loader.start(head_rows<D>(a.c, (size_t)b * a.c.heads + h), first * TK, step, lane);
+    const uint32_t lane_chunk = L::chunk_pos(lane / L::CPR, lane % L::CPR) * 16;
+    int fill = 0;  // byte offset of the stage that the next tile goes to
     auto issue = [&](int k) {
-        if (k < mine) load_tile<D>(ring + (k % ASTAGES) * L::BYTES, rows, (first + k * step) * TK, T, lane);
+        if (k < mine) loader.copy(ring + fill, ring + fill + lane_chunk, T, lane);
         cp_async_commit();
+        fill = fill == (ASTAGES - 1) * L::BYTES ? 0 : fill + L::BYTES;
     };
 #pragma unroll
     for (int k = 0; k < ASTAGES - 1; ++k) issue(k);
@@ -264,16 +268,18 @@ QW_DEV void run_tiles(const Kv4AttnArgs& a, const Kv4Rows& rw, int b, int h, int
         }
     }
     const int all = a.causal ? min(T, rw.off + cb * CB / G + 1) : T;  // keys that every column sees
+    const unsigned char* tile = ringp;
+    int key0 = first * TK;
     for (int k = 0; k < mine; ++k) {
         cp_async_wait<ASTAGES - 2>();
         __syncwarp();
         issue(k + ASTAGES - 1);  // into the stage that the warp left in the turn before
-        const int key0 = (first + k * step) * TK;
-        const unsigned char* tile = ringp + (k % ASTAGES) * L::BYTES;
         if (key0 + TK <= all)
             attend_tile<D, NT, false>(st, cols, tile, key0, T, vis, lane);
         else
             attend_tile<D, NT, true>(st, cols, tile, key0, T, vis, lane);
+        key0 += step * TK;
+        tile = tile == ringp + (ASTAGES - 1) * L::BYTES ? ringp : tile + L::BYTES;
         __syncwarp();
     }
     cp_async_wait<0>();

@@ -72,41 +72,56 @@ QW_DEV Rows head_rows(const Kv4View& c, size_t bh) {
     return r;
 }
 
-// Keys [key0, key0 + 32) into the tile at shared address `dst`, by the lanes of
-// one warp; rows from T on arrive as zeros (scales and biases in pieces of 16
-// bytes, so up to 7 rows past T may hold what the cache has there).
+// Copies tiles of 32 keys, key0, key0 + 32 step, ... into shared memory, by the
+// lanes of one warp; rows from T on arrive as zeros (scales and biases in pieces
+// of 16 bytes, so up to 7 rows past T may hold what the cache has there).  The
+// addresses only move by constants from tile to tile.
 template <int D>
-QW_DEV void load_tile(uint32_t dst, const Rows& r, int key0, int T, int lane) {
+struct TileLoader {
     using L = Tile<D>;
-    constexpr int CH = TK * L::CPR;              // 16-byte chunks of the tile's words
-    constexpr int SC = L::SBB / 16, KPC = TK / SC;  // 16-byte pieces of a scale array, keys of a piece
-    // a row group of 32 chunks further on is a fixed distance away on both sides
-    const uint32_t d = dst + L::chunk_pos(lane / L::CPR, lane % L::CPR) * 16;
-    const unsigned char* s[2] = {r.w[0] + (size_t)key0 * L::ROWB + lane * 16, r.w[1] + (size_t)key0 * L::ROWB + lane * 16};
-    const int arr = lane / SC, piece = lane % SC;
-    const unsigned char* sb = (arr & 2 ? (arr & 1 ? r.b[1] : r.s[1]) : (arr & 1 ? r.b[0] : r.s[0])) +
-                              (size_t)key0 * (2 * L::GR) + piece * 16;
-    const uint32_t sd = dst + L::SB + lane * 16;
-    if (key0 + TK <= T) {
-#pragma unroll
-        for (int w = 0; w < 2; ++w)
-#pragma unroll
-            for (int i = 0; i < CH / 32; ++i) cp_async16(d + w * L::VW + i * 512, s[w] + i * 512);
-        if (lane < 4 * SC) cp_async16(sd, sb);
-    } else {
-#pragma unroll
-        for (int w = 0; w < 2; ++w)
+    static constexpr int CH = TK * L::CPR;                 // 16-byte chunks of the tile's words
+    static constexpr int SC = L::SBB / 16, KPC = TK / SC;  // 16-byte pieces of a scale array, keys of a piece
+    const unsigned char *w0, *w1, *sb;                     // this lane's first chunk of K and V words, its scale piece
+    const unsigned char* safe;                             // a readable address for chunks that are not copied
+    int key, keys;                                         // first key of the next tile, keys from tile to tile
+    QW_DEV void start(const Rows& r, int key0, int step, int lane) {
+        const int arr = (lane / SC) & 3, piece = lane % SC;
+        key = key0;
+        keys = step * TK;
+        safe = r.w[0];
+        w0 = r.w[0] + (size_t)key0 * L::ROWB + lane * 16;
+        w1 = r.w[1] + (size_t)key0 * L::ROWB + lane * 16;
+        sb = (arr & 2 ? (arr & 1 ? r.b[1] : r.s[1]) : (arr & 1 ? r.b[0] : r.s[0])) + (size_t)key0 * (2 * L::GR) + piece * 16;
+    }
+    // into the tile at shared address `dst`, of which `to` is this lane's first chunk of words
+    QW_DEV void copy(uint32_t dst, uint32_t to, int T, int lane) {
+        const uint32_t sd = dst + L::SB + lane * 16;
+        if (key + TK <= T) {
+            // a row group of 32 chunks further on is a fixed distance away on both sides
 #pragma unroll
             for (int i = 0; i < CH / 32; ++i) {
-                const bool ok = key0 + (lane + 32 * i) / L::CPR < T;
-                cp_async16_zfill(d + w * L::VW + i * 512, ok ? s[w] + i * 512 : r.w[w], ok);
+                cp_async16(to + i * 512, w0 + i * 512);
+                cp_async16(to + L::VW + i * 512, w1 + i * 512);
             }
-        if (lane < 4 * SC) {
-            const bool ok = key0 + piece * KPC < T;
-            cp_async16_zfill(sd, ok ? sb : r.s[0], ok);
+            if (lane < 4 * SC) cp_async16(sd, sb);
+        } else {
+#pragma unroll
+            for (int i = 0; i < CH / 32; ++i) {
+                const bool ok = key + (lane + 32 * i) / L::CPR < T;
+                cp_async16_zfill(to + i * 512, ok ? w0 + i * 512 : safe, ok);
+                cp_async16_zfill(to + L::VW + i * 512, ok ? w1 + i * 512 : safe, ok);
+            }
+            if (lane < 4 * SC) {
+                const bool ok = key + lane % SC * KPC < T;
+                cp_async16_zfill(sd, ok ? sb : safe, ok);
+            }
         }
+        key += keys;
+        w0 += (size_t)keys * L::ROWB;
+        w1 += (size_t)keys * L::ROWB;
+        sb += (size_t)keys * (2 * L::GR);
     }
-}
+};
 
 // Query columns of a warp: 8 NT of them.
 template <int D, int NT>
