@@ -20,7 +20,7 @@
 namespace qw {
 namespace {
 
-constexpr int SEL_NT = 1024;
+constexpr int SEL_NT = 512, SEL_W = SEL_NT / 32;
 constexpr int BINS = 2048;
 constexpr int SEL_MAX_CLUSTER = 8;
 constexpr int SEL_KEYS = 40960;  // keys of a slice held in shared memory; longer slices are read again per pass
@@ -39,7 +39,7 @@ QW_DEV void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
-// The pair of ints at `p` in the cluster's block `rank`.
+// Ints at `p` in the cluster's block `rank`.
 QW_DEV uint32_t cluster_addr(const int* p, int rank) {
     uint32_t addr;
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(rank));
@@ -48,6 +48,14 @@ QW_DEV uint32_t cluster_addr(const int* p, int rank) {
 QW_DEV int2 cluster_load2(const int* p, int rank) {
     int2 v;
     asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(cluster_addr(p, rank)) : "memory");
+    return v;
+}
+QW_DEV int4 cluster_load4(const int* p, int rank) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(cluster_addr(p, rank))
+                 : "memory");
     return v;
 }
 
@@ -65,14 +73,13 @@ QW_DEV void block_scan2(int& v, int& w, int2* red, int2& total) {
     }
     if (lane == 31) red[warp] = make_int2(s, r);
     __syncthreads();
-    const int2 p = red[lane];  // every warp: the warps before it, and all
+    const int2 p = lane < SEL_W ? red[lane] : make_int2(0, 0);  // every warp: the warps before it, and all
     total = make_int2(__reduce_add_sync(0xffffffffu, p.x), __reduce_add_sync(0xffffffffu, p.y));
     v = s - v + __reduce_add_sync(0xffffffffu, lane < warp ? p.x : 0);
     w = r - w + __reduce_add_sync(0xffffffffu, lane < warp ? p.y : 0);
 }
 
 // index[b][h][0..new length): the kept positions in increasing order.
-// (two blocks per SM: at most 32 registers a thread)
 __global__ void __launch_bounds__(SEL_NT, 2) kv4_select_kernel(const Kv4EvictArgs a, int cluster, int slice_keys, int* index,
                                                             int* count) {
     extern __shared__ __align__(16) int sel_smem[];
@@ -113,55 +120,69 @@ __global__ void __launch_bounds__(SEL_NT, 2) kv4_select_kernel(const Kv4EvictArg
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
             const uint32_t mask = pass == 2 ? 1023u : 2047u;
             int* hp = hist + pass * BINS;
-            for (int j = j0 + tid; j < jo; j += SEL_NT) {
-                uint32_t k;
-                if (pass == 0) {
-                    k = order_key(mass[j]);
-                    if (held) sk[j - j0] = k;
-                } else {
-                    k = key(j);
-                    // every higher digit has to agree
-                    if ((k >> (pass == 1 ? 21 : 10)) != (prefix >> (pass == 1 ? 21 : 10))) continue;
+            if (pass == 0) {
+                for (int j = j0 + tid; j < jo; j += 8 * SEL_NT) {  // eight loads in flight
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = j + e * SEL_NT < jo ? mass[j + e * SEL_NT] : 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (j + e * SEL_NT < jo) {
+                            const uint32_t k = order_key(v[e]);
+                            if (held) sk[j + e * SEL_NT - j0] = k;
+                            atomicAdd(&hp[k >> shift], 1);
+                        }
                 }
-                atomicAdd(&hp[(k >> shift) & mask], 1);
+            } else {
+                const int above = pass == 1 ? 21 : 10;  // every higher digit has to agree
+                for (int j = j0 + tid; j < jo; j += SEL_NT) {
+                    const uint32_t k = key(j);
+                    if ((k >> above) == (prefix >> above)) atomicAdd(&hp[(k >> shift) & mask], 1);
+                }
             }
             if (cluster > 1)
                 cluster_sync();
             else
                 __syncthreads();
-            // warp w counts the 64 bins from 64 (31 - w) on, lane l the pair 2 (31 - l) of them:
-            // both in order from the largest digit down
-            const int d0 = 64 * (31 - warp) + 2 * (31 - lane);
-            int c1 = 0, c0 = 0;
+            // warp w counts the 128 bins from 128 (15 - w) on, lane l four of them from 4 (31 - l) on: warps, lanes
+            // and c[0..3] in order from the largest digit down
+            static_assert(BINS == 4 * SEL_NT, "four bins per thread");
+            const int d0 = 128 * (SEL_W - 1 - warp) + 4 * (31 - lane);
+            int c[4] = {0, 0, 0, 0};
             if (cluster > 1) {
-                int2 c[SEL_MAX_CLUSTER];
+                int4 v[SEL_MAX_CLUSTER];
 #pragma unroll
-                for (int r = 0; r < SEL_MAX_CLUSTER; ++r) c[r] = r < cluster ? cluster_load2(&hp[d0], r) : make_int2(0, 0);
+                for (int r = 0; r < SEL_MAX_CLUSTER; ++r) v[r] = r < cluster ? cluster_load4(&hp[d0], r) : make_int4(0, 0, 0, 0);
 #pragma unroll
                 for (int r = 0; r < SEL_MAX_CLUSTER; ++r) {
-                    c0 += c[r].x;
-                    c1 += c[r].y;
+                    c[0] += v[r].w;
+                    c[1] += v[r].z;
+                    c[2] += v[r].y;
+                    c[3] += v[r].x;
                 }
             } else {
-                c0 = hp[d0];
-                c1 = hp[d0 + 1];
+                const int4 v = *reinterpret_cast<const int4*>(&hp[d0]);
+                c[0] = v.w, c[1] = v.z, c[2] = v.y, c[3] = v.x;
             }
-            const int mine = __reduce_add_sync(0xffffffffu, c0 + c1);
+            const int own = c[0] + c[1] + c[2] + c[3], mine = __reduce_add_sync(0xffffffffu, own);
             if (lane == 0) wsum[pass][warp] = mine;
             __syncthreads();
             const int before = __reduce_add_sync(0xffffffffu, lane < warp ? wsum[pass][lane] : 0);
             if (before < left && left <= before + mine) {  // this warp's bins hold the threshold
-                int s = c0 + c1;
+                int s = own;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const int v = __shfl_up_sync(0xffffffffu, s, o);
                     if (lane >= o) s += v;
                 }
-                const int above = before + s - c0 - c1;
-                if (above < left && left <= above + c0 + c1) {
-                    const bool hi = left <= above + c1;
-                    pick[pass][0] = hi ? d0 + 1 : d0;
-                    pick[pass][1] = left - above - (hi ? 0 : c1);
+                int above = before + s - own;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (above < left && left <= above + c[e]) {
+                        pick[pass][0] = d0 + 3 - e;
+                        pick[pass][1] = left - above;
+                    }
+                    above += c[e];
                 }
             }
             __syncthreads();
@@ -273,12 +294,13 @@ __global__ void __launch_bounds__(256) kv4_move_kernel(const Kv4EvictArgs a, con
     }
 }
 
-// In place: one CTA per (sequence, head, K words | V words | the rest) walks the
-// kept rows in order, a chunk at a time: read, barrier, write.  index[r] >= r,
-// so the rows a chunk overwrites are never read by a later chunk.
+// In place: one block per (sequence, head, K words | V words | the rest) walks
+// the kept rows in order, a chunk at a time: read, barrier, write.  index[r] >= r,
+// so the rows a chunk overwrites are never read by a later chunk.  MR rows per
+// thread and chunk: a chunk costs two memory latencies and two barriers.
 template <int D>
 __global__ void __launch_bounds__(1024) kv4_move_inplace_kernel(const Kv4EvictArgs a, const int* index, const int* count) {
-    constexpr int P = D / 32;
+    constexpr int P = D / 32, GR = D / 64, RB = 1024 / P;
     const int part = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const size_t bh = (size_t)b * a.src.heads + h;
     pdl_wait();
@@ -286,31 +308,38 @@ __global__ void __launch_bounds__(1024) kv4_move_inplace_kernel(const Kv4EvictAr
     const int n = count[b];
     const int* idx = index + bh * a.keep;
     const size_t row0 = bh * a.src.max_pos;
+    if (part == 2 && h == 0 && tid == 0) a.new_len[b] = n;
+    if (n == 0 || idx[n - 1] == n - 1) return;  // every row stays where it is
     if (part < 2) {
-        uint4* w = reinterpret_cast<uint4*>(a.dst.p[part].w) + row0 * P;
-        for (int r0 = 0; r0 < n; r0 += 1024 / P) {
-            const int r = r0 + tid / P, e = tid % P;
-            uint4 v;
-            if (r < n) v = w[(size_t)idx[r] * P + e];
+        uint4* w = reinterpret_cast<uint4*>(a.dst.p[part].w) + row0 * P + tid % P;
+        for (int r0 = tid / P; r0 - tid / P < n; r0 += MR * RB) {
+            int j[MR];
+            uint4 v[MR];
+#pragma unroll
+            for (int i = 0; i < MR; ++i) j[i] = r0 + i * RB < n ? idx[r0 + i * RB] : -1;
+#pragma unroll
+            for (int i = 0; i < MR; ++i)
+                if (j[i] >= 0) v[i] = w[(size_t)j[i] * P];
             __syncthreads();
-            if (r < n) w[(size_t)r * P + e] = v;
+#pragma unroll
+            for (int i = 0; i < MR; ++i)
+                if (j[i] >= 0) w[(size_t)(r0 + i * RB) * P] = v[i];
             __syncthreads();
         }
         return;
     }
-    if (h == 0 && tid == 0) a.new_len[b] = n;
     for (int r0 = 0; r0 < n; r0 += 1024) {
         const int r = r0 + tid;
-        bf16 v[4 * (D / 64)];
+        bf16 v[4 * GR];
         float m = 0.f;
         if (r < n) {
             const size_t sr = row0 + idx[r];
 #pragma unroll
-            for (int g = 0; g < D / 64; ++g) {
-                v[4 * g] = a.dst.p[0].s[sr * (D / 64) + g];
-                v[4 * g + 1] = a.dst.p[0].b[sr * (D / 64) + g];
-                v[4 * g + 2] = a.dst.p[1].s[sr * (D / 64) + g];
-                v[4 * g + 3] = a.dst.p[1].b[sr * (D / 64) + g];
+            for (int g = 0; g < GR; ++g) {
+                v[4 * g] = a.dst.p[0].s[sr * GR + g];
+                v[4 * g + 1] = a.dst.p[0].b[sr * GR + g];
+                v[4 * g + 2] = a.dst.p[1].s[sr * GR + g];
+                v[4 * g + 3] = a.dst.p[1].b[sr * GR + g];
             }
             m = a.mass_dst[sr];
         }
@@ -318,11 +347,11 @@ __global__ void __launch_bounds__(1024) kv4_move_inplace_kernel(const Kv4EvictAr
         if (r < n) {
             const size_t dr = row0 + r;
 #pragma unroll
-            for (int g = 0; g < D / 64; ++g) {
-                a.dst.p[0].s[dr * (D / 64) + g] = v[4 * g];
-                a.dst.p[0].b[dr * (D / 64) + g] = v[4 * g + 1];
-                a.dst.p[1].s[dr * (D / 64) + g] = v[4 * g + 2];
-                a.dst.p[1].b[dr * (D / 64) + g] = v[4 * g + 3];
+            for (int g = 0; g < GR; ++g) {
+                a.dst.p[0].s[dr * GR + g] = v[4 * g];
+                a.dst.p[0].b[dr * GR + g] = v[4 * g + 1];
+                a.dst.p[1].s[dr * GR + g] = v[4 * g + 2];
+                a.dst.p[1].b[dr * GR + g] = v[4 * g + 3];
             }
             a.mass_dst[dr] = m;
         }
