@@ -830,6 +830,7 @@ void kv4_rows_arg(int S) { need(S >= 1 && S <= (1 << 24), "kv4: S must be 1..2^2
 void kv4_heads_arg(const qw::Kv4View& v, int S, int heads) {
     kv4_rows_arg(S);
     need(heads >= 1 && heads <= 65535 && heads % v.heads == 0, "kv4: heads must be a positive multiple of kv_heads");
+    need((long long)S * heads <= (1ll << 30), "kv4: S * heads must not exceed 2^30");
 }
 
 bool overlaps(const void* a, size_t na, const void* b, size_t nb) {
@@ -909,6 +910,9 @@ extern "C" int qw_kv4_attention(const qw_kv4* cache, const void* q, const int64_
              "kv4: q, out and scratch must be 16-byte aligned");
         need((a.os.b != 0 || a.c.batch == 1) && (a.os.s != 0 || S == 1) && (a.os.h != 0 || heads == 1),
              "kv4: out has a zero stride");
+        // every form reads a row's query before it writes that row, but the weights are computed after the output
+        need(q != out || (!mass && a.qs.b == a.os.b && a.qs.s == a.os.s && a.qs.h == a.os.h),
+             "kv4: out may be q only with the same strides and without mass");
         a.S = S;
         a.Hq = heads;
         a.causal = causal ? 1 : 0;

@@ -334,7 +334,8 @@ QW_API int qw_quantized_matmul_argmax_static(const void* x, const void* w, const
  *     rows; n_new_dev[b] (NULL: S) says how many of the S rows sequence b has.
  *     Rows that would lie past max_pos are left out, a sequence whose seq_len
  *     is outside [0, max_pos] counts as empty and without rows; a call that
- *     meets either sets bit 0 of *err_dev (int32, may be NULL).
+ *     meets either sets bit 0 of *err_dev (int32, may be NULL).  Bit 3 means
+ *     that a kernel's bounded wait gave up: its results are not valid.
  *   - strides are in elements, {sequence, row, head}, of a tensor
  *     [batch][S][heads][head_dim] with contiguous head_dim; NULL: contiguous.
  *   - no call allocates; scratch is the caller's (16-byte aligned, no initial
@@ -367,7 +368,12 @@ QW_API int qw_kv4_attention_scratch(const qw_kv4* cache, int S, int heads, size_
  * out[b][i][h] = softmax(scale * <q[b][i][h], k_j>) . v_j over the keys
  * j < seq_len[b] + n_new[b] of kv head h / (heads / kv_heads), with causal != 0
  * only j <= seq_len[b] + i.  q and out are bf16 (16-byte aligned, strides a
- * multiple of 8 elements).  lse (fp32 [batch][S][heads], may be NULL) receives
+ * multiple of 8 elements; out may be q itself, with the same strides and without
+ * mass, and shares no memory with it otherwise); S * heads is at most
+ * 2^30.  Stored values may come from another quantizer (negative scales
+ * included); a NaN among a row's visible K or V rows makes the output row NaN,
+ * as a whole or in the 64 dimensions of a NaN in V, and reaches no row that
+ * does not see it.  lse (fp32 [batch][S][heads], may be NULL) receives
  * the natural logarithm of each row's sum of exponentials; a row without keys
  * gives out = 0, lse = -inf.  mass (fp32 [batch][kv_heads][max_pos], may be
  * NULL) has every key's probability, summed over the sequence's rows and the

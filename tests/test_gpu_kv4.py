@@ -453,15 +453,13 @@ def test_attention_is_repeatable(S, G, T):
     assert torch.equal(one, two) and torch.equal(l1, l2) and torch.equal(*m)
 
 
-@pytest.mark.parametrize("S,Hq,Hkv,T,B", [(1, 32, 8, 20000, 1), (1, 8, 1, 9000, 2), (1, 16, 4, 700, 40),
-                                          (16, 16, 1, 4000, 1), (300, 4, 1, 3000, 1)])
-def test_attention_long(S, Hq, Hkv, T, B):
-    """Lengths that are split over many thread blocks, against a 64-bit computation on the GPU."""
+def _long(S, Hq, Hkv, T, B, D):
+    """A ragged call against a 64-bit computation on the GPU."""
     torch = _torch()
-    c = _filled(B, Hkv, T, 128)
+    c = _filled(B, Hkv, T, D)
     g = np.random.default_rng(T)
     total = [T] + [int(t) for t in g.integers(S, T + 1, B - 1)]
-    x = _rand((B, S, Hq, 128), 12, 1.5).cuda()
+    x = _rand((B, S, Hq, D), 12, 1.5).cuda()
     m = torch.zeros(B, Hkv, c.max_pos, device="cuda")
     out, lse = _attend(c, x, _dev([t - S for t in total]), mass=m)
     K, V = c.values64(0).cuda(), c.values64(1).cuda()
@@ -471,13 +469,13 @@ def test_attention_long(S, Hq, Hkv, T, B):
         for h in range(Hkv):
             qr = x[b, :, h * G:(h + 1) * G].double()
             k, v = K[b, h, :t], V[b, h, :t]
-            s = torch.einsum("igd,jd->igj", qr, k) * 128 ** -0.5
+            s = torch.einsum("igd,jd->igj", qr, k) * D ** -0.5
             hide = torch.arange(t, device="cuda")[None, :] > torch.arange(t - S, t, device="cuda")[:, None]
             s = s.masked_fill(hide[:, None], -float("inf"))
             z = torch.logsumexp(s, -1)
             p = torch.exp(s - z[..., None])
             ref = torch.einsum("igj,jd->igd", p, v)
-            e = (2.0 ** -11 + 2.0 ** -16) * 128 ** -0.5 * torch.einsum("igd,jd->igj", qr.abs(), k.abs()).amax(-1)
+            e = (2.0 ** -11 + 2.0 ** -16) * D ** -0.5 * torch.einsum("igd,jd->igj", qr.abs(), k.abs()).amax(-1)
             tol = 3 * v.abs().max() * (2.0 ** -10 + torch.expm1(2 * e))[..., None] + 2.0 ** -8 * ref.abs()
             assert ((out[b, :, h * G:(h + 1) * G].double() - ref).abs() <= tol).all()
             assert ((lse[b, :, h * G:(h + 1) * G].double() - z).abs() <= e + 2.0 ** -20 * (1 + z.abs())).all()
@@ -485,6 +483,97 @@ def test_attention_long(S, Hq, Hkv, T, B):
             pm = p.sum((0, 1))
             assert ((m[b, h, :t].double() - pm).abs() <= em + 2.0 ** -18 * (1 + pm)).all()
         assert (m[b, :, t:] == 0).all()
+
+
+@pytest.mark.parametrize("S,Hq,Hkv,T,B", [(1, 32, 8, 20000, 1), (1, 8, 1, 9000, 2), (1, 16, 4, 700, 40),
+                                          (16, 16, 1, 4000, 1), (300, 4, 1, 3000, 1)])
+def test_attention_long(S, Hq, Hkv, T, B):
+    """Lengths that are split over many thread blocks."""
+    _long(S, Hq, Hkv, T, B, 128)
+
+
+@pytest.mark.parametrize("S,Hq,Hkv,T,B,D", [(1, 16, 1, 9000, 2, 128), (5, 8, 2, 9001, 1, 128), (5, 8, 2, 5000, 3, 64),
+                                            (1, 6, 1, 12345, 1, 64), (1, 64, 1, 3001, 2, 128), (130, 2, 1, 4111, 2, 64),
+                                            (40, 8, 2, 2500, 3, 128), (700, 2, 1, 701, 1, 128)])
+def test_attention_long_forms(S, Hq, Hkv, T, B, D):
+    """More columns per kv head and both head sizes, where the keys are split."""
+    _long(S, Hq, Hkv, T, B, D)
+
+
+def test_attention_of_many_sequences_in_a_long_cache():
+    """More sequences than a warp plans for, many of them empty, some without new rows."""
+    torch = _torch()
+    B, H, D, T = 150, 1, 64, 2048
+    c = Cache(B, H, T, D)
+    g = np.random.default_rng(5)
+    total = g.integers(1, 300, B)
+    total[::7] = 0
+    total[3] = 2048
+    n = np.where(total > 0, 1, 0)
+    k = _rand((B, 2048, H, D), 1).cuda()
+    _append(c, k, k, _dev([0] * B), _dev(total))
+    x = _rand((B, 1, 4, D), 2).cuda()
+    seq, new = _dev(total - n), _dev(n)
+    err = _dev([0])
+    _check_attention(c, x, seq, new, mass=True, err=err)
+    assert int(err) == 0
+
+
+@pytest.mark.parametrize("S,Hq", [(96, 4), (200, 2), (7, 4)])
+def test_attention_padded_batch_in_a_long_cache(S, Hq):
+    """Rows past n_new and empty sequences where the keys are split over thread blocks; padding queries are NaN."""
+    torch = _torch()
+    B, H, D, T = 4, 2, 128, 6000
+    c = Cache(B, H, 6400, D)
+    k = _rand((B, T, H, D), 1).cuda()
+    lens, n = [5000, 0, 0, 17], [S, 3, 0, S // 2]
+    for b in range(B):
+        t = lens[b] + n[b]
+        _append(c, k, k, _dev([0] * B), _dev([t if i == b else 0 for i in range(B)]))
+    x = _rand((B, S, Hq, D), 4)
+    for b in range(B):
+        x[b, n[b]:] = float("nan")
+    out, lse = _attend(c, x.cuda(), _dev(lens), _dev(n))
+    ref = _attend(c, torch.nan_to_num(x).cuda(), _dev(lens), _dev(n))
+    assert torch.equal(out, ref[0]) and torch.equal(lse, ref[1])
+    for b in range(B):
+        assert (out[b, n[b]:] == 0).all() and (lse[b, n[b]:] == -float("inf")).all()
+        assert torch.isfinite(out[b, :n[b]].float()).all()
+    rows = [0, 1, 2, n[3] - 1]  # a few rows against the formula
+    K, V = c.values64(0).cuda(), c.values64(1).cuda()
+    for b in (0, 1, 3):
+        for i in [r for r in rows if r < n[b]]:
+            for h in range(Hq):
+                kk, vv = K[b, h // (Hq // H), :lens[b] + i + 1], V[b, h // (Hq // H), :lens[b] + i + 1]
+                s = (kk @ x[b, i, h].cuda().double()) * D ** -0.5
+                p = torch.softmax(s, 0)
+                e = (2.0 ** -11 + 2.0 ** -16) * D ** -0.5 * float((kk.abs() @ x[b, i, h].cuda().double().abs()).max())
+                o = p @ vv
+                tol = 3 * vv.abs().max() * (2.0 ** -10 + np.expm1(2 * e)) + 2.0 ** -8 * o.abs()
+                assert ((out[b, i, h].double() - o).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("S,T", [(1, 700), (1, 9000), (90, 700)])
+def test_attention_over_negative_scales(S, T):
+    """A cache whose scales are negative (bias at the group's largest value), as another quantizer may leave it."""
+    torch = _torch()
+    a = _filled(1, 2, T, 128)
+    b = Cache(1, 2, a.max_pos, 128)
+    for w in (0, 3):  # q -> 15 - q, bias -> bias + 15 scale, scale -> -scale: exact where bias + 15 scale is a bf16
+        s = a.t[w + 1].view(torch.bfloat16).float()
+        b.t[w].copy_(~a.t[w])
+        b.t[w + 1].copy_((-s).bfloat16().view(torch.int16))
+        b.t[w + 2].copy_((a.t[w + 2].view(torch.bfloat16).float() + 15 * s).bfloat16().view(torch.int16))
+    x = _rand((1, S, 4, 128), 3).cuda()
+    out, lse = _attend(b, x, _dev([T - S]))
+    K, V = b.values64(0)[0, :, :T].cuda(), b.values64(1)[0, :, :T].cuda()
+    for h in range(4):
+        s = torch.einsum("id,jd->ij", x[0, :, h].double(), K[h // 2]) * 128 ** -0.5
+        s = s.masked_fill(torch.arange(T, device="cuda")[None] > torch.arange(T - S, T, device="cuda")[:, None], -float("inf"))
+        p = torch.softmax(s, -1)
+        o = p @ V[h // 2]
+        e = (2.0 ** -11 + 2.0 ** -16) * 128 ** -0.5 * (x[0, :, h].double().abs() @ K[h // 2].abs().T).max()
+        assert ((out[0, :, h].double() - o).abs() <= 3 * V.abs().max() * (2.0 ** -10 + torch.expm1(2 * e)) + 2.0 ** -8 * o.abs()).all()
 
 
 def test_offsets_past_32_bits():
@@ -718,6 +807,20 @@ def test_other_stream_and_two_calls_at_once():
                 got.append(_attend(c, x, lens)[0])
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("S,T", [(1, 300), (1, 9000), (90, 700), (90, 9000)])
+def test_attention_in_place(S, T):
+    torch, q = _torch(), _api()
+    c = _filled(1, 2, T, 128)
+    x = _rand((1, S, 8, 128), 3).cuda()
+    lens = _dev([T - S])
+    want = _attend(c, x, lens)[0]
+    n = q.kv4_attention_scratch_bytes(c.h, S, 8)
+    scratch = torch.empty(n, dtype=torch.uint8, device="cuda")
+    q.kv4_attention(c.h, x.data_ptr(), x.data_ptr(), S, 8, 128 ** -0.5, lens.data_ptr(), scratch.data_ptr(), n,
+                    stream=torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(x, want)
 
 
 def test_host_memory_and_short_scratch_are_refused():

@@ -74,6 +74,9 @@ def test_attention_refusals():
     _refused(call(scale=float("inf")), text="scale")
     _refused(call(q_ptr=BASE + 2), text="16-byte")
     _refused(call(scratch=BASE + 4), text="16-byte")
+    _refused(call(mass_ptr=BASE), text="out may be q only")
+    _refused(call(S=2, q_strides=(1024, 512, 128), out_strides=(2048, 1024, 128)), text="out may be q only")
+    _refused(call(S=1 << 24, heads=128), text="2^30")
     _refused(call(q_strides=(512, 513, 128)), text="strides")
     _refused(call(out_strides=(512, 512, 4)), text="strides")
     _refused(call(out_strides=(0, 512, 128)), text="zero stride")
