@@ -54,15 +54,18 @@ QW_DEV float4 cluster_load4(const float* p, int rank) {
 
 // Scratch: [0] tiles per share, [1 + b] first tile of sequence b; then the
 // partials [2 shares][columns][D] and their (base exponent, sum); then the lse of a
-// call that accumulates weights but returns none.  (The tcgen05 form has no plan.)
+// call that accumulates weights but returns none, and what the attention kernel keeps
+// for the weights kernel (scores, or the tcgen05 form's Q operands).  (The tcgen05
+// form has no plan.)
 struct Scratch {
     int* plan;
     float* part;
     float2* ml;
     float* lse;
+    float* kept;
     size_t bytes;
 };
-Scratch scratch_of(void* base, const Kv4View& c, int S, int Hq, size_t part_rows) {
+Scratch scratch_of(void* base, const Kv4View& c, int S, int Hq, size_t part_rows, size_t kept_bytes) {
     Scratch s;
     unsigned char* p = static_cast<unsigned char*>(base);
     auto take = [&](size_t n) {
@@ -74,6 +77,7 @@ Scratch scratch_of(void* base, const Kv4View& c, int S, int Hq, size_t part_rows
     s.part = reinterpret_cast<float*>(take(part_rows * c.D * 4));
     s.ml = reinterpret_cast<float2*>(take(part_rows * 8));
     s.lse = reinterpret_cast<float*>(take((size_t)c.batch * S * Hq * 4));
+    s.kept = reinterpret_cast<float*>(take(kept_bytes));
     s.bytes = (size_t)(p - static_cast<unsigned char*>(base));
     return s;
 }
@@ -228,10 +232,10 @@ QW_DEV void fetch_cols(const Kv4AttnArgs& a, int b, int h, int cb, RawCol<D> (&r
 // This warp's tiles first, first + step, ... below t1 of column block cb of (b, h):
 // every warp has its own columns' state and its own ring of
 // tiles (cp.async, so no warp waits for another).  Leaves (base exponent, sum) of every warp and column in
-// wml and the warps' outputs, relative to the block's base, in wo.
-template <int D, int NT>
+// wml and the warps' outputs, relative to the block's base, in wo.  WEIGHTS: the scores are kept too.
+template <int D, int NT, bool WEIGHTS>
 QW_DEV void run_tiles(const Kv4AttnArgs& a, const Kv4Rows& rw, int b, int h, int cb, const RawCol<D> (&raw)[NT], int first, int step, int t1,
-                      unsigned char* smem) {
+                      unsigned char* smem, float* scores, int cp) {
     using L = Tile<D>;
     using SM = SplitSmem<D, NT>;
     constexpr int CB = SM::CB;
@@ -270,15 +274,17 @@ QW_DEV void run_tiles(const Kv4AttnArgs& a, const Kv4Rows& rw, int b, int h, int
     const int all = a.causal ? min(T, rw.off + cb * CB / G + 1) : T;  // keys that every column sees
     const unsigned char* tile = ringp;
     int key0 = first * TK;
+    if (WEIGHTS) scores += (((size_t)b * a.c.heads + h) * a.c.max_pos + key0) * cp;
     for (int k = 0; k < mine; ++k) {
         cp_async_wait<ASTAGES - 2>();
         __syncwarp();
         issue(k + ASTAGES - 1);  // into the stage that the warp left in the turn before
         if (key0 + TK <= all)
-            attend_tile<D, NT, false>(st, cols, tile, key0, T, vis, lane);
+            attend_tile<D, NT, false, WEIGHTS>(st, cols, tile, key0, T, vis, lane, scores, cp);
         else
-            attend_tile<D, NT, true>(st, cols, tile, key0, T, vis, lane);
+            attend_tile<D, NT, true, WEIGHTS>(st, cols, tile, key0, T, vis, lane, scores, cp);
         key0 += step * TK;
+        if (WEIGHTS) scores += (size_t)(step * TK) * cp;
         tile = tile == ringp + (ASTAGES - 1) * L::BYTES ? ringp : tile + L::BYTES;
         __syncwarp();
     }
@@ -356,8 +362,9 @@ QW_DEV void write_out(const Kv4AttnArgs& a, const Kv4Rows& rw, int b, int h, int
     if (d == 0 && a.lse) a.lse[((size_t)b * a.S + i) * a.Hq + h * G + c % G] = has ? (M + log2f(l)) * LN2 : -INFINITY;
 }
 
-template <int D, int NT>
-__global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(const Kv4AttnArgs a, int ncb, int* plan, float* part, float2* pml) {
+template <int D, int NT, bool WEIGHTS>
+__global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(const Kv4AttnArgs a, int ncb, int* plan, float* part, float2* pml,
+                                                                              float* scores, int cp) {
     constexpr int CB = 8 * NT;
     extern __shared__ __align__(128) unsigned char smem[];
     const int tid = threadIdx.x, C = a.Hq / a.c.heads * a.S;
@@ -382,7 +389,7 @@ __global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(co
         const int h = ncb == 1 ? seg : seg / ncb, cb = seg - h * ncb;
         RawCol<D> raw[NT];
         fetch_cols<D, NT>(a, b, h, cb, raw);
-        run_tiles<D, NT>(a, rw, b, h, cb, raw, t0 + (tid >> 5), AW, t1, smem);
+        run_tiles<D, NT, WEIGHTS>(a, rw, b, h, cb, raw, t0 + (tid >> 5), AW, t1, smem, scores, cp);
         const bool whole = t0 == 0 && t1 == nt;
         const size_t slot = 2 * (size_t)blockIdx.x + (u == sh.begin ? 0 : 1);
         for (int idx = tid; idx < CB * (D / 4); idx += ANT) {
@@ -404,8 +411,8 @@ __global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(co
 
 // Short caches: a cluster of `cluster` blocks takes a whole segment, tile k by block k % cluster, and joins
 // through distributed shared memory -- one launch and no partials in memory.
-template <int D, int NT>
-__global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_cluster_kernel(const Kv4AttnArgs a, int ncb, int cluster) {
+template <int D, int NT, bool WEIGHTS>
+__global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_cluster_kernel(const Kv4AttnArgs a, int ncb, int cluster, float* scores, int cp) {
     using SM = SplitSmem<D, NT>;
     constexpr int CB = SM::CB;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -419,7 +426,7 @@ __global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_cluster_kernel(
     RawCol<D> raw[NT];
     fetch_cols<D, NT>(a, b, h, cb, raw);  // before the length arrives
     const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, a.err, rank == 0 && h == 0 && cb == 0 && tid == 0);
-    run_tiles<D, NT>(a, rw, b, h, cb, raw, (tid >> 5) * cluster + rank, AW * cluster, tiles_of(rw), smem);
+    run_tiles<D, NT, WEIGHTS>(a, rw, b, h, cb, raw, (tid >> 5) * cluster + rank, AW * cluster, tiles_of(rw), smem, scores, cp);
     const int nt = tiles_of(rw);
     for (int idx = tid; idx < CB * (D / 4); idx += ANT) {
         const int col = idx / (D / 4), d = 4 * (idx % (D / 4)), c = cb * CB + col;
@@ -576,42 +583,40 @@ QW_DEV void store_weights(float (&sum)[2 * KB], float* mass, int key0, int T, in
         if (t == r && key0 + 8 * r + g < T) mass[key0 + 8 * r + g] += sum[r];
 }
 
-// Up to 16 columns: a warp keeps them in registers and walks tiles of 32 keys, the next tile's rows in flight.
-template <int D, int NT>
-__global__ void __launch_bounds__(ANT, 2) kv4_mass_few_kernel(const Kv4AttnArgs a) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3;
-    const int h = blockIdx.y, b = blockIdx.z, G = a.Hq / a.c.heads, C = G * a.S;
-    RawCol<D> raw[NT];
-    fetch_cols<D, NT>(a, b, h, 0, raw);
+// Up to SCORE_COLUMNS columns: the attention kernels leave their scores [batch][kv head][key][cp] (base 2; at eight
+// columns 32 bytes a key next to the 72 of its K row), so that this pass reads them from L2 and takes no products.
+// 4 sequences of up to 16000 keys, 8 columns: 30.8 us with the attention, 39.0 us with scores recomputed from K.
+// A thread adds one key's columns in their order.
+constexpr int SCORE_COLUMNS = 16, WNT = 256;
+template <int VEC>
+__global__ void __launch_bounds__(WNT) kv4_mass_scores_kernel(const Kv4AttnArgs a, const float* scores, int cp) {
+    __shared__ float base[SCORE_COLUMNS];  // the columns' log2-sum-exp; +inf for a row that is padding
+    const int h = blockIdx.y, b = blockIdx.z, G = a.Hq / a.c.heads, C = G * a.S, key = blockIdx.x * WNT + threadIdx.x;
     const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
-    const int T = rw.off + rw.n, nt = tiles_of(rw), step = gridDim.x * AW;
-    const size_t bh = (size_t)b * a.c.heads + h;
-    int k = blockIdx.x * AW + warp;
-    MassKeys<D, 2> cur;
-    fetch_keys<D, 2>(cur, a.c, bh, k * TK, T, lane);
-    Cols<D, NT> cols;
-    float base[NT][4];
-    int vis[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) load_cols<D, NT>(cols, n, raw[n], a.scale, lane);
-    pdl_wait();  // the rows' log-sum-exp are the attention kernel's
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int c = 8 * n + 2 * t + e, i = c / G;
-            const bool has = c < C && i < rw.n;
-            base[n][e] = base[n][2 + e] = has ? -a.lse[((size_t)b * a.S + i) * a.Hq + h * G + c % G] * LOG2E : -INFINITY;
-            vis[n][e] = has ? (a.causal ? min(T, rw.off + i + 1) : T) : 0;
-        }
-    for (; k < nt; k += step) {
-        MassKeys<D, 2> next;
-        fetch_keys<D, 2>(next, a.c, bh, (k + step) * TK, T, lane);
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        add_weights<D, 2, NT>(sum, cur, cols, base, vis, k * TK, lane);
-        store_weights<2>(sum, a.mass + bh * a.c.max_pos, k * TK, T, lane);
-        cur = next;
+    pdl_wait();
+    if (blockIdx.x * WNT >= rw.off + rw.n) return;
+    if (threadIdx.x < cp) {
+        const int c = threadIdx.x, i = c / G;
+        base[c] = c < C && i < rw.n ? a.lse[((size_t)b * a.S + i) * a.Hq + h * G + c % G] * LOG2E : INFINITY;
     }
+    const size_t at = ((size_t)b * a.c.heads + h) * a.c.max_pos + key;
+    const bool ok = key < rw.off + rw.n;
+    float v[SCORE_COLUMNS];
+#pragma unroll
+    for (int c = 0; c < SCORE_COLUMNS; c += VEC)
+        if (ok && c < cp) {
+            if (VEC == 4)
+                *reinterpret_cast<float4*>(v + c) = *reinterpret_cast<const float4*>(scores + at * cp + c);
+            else
+                *reinterpret_cast<float2*>(v + c) = *reinterpret_cast<const float2*>(scores + at * cp + c);
+        }
+    __syncthreads();
+    if (!ok) return;
+    float sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < SCORE_COLUMNS; ++c)
+        if (c < cp) sum += base[c] == INFINITY ? 0.f : ex2(v[c] - base[c]);
+    a.mass[at] += sum;
 }
 
 // More columns: a warp keeps 16 keys (eight warps of 16: with 32 a chunk of 512 rows on 4096 keys left half of the
@@ -727,6 +732,8 @@ struct Shape {
     bool tc;
     TcShape t;
     int nt, cb, ncb, shares;
+    int cp;       // columns of a kept score row, 0: the scores are not kept
+    size_t kept_bytes;
     int cluster;  // blocks of a segment in the cluster form, 0: shares
     size_t part_rows;
 };
@@ -742,6 +749,8 @@ Shape shape_of(const Kv4View& c, int S, int Hq, int num_sms) {
     s.nt = C <= 8 ? 1 : 2;
     s.cb = 8 * s.nt;
     s.ncb = (int)((C + s.cb - 1) / s.cb);
+    s.cp = C <= SCORE_COLUMNS ? (int)(C + 1) / 2 * 2 : 0;
+    s.kept_bytes = (size_t)c.batch * c.heads * c.max_pos * s.cp * 4;
     s.shares = s.nt == 1 ? 2 * num_sms : num_sms;
     // The cluster form, when the longest sequence the cache can hold is at most CLUSTER_TILES tiles a warp (what a
     // ragged batch loses to its longest sequence then costs less than the joining kernel) and its blocks fit at once.
@@ -758,37 +767,36 @@ Shape shape_of(const Kv4View& c, int S, int Hq, int num_sms) {
     return s;
 }
 
-template <int D, int NT>
+template <int D, int NT, bool WEIGHTS>
 cudaError_t launch_split(const Kv4AttnArgs& a, const Shape& sp, const Scratch& sc, cudaStream_t st) {
     constexpr int smem = SplitSmem<D, NT>::BYTES;
     if (sp.cluster) {
-        const cudaError_t e = ensure_max_dyn_smem(kv4_attn_cluster_kernel<D, NT>, smem);
+        const cudaError_t e = ensure_max_dyn_smem(kv4_attn_cluster_kernel<D, NT, WEIGHTS>, smem);
         if (e != cudaSuccess) return e;
         const unsigned blocks = (unsigned)(sp.cluster * sp.ncb * a.c.heads) * (unsigned)a.c.batch;
-        return launch(kv4_attn_cluster_kernel<D, NT>, dim3(blocks), dim3(ANT), smem, st, true, sp.cluster, a, sp.ncb, sp.cluster);
+        return launch(kv4_attn_cluster_kernel<D, NT, WEIGHTS>, dim3(blocks), dim3(ANT), smem, st, true, sp.cluster, a, sp.ncb, sp.cluster, sc.kept,
+                      sp.cp);
     }
-    cudaError_t e = ensure_max_dyn_smem(kv4_attn_split_kernel<D, NT>, smem);
+    cudaError_t e = ensure_max_dyn_smem(kv4_attn_split_kernel<D, NT, WEIGHTS>, smem);
     if (e != cudaSuccess) return e;
-    e = launch(kv4_attn_split_kernel<D, NT>, dim3(sp.shares), dim3(ANT), smem, st, true, 1, a, sp.ncb, sc.plan, sc.part, sc.ml);
+    e = launch(kv4_attn_split_kernel<D, NT, WEIGHTS>, dim3(sp.shares), dim3(ANT), smem, st, true, 1, a, sp.ncb, sc.plan, sc.part, sc.ml, sc.kept,
+               sp.cp);
     if (e != cudaSuccess) return e;
     return launch(kv4_attn_join_kernel<D>, dim3((unsigned)(a.S * a.Hq), a.c.batch), dim3(32 * JOIN_WARPS), 0, st, true, 1, a, sp.cb, sp.ncb,
                   sp.shares, (const int*)sc.plan, (const float*)sc.part, (const float2*)sc.ml);
 }
 
 template <int D>
-cudaError_t launch_d(const Kv4AttnArgs& a, const Shape& sp, const Scratch& sc, int num_sms, cudaStream_t st) {
-    const cudaError_t e = sp.tc      ? launch_kv4_attn_tc(a, sp.t, sc.part, sc.ml, st)
-                          : sp.nt == 1 ? launch_split<D, 1>(a, sp, sc, st)
-                                       : launch_split<D, 2>(a, sp, sc, st);
+cudaError_t launch_d(const Kv4AttnArgs& a, const Shape& sp, const Scratch& sc, cudaStream_t st) {
+    const bool keep = a.mass && sp.cp;
+    const cudaError_t e = sp.tc          ? launch_kv4_attn_tc(a, sp.t, sc.part, sc.ml, st)
+                          : sp.nt == 1 ? (keep ? launch_split<D, 1, true>(a, sp, sc, st) : launch_split<D, 1, false>(a, sp, sc, st))
+                                       : (keep ? launch_split<D, 2, true>(a, sp, sc, st) : launch_split<D, 2, false>(a, sp, sc, st));
     if (e != cudaSuccess || !a.mass) return e;
-    const long long C = (long long)(a.Hq / a.c.heads) * a.S;
-    if (C <= 16) {
-        // about two rounds of blocks, and no more than the cache can hold tiles for
-        const int most = (a.c.max_pos + AW * TK - 1) / (AW * TK);
-        const int x = (int)std::max(1ll, std::min<long long>(most, (4ll * num_sms + a.c.heads * a.c.batch - 1) / (a.c.heads * a.c.batch)));
-        const dim3 grid(x, a.c.heads, a.c.batch);
-        return C <= 8 ? launch(kv4_mass_few_kernel<D, 1>, grid, dim3(ANT), 0, st, true, 1, a)
-                      : launch(kv4_mass_few_kernel<D, 2>, grid, dim3(ANT), 0, st, true, 1, a);
+    if (keep) {
+        const dim3 grid((a.c.max_pos + WNT - 1) / WNT, a.c.heads, a.c.batch);
+        return launch(sp.cp % 4 == 0 ? kv4_mass_scores_kernel<4> : kv4_mass_scores_kernel<2>, grid, dim3(WNT), 0, st, true, 1, a,
+                      (const float*)sc.kept, sp.cp);
     }
     const dim3 grid((a.c.max_pos + AW * 16 - 1) / (AW * 16), a.c.heads, a.c.batch);
     return launch(kv4_mass_kernel<D>, grid, dim3(ANT), 0, st, true, 1, a);
@@ -798,7 +806,7 @@ cudaError_t launch_d(const Kv4AttnArgs& a, const Shape& sp, const Scratch& sc, i
 
 size_t kv4_attn_scratch_bytes(const Kv4View& c, int S, int Hq, int num_sms) {
     const Shape sp = shape_of(c, S, Hq, num_sms);
-    return scratch_of(nullptr, c, S, Hq, sp.part_rows).bytes;
+    return scratch_of(nullptr, c, S, Hq, sp.part_rows, sp.kept_bytes).bytes;
 }
 
 cudaError_t launch_kv4_attention(const Kv4AttnArgs& in, void* scratch, int num_sms, cudaStream_t st) {
@@ -806,9 +814,9 @@ cudaError_t launch_kv4_attention(const Kv4AttnArgs& in, void* scratch, int num_s
     const Shape sp = shape_of(a.c, a.S, a.Hq, num_sms);
     // tiles are counted in 32 bits (180 GB of cache are less than 2^26 tiles of one column block)
     if (!sp.tc && !sp.cluster && (long long)a.c.batch * a.c.heads * sp.ncb * ((a.c.max_pos + TK - 1) / TK) > 0x7FFFFFFF) return cudaErrorInvalidValue;
-    const Scratch sc = scratch_of(scratch, a.c, a.S, a.Hq, sp.part_rows);
+    const Scratch sc = scratch_of(scratch, a.c, a.S, a.Hq, sp.part_rows, sp.kept_bytes);
     if (a.mass && !a.lse) a.lse = sc.lse;
-    return a.c.D == 128 ? launch_d<128>(a, sp, sc, num_sms, st) : launch_d<64>(a, sp, sc, num_sms, st);
+    return a.c.D == 128 ? launch_d<128>(a, sp, sc, st) : launch_d<64>(a, sp, sc, st);
 }
 
 }  // namespace qw

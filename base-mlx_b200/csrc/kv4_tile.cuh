@@ -339,9 +339,10 @@ struct State {
 
 // One tile: keys [key0, key0 + 32) of which vis[n][e] (absolute) are visible to
 // column (n, e).  EDGE: some key of the tile is not visible to some column.
-template <int D, int NT, bool EDGE>
+// WEIGHTS: the scores (base 2, -inf for hidden keys) go to scores[key - key0][column], rows of cp columns.
+template <int D, int NT, bool EDGE, bool WEIGHTS>
 QW_DEV void attend_tile(State<D, NT>& st, const Cols<D, NT>& cols, const unsigned char* tile, int key0, int T,
-                        const int (&vis)[NT][2], int lane) {
+                        const int (&vis)[NT][2], int lane, float* scores, int cp) {
     const uint32_t tile_s = smem_u32(tile);
     using L = Tile<D>;
     constexpr int GR = L::GR;
@@ -425,6 +426,16 @@ QW_DEV void attend_tile(State<D, NT>& st, const Cols<D, NT>& cols, const unsigne
                     st.o[i][n][2 + e] = st.o[i][n][2 + e] * al * al;
                 }
             }
+    }
+    if (WEIGHTS) {
+        float* row = scores + g * cp + 2 * (lane & 3);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                if (8 * n + 2 * (lane & 3) < cp && (!EDGE || key0 + 8 * r + g < T))
+                    *reinterpret_cast<float2*>(row + 8 * r * cp + 8 * n) =
+                        make_float2(x[r >> 1][n][2 * (r & 1)] - st.nm[n][0], x[r >> 1][n][2 * (r & 1) + 1] - st.nm[n][1]);
     }
     // probabilities, their sums, and p s in the B-operand layout (keys along k)
     uint32_t pb[2][GR][NT][2];
