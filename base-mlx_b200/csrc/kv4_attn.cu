@@ -19,6 +19,7 @@
 #include <algorithm>
 
 #include "kv4_join.cuh"
+#include "kv4_launch.h"
 #include "kv4_tc.h"
 #include "kv4_tile.cuh"
 #include "smem_attr.h"
@@ -700,30 +701,6 @@ __global__ void __launch_bounds__(ANT, 2) kv4_mass_kernel(const Kv4AttnArgs a) {
     store_weights<1>(sum, a.mass + bh * a.c.max_pos, key0, T, lane);
 }
 
-template <typename K, typename... Args>
-cudaError_t launch(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl, int cluster, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    int n = 0;
-    if (pdl) {
-        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[n++].val.programmaticStreamSerializationAllowed = 1;
-    }
-    if (cluster > 1) {
-        attr[n].id = cudaLaunchAttributeClusterDimension;
-        attr[n].val.clusterDim.x = cluster;
-        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
-        ++n;
-    }
-    cfg.attrs = attr;
-    cfg.numAttrs = n;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 // Form of a call: from TC_COLUMNS columns per kv head the tcgen05 kernel, below it the split kernel
 // with column blocks of 8 (two blocks of threads per SM) or 16.
 constexpr int TC_COLUMNS = 64;
@@ -744,6 +721,7 @@ Shape shape_of(const Kv4View& c, int S, int Hq, int num_sms) {
     if (s.tc) {
         s.t = kv4_tc_shape(c, S, Hq, num_sms);
         s.part_rows = s.t.part_rows;
+        s.kept_bytes = s.t.kept_bytes;
         return s;
     }
     s.nt = C <= 8 ? 1 : 2;
@@ -774,32 +752,32 @@ cudaError_t launch_split(const Kv4AttnArgs& a, const Shape& sp, const Scratch& s
         const cudaError_t e = ensure_max_dyn_smem(kv4_attn_cluster_kernel<D, NT, WEIGHTS>, smem);
         if (e != cudaSuccess) return e;
         const unsigned blocks = (unsigned)(sp.cluster * sp.ncb * a.c.heads) * (unsigned)a.c.batch;
-        return launch(kv4_attn_cluster_kernel<D, NT, WEIGHTS>, dim3(blocks), dim3(ANT), smem, st, true, sp.cluster, a, sp.ncb, sp.cluster, sc.kept,
+        return launch(kv4_attn_cluster_kernel<D, NT, WEIGHTS>, dim3(blocks), dim3(ANT), smem, sp.cluster, st, a, sp.ncb, sp.cluster, sc.kept,
                       sp.cp);
     }
     cudaError_t e = ensure_max_dyn_smem(kv4_attn_split_kernel<D, NT, WEIGHTS>, smem);
     if (e != cudaSuccess) return e;
-    e = launch(kv4_attn_split_kernel<D, NT, WEIGHTS>, dim3(sp.shares), dim3(ANT), smem, st, true, 1, a, sp.ncb, sc.plan, sc.part, sc.ml, sc.kept,
+    e = launch(kv4_attn_split_kernel<D, NT, WEIGHTS>, dim3(sp.shares), dim3(ANT), smem, 1, st, a, sp.ncb, sc.plan, sc.part, sc.ml, sc.kept,
                sp.cp);
     if (e != cudaSuccess) return e;
-    return launch(kv4_attn_join_kernel<D>, dim3((unsigned)(a.S * a.Hq), a.c.batch), dim3(32 * JOIN_WARPS), 0, st, true, 1, a, sp.cb, sp.ncb,
+    return launch(kv4_attn_join_kernel<D>, dim3((unsigned)(a.S * a.Hq), a.c.batch), dim3(32 * JOIN_WARPS), 0, 1, st, a, sp.cb, sp.ncb,
                   sp.shares, (const int*)sc.plan, (const float*)sc.part, (const float2*)sc.ml);
 }
 
 template <int D>
 cudaError_t launch_d(const Kv4AttnArgs& a, const Shape& sp, const Scratch& sc, cudaStream_t st) {
+    if (sp.tc) return launch_kv4_attn_tc(a, sp.t, sc.part, sc.ml, sc.kept, st);
     const bool keep = a.mass && sp.cp;
-    const cudaError_t e = sp.tc          ? launch_kv4_attn_tc(a, sp.t, sc.part, sc.ml, st)
-                          : sp.nt == 1 ? (keep ? launch_split<D, 1, true>(a, sp, sc, st) : launch_split<D, 1, false>(a, sp, sc, st))
-                                       : (keep ? launch_split<D, 2, true>(a, sp, sc, st) : launch_split<D, 2, false>(a, sp, sc, st));
+    const cudaError_t e = sp.nt == 1 ? (keep ? launch_split<D, 1, true>(a, sp, sc, st) : launch_split<D, 1, false>(a, sp, sc, st))
+                                     : (keep ? launch_split<D, 2, true>(a, sp, sc, st) : launch_split<D, 2, false>(a, sp, sc, st));
     if (e != cudaSuccess || !a.mass) return e;
     if (keep) {
         const dim3 grid((a.c.max_pos + WNT - 1) / WNT, a.c.heads, a.c.batch);
-        return launch(sp.cp % 4 == 0 ? kv4_mass_scores_kernel<4> : kv4_mass_scores_kernel<2>, grid, dim3(WNT), 0, st, true, 1, a,
+        return launch(sp.cp % 4 == 0 ? kv4_mass_scores_kernel<4> : kv4_mass_scores_kernel<2>, grid, dim3(WNT), 0, 1, st, a,
                       (const float*)sc.kept, sp.cp);
     }
     const dim3 grid((a.c.max_pos + AW * 16 - 1) / (AW * 16), a.c.heads, a.c.batch);
-    return launch(kv4_mass_kernel<D>, grid, dim3(ANT), 0, st, true, 1, a);
+    return launch(kv4_mass_kernel<D>, grid, dim3(ANT), 0, 1, st, a);
 }
 
 }  // namespace

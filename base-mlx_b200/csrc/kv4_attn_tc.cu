@@ -29,8 +29,9 @@
 // chains.)  Every wait is bounded: a lost arrival sets QW_DERR_TIMEOUT and the
 // block still frees its TMEM and ends.
 #include "kv4_join.cuh"
+#include "kv4_launch.h"
 #include "kv4_tc.h"
-#include "kv4_tile.cuh"
+#include "kv4_tcgen.cuh"
 #include "smem_attr.h"
 
 namespace qw {
@@ -38,8 +39,6 @@ namespace {
 
 using namespace kv4;
 
-constexpr int CM = 128;      // columns of a column block
-constexpr int KT = 128;      // keys of a tile
 template <int NB>
 constexpr int THREADS = 256 * NB + 32;
 constexpr float BASE = 7.f;           // P = 2^(x - max + 7): normal fp16 numbers down to 2^-21 of the largest
@@ -50,7 +49,7 @@ constexpr float UNSET = -3.0e38f;
 template <int D, int NB>
 struct Plan {
     static constexpr int GR = D / 64;
-    static constexpr int QB = GR * CM * 128 + CM * 32, KB = GR * KT * 128 + KT * 32, VB = GR * KT * 128;
+    static constexpr int QB = q_block_bytes(D), KB = GR * KT * 128 + KT * 32, VB = GR * KT * 128;
     static constexpr int Q = 5120;           // after the barriers and two exchange arrays: [NB]{[GR][128 rows][128 B] swizzled; Q*}
     static constexpr int K = Q + NB * QB;    // [2]{[GR][128 keys][128 B] swizzled; C*}
     static constexpr int V = K + 2 * KB;     // [2][GR][128 keys][128 B], swizzled, read along the keys
@@ -59,102 +58,14 @@ struct Plan {
     static constexpr uint32_t TO = KT, TB = KT + D, TMEM = NB * TB <= 256 ? 256 : 512;
 };
 
-// Bounded wait: every poll suspends for a while, 2^22 of them are far beyond any tile's time.
-QW_DEV bool wait_bar(uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity); }
-QW_DEV void arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-QW_DEV void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-QW_DEV void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// The product warp runs as a whole, so that its control flow and descriptors stay in uniform
-// registers; one elected lane issues.
-QW_DEV void commit(uint64_t* bar) {
-    asm volatile(
-        "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
-        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar))
-        : "memory");
-}
-// 128-byte-swizzled operand rows of 64 fp16: descriptor version 1, 1 KB between 8-row groups; along_keys:
-// the matrix' k runs over the rows and its 64-element blocks lie `lead` bytes apart.
-QW_DEV uint64_t desc(uint32_t addr, uint32_t lead) {
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) |
-           (2ull << 61);
-}
-// The 16-wide extra operand: 8 rows x 16 bytes make a block of 128 bytes, [row / 8][k / 8][row % 8][16 B], no swizzle.
-QW_DEV uint64_t desc16(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(128u >> 4) << 16) | ((uint64_t)(256u >> 4) << 32) | (1ull << 46);
-}
-QW_DEV uint32_t at16(int row, int khalf) { return (uint32_t)(row >> 3) * 256 + khalf * 128 + (row & 7) * 16; }
-// kind::f16, fp32 sums, fp16 operands, A along k, B along k or (bit 16) along n; M = 128.
-__host__ __device__ constexpr uint32_t idesc(int n, bool b_along_n) {
-    return (1u << 4) | (b_along_n ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(CM >> 4) << 24);
-}
-QW_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate)
-        : "memory");
-}
-QW_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate)
-        : "memory");
-}
-QW_DEV void ld16(uint32_t addr, float (&v)[16]) {
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(addr)
-        : "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
-QW_DEV void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-QW_DEV void st16(uint32_t addr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
-QW_DEV void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-QW_DEV uint32_t h2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-QW_DEV __half2 as_h2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
-QW_DEV uint32_t as_u(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
-
-// 16-byte chunk c of a swizzled operand row.  A word fills one chunk, its elements in the order 0, 4, 1, 5, 2, 6, 3, 7.
-QW_DEV uint32_t chunk_at(int row, int c) { return (uint32_t)row * 128 + (uint32_t)((c ^ (row & 7)) << 4); }
-
 QW_DEV float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-QW_DEV unsigned long long pack2(float lo, float hi) {
-    unsigned long long r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-QW_DEV void unpack2(unsigned long long v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-QW_DEV unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
-    unsigned long long r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-QW_DEV unsigned long long add2(unsigned long long a, unsigned long long b) {
-    unsigned long long r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-
 template <int D, int NB>
-__global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4AttnArgs a, int ncb, int nsplit, float* part, float2* pml) {
+__global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4AttnArgs a, int ncb, int nsplit, float* part, float2* pml,
+                                                                        unsigned char* qkeep) {
     using P = Plan<D, NB>;
     constexpr int GR = P::GR, CB = CM * NB, PW0 = 8 * NB;  // columns of the block, first producer warp
     extern __shared__ unsigned char tc_raw[];
@@ -304,13 +215,19 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
     fence_before();
     __syncthreads();
     fence_after();
+    if (qkeep && sp == nsplit - 1) {  // (the last split of a block with rows has tiles)
+        uint4* dst = reinterpret_cast<uint4*>(qkeep + seg * NB * P::QB);
+        for (int p = tid; p < NB * P::QB / 16; p += THREADS<NB>) dst[p] = reinterpret_cast<const uint4*>(sm + P::Q)[p];
+        if (warp < PW0 && half == 0)
+            reinterpret_cast<float*>(qkeep + (size_t)a.c.batch * a.c.heads * ncb * NB * P::QB)[seg * CB + col] = cc;
+    }
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
     // exponents of the largest values: K enters times 2^(7 - ek), V times 2^(13 - ev)
     auto exponent = [&](int v) {
         float m = 0.f;
 #pragma unroll
         for (int w = 0; w < PW0; ++w) m = fmaxf(m, kvmax[2 * w + v]);
-        return max((int)(__float_as_uint(fminf(m, 3.0e38f)) >> 23) - 127, -100);
+        return top_exponent(m);
     };
     const int ek = exponent(0), ev = exponent(1);
     const int n_tiles = t1 - t0;
@@ -326,9 +243,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
         const unsigned long long c2 = pack2(cc, cc);
 
         // ---- expansion of this thread's share of a tile --------------------------------------------------
-        // A thread takes 16-byte pieces (4 words of a row), thread after thread: piece p of a tile is words
-        // 4 (p % CPR) .. of key p / CPR.  With two groups the second one's words go out in another order
-        // (e ^ 2): the eight lanes of a store phase (two keys, all pieces) hit eight different chunk columns.
+        // A thread takes 16-byte pieces (4 words of a row), thread after thread.
         constexpr int CPR = D / 32, PIECES = KT * CPR, NTH = 256 * NB, PER = PIECES >= NTH ? PIECES / NTH : 1;
         const bool has_piece = tid < PIECES;  // D = 64 and two column blocks: half of the threads
         const float kup = __uint_as_float((uint32_t)(127 + 7 - ek) << 23), vup = __uint_as_float((uint32_t)(127 + 13 - ev) << 23);
@@ -340,9 +255,6 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
             uint16_t s[PER], z[PER];  // scale and bias of the piece's group
         } ks, vs;
         uint32_t cs = 0, cz = 0;  // threads 0 .. 127: scales and biases of one key of the tile, every group
-        auto packed = [&](const unsigned char* base, int key) {
-            return GR == 2 ? *reinterpret_cast<const uint32_t*>(base + (size_t)key * 4) : (uint32_t)*reinterpret_cast<const uint16_t*>(base + (size_t)key * 2);
-        };
         // A block-wide base and a 32-bit offset of the thread's own each.
         const uint32_t po = (uint32_t)tid, so = (uint32_t)(tid / CPR * GR + ((tid % CPR) >> 1));
         constexpr uint32_t PSTEP = NTH, SSTEP = NTH / CPR * GR;
@@ -372,61 +284,30 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
             if (i >= n_tiles) return;
             load(ks, 0, i);
             const int key = (t0 + i) * KT + tid;
-            cs = tid < KT && key < T ? packed(rows.s[0], key) : 0u;
-            cz = tid < KT && key < T ? packed(rows.b[0], key) : 0u;
+            cs = tid < KT && key < T ? group_pair<GR>(rows.s[0], key) : 0u;
+            cz = tid < KT && key < T ? group_pair<GR>(rows.b[0], key) : 0u;
         };
         auto load_v = [&](int i) {
             if (i < n_tiles) load(vs, 1, i);
-        };
-        auto expand = [&](const uint4& w, int p, unsigned char* dst, auto&& value) {
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-            const int key = p / CPR, q = p % CPR, g = q >> 1;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t v = g ? u[e ^ 2] : u[e];
-                uint32_t o[4];
-#pragma unroll
-                for (int n = 0; n < 4; ++n) o[n] = value(((v >> (4 * n)) & 0x000F000Fu) | 0x64006400u);  // (1024 + n_j, 1024 + n_{j+4})
-                *reinterpret_cast<uint4*>(dst + g * KT * 128 + chunk_at(key, 4 * (q & 1) + (g ? e ^ 2 : e))) = make_uint4(o[0], o[1], o[2], o[3]);
-            }
         };
         auto store_k = [&](int i) {  // tile i's K operand from ks, cs, cz
             if (i >= n_tiles) return;
             if (ok && i > 1 && !wait_bar(k_free + (i & 1), ((i - 2) >> 1) & 1)) ok = false;
             unsigned char* dst = sm + P::K + (i & 1) * P::KB;
-            const __half2 k1032 = __float2half2_rn(1032.f);
             if (has_piece)
 #pragma unroll
                 for (int j = 0; j < PER; ++j) {
                     const __half2 s2 = __float2half2_rn(u16_to_f(ks.s[j]) * kup);
-                    expand(ks.w[j], tid + NTH * j, dst, [&](uint32_t n) { return as_u(__hmul2(__hsub2(as_h2(n), k1032), s2)); });
+                    expand_piece<D>(ks.w[j], tid + NTH * j, dst, [&](uint32_t n) { return centred(n, s2); });
                 }
             if (tid < KT) {
-                // C*: 2^6 c in two fp16 terms, k = 5 g + {0..4}: hi, lo, hi, lo, hi
                 bool nan = false;
                 const int key = (t0 + i) * KT + tid;
                 if (partial(i) && key < T) {
-                    const uint32_t s = packed(rows.s[1], key), z = packed(rows.b[1], key);
+                    const uint32_t s = group_pair<GR>(rows.s[1], key), z = group_pair<GR>(rows.b[1], key);
                     nan = !(fabsf(bits_lo_f(s)) + fabsf(bits_lo_f(z)) < INFINITY) || !(fabsf(bits_hi_f(s)) + fabsf(bits_hi_f(z)) < INFINITY);
                 }
-                __half c[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) c[e] = __float2half_rn(0.f);
-#pragma unroll
-                for (int g = 0; g < GR; ++g) {
-                    float x = fmaf(8.f, g ? bits_hi_f(cs) : bits_lo_f(cs), g ? bits_hi_f(cz) : bits_lo_f(cz)) * kup * 64.f;
-                    if (nan) x = __int_as_float(0x7FC00000);
-                    const __half hi = __float2half_rn(x), lo = __float2half_rn(x - __half2float(hi));
-                    c[5 * g] = c[5 * g + 2] = c[5 * g + 4] = hi;
-                    c[5 * g + 1] = c[5 * g + 3] = lo;
-                }
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    uint32_t r[4];
-#pragma unroll
-                    for (int f = 0; f < 4; ++f) r[f] = as_u(__halves2half2(c[8 * e + 2 * f], c[8 * e + 2 * f + 1]));
-                    *reinterpret_cast<uint4*>(dst + GR * KT * 128 + at16(tid, e)) = make_uint4(r[0], r[1], r[2], r[3]);
-                }
+                store_offsets<GR>(dst + GR * KT * 128, tid, cs, cz, kup, nan);
             }
         };
         auto store_v = [&](int i) {
@@ -440,7 +321,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
                     float s = u16_to_f(vs.s[j]), z = u16_to_f(vs.z[j]);
                     if (partial(i) && !(fabsf(s) + fabsf(z) < INFINITY)) s = z = 0.f;
                     const __half2 s2 = __float2half2_rn(s * vup), z2 = __float2half2_rn(z * vup);
-                    expand(vs.w[j], tid + NTH * j, dst, [&](uint32_t n) { return as_u(__hfma2(__hsub2(as_h2(n), k1024), s2, z2)); });
+                    expand_piece<D>(vs.w[j], tid + NTH * j, dst, [&](uint32_t n) { return as_u(__hfma2(__hsub2(as_h2(n), k1024), s2, z2)); });
                 }
         };
         // Stores first, then one fence, then the loads: a fence waits for the thread's loads in flight.
@@ -672,31 +553,17 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) kv4_attn_tc_join_kernel(const
     join_row<D, 1>(nsplit, 0, slot, part, pml, nullptr, dst, lse);
 }
 
-template <typename K, typename... Args>
-cudaError_t launch(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <int D, int NB>
-cudaError_t launch_tc(const Kv4AttnArgs& a, const TcShape& sp, float* part, float2* ml, cudaStream_t st) {
+cudaError_t launch_tc(const Kv4AttnArgs& a, const TcShape& sp, float* part, float2* ml, unsigned char* qkeep, cudaStream_t st) {
     constexpr int smem = Plan<D, NB>::BYTES;
     cudaError_t e = ensure_max_dyn_smem(kv4_attn_tc_kernel<D, NB>, smem);
     if (e != cudaSuccess) return e;
     const long long blocks = (long long)sp.ncb * sp.nsplit * a.c.heads * a.c.batch;
     if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
-    e = launch(kv4_attn_tc_kernel<D, NB>, dim3((unsigned)blocks), dim3(THREADS<NB>), smem, st, true, a, sp.ncb, sp.nsplit, part, ml);
+    e = launch(kv4_attn_tc_kernel<D, NB>, dim3((unsigned)blocks), dim3(THREADS<NB>), smem, 1, st, a, sp.ncb, sp.nsplit, part, ml,
+               qkeep);
     if (e != cudaSuccess || sp.nsplit == 1) return e;
-    return launch(kv4_attn_tc_join_kernel<D>, dim3((unsigned)((a.S * (long long)a.Hq + JOIN_WARPS - 1) / JOIN_WARPS), a.c.batch), dim3(32 * JOIN_WARPS), 0, st, true, a, CM * NB, sp.ncb,
+    return launch(kv4_attn_tc_join_kernel<D>, dim3((unsigned)((a.S * (long long)a.Hq + JOIN_WARPS - 1) / JOIN_WARPS), a.c.batch), dim3(32 * JOIN_WARPS), 0, 1, st, a, CM * NB, sp.ncb,
                   sp.nsplit, (const float*)part, (const float2*)ml);
 }
 
@@ -720,12 +587,16 @@ TcShape kv4_tc_shape(const Kv4View& c, int S, int Hq, int num_sms) {
         }
     }
     s.part_rows = s.nsplit > 1 ? (size_t)segs * s.nsplit * CM * s.nb : 0;
+    s.kept_bytes = (size_t)segs * s.nb * (q_block_bytes(c.D) + CM * 4);
     return s;
 }
 
-cudaError_t launch_kv4_attn_tc(const Kv4AttnArgs& a, const TcShape& s, float* part, float2* ml, cudaStream_t st) {
-    if (a.c.D == 128) return s.nb == 2 ? launch_tc<128, 2>(a, s, part, ml, st) : launch_tc<128, 1>(a, s, part, ml, st);
-    return s.nb == 2 ? launch_tc<64, 2>(a, s, part, ml, st) : launch_tc<64, 1>(a, s, part, ml, st);
+cudaError_t launch_kv4_attn_tc(const Kv4AttnArgs& a, const TcShape& s, float* part, float2* ml, void* kept, cudaStream_t st) {
+    unsigned char* q = a.mass ? static_cast<unsigned char*>(kept) : nullptr;
+    const cudaError_t e = a.c.D == 128 ? (s.nb == 2 ? launch_tc<128, 2>(a, s, part, ml, q, st) : launch_tc<128, 1>(a, s, part, ml, q, st))
+                                       : (s.nb == 2 ? launch_tc<64, 2>(a, s, part, ml, q, st) : launch_tc<64, 1>(a, s, part, ml, q, st));
+    if (e != cudaSuccess || !a.mass) return e;
+    return launch_kv4_mass_tc(a, s, q, st);
 }
 
 }  // namespace qw

@@ -15,6 +15,7 @@
 #include <algorithm>
 
 #include "kv4.h"
+#include "kv4_launch.h"
 #include "smem_attr.h"
 
 namespace qw {
@@ -359,30 +360,6 @@ __global__ void __launch_bounds__(1024) kv4_move_inplace_kernel(const Kv4EvictAr
     }
 }
 
-template <typename K, typename... Args>
-cudaError_t launch(K kernel, dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t st, bool pdl, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    int n = 0;
-    if (pdl) {
-        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[n++].val.programmaticStreamSerializationAllowed = 1;
-    }
-    if (cluster > 1) {
-        attr[n].id = cudaLaunchAttributeClusterDimension;
-        attr[n].val.clusterDim.x = cluster;
-        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
-        ++n;
-    }
-    cfg.attrs = attr;
-    cfg.numAttrs = n;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 }  // namespace
 
 size_t kv4_evict_scratch_bytes(const Kv4View& src, int keep) {
@@ -401,19 +378,19 @@ cudaError_t launch_kv4_evict(const Kv4EvictArgs& a, void* scratch, cudaStream_t 
     const int smem = (3 * BINS + keys) * (int)sizeof(int);
     cudaError_t e = ensure_max_dyn_smem(kv4_select_kernel, (3 * BINS + SEL_KEYS) * (int)sizeof(int));
     if (e != cudaSuccess) return e;
-    e = launch(kv4_select_kernel, dim3(a.src.heads * cluster, a.src.batch), dim3(SEL_NT), smem, cluster, st, true, a, cluster,
+    e = launch(kv4_select_kernel, dim3(a.src.heads * cluster, a.src.batch), dim3(SEL_NT), smem, cluster, st, a, cluster,
                keys, index, count);
     if (e != cudaSuccess) return e;
     const bool wide = a.src.D == 128;
     if (a.dst.p[0].w == a.src.p[0].w) {
         const dim3 grid(3, a.src.heads, a.src.batch);
-        return wide ? launch(kv4_move_inplace_kernel<128>, grid, dim3(1024), 0, 1, st, true, a, (const int*)index, (const int*)count)
-                    : launch(kv4_move_inplace_kernel<64>, grid, dim3(1024), 0, 1, st, true, a, (const int*)index, (const int*)count);
+        return wide ? launch(kv4_move_inplace_kernel<128>, grid, dim3(1024), 0, 1, st, a, (const int*)index, (const int*)count)
+                    : launch(kv4_move_inplace_kernel<64>, grid, dim3(1024), 0, 1, st, a, (const int*)index, (const int*)count);
     }
     const int rows = MR * 256 / (a.src.D / 32);
     const dim3 grid((a.keep + rows - 1) / rows, 3 * a.src.heads, a.src.batch);
-    return wide ? launch(kv4_move_kernel<128>, grid, dim3(256), 0, 1, st, true, a, (const int*)index, (const int*)count)
-                : launch(kv4_move_kernel<64>, grid, dim3(256), 0, 1, st, true, a, (const int*)index, (const int*)count);
+    return wide ? launch(kv4_move_kernel<128>, grid, dim3(256), 0, 1, st, a, (const int*)index, (const int*)count)
+                : launch(kv4_move_kernel<64>, grid, dim3(256), 0, 1, st, a, (const int*)index, (const int*)count);
 }
 
 }  // namespace qw
