@@ -541,6 +541,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) kv4_attn_tc_join_kernel(const
     float* lse = a.lse ? a.lse + ((size_t)b * a.S + i) * a.Hq + h : nullptr;
     const size_t s0 = ((((size_t)b * a.c.heads + h / G) * ncb + cb) * nsplit) * cb_size + c % cb_size;
     pdl_wait();
+    pdl_launch_dependents();  // the weights kernel expands its keys meanwhile
     if (i >= rw.n) {
         if (lane < D / 8) *reinterpret_cast<uint4*>(dst + 8 * lane) = make_uint4(0u, 0u, 0u, 0u);
         if (lse && lane == 0) *lse = -INFINITY;

@@ -116,29 +116,36 @@ __global__ void __launch_bounds__(MTHREADS, 1) kv4_mass_tc_kernel(const Kv4AttnA
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    // the next tile's Q operand (product warp)
+    int issued = 0;
+    auto load = [&](size_t image) {
+        if (issued >= n_tiles) return;
+        if (lane == 0) {
+            mbar_arrive_expect_tx(q_full + issued % QSTAGES, P::QB);
+            bulk_g2s(sm + P::Q + issued % QSTAGES * P::QB, kept + (image + issued) * P::QB, P::QB, q_full + issued % QSTAGES);
+        }
+        ++issued;
+    };
     const size_t image = ((size_t)b * a.c.heads + h) * blocks + c_first / CM;
+    if (warp == PW)
+        for (int i = 0; i < QSTAGES; ++i) load(image);
     const float* factor = reinterpret_cast<const float*>(kept + (size_t)a.c.batch * a.c.heads * blocks * P::QB) + image * CM;
-    float cc = 0.f, nl = -INFINITY;  // threads 0 .. 127: factor and -log2-sum-exp of a column (2^-inf where there is none)
+    // threads 0 .. 127: factor and log-sum-exp of a column (2^-inf where there is none)
     auto fetch = [&](int i) {
         const int c = c_first + i * CM + tid;
-        cc = 0.f;
-        nl = -INFINITY;
-        if (tid < CM && c < c_end) {
-            cc = factor[i * CM + tid];
-            nl = a.lse[((size_t)b * a.S + c / G) * a.Hq + h * G + c % G];
-        }
+        if (tid >= CM || c >= c_end) return make_float2(0.f, INFINITY);
+        return make_float2(factor[i * CM + tid], a.lse[((size_t)b * a.S + c / G) * a.Hq + h * G + c % G]);
     };
-    auto put = [&](int i) {
+    auto put = [&](int i, float2 v) {
         if (tid >= CM) return;
         float* t = tab + (i & 3) * 2 * CM + (tid >> 1) * 4 + (tid & 1);
-        t[0] = ldexpf(cc, ek - 7);
-        t[2] = nl == -INFINITY && cc == 0.f ? nl : -nl * LOG2E;
+        t[0] = ldexpf(v.x, ek - 7);
+        t[2] = -v.y * LOG2E;
     };
-    fetch(0);
-    put(0);
-    fetch(1);
-    put(1);
-    fetch(2);
+    const float2 v0 = fetch(0), v1 = fetch(1);
+    float2 ahead = fetch(2);
+    put(0, v0);
+    put(1, v1);
     fence_proxy_async_smem();
     fence_before();
     __syncthreads();
@@ -158,8 +165,8 @@ __global__ void __launch_bounds__(MTHREADS, 1) kv4_mass_tc_kernel(const Kv4AttnA
             if (ok && i > 1 && !wait_bar(s_free + buf, ((i - 2) >> 1) & 1)) ok = false;
             if (ok && !wait_bar(s_full + buf * KBLOCKS + kb, (i >> 1) & 1)) ok = false;
             fence_after();
-            put(i + 2);  // over the table of tile i - 2, which every thread has left
-            fetch(i + 3);
+            put(i + 2, ahead);  // over the table of tile i - 2, which every thread has left
+            ahead = fetch(i + 3);
             const bool seen = k0 < T && c0 + CM > c_some;
             unsigned long long s2[2] = {0ull, 0ull};
 #pragma unroll 1
@@ -204,16 +211,6 @@ __global__ void __launch_bounds__(MTHREADS, 1) kv4_mass_tc_kernel(const Kv4AttnA
         const uint32_t qa = smem_u32(sm + P::Q), ka = smem_u32(sm + P::K);
         const uint64_t qd = desc(qa, 16), kd = desc(ka, 16), qx = desc16(qa + GR * CM * 128), kx = desc16(ka + GR * KT * 128);
         auto at = [](uint64_t d, uint32_t bytes) { return d + (bytes >> 4); };
-        int issued = 0;
-        auto load = [&]() {  // the next tile's Q operand
-            if (issued >= n_tiles) return;
-            if (lane == 0) {
-                mbar_arrive_expect_tx(q_full + issued % QSTAGES, P::QB);
-                bulk_g2s(sm + P::Q + issued % QSTAGES * P::QB, kept + (image + issued) * P::QB, P::QB, q_full + issued % QSTAGES);
-            }
-            ++issued;
-        };
-        for (int i = 0; i < QSTAGES; ++i) load();
         int i = 0;
         for (; i < n_tiles; ++i) {
             const int buf = i & 1;
@@ -237,7 +234,7 @@ __global__ void __launch_bounds__(MTHREADS, 1) kv4_mass_tc_kernel(const Kv4AttnA
                 if (!wait_bar(s_full + (buf ^ 1) * KBLOCKS + KBLOCKS - 1, ((i - 1) >> 1) & 1)) ok = false;
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                load();
+                load(image);
             }
         }
         for (; !ok && i < issued; ++i) wait_bar(q_full + i % QSTAGES, (i / QSTAGES) & 1);  // copies still on their way
