@@ -8,9 +8,12 @@
 // tiles of 128 keys expanded in shared memory and walks the columns, 128 at a
 // time: the Q operand that the attention kernel built and kept arrives by one
 // bulk copy (one tile of keys per block instead would read 36 KB of Q from L2 per
-// 128 x 128 scores, more than L2 gives).  Per key tile two threads a key take
-// half the columns each; S is double buffered in TMEM, Q three times in shared
-// memory.  What bounds it is 2^x (16 a clock and SM).  512 rows of 16 heads on 8
+// 128 x 128 scores, more than L2 gives).  A thread takes one key of either tile
+// and a quarter of the columns, so that a column's factor and log-sum-exp, read
+// from shared memory, serve two scores (serving one, those reads were the bound:
+// a broadcast of 16 bytes takes four of the 128-byte cycles); S is double buffered
+// in TMEM, Q three times in shared memory.  What bounds it is 2^x (16 a clock and
+// SM) next to shared memory.  512 rows of 16 heads on 8
 // kv heads, 4096 keys: TIME (with scores by mma.sync: 63 us).
 #include "kv4_launch.h"
 #include "kv4_tc.h"
@@ -23,7 +26,7 @@ namespace {
 using namespace kv4;
 
 constexpr int KBLOCKS = 2;                    // key tiles of a thread block
-constexpr int PW = 8 * KBLOCKS;               // the product warp; the others: two threads a key
+constexpr int PW = 16;                        // the product warp; the others: a quarter of the columns per 4 warps
 constexpr int MTHREADS = 32 * PW + 32;
 constexpr int QSTAGES = 3;
 constexpr uint32_t MASS_TMEM = 2 * KBLOCKS * CM;
@@ -34,8 +37,8 @@ struct MassPlan {
     static constexpr int GR = D / 64;
     static constexpr int KB = GR * KT * 128 + KT * 32, QB = q_block_bytes(D);
     static constexpr int TAB = 1024;                   // [4][64 column pairs]{factor x 2, -log2-sum-exp x 2}
-    static constexpr int SUM = TAB + 4 * CM * 8;       // [key tile][key]
-    static constexpr int K = SUM + KBLOCKS * KT * 4;   // [key tile]{[GR][128 keys][128 B] swizzled; C*}
+    static constexpr int SUM = TAB + 4 * CM * 8;       // [column quarter][key tile][key]
+    static constexpr int K = SUM + 4 * KBLOCKS * KT * 4;   // [key tile]{[GR][128 keys][128 B] swizzled; C*}
     static constexpr int Q = K + KBLOCKS * KB;
     static constexpr int BYTES = Q + QSTAGES * QB + 1024;
     static_assert(K % 1024 == 0 && KB % 1024 == 0 && QB % 1024 == 0, "swizzled rows start at a multiple of 1 KB");
@@ -48,8 +51,8 @@ __global__ void __launch_bounds__(MTHREADS, 1) kv4_mass_tc_kernel(const Kv4AttnA
     extern __shared__ unsigned char mass_raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>(((uintptr_t)mass_raw + 1023) & ~(uintptr_t)1023);
     uint64_t* q_full = reinterpret_cast<uint64_t*>(sm);  // [QSTAGES] Q operand arrived
-    uint64_t* s_full = q_full + QSTAGES;                 // [2][KBLOCKS] scores in TMEM
-    uint64_t* s_free = s_full + 2 * KBLOCKS;             // [2] scores read, and the table two tiles on written
+    uint64_t* s_full = q_full + QSTAGES;                 // [2] scores in TMEM
+    uint64_t* s_free = s_full + 2;                       // [2] scores read, and the table two tiles on written
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_free + 2);
     float* kmax = reinterpret_cast<float*>(tmem_slot + 2);  // [8]
     float* tab = reinterpret_cast<float*>(sm + P::TAB);
@@ -68,8 +71,10 @@ __global__ void __launch_bounds__(MTHREADS, 1) kv4_mass_tc_kernel(const Kv4AttnA
     const int n_tiles = (c_end - c_first + CM - 1) / CM;
     if (tid == 0) {
         for (int i = 0; i < QSTAGES; ++i) mbar_init(q_full + i, 1);
-        for (int i = 0; i < 2 * KBLOCKS; ++i) mbar_init(s_full + i, 1);
-        for (int i = 0; i < 2; ++i) mbar_init(s_free + i, 256 * KBLOCKS);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_full + i, 1);
+            mbar_init(s_free + i, 32 * PW);
+        }
         fence_mbar_init();
     }
 
@@ -92,10 +97,9 @@ __global__ void __launch_bounds__(MTHREADS, 1) kv4_mass_tc_kernel(const Kv4AttnA
     for (int w = 0; w < KBLOCKS * KT / 32; ++w) m = fmaxf(m, kmax[w]);
     const int ek = top_exponent(m);
     const float kup = __uint_as_float((uint32_t)(127 + 7 - ek) << 23);
-    const int kb = warp >> 3, half = (warp >> 2) & 1;
     if (warp < PW) {
         constexpr int CPR = D / 32, PER = KT * CPR / 256;
-        const int k0 = key0 + kb * KT;
+        const int kb = warp >> 3, k0 = key0 + kb * KT;
         const uint4* src = reinterpret_cast<const uint4*>(rows.w[0]) + (size_t)k0 * CPR;
         const uint16_t* s = reinterpret_cast<const uint16_t*>(rows.s[0]) + (size_t)k0 * GR;
 #pragma unroll
@@ -154,59 +158,75 @@ __global__ void __launch_bounds__(MTHREADS, 1) kv4_mass_tc_kernel(const Kv4AttnA
     bool ok = true;
 
     if (warp < PW) {
-        const int k0 = key0 + kb * KT, row = 32 * (warp & 3) + lane, key = k0 + row;
-        const uint32_t tm = tmem + kb * CM + half * 64 + ((uint32_t)(32 * (warp & 3)) << 16);
-        // first column that sees the thread's key, the tile's first and its last
+        const int quarter = warp >> 2, row = 32 * (warp & 3) + lane;
+        const uint32_t tm = tmem + quarter * 32 + ((uint32_t)(32 * (warp & 3)) << 16);
+        // first column that sees a key: the thread's two, the block's first, its last
         auto first_of = [&](int k) { return a.causal ? max(0, k - rw.off) * G : 0; };
-        const int mine = first_of(key) - half * 64, c_some = first_of(k0), c_all = first_of(k0 + KT - 1);
-        float total = 0.f;
+        int mine[KBLOCKS];
+#pragma unroll
+        for (int n = 0; n < KBLOCKS; ++n) mine[n] = first_of(key0 + n * KT + row) - c_first - quarter * 32;
+        const int c_all = first_of(key0 + KBLOCKS * KT - 1);
+        float total[KBLOCKS] = {0.f, 0.f};
         for (int i = 0; i < n_tiles; ++i) {
-            const int buf = i & 1, c0 = c_first + i * CM;
+            const int buf = i & 1;
             if (ok && i > 1 && !wait_bar(s_free + buf, ((i - 2) >> 1) & 1)) ok = false;
-            if (ok && !wait_bar(s_full + buf * KBLOCKS + kb, (i >> 1) & 1)) ok = false;
+            if (ok && !wait_bar(s_full + buf, (i >> 1) & 1)) ok = false;
             fence_after();
             put(i + 2, ahead);  // over the table of tile i - 2, which every thread has left
             ahead = fetch(i + 3);
-            const bool seen = k0 < T && c0 + CM > c_some;
-            unsigned long long s2[2] = {0ull, 0ull};
+            unsigned long long s2[KBLOCKS] = {0ull, 0ull};
 #pragma unroll 1
-            for (int r = 0; r < 64; r += 32) {  // 32 columns at a time: 64 would spill
-                float x[32];
-                ld16(tm + buf * KBLOCKS * CM + r, *reinterpret_cast<float(*)[16]>(&x[0]));
-                ld16(tm + buf * KBLOCKS * CM + r + 16, *reinterpret_cast<float(*)[16]>(&x[16]));
+            for (int r = 0; r < 32; r += 16) {  // 16 columns of both tiles at a time: 32 would spill
+                float x[KBLOCKS][16];
+#pragma unroll
+                for (int n = 0; n < KBLOCKS; ++n) ld16(tm + (buf * KBLOCKS + n) * CM + r, x[n]);
                 wait_ld();
-                if (r == 32) {
+                if (r == 16) {
                     fence_before();
                     arrive(s_free + buf);
                 }
-                if (!seen) continue;
-                const ulonglong2* t = reinterpret_cast<const ulonglong2*>(tab + (i & 3) * 2 * CM) + half * 32 + r / 2;
-                if (c0 >= c_all) {
+                const ulonglong2* t = reinterpret_cast<const ulonglong2*>(tab + (i & 3) * 2 * CM) + quarter * 16 + r / 2;
+                if (c_first + i * CM >= c_all) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
+                    for (int e = 0; e < 8; ++e) {
                         const ulonglong2 f = t[e];
-                        float p0, p1;
-                        unpack2(fma2(pack2(x[2 * e], x[2 * e + 1]), f.x, f.y), p0, p1);
-                        s2[e & 1] = add2(s2[e & 1], pack2(ex2(p0), ex2(p1)));
+#pragma unroll
+                        for (int n = 0; n < KBLOCKS; ++n) {
+                            float p0, p1;
+                            unpack2(fma2(pack2(x[n][2 * e], x[n][2 * e + 1]), f.x, f.y), p0, p1);
+                            s2[n] = add2(s2[n], pack2(ex2(p0), ex2(p1)));
+                        }
                     }
                 } else {
-                    const int from = mine - c0 - r;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
+                    for (int e = 0; e < 8; ++e) {
                         const ulonglong2 f = t[e];
-                        float p0, p1;
-                        unpack2(fma2(pack2(x[2 * e], x[2 * e + 1]), f.x, f.y), p0, p1);
-                        s2[e & 1] = add2(s2[e & 1], pack2(2 * e < from ? 0.f : ex2(p0), 2 * e + 1 < from ? 0.f : ex2(p1)));
+#pragma unroll
+                        for (int n = 0; n < KBLOCKS; ++n) {
+                            const int from = mine[n] - i * CM - r;
+                            float p0, p1;
+                            unpack2(fma2(pack2(x[n][2 * e], x[n][2 * e + 1]), f.x, f.y), p0, p1);
+                            s2[n] = add2(s2[n], pack2(2 * e < from ? 0.f : ex2(p0), 2 * e + 1 < from ? 0.f : ex2(p1)));
+                        }
                     }
                 }
             }
-            float s0, s1;
-            unpack2(add2(s2[0], s2[1]), s0, s1);
-            total += s0 + s1;
+#pragma unroll
+            for (int n = 0; n < KBLOCKS; ++n) {
+                float s0, s1;
+                unpack2(s2[n], s0, s1);
+                total[n] += s0 + s1;
+            }
         }
-        if (half == 1) sums[kb * KT + row] = total;
-        asm volatile("bar.sync %0, 64;" ::"r"(1 + kb * 4 + (warp & 3)) : "memory");
-        if (half == 0 && key < T && ok) a.mass[((size_t)b * a.c.heads + h) * a.c.max_pos + key] += total + sums[kb * KT + row];
+#pragma unroll
+        for (int n = 0; n < KBLOCKS; ++n) sums[(quarter * KBLOCKS + n) * KT + row] = total[n];
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * PW) : "memory");
+        if (tid < KBLOCKS * KT && key0 + tid < T && ok) {
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) sum += sums[w * KBLOCKS * KT + tid];
+            a.mass[((size_t)b * a.c.heads + h) * a.c.max_pos + key0 + tid] += sum;
+        }
     } else {
         const uint32_t qa = smem_u32(sm + P::Q), ka = smem_u32(sm + P::K);
         const uint64_t qd = desc(qa, 16), kd = desc(ka, 16), qx = desc16(qa + GR * CM * 128), kx = desc16(ka + GR * KT * 128);
@@ -228,10 +248,10 @@ __global__ void __launch_bounds__(MTHREADS, 1) kv4_mass_tc_kernel(const Kv4AttnA
                     mma_ss(d, at(kd, ko + (k >> 2) * KT * 128 + 32 * (k & 3)), at(qd, qo + (k >> 2) * CM * 128 + 32 * (k & 3)), idesc(CM, false),
                            k != 0 ? 1u : 0u);
                 mma_ss(d, at(kx, ko), at(qx, qo), idesc(CM, false), 1u);
-                commit(s_full + buf * KBLOCKS + n);
             }
+            commit(s_full + buf);
             if (i > 0 && issued < n_tiles) {  // the stage of tile i - 1 is free once its products are done
-                if (!wait_bar(s_full + (buf ^ 1) * KBLOCKS + KBLOCKS - 1, ((i - 1) >> 1) & 1)) ok = false;
+                if (!wait_bar(s_full + (buf ^ 1), ((i - 1) >> 1) & 1)) ok = false;
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 load(image);
