@@ -129,70 +129,65 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
 
+    // the two warps that share 32 columns meet
+    auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp >> 3) * 4 + (warp & 3)) : "memory"); };
     const Rows rows = head_rows<D>(a.c, (size_t)b * a.c.heads + h);
     const int key_end = min(T, t1 * KT);  // this block's keys end here
+    const int n_tiles = t1 - t0;
+    // Expansion: a thread takes 16-byte pieces (4 words of a row), thread after thread.
+    constexpr int CPR = D / 32, PIECES = KT * CPR, NTH = 256 * NB, PER = PIECES >= NTH ? PIECES / NTH : 1;
+    const bool has_piece = tid < PIECES;  // D = 64 and two column blocks: half of the threads
+    struct Share {
+        uint4 w[PER];
+        uint16_t s[PER], z[PER];  // scale and bias of the piece's group
+    } ks, vs;
+    uint32_t cs = 0, cz = 0;  // threads 0 .. 127: scales and biases of one key of the tile, every group
+    // A block-wide base and a 32-bit offset of the thread's own each.
+    const uint32_t po = (uint32_t)tid, so = (uint32_t)(tid / CPR * GR + ((tid % CPR) >> 1));
+    constexpr uint32_t PSTEP = NTH, SSTEP = NTH / CPR * GR;
+    auto load = [&](Share& x, int which, int i) {  // zeros past the last key
+        const int k0 = (t0 + i) * KT;
+        const uint4* src = reinterpret_cast<const uint4*>(rows.w[which] + (size_t)k0 * (D / 2));
+        const uint16_t* s = reinterpret_cast<const uint16_t*>(rows.s[which]) + (size_t)k0 * GR;
+        const uint16_t* z = reinterpret_cast<const uint16_t*>(rows.b[which]) + (size_t)k0 * GR;
+        if (k0 + KT <= T && (PIECES >= NTH || has_piece)) {
+#pragma unroll
+            for (uint32_t j = 0; j < PER; ++j) {
+                x.w[j] = src[po + PSTEP * j];
+                x.s[j] = s[so + SSTEP * j];
+                if (which) x.z[j] = z[so + SSTEP * j];
+            }
+            return;
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < PER; ++j) {
+            const bool in = has_piece && k0 + (tid + NTH * (int)j) / CPR < T;
+            x.w[j] = in ? src[po + PSTEP * j] : make_uint4(0u, 0u, 0u, 0u);
+            x.s[j] = in ? s[so + SSTEP * j] : (uint16_t)0;
+            if (which) x.z[j] = in ? z[so + SSTEP * j] : (uint16_t)0;
+        }
+    };
+    auto load_k = [&](int i) {
+        if (i >= n_tiles) return;
+        load(ks, 0, i);
+        const int key = (t0 + i) * KT + tid;
+        cs = tid < KT && key < T ? group_pair<GR>(rows.s[0], key) : 0u;
+        cz = tid < KT && key < T ? group_pair<GR>(rows.b[0], key) : 0u;
+    };
+    auto load_v = [&](int i) {
+        if (i < n_tiles) load(vs, 1, i);
+    };
     float cc = 0.f;  // score of a column = cc * S (softmax threads; K's power of two comes in below)
     if (warp < PW0) {
-        // Q operand: column `col`, the thread's half of its chunks, elements in the order of an expanded word
-        const bf16* src = a.q + (b * a.qs.b + (long long)i_row * a.qs.s + (long long)head * a.qs.h);
-        float mx = 0.f, sum[GR];
+        // Q operand: column `col`, the thread's half of its chunks, elements in the order of an expanded word.  Everything
+        // that the block begins with is on its way at once: the queries, the first tile's rows, the scales and biases.
+        constexpr int QW = 4 * GR;  // chunks of a thread: with two groups one of them
+        const bf16* src = a.q + (b * a.qs.b + (long long)i_row * a.qs.s + (long long)head * a.qs.h) + half * 8 * QW;
+        uint4 raw[QW];
 #pragma unroll
-        for (int g = 0; g < GR; ++g) {
-            sum[g] = 0.f;
-            if (row)
-#pragma unroll 4
-                for (int k = 0; k < 8; ++k) {
-                    const uint4 u = *reinterpret_cast<const uint4*>(src + 64 * g + 8 * k);
-                    const uint32_t X[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float lo = bits_lo_f(X[e]), hi = bits_hi_f(X[e]);
-                        sum[g] += lo + hi;
-                        mx = fmaxf(mx, fmaxf(fabsf(lo), fabsf(hi)));
-                    }
-                }
-        }
-        const int ex = max((int)(__float_as_uint(mx) >> 23) - 127, -100);
-        const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
-        cc = ldexpf(a.scale * LOG2E, ex - 14);
-        unsigned char* qo = sm + P::Q + (col >> 7) * P::QB;
-#pragma unroll 4
-        for (int j = 0; j < 4 * GR; ++j) {
-            const int g = (half * 4 * GR + j) / 8, k = (half * 4 * GR + j) % 8;
-            uint4 u = make_uint4(0u, 0u, 0u, 0u);
-            if (row) u = *reinterpret_cast<const uint4*>(src + 64 * g + 8 * k);
-            const uint32_t X[4] = {u.x, u.y, u.z, u.w};
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[2 * e] = bits_lo_f(X[e]) * up;
-                x[2 * e + 1] = bits_hi_f(X[e]) * up;
-            }
-            *reinterpret_cast<uint4*>(qo + g * CM * 128 + chunk_at(col & 127, k)) =
-                make_uint4(h2(x[0], x[4]), h2(x[1], x[5]), h2(x[2], x[6]), h2(x[3], x[7]));
-        }
-        // Q*: a group's sum times 2^-6 in three fp16 terms, k = 5 g + {0..4}: hi, hi, mid, mid, lo
-        // (against the two terms of 2^6 c: hi, lo, hi, lo, hi)
-        if (half == 0) {
-            __half t[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) t[e] = __float2half_rn(0.f);
-#pragma unroll
-            for (int g = 0; g < GR; ++g) {
-                const float v = sum[g] * up * 0.015625f;
-                const __half hi = __float2half_rn(v), mid = __float2half_rn(v - __half2float(hi));
-                t[5 * g] = t[5 * g + 1] = hi;
-                t[5 * g + 2] = t[5 * g + 3] = mid;
-                t[5 * g + 4] = __float2half_rn(v - __half2float(hi) - __half2float(mid));
-            }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                uint32_t r[4];
-#pragma unroll
-                for (int f = 0; f < 4; ++f) r[f] = as_u(__halves2half2(t[8 * e + 2 * f], t[8 * e + 2 * f + 1]));
-                *reinterpret_cast<uint4*>(qo + GR * CM * 128 + at16(col & 127, e)) = make_uint4(r[0], r[1], r[2], r[3]);
-            }
-        }
+        for (int k = 0; k < QW; ++k) raw[k] = row ? *reinterpret_cast<const uint4*>(src + 8 * k) : make_uint4(0u, 0u, 0u, 0u);
+        load_k(0);
+        load_v(0);
         // largest magnitudes that the block's rows can stand for: max(|b|, |b + 15 s|) (a NaN counts as nothing here)
         constexpr int KW = 2 / GR;  // keys of a 32-bit word of scales (rows end at a multiple of 16)
 #pragma unroll
@@ -210,6 +205,61 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
             }
             mx = warp_max(mx);
             if (lane == 0) kvmax[2 * warp + v] = mx;
+        }
+        float mx = 0.f, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < QW; ++k) {
+            const uint32_t X[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float lo = bits_lo_f(X[e]), hi = bits_hi_f(X[e]);
+                sum += lo + hi;
+                mx = fmaxf(mx, fmaxf(fabsf(lo), fabsf(hi)));
+            }
+        }
+        xch[half * CB + col] = mx;
+        xch[(2 + half) * CB + col] = sum;
+        pair_sync();
+        mx = fmaxf(xch[col], xch[CB + col]);
+        const int ex = max((int)(__float_as_uint(mx) >> 23) - 127, -100);
+        const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
+        cc = ldexpf(a.scale * LOG2E, ex - 14);
+        unsigned char* qo = sm + P::Q + (col >> 7) * P::QB;
+#pragma unroll
+        for (int j = 0; j < QW; ++j) {
+            const int g = (half * QW + j) / 8, k = (half * QW + j) % 8;
+            const uint32_t X[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[2 * e] = bits_lo_f(X[e]) * up;
+                x[2 * e + 1] = bits_hi_f(X[e]) * up;
+            }
+            *reinterpret_cast<uint4*>(qo + g * CM * 128 + chunk_at(col & 127, k)) =
+                make_uint4(h2(x[0], x[4]), h2(x[1], x[5]), h2(x[2], x[6]), h2(x[3], x[7]));
+        }
+        // Q*: a group's sum times 2^-6 in three fp16 terms, k = 5 g + {0..4}: hi, hi, mid, mid, lo
+        // (against the two terms of 2^6 c: hi, lo, hi, lo, hi)
+        if (half == 0) {
+            __half t[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) t[e] = __float2half_rn(0.f);
+#pragma unroll
+            for (int g = 0; g < GR; ++g) {
+                const float s = GR == 2 ? xch[(2 + g) * CB + col] : xch[2 * CB + col] + xch[3 * CB + col];
+                const float v = s * up * 0.015625f;
+                const __half hi = __float2half_rn(v), mid = __float2half_rn(v - __half2float(hi));
+                t[5 * g] = t[5 * g + 1] = hi;
+                t[5 * g + 2] = t[5 * g + 3] = mid;
+                t[5 * g + 4] = __float2half_rn(v - __half2float(hi) - __half2float(mid));
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                uint32_t r[4];
+#pragma unroll
+                for (int f = 0; f < 4; ++f) r[f] = as_u(__halves2half2(t[8 * e + 2 * f], t[8 * e + 2 * f + 1]));
+                *reinterpret_cast<uint4*>(qo + GR * CM * 128 + at16(col & 127, e)) = make_uint4(r[0], r[1], r[2], r[3]);
+            }
         }
     }
     fence_before();
@@ -230,7 +280,6 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
         return top_exponent(m);
     };
     const int ek = exponent(0), ev = exponent(1);
-    const int n_tiles = t1 - t0;
     bool ok = true;
 
     if (warp < PW0) {
@@ -243,53 +292,10 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
         const unsigned long long c2 = pack2(cc, cc);
 
         // ---- expansion of this thread's share of a tile --------------------------------------------------
-        // A thread takes 16-byte pieces (4 words of a row), thread after thread.
-        constexpr int CPR = D / 32, PIECES = KT * CPR, NTH = 256 * NB, PER = PIECES >= NTH ? PIECES / NTH : 1;
-        const bool has_piece = tid < PIECES;  // D = 64 and two column blocks: half of the threads
         const float kup = __uint_as_float((uint32_t)(127 + 7 - ek) << 23), vup = __uint_as_float((uint32_t)(127 + 13 - ev) << 23);
         // A NaN in V: where every column sees the key its value is simply NaN; in a tile that some column sees in
         // part only, the value is left out and the key's score made NaN, which reaches just the rows that see it.
         auto partial = [&](int i) { return (t0 + i + 1) * KT > all; };
-        struct Share {
-            uint4 w[PER];
-            uint16_t s[PER], z[PER];  // scale and bias of the piece's group
-        } ks, vs;
-        uint32_t cs = 0, cz = 0;  // threads 0 .. 127: scales and biases of one key of the tile, every group
-        // A block-wide base and a 32-bit offset of the thread's own each.
-        const uint32_t po = (uint32_t)tid, so = (uint32_t)(tid / CPR * GR + ((tid % CPR) >> 1));
-        constexpr uint32_t PSTEP = NTH, SSTEP = NTH / CPR * GR;
-        auto load = [&](Share& x, int which, int i) {  // zeros past the last key
-            const int k0 = (t0 + i) * KT;
-            const uint4* src = reinterpret_cast<const uint4*>(rows.w[which] + (size_t)k0 * (D / 2));
-            const uint16_t* s = reinterpret_cast<const uint16_t*>(rows.s[which]) + (size_t)k0 * GR;
-            const uint16_t* z = reinterpret_cast<const uint16_t*>(rows.b[which]) + (size_t)k0 * GR;
-            if (k0 + KT <= T && (PIECES >= NTH || has_piece)) {
-#pragma unroll
-                for (uint32_t j = 0; j < PER; ++j) {
-                    x.w[j] = src[po + PSTEP * j];
-                    x.s[j] = s[so + SSTEP * j];
-                    if (which) x.z[j] = z[so + SSTEP * j];
-                }
-                return;
-            }
-#pragma unroll
-            for (uint32_t j = 0; j < PER; ++j) {
-                const bool in = has_piece && k0 + (tid + NTH * (int)j) / CPR < T;
-                x.w[j] = in ? src[po + PSTEP * j] : make_uint4(0u, 0u, 0u, 0u);
-                x.s[j] = in ? s[so + SSTEP * j] : (uint16_t)0;
-                if (which) x.z[j] = in ? z[so + SSTEP * j] : (uint16_t)0;
-            }
-        };
-        auto load_k = [&](int i) {
-            if (i >= n_tiles) return;
-            load(ks, 0, i);
-            const int key = (t0 + i) * KT + tid;
-            cs = tid < KT && key < T ? group_pair<GR>(rows.s[0], key) : 0u;
-            cz = tid < KT && key < T ? group_pair<GR>(rows.b[0], key) : 0u;
-        };
-        auto load_v = [&](int i) {
-            if (i < n_tiles) load(vs, 1, i);
-        };
         auto store_k = [&](int i) {  // tile i's K operand from ks, cs, cz
             if (i >= n_tiles) return;
             if (ok && i > 1 && !wait_bar(k_free + (i & 1), ((i - 2) >> 1) & 1)) ok = false;
@@ -330,8 +336,6 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
             if (iv < n_tiles) arrive(v_full + (iv & 1));
             if (ik < n_tiles) arrive(k_full + (ik & 1));
         };
-        load_k(0);
-        load_v(0);
         store_k(0);
         store_v(0);
         publish(0, 0);  // and the Q operand
@@ -365,7 +369,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
 #pragma unroll
                 for (int k = 0; k < KH; k += 2) top = max3(top, x[k], x[k + 1]);
                 xch[(2 * m + half) * CB + col] = top;
-                asm volatile("bar.sync %0, 64;" ::"r"(2 + blk * 4 + (warp & 3)) : "memory");
+                pair_sync();
                 top = fmaxf(top, xch[(2 * m + (half ^ 1)) * CB + col]);
                 if (__any_sync(0xffffffffu, top > thr)) {
                     // raise the maximum of the columns that ask for it, and rescale what they have summed
@@ -426,7 +430,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
             load_k(i + 3);
         }
         xch[half * CB + col] = l;
-        asm volatile("bar.sync %0, 64;" ::"r"(2 + blk * 4 + (warp & 3)) : "memory");
+        pair_sync();
         l = xch[col] + xch[CB + col];
         if (ok && !wait_bar(pv_done + blk, (n_tiles - 1) & 1)) ok = false;
         fence_after();
