@@ -102,12 +102,16 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
     const int half = (warp >> 2) & 1;  // softmax threads: half of a tile's keys
     const int col = min((warp >> 3) * CM + (tid & 127), CB - 1), c = cb * CB + col, i_row = c / G, head = h * G + c % G;
     const bool row = c < C && i_row < rw.n;
-    bf16* out = a.out + (b * a.os.b + (long long)i_row * a.os.s + (long long)head * a.os.h);
-    const size_t lse_at = ((size_t)b * a.S + i_row) * a.Hq + head;
+    // (worked out where they are used: between the block's begin and end registers are short)
+    auto out_row = [&] {
+        const int i = c / G;
+        return a.out + (b * a.os.b + (long long)i * a.os.s + (long long)(h * G + (c - i * G)) * a.os.h);
+    };
+    auto lse_at = [&] { return a.lse + (((size_t)b * a.S + c / G) * a.Hq + h * G + c % G); };
     if (t0 == t1) {  // nothing to see: zeros (a split's empty share is skipped by the joining kernel)
         if (nsplit == 1 && warp < PW0 && half == 0 && c < C) {
-            for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(out + d) = make_uint4(0u, 0u, 0u, 0u);
-            if (a.lse) a.lse[lse_at] = -INFINITY;
+            for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(out_row() + d) = make_uint4(0u, 0u, 0u, 0u);
+            if (a.lse) *lse_at() = -INFINITY;
         }
         return;
     }
@@ -181,13 +185,23 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
     if (warp < PW0) {
         // Q operand: column `col`, the thread's half of its chunks, elements in the order of an expanded word.  Everything
         // that the block begins with is on its way at once: the queries, the first tile's rows, the scales and biases.
+        // (The queries come row by row into their places, to be converted there: a row per lane is 32 lines a load, which
+        // alone took 4000 cycles.)
         constexpr int QW = 4 * GR;  // chunks of a thread: with two groups one of them
-        const bf16* src = a.q + (b * a.qs.b + (long long)i_row * a.qs.s + (long long)head * a.qs.h) + half * 8 * QW;
-        uint4 raw[QW];
-#pragma unroll
-        for (int k = 0; k < QW; ++k) raw[k] = row ? *reinterpret_cast<const uint4*>(src + 8 * k) : make_uint4(0u, 0u, 0u, 0u);
+        auto all_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(256 * NB) : "memory"); };
+        long long* off = reinterpret_cast<long long*>(xch);  // [CB]
+        if (half == 0) off[col] = row ? b * a.qs.b + (long long)i_row * a.qs.s + (long long)head * a.qs.h : -1;
         load_k(0);
         load_v(0);
+        all_sync();
+#pragma unroll
+        for (int j = 0; j < QW; ++j) {
+            const int p = tid + 256 * NB * j, qc = p / (D / 8), k = p % (D / 8);
+            const long long o = off[qc];
+            cp_async16_zfill(smem_u32(sm + P::Q + (qc >> 7) * P::QB + (k >> 3) * CM * 128 + chunk_at(qc & 127, k & 7)),
+                       o < 0 ? a.q : a.q + o + 8 * k, o >= 0);
+        }
+        cp_async_commit();
         // largest magnitudes that the block's rows can stand for: max(|b|, |b + 15 s|) (a NaN counts as nothing here)
         constexpr int KW = 2 / GR;  // keys of a 32-bit word of scales (rows end at a multiple of 16)
 #pragma unroll
@@ -195,7 +209,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
             float mx = 0.f;
             const uint32_t* s = reinterpret_cast<const uint32_t*>(rows.s[v]);
             const uint32_t* z = reinterpret_cast<const uint32_t*>(rows.b[v]);
-#pragma unroll 8
+#pragma unroll 4
             for (int w = t0 * KT / KW + tid; w < (key_end + KW - 1) / KW; w += 256 * NB) {
                 const uint32_t us = s[w], uz = z[w];
                 const float z0 = bits_lo_f(uz), z1 = bits_hi_f(uz);
@@ -206,10 +220,15 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
             mx = warp_max(mx);
             if (lane == 0) kvmax[2 * warp + v] = mx;
         }
+        cp_async_wait<0>();
+        all_sync();
+        unsigned char* qo = sm + P::Q + (col >> 7) * P::QB;
+        auto mine = [&](int k) { return reinterpret_cast<uint4*>(qo + (half * QW + k) / 8 * CM * 128 + chunk_at(col & 127, (half * QW + k) % 8)); };
         float mx = 0.f, sum = 0.f;
-#pragma unroll
+#pragma unroll 2
         for (int k = 0; k < QW; ++k) {
-            const uint32_t X[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+            const uint4 raw = *mine(k);
+            const uint32_t X[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float lo = bits_lo_f(X[e]), hi = bits_hi_f(X[e]);
@@ -224,19 +243,17 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
         const int ex = max((int)(__float_as_uint(mx) >> 23) - 127, -100);
         const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
         cc = ldexpf(a.scale * LOG2E, ex - 14);
-        unsigned char* qo = sm + P::Q + (col >> 7) * P::QB;
-#pragma unroll
+#pragma unroll 2
         for (int j = 0; j < QW; ++j) {
-            const int g = (half * QW + j) / 8, k = (half * QW + j) % 8;
-            const uint32_t X[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+            const uint4 raw = *mine(j);
+            const uint32_t X[4] = {raw.x, raw.y, raw.z, raw.w};
             float x[8];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 x[2 * e] = bits_lo_f(X[e]) * up;
                 x[2 * e + 1] = bits_hi_f(X[e]) * up;
             }
-            *reinterpret_cast<uint4*>(qo + g * CM * 128 + chunk_at(col & 127, k)) =
-                make_uint4(h2(x[0], x[4]), h2(x[1], x[5]), h2(x[2], x[6]), h2(x[3], x[7]));
+            *mine(j) = make_uint4(h2(x[0], x[4]), h2(x[1], x[5]), h2(x[2], x[6]), h2(x[3], x[7]));
         }
         // Q*: a group's sum times 2^-6 in three fp16 terms, k = 5 g + {0..4}: hi, hi, mid, mid, lo
         // (against the two terms of 2^6 c: hi, lo, hi, lo, hi)
@@ -439,31 +456,59 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
         const float f = nsplit == 1 ? (has ? 1.f / l : 0.f) : 1.f;
         const float e0 = __uint_as_float((uint32_t)(127 - 13) << 23), e1 = __uint_as_float((uint32_t)(127 + ev) << 23);
         const size_t slot = (seg * nsplit + sp) * CB + col;
+        // Through shared memory (the Q and K operands, of which every product is done), so that lanes write along
+        // rows: [32 columns][128 B], swizzled.
+        const bf16* out = out_row();
+        unsigned char* stage = sm + P::Q + warp * 4096;
+        auto piece = [&](int r, int ch) { return reinterpret_cast<uint4*>(stage + chunk_at(r, ch)); };
+        const int c_warp = cb * CB + (warp >> 3) * CM + 32 * (warp & 3);  // the warp's first column
+        constexpr int STEP = D / 2 < 32 ? D / 2 : 32;
 #pragma unroll 1
-        for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 16) {
-            float o[16];
-            ld16(tm + P::TO + d, o);
-            wait_ld();
+        for (int d0 = half * (D / 2); d0 < (half + 1) * (D / 2); d0 += nsplit == 1 ? D / 2 : STEP) {
+#pragma unroll 1
+            for (int d = 0; d < (nsplit == 1 ? D / 2 : STEP); d += 16) {
+                float o[16];
+                ld16(tm + P::TO + d0 + d, o);
+                wait_ld();
 #pragma unroll
-            for (int g = 0; g < 16; g += 8) {
-                float v[8];
+                for (int g = 0; g < 16; g += 8) {
+                    float v[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = o[g + (e < 4 ? 2 * e : 2 * e - 7)] * f * e0 * e1;  // columns hold 0, 4, 1, 5, ...
-                if (!ok || c >= C) continue;
-                if (nsplit == 1) {
-                    *reinterpret_cast<uint4*>(out + d + g) =
-                        has ? make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]))
-                            : make_uint4(0u, 0u, 0u, 0u);
-                } else {
-                    float* dst = part + slot * D + d + g;
-                    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
-                    *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                    for (int e = 0; e < 8; ++e) v[e] = o[g + (e < 4 ? 2 * e : 2 * e - 7)] * f * e0 * e1;  // columns hold 0, 4, 1, 5, ...
+                    if (nsplit == 1) {
+                        *piece(lane, (d + g) / 8) =
+                            has ? make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]))
+                                : make_uint4(0u, 0u, 0u, 0u);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; e += 4)
+                            *piece(lane, (d + g + e) / 4) =
+                                make_uint4(__float_as_uint(v[e]), __float_as_uint(v[e + 1]), __float_as_uint(v[e + 2]), __float_as_uint(v[e + 3]));
+                    }
                 }
             }
+            __syncwarp();
+            if (nsplit == 1) {
+                constexpr int NCH = D / 16;  // 16-byte chunks of a row's half
+#pragma unroll
+                for (int it = 0; it < NCH; ++it) {
+                    const int r = it * (32 / NCH) + lane / NCH, ch = lane % NCH;
+                    bf16* dst = reinterpret_cast<bf16*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), r));
+                    if (ok && c_warp + r < C) *reinterpret_cast<uint4*>(dst + d0 + 8 * ch) = *piece(r, ch);
+                }
+            } else {
+                constexpr int NCH = STEP / 4;
+#pragma unroll
+                for (int it = 0; it < NCH; ++it) {
+                    const int r = it * (32 / NCH) + lane / NCH, ch = lane % NCH;
+                    if (ok && c_warp + r < C) *reinterpret_cast<uint4*>(part + (slot - lane + r) * D + d0 + 4 * ch) = *piece(r, ch);
+                }
+            }
+            __syncwarp();
         }
         if (ok && c < C && half == 0) {
             if (nsplit == 1) {
-                if (a.lse) a.lse[lse_at] = has ? (log2f(l) - nm) * LN2 : -INFINITY;
+                if (a.lse) *lse_at() = has ? (log2f(l) - nm) * LN2 : -INFINITY;
             } else {
                 pml[slot] = make_float2(l != 0.f ? -nm : M0, l);
             }
