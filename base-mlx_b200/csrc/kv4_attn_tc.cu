@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
             reinterpret_cast<float*>(qkeep + (size_t)a.c.batch * a.c.heads * ncb * NB * P::QB)[seg * CB + col] = cc;
     }
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-    // exponents of the largest values: K enters times 2^(7 - ek), V times 2^(13 - ev)
+    // exponents of the largest values
     auto exponent = [&](int v) {
         float m = 0.f;
 #pragma unroll
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
         const unsigned long long c2 = pack2(cc, cc);
 
         // ---- expansion of this thread's share of a tile --------------------------------------------------
-        const float kup = __uint_as_float((uint32_t)(127 + 7 - ek) << 23), vup = __uint_as_float((uint32_t)(127 + 13 - ev) << 23);
+        const float kup = __uint_as_float((uint32_t)(127 + 7 - ek) << 23), vup = __uint_as_float((uint32_t)(127 + 16 - ev) << 23);
         // A NaN in V: where every column sees the key its value is simply NaN; in a tile that some column sees in
         // part only, the value is left out and the key's score made NaN, which reaches just the rows that see it.
         auto partial = [&](int i) { return (t0 + i + 1) * KT > all; };
@@ -319,10 +319,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
             unsigned char* dst = sm + P::K + (i & 1) * P::KB;
             if (has_piece)
 #pragma unroll
-                for (int j = 0; j < PER; ++j) {
-                    const __half2 s2 = __float2half2_rn(u16_to_f(ks.s[j]) * kup);
-                    expand_piece<D>(ks.w[j], tid + NTH * j, dst, [&](uint32_t n) { return centred(n, s2); });
-                }
+                for (int j = 0; j < PER; ++j) expand_piece<D>(ks.w[j], tid + NTH * j, dst, Centred(u16_to_f(ks.s[j]) * kup));
             if (tid < KT) {
                 bool nan = false;
                 const int key = (t0 + i) * KT + tid;
@@ -337,14 +334,14 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
             if (i >= n_tiles) return;
             if (ok && i > 1 && !wait_bar(v_free + (i & 1), ((i - 2) >> 1) & 1)) ok = false;
             unsigned char* dst = sm + P::V + (i & 1) * P::VB;
-            const __half2 k1024 = __float2half2_rn(1024.f);
             if (has_piece)
 #pragma unroll
                 for (int j = 0; j < PER; ++j) {
                     float s = u16_to_f(vs.s[j]), z = u16_to_f(vs.z[j]);
                     if (partial(i) && !(fabsf(s) + fabsf(z) < INFINITY)) s = z = 0.f;
-                    const __half2 s2 = __float2half2_rn(s * vup), z2 = __float2half2_rn(z * vup);
-                    expand_piece<D>(vs.w[j], tid + NTH * j, dst, [&](uint32_t n) { return as_u(__hfma2(__hsub2(as_h2(n), k1024), s2, z2)); });
+                    // n 2^-18 times 2^18 s plus z, times 2^(-2 - ev): s is at most 2/15 of the largest value
+                    const __half2 s2 = __float2half2_rn(s * vup), z2 = __float2half2_rn(z * vup * 0x1p-18f);
+                    expand_piece<D>(vs.w[j], tid + NTH * j, dst, [&](uint32_t n) { return as_u(__hfma2(as_h2(n), s2, z2)); });
                 }
         };
         // Stores first, then one fence, then the loads: a fence waits for the thread's loads in flight.
@@ -454,7 +451,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
         // ---- output ---------------------------------------------------------------------------------
         const bool has = row && l != 0.f;
         const float f = nsplit == 1 ? (has ? 1.f / l : 0.f) : 1.f;
-        const float e0 = __uint_as_float((uint32_t)(127 - 13) << 23), e1 = __uint_as_float((uint32_t)(127 + ev) << 23);
+        const float e0 = 4.f, e1 = __uint_as_float((uint32_t)(127 + ev) << 23);
         const size_t slot = (seg * nsplit + sp) * CB + col;
         // Through shared memory (the Q and K operands, of which every product is done), so that lanes write along
         // rows: [32 columns][128 B], swizzled.

@@ -107,8 +107,7 @@ __global__ void __launch_bounds__(MTHREADS, 1) kv4_mass_tc_kernel(const Kv4AttnA
             const int p = (tid & 255) + 256 * j, key = p / CPR;
             const bool in = k0 + key < T;
             const uint4 w = in ? src[p] : make_uint4(0u, 0u, 0u, 0u);
-            const __half2 s2 = __float2half2_rn(in ? u16_to_f(s[key * GR + ((p % CPR) >> 1)]) * kup : 0.f);
-            expand_piece<D>(w, p, sm + P::K + kb * P::KB, [&](uint32_t n) { return centred(n, s2); });
+            expand_piece<D>(w, p, sm + P::K + kb * P::KB, Centred(in ? u16_to_f(s[key * GR + ((p % CPR) >> 1)]) * kup : 0.f));
         }
         if (tid < KBLOCKS * KT)
             store_offsets<GR>(sm + P::K + tid / KT * P::KB + GR * KT * 128, tid % KT, cs, cz, kup, false);

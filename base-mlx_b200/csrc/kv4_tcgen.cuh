@@ -102,7 +102,7 @@ QW_DEV unsigned long long add2(unsigned long long a, unsigned long long b) {
 }
 
 // Piece p (words 4 (p % CPR) .. of key p / CPR) of a tile's packed rows to the swizzled operand rows at dst, each
-// word's nibble pairs (1024 + n_j, 1024 + n_{j + 4}) through `value`.  With two groups the second one's words go out
+// word's nibble pairs through `value`, which gets (n_j, n_{j + 4}) at bits 6 .. 9 of its halves: n 2^-18 as fp16.  With two groups the second one's words go out
 // in another order (e ^ 2): the eight lanes of a store phase (two keys, all pieces) hit eight different chunk columns.
 template <int D, typename F>
 QW_DEV void expand_piece(const uint4& w, int p, unsigned char* dst, F&& value) {
@@ -114,12 +114,16 @@ QW_DEV void expand_piece(const uint4& w, int p, unsigned char* dst, F&& value) {
         const uint32_t v = g ? u[e ^ 2] : u[e];
         uint32_t o[4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) o[n] = value(((v >> (4 * n)) & 0x000F000Fu) | 0x64006400u);
+        for (int n = 0; n < 4; ++n) o[n] = value((n < 2 ? v << (6 - 4 * n) : v >> (4 * n - 6)) & 0x03C003C0u);
         *reinterpret_cast<uint4*>(dst + g * KT * 128 + chunk_at(key, 4 * (q & 1) + (g ? e ^ 2 : e))) = make_uint4(o[0], o[1], o[2], o[3]);
     }
 }
-// K' of a pair: s (n - 8), exact.
-QW_DEV uint32_t centred(uint32_t n, __half2 s2) { return as_u(__hmul2(__hsub2(as_h2(n), __float2half2_rn(1032.f)), s2)); }
+// K' of a pair: s (n - 8) = (16 + n) s - 24 s in one exact step (24 s has 10 bits).
+struct Centred {
+    __half2 s2, m24;
+    QW_DEV explicit Centred(float s) : s2(__float2half2_rn(s)), m24(__hmul2(s2, __float2half2_rn(-24.f))) {}
+    QW_DEV uint32_t operator()(uint32_t n) const { return as_u(__hfma2(as_h2(n | 0x4C004C00u), s2, m24)); }
+};
 // C* of one key (`scale`, `bias`: its groups' bf16 pairs): 2^6 c kup in two fp16 terms, k = 5 g + {0..4}: hi, lo, hi, lo, hi.
 template <int GR>
 QW_DEV void store_offsets(unsigned char* dst, int row, uint32_t scale, uint32_t bias, float kup, bool nan) {
@@ -142,7 +146,7 @@ QW_DEV void store_offsets(unsigned char* dst, int row, uint32_t scale, uint32_t 
         *reinterpret_cast<uint4*>(dst + at16(row, e)) = make_uint4(r[0], r[1], r[2], r[3]);
     }
 }
-// The exponent of a largest magnitude m: K enters times 2^(7 - ek), V times 2^(13 - ev).
+// The exponent of a largest magnitude m: K enters times 2^(7 - ek), V times 2^(-2 - ev).
 QW_DEV int top_exponent(float m) { return max((int)(__float_as_uint(fminf(m, 3.0e38f)) >> 23) - 127, -100); }
 // The bf16 of every group of a key.
 template <int GR>
