@@ -135,6 +135,15 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
 
     // the two warps that share 32 columns meet
     auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp >> 3) * 4 + (warp & 3)) : "memory"); };
+    auto pair_any = [&](bool v) {
+        uint32_t r;
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %2, 0;\n\tbarrier.cta.red.or.pred q, %1, 64, p;\n\tselp.b32 %0, 1, 0, q;\n\t}\n"
+            : "=r"(r)
+            : "r"(2 + (warp >> 3) * 4 + (warp & 3)), "r"((int)v)
+            : "memory");
+        return r != 0;
+    };
     const Rows rows = head_rows<D>(a.c, (size_t)b * a.c.heads + h);
     const int key_end = min(T, t1 * KT);  // this block's keys end here
     const int n_tiles = t1 - t0;
@@ -364,7 +373,8 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
             if (ok && !wait_bar(s_full + blk, i & 1)) ok = false;
             fence_after();
             // Two rounds of 64 keys, 32 of them this thread's.  P of a round lies over columns of S that this
-            // round or the one before has read; the two warps of the column meet after each read.
+            // round or the one before has read; the two warps of the column meet after each read, and hear
+            // whether either of them met a larger score.
 #pragma unroll 1
             for (int m = 0; m < 2; ++m) {
                 const int k0 = 64 * m + 32 * half, key0 = (t0 + i) * KT + k0;
@@ -382,10 +392,10 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
                 float top = -INFINITY;
 #pragma unroll
                 for (int k = 0; k < KH; k += 2) top = max3(top, x[k], x[k + 1]);
-                xch[(2 * m + half) * CB + col] = top;
-                pair_sync();
-                top = fmaxf(top, xch[(2 * m + (half ^ 1)) * CB + col]);
-                if (__any_sync(0xffffffffu, top > thr)) {
+                if (pair_any(top > thr)) {
+                    xch[(2 * m + half) * CB + col] = top;
+                    pair_sync();
+                    top = fmaxf(top, xch[(2 * m + (half ^ 1)) * CB + col]);
                     // raise the maximum of the columns that ask for it, and rescale what they have summed
                     float al = 1.f;
                     if (top > thr) {
