@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) kv4_attn_join_kernel(const Kv
     if (first == last) return;
     // the first share's partial of this segment is its second one if the share began before it
     auto slot = [&](int k) { return (2ll * (first + k) + (k == 0 && first * per < s0 ? 1 : 0)) * cb_size + col; };
-    join_row<D, JOIN_WARPS>(last - first + 1, warp, slot, part, pml, sh, dst, lse);
+    join_row<D, JOIN_WARPS, 8>(last - first + 1, warp, slot, part, pml, sh, dst, lse);
 }
 
 // ---- attention weights ------------------------------------------------------

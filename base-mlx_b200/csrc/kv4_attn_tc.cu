@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
     // rows of the block's columns, keys they see, this split's tiles
     const int i_first = cb * CB / G, i_last = min(rw.n, (min(C, (cb + 1) * CB) - 1) / G + 1) - 1;
     const int keys = i_last < i_first ? 0 : a.causal ? min(T, rw.off + i_last + 1) : T;
-    const int nt = (keys + KT - 1) / KT, t0 = (int)((long long)nt * sp / nsplit), t1 = (int)((long long)nt * (sp + 1) / nsplit);
+    const int nt = (keys + KT - 1) / KT, t0 = nt * sp / nsplit, t1 = nt * (sp + 1) / nsplit;  // (nt < 2^24, nsplit <= 64)
     const int all = a.causal ? min(T, rw.off + i_first + 1) : T;  // keys that every column sees
     const size_t seg = ((size_t)b * a.c.heads + h) * ncb + cb;
 
@@ -605,9 +605,9 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) kv4_attn_tc_join_kernel(const
     }
     // a split without tiles has left nothing
     auto slot = [&](int k) {
-        return (long long)nt * k / nsplit == (long long)nt * (k + 1) / nsplit ? -1ll : (long long)(s0 + (size_t)k * cb_size);
+        return nt * k / nsplit == nt * (k + 1) / nsplit ? -1ll : (long long)(s0 + (size_t)k * cb_size);
     };
-    join_row<D, 1>(nsplit, 0, slot, part, pml, nullptr, dst, lse);
+    join_row<D, 1, 4>(nsplit, 0, slot, part, pml, nullptr, dst, lse);
 }
 
 template <int D, int NB>

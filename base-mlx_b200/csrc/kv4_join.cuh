@@ -8,8 +8,8 @@ namespace kv4 {
 
 // The WPR warps of a row take its n partials in turn; slot(k) is partial k's row in `part` and `pml`,
 // or negative if it was left empty.  The caller's warps are `wi` of the row (all of them or none take part);
-// `sh` is shared memory of WPR x (D + 2) floats per row.  Lane l holds dimensions l D / 32 ...
-template <int D, int WPR, typename Slot>
+// `sh` is shared memory of WPR x (D + 2) floats per row; UNROLL partials are in flight at a time.  Lane l holds dimensions l D / 32 ...
+template <int D, int WPR, int UNROLL, typename Slot>
 QW_DEV void join_row(int n, int wi, Slot slot, const float* part, const float2* pml, float* sh, bf16* dst, float* lse) {
     constexpr int V = D / 32;
     const int lane = threadIdx.x & 31;
@@ -27,10 +27,10 @@ QW_DEV void join_row(int n, int wi, Slot slot, const float* part, const float2* 
         for (int e = 0; e < V; ++e) o[e] = o[e] * al * al;
         M = m;
         const int cnt = min(32, (n - k0 + WPR - 1) / WPR);
-        for (int j = 0; j < cnt; j += 8) {
-            float v[8][V];
+        for (int j = 0; j < cnt; j += UNROLL) {
+            float v[UNROLL][V];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < UNROLL; ++e) {
                 const long long t = __shfl_sync(0xffffffffu, s, min(j + e, 31));
                 const bool in = j + e < cnt && t >= 0;
                 const float* p = part + (in ? (size_t)t * D : 0) + lane * V;
@@ -43,7 +43,7 @@ QW_DEV void join_row(int n, int wi, Slot slot, const float* part, const float2* 
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < UNROLL; ++e) {
                 const float fe = j + e < cnt ? __shfl_sync(0xffffffffu, f, min(j + e, 31)) : 0.f;
 #pragma unroll
                 for (int d = 0; d < V; ++d) o[d] = fmaf(v[e][d] * fe, fe, o[d]);
