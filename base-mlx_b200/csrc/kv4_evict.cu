@@ -12,6 +12,11 @@
 //      how many of its equals stay, one prefix over the threads' consecutive
 //      positions writes the kept ones in order.
 //   2. move: dst row r = src row index[r].
+//
+// 8 sequences of up to 16384 positions, 8 heads, half of them kept: 46 us, of them
+// 24 for the move (117 MB at 4.8 TB/s, waiting on its gathers) and 16 for the
+// selection, which is bound by the latency of its passes: weights to keys, three
+// histograms with a cluster barrier each, the prefix.
 #include <algorithm>
 
 #include "kv4.h"
@@ -298,7 +303,8 @@ __global__ void __launch_bounds__(256) kv4_move_kernel(const Kv4EvictArgs a, con
 // In place: one block per (sequence, head, K words | V words | the rest) walks
 // the kept rows in order, a chunk at a time: read, barrier, write.  index[r] >= r,
 // so the rows a chunk overwrites are never read by a later chunk.  MR rows per
-// thread and chunk: a chunk costs two memory latencies and two barriers.
+// thread and chunk: a chunk costs two memory latencies and two barriers (the case
+// above: 35 us, against 24 out of place).
 template <int D>
 __global__ void __launch_bounds__(1024) kv4_move_inplace_kernel(const Kv4EvictArgs a, const int* index, const int* count) {
     constexpr int P = D / 32, GR = D / 64, RB = 1024 / P;

@@ -593,7 +593,8 @@ def kv4_evict(src: Kv4, dst: Kv4, mass_src_ptr: int, mass_dst_ptr: int, seq_len_
               stream: int = 0) -> None:
     """Cut sequences longer than `keep` to `keep` positions per kv head: the last
     `recent` and the others of largest accumulated weight, moved to the front
-    of dst (src itself, or a cache apart from it) in their old order."""
+    of dst (src itself, or a cache apart from it) in their old order.  Rows and
+    weights behind the new lengths are left: clear those weights before adding to them."""
     check(lib().qw_kv4_evict(ctypes.byref(src), ctypes.byref(dst), mass_src_ptr, mass_dst_ptr, seq_len_ptr,
                              new_len_ptr, keep, recent, index_ptr or None, scratch_ptr, scratch_bytes,
                              stream or None))

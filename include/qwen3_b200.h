@@ -361,7 +361,11 @@ QW_API int qw_kv4_append(const qw_kv4* cache, const void* k, const int64_t* k_st
 QW_API int qw_kv4_read(const qw_kv4* cache, void* k_out, void* v_out, int S, const int32_t* seq_len_dev,
                        const int32_t* n_new_dev, int32_t* err_dev, void* stream);
 
-/* Scratch of qw_kv4_attention for S rows of `heads` query heads on the cache's GPU. */
+/* Scratch of qw_kv4_attention for S rows of `heads` query heads on the cache's
+ * GPU, with or without mass.  With at most 16 columns (S * heads / kv_heads) it
+ * holds their scores, up to 64 bytes per position of the cache and kv head; with
+ * 64 or more, a copy of the queries.  One scratch serves the calls of one
+ * stream, one after another; calls that may overlap need one each. */
 QW_API int qw_kv4_attention_scratch(const qw_kv4* cache, int S, int heads, size_t* bytes);
 
 /* Attention of S new rows per sequence (already appended) over the cache:
@@ -397,7 +401,8 @@ QW_API int qw_kv4_evict_scratch(const qw_kv4* src, int keep, size_t* bytes);
  * them.  dst is src itself (in place; then mass_dst = mass_src, and
  * new_len_dev may be seq_len_dev) or a cache that does not overlap it, of the
  * same batch, kv_heads and head_dim with max_pos >= keep; its rows past
- * new_len are left as they are.  Keys keep the positions they were rotated
+ * new_len are left as they are, and so are the weights there: a caller that
+ * appends rows and accumulates on clears those first.  Keys keep the positions they were rotated
  * with: rows appended later count seq_len from the new length, rotary
  * positions go on from the old one. */
 QW_API int qw_kv4_evict(const qw_kv4* src, const qw_kv4* dst, const float* mass_src, float* mass_dst,
