@@ -809,6 +809,46 @@ def test_other_stream_and_two_calls_at_once():
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("S,Hq,Hkv", [(1, 1, 1), (1, 6, 2), (5, 1, 1), (7, 2, 2), (2, 8, 2), (3, 3, 1), (15, 1, 1), (4, 4, 1),
+                                      (17, 1, 1), (5, 16, 2), (63, 1, 1), (16, 4, 1), (13, 5, 1), (127, 1, 1), (32, 8, 2),
+                                      (43, 3, 1), (51, 5, 1), (86, 3, 1)])
+def test_weights_at_every_number_of_columns(S, Hq, Hkv, D):
+    """1 to 258 columns per kv head: scores kept, recomputed and from kept queries; one sequence without rows, one that
+    ends inside a tile, one whose queries past its rows are NaN."""
+    torch = _torch()
+    c = Cache(3, Hkv, 608, D)
+    total = [601, 0, 258 + S]
+    k = _rand((3, 601, Hkv, D), 1, outliers=True).cuda()
+    _append(c, k, _rand((3, 601, Hkv, D), 2).cuda(), _dev([0, 0, 0]), _dev(total))
+    n = [S, 0, (S + 1) // 2]
+    x = _rand((3, S, Hq, D), 3)
+    lens, new = _dev([t - r for t, r in zip(total, n)]), _dev(n)
+    for causal in (True, False):
+        _check_attention(c, x.cuda(), lens, new, causal=causal, mass=True)
+    m = [torch.zeros(3, Hkv, c.max_pos, device="cuda") for _ in range(2)]
+    _attend(c, x.cuda(), lens, new, mass=m[0])
+    x[1] = x[2, n[2]:] = float("nan")
+    _attend(c, x.cuda(), lens, new, mass=m[1])
+    assert torch.equal(m[0], m[1]) and (m[0][1] == 0).all() and (m[0][2, :, total[2]:] == 0).all()
+
+
+@pytest.mark.parametrize("S", [1, 8, 20, 64, 130])
+def test_weights_beside_a_nan(S):
+    """A NaN key makes the weights of the keys that its rows see NaN, and leaves those of other sequences and heads."""
+    torch = _torch()
+    c = Cache(2, 2, 320, 64)
+    k = _rand((2, 300, 2, 64), 1)
+    k[0, 299, 1] = float("nan")  # seen by the last row alone
+    _append(c, k.cuda(), _rand((2, 300, 2, 64), 2).cuda(), _dev([0, 0]))
+    x = _rand((2, S, 2, 64), 3).cuda()
+    m = torch.zeros(2, 2, c.max_pos, device="cuda")
+    out, _ = _attend(c, x, _dev([300 - S] * 2), mass=m)
+    assert torch.isnan(m[0, 1, :300]).all() and (m[0, 1, 300:] == 0).all()
+    assert torch.isfinite(m[1]).all() and torch.isfinite(m[0, 0]).all()
+    assert torch.isfinite(out[0, :S - 1].float()).all() and torch.isfinite(out[1].float()).all()
+
+
 @pytest.mark.parametrize("S,T", [(1, 300), (1, 9000), (90, 700), (90, 9000)])
 def test_attention_in_place(S, T):
     torch, q = _torch(), _api()
