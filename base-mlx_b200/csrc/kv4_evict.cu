@@ -65,26 +65,6 @@ QW_DEV int4 cluster_load4(const int* p, int rank) {
     return v;
 }
 
-// Exclusive prefixes of v and w over the block (SEL_NT threads) and the block totals.
-QW_DEV void block_scan2(int& v, int& w, int2* red, int2& total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int s = v, r = w;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int t = __shfl_up_sync(0xffffffffu, s, o), u = __shfl_up_sync(0xffffffffu, r, o);
-        if (lane >= o) {
-            s += t;
-            r += u;
-        }
-    }
-    if (lane == 31) red[warp] = make_int2(s, r);
-    __syncthreads();
-    const int2 p = lane < SEL_W ? red[lane] : make_int2(0, 0);  // every warp: the warps before it, and all
-    total = make_int2(__reduce_add_sync(0xffffffffu, p.x), __reduce_add_sync(0xffffffffu, p.y));
-    v = s - v + __reduce_add_sync(0xffffffffu, lane < warp ? p.x : 0);
-    w = r - w + __reduce_add_sync(0xffffffffu, lane < warp ? p.y : 0);
-}
-
 // index[b][h][0..new length): the kept positions in increasing order.
 __global__ void __launch_bounds__(SEL_NT, 2) kv4_select_kernel(const Kv4EvictArgs a, int cluster, int slice_keys, int* index,
                                                             int* count) {
@@ -196,22 +176,29 @@ __global__ void __launch_bounds__(SEL_NT, 2) kv4_select_kernel(const Kv4EvictArg
             left = pick[pass][1];
         }
     }
-    // consecutive positions per thread, in order
-    const int kpt = (slice + SEL_NT - 1) / SEL_NT, t0 = min(j1, j0 + tid * kpt), t1 = min(j1, t0 + kpt);
-    int above = 0, equal = 0;
-    for (int j = t0; j < t1; ++j) {
-        if (j >= jo) {
-            ++above;
-        } else if (want > 0) {
-            const uint32_t k = key(j);
-            above += k > prefix;
-            equal += k == prefix;
-        }
+    // A warp takes consecutive positions, 32 at a time, and ranks the kept ones by votes: its lanes read neighbouring
+    // keys and write neighbouring indices.
+    const unsigned below = (1u << lane) - 1u;
+    const int span = ((slice + SEL_W - 1) / SEL_W + 31) & ~31, w0 = min(j1, j0 + warp * span), w1 = min(j1, w0 + span);
+    auto votes = [&](int j, unsigned& above, unsigned& equal) {  // positions that stay for certain; that equal the threshold
+        const bool in = j < w1, low = in && j < jo;
+        const uint32_t k = low && want > 0 ? key(j) : 0u;
+        above = __ballot_sync(0xffffffffu, (in && j >= jo) || (low && want > 0 && k > prefix));
+        equal = __ballot_sync(0xffffffffu, low && want > 0 && k == prefix);
+    };
+    int2 mine = make_int2(0, 0);
+    for (int j = w0; j < w1; j += 32) {
+        unsigned above, equal;
+        votes(j + lane, above, equal);
+        mine.x += __popc(above);
+        mine.y += __popc(equal);
     }
-    int a_before = above, e_before = equal;
-    int2 total;
-    block_scan2(a_before, e_before, red, total);
+    if (lane == 0) red[warp] = mine;
+    __syncthreads();
+    const int2 p = lane < SEL_W ? red[lane] : make_int2(0, 0);
+    int a_before = __reduce_add_sync(0xffffffffu, lane < warp ? p.x : 0), e_before = __reduce_add_sync(0xffffffffu, lane < warp ? p.y : 0);
     if (cluster > 1) {
+        const int2 total = make_int2(__reduce_add_sync(0xffffffffu, p.x), __reduce_add_sync(0xffffffffu, p.y));
         if (tid == 0) tally = total;
         cluster_sync();
         int2 c[SEL_MAX_CLUSTER];
@@ -225,18 +212,18 @@ __global__ void __launch_bounds__(SEL_NT, 2) kv4_select_kernel(const Kv4EvictArg
         cluster_sync();  // a block's tally is read until here
     }
     int at = a_before + min(e_before, left);
-    for (int j = t0; j < t1; ++j) {
-        bool keep = j >= jo;
-        if (!keep && want > 0) {
-            const uint32_t k = key(j);
-            keep = k > prefix || (k == prefix && e_before < left);
-            e_before += k == prefix;
+    for (int j = w0; j < w1; j += 32) {
+        unsigned above, equal;
+        votes(j + lane, above, equal);
+        const bool tie = (equal >> lane & 1u) && e_before + __popc(equal & below) < left;  // the lowest of the equals stay
+        const unsigned kept = above | __ballot_sync(0xffffffffu, tie);
+        if (kept >> lane & 1u) {
+            const int r = at + __popc(kept & below);
+            idx[r] = j + lane;
+            if (out) out[r] = j + lane;
         }
-        if (keep) {
-            idx[at] = j;
-            if (out) out[at] = j;
-            ++at;
-        }
+        at += __popc(kept);
+        e_before += __popc(equal);
     }
 }
 
