@@ -5,18 +5,18 @@
 // position wins a tie).  The kept rows move to the front in position order,
 // with their weights; n <= keep keeps every row.
 //
-//   1. select: weights become unsigned keys of the same order.  A cluster of
-//      thread blocks takes a (sequence, head), each block a slice of its
-//      positions; three histogram passes (11, 11 and 10 bits, summed over the
-//      cluster through distributed shared memory) find the threshold key and
-//      how many of its equals stay, one prefix over the threads' consecutive
-//      positions writes the kept ones in order.
+//   1. select: weights become unsigned keys of the same order.  A thread block
+//      holds the keys of a (sequence, head) in registers, 16384 of them; more
+//      positions take a cluster of blocks, a slice each.  Three histogram passes
+//      (11, 11 and 10 bits, summed over the cluster through distributed shared
+//      memory) find the threshold key and how many of its equals stay; votes rank
+//      the kept positions.
 //   2. move: dst row r = src row index[r].
 //
-// 8 sequences of up to 16384 positions, 8 heads, half of them kept: 46 us, of them
-// 24 for the move (117 MB at 4.8 TB/s, waiting on its gathers) and 16 for the
-// selection, which is bound by the latency of its passes: weights to keys, three
-// histograms with a cluster barrier each, the prefix.
+// 8 sequences of up to 16384 positions, 8 heads, half of them kept: 43 us, of them
+// 24 for the move (117 MB at 4.8 TB/s, waiting on its gathers) and 14 for the
+// selection, which is bound by the latency of its passes (with clusters of four
+// blocks 16: a cluster barrier and the remote reads behind it take 1.8 us).
 #include <algorithm>
 
 #include "kv4.h"
@@ -26,10 +26,10 @@
 namespace qw {
 namespace {
 
-constexpr int SEL_NT = 512, SEL_W = SEL_NT / 32;
+constexpr int SEL_NT = 1024, SEL_W = SEL_NT / 32;
 constexpr int BINS = 2048;
 constexpr int SEL_MAX_CLUSTER = 8;
-constexpr int SEL_KEYS = 40960;  // keys of a slice held in shared memory; longer slices are read again per pass
+constexpr int SLICE = 16384;             // keys a block holds in shared memory; further ones are read again per pass
 
 // Unsigned key of the same order as the float; -0 equals +0, NaN is above everything.
 QW_DEV uint32_t order_key(float v) {
@@ -56,21 +56,11 @@ QW_DEV int2 cluster_load2(const int* p, int rank) {
     asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(cluster_addr(p, rank)) : "memory");
     return v;
 }
-QW_DEV int4 cluster_load4(const int* p, int rank) {
-    int4 v;
-    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "r"(cluster_addr(p, rank))
-                 : "memory");
-    return v;
-}
-
 // index[b][h][0..new length): the kept positions in increasing order.
-__global__ void __launch_bounds__(SEL_NT, 2) kv4_select_kernel(const Kv4EvictArgs a, int cluster, int slice_keys, int* index,
-                                                            int* count) {
+__global__ void __launch_bounds__(SEL_NT, 1) kv4_select_kernel(const Kv4EvictArgs a, int cluster, int* index, int* count) {
     extern __shared__ __align__(16) int sel_smem[];
-    int* hist = sel_smem;                                                // [3][BINS]
-    uint32_t* sk = reinterpret_cast<uint32_t*>(sel_smem + 3 * BINS);     // [slice_keys]
+    int* hist = sel_smem;                                             // [3][BINS]
+    uint32_t* held = reinterpret_cast<uint32_t*>(sel_smem + 3 * BINS);  // keys of the slice's first SLICE positions
     __shared__ int2 red[32], tally;
     __shared__ int wsum[3][32], pick[3][2];
     const int rank = blockIdx.x % cluster, h = blockIdx.x / cluster, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31,
@@ -90,67 +80,77 @@ __global__ void __launch_bounds__(SEL_NT, 2) kv4_select_kernel(const Kv4EvictArg
         }
         return;
     }
+    // as many blocks of the cluster as the positions need (each cluster barrier costs a microsecond)
+    const int active = min(cluster, (n + SLICE - 1) / SLICE);
+    if (active == 1 && rank > 0) return;
     const float* mass = a.mass_src + bh * a.src.max_pos;
     const int old = n - a.recent, want = a.keep - a.recent;
-    const int slice = (n + cluster - 1) / cluster, j0 = min(n, rank * slice), j1 = min(n, j0 + slice);
+    const int slice = (n + active - 1) / active, j0 = min(n, rank * slice), j1 = min(n, j0 + slice);
     const int jo = max(j0, min(j1, old));  // [j0, jo): may be dropped; [jo, j1): recent
-    const bool held = slice <= slice_keys;
-    for (int i = tid; i < 3 * BINS; i += SEL_NT) hist[i] = 0;
+    // A warp takes consecutive positions [w0, w1), a lane every 32nd of them.
+    const int span = ((slice + SEL_W - 1) / SEL_W + 31) & ~31, w0 = min(j1, j0 + warp * span), w1 = min(j1, w0 + span);
+    auto load = [&](int j) { return j < w1 && j < jo ? mass[j] : 0.f; };
+    const int most = min(w1, j0 + SLICE);  // [w0, most): held
+    for (int j = w0 + lane; j < most; j += 32 * 8) {  // eight loads in flight
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = load(j + 32 * e);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (j + 32 * e < most) held[j + 32 * e - j0] = order_key(v[e]);
+    }
+    for (int i = tid; i < 3 * BINS / 4; i += SEL_NT) reinterpret_cast<int4*>(hist)[i] = make_int4(0, 0, 0, 0);
     __syncthreads();
-    auto key = [&](int j) { return held ? sk[j - j0] : order_key(mass[j]); };
+    // f(position, key) of the warp's positions, by whole warps.  (Rolled, as the passes are: the block is short and
+    // runs at the pace of instruction fetch; with 16 keys a thread in registers it took 12.3 us for 700 positions.)
+    auto each = [&](auto f) {
+        int j = w0;
+#pragma unroll 1
+        for (; j + 128 <= most; j += 128) {
+            uint32_t k[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) k[e] = held[j + 32 * e + lane - j0];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f(j + 32 * e + lane, k[e]);
+        }
+#pragma unroll 1
+        for (; j < w1; j += 32) f(j + lane, j + lane < most ? held[j + lane - j0] : order_key(load(j + lane)));
+    };
     uint32_t prefix = 0;
     int left = want;
     if (want > 0) {
-#pragma unroll
+#pragma unroll 1
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
             const uint32_t mask = pass == 2 ? 1023u : 2047u;
+            const int above_bits = pass == 0 ? 31 : pass == 1 ? 21 : 10;  // every higher digit has to agree
             int* hp = hist + pass * BINS;
-            if (pass == 0) {
-                for (int j = j0 + tid; j < jo; j += 8 * SEL_NT) {  // eight loads in flight
-                    float v[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = j + e * SEL_NT < jo ? mass[j + e * SEL_NT] : 0.f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (j + e * SEL_NT < jo) {
-                            const uint32_t k = order_key(v[e]);
-                            if (held) sk[j + e * SEL_NT - j0] = k;
-                            atomicAdd(&hp[k >> shift], 1);
-                        }
-                }
-            } else {
-                const int above = pass == 1 ? 21 : 10;  // every higher digit has to agree
-                for (int j = j0 + tid; j < jo; j += SEL_NT) {
-                    const uint32_t k = key(j);
-                    if ((k >> above) == (prefix >> above)) atomicAdd(&hp[(k >> shift) & mask], 1);
-                }
-            }
-            if (cluster > 1)
+            each([&](int j, uint32_t k) {
+                if (j < w1 && j < jo && (pass == 0 || (k >> above_bits) == (prefix >> above_bits))) atomicAdd(&hp[(k >> shift) & mask], 1);
+            });
+            if (active > 1)
                 cluster_sync();
             else
                 __syncthreads();
-            // warp w counts the 128 bins from 128 (15 - w) on, lane l four of them from 4 (31 - l) on: warps, lanes
-            // and c[0..3] in order from the largest digit down
-            static_assert(BINS == 4 * SEL_NT, "four bins per thread");
-            const int d0 = 128 * (SEL_W - 1 - warp) + 4 * (31 - lane);
-            int c[4] = {0, 0, 0, 0};
-            if (cluster > 1) {
-                int4 v[SEL_MAX_CLUSTER];
+            // warp w counts the 64 bins from 64 (31 - w) on, lane l two of them from 2 (31 - l) on: warps, lanes
+            // and c[0], c[1] in order from the largest digit down
+            static_assert(BINS == 2 * SEL_NT, "two bins per thread");
+            const int d0 = 64 * (SEL_W - 1 - warp) + 2 * (31 - lane);
+            int c[2] = {0, 0};
+            if (active > 1) {
+                int2 v[SEL_MAX_CLUSTER];
 #pragma unroll
-                for (int r = 0; r < SEL_MAX_CLUSTER; ++r) v[r] = r < cluster ? cluster_load4(&hp[d0], r) : make_int4(0, 0, 0, 0);
+                for (int r = 0; r < SEL_MAX_CLUSTER; ++r) v[r] = r < active ? cluster_load2(&hp[d0], r) : make_int2(0, 0);
 #pragma unroll
                 for (int r = 0; r < SEL_MAX_CLUSTER; ++r) {
-                    c[0] += v[r].w;
-                    c[1] += v[r].z;
-                    c[2] += v[r].y;
-                    c[3] += v[r].x;
+                    c[0] += v[r].y;
+                    c[1] += v[r].x;
                 }
             } else {
-                const int4 v = *reinterpret_cast<const int4*>(&hp[d0]);
-                c[0] = v.w, c[1] = v.z, c[2] = v.y, c[3] = v.x;
+                const int2 v = *reinterpret_cast<const int2*>(&hp[d0]);
+                c[0] = v.y, c[1] = v.x;
             }
-            const int own = c[0] + c[1] + c[2] + c[3], mine = __reduce_add_sync(0xffffffffu, own);
+            const int own = c[0] + c[1], mine = __reduce_add_sync(0xffffffffu, own);
             if (lane == 0) wsum[pass][warp] = mine;
             __syncthreads();
             const int before = __reduce_add_sync(0xffffffffu, lane < warp ? wsum[pass][lane] : 0);
@@ -163,9 +163,9 @@ __global__ void __launch_bounds__(SEL_NT, 2) kv4_select_kernel(const Kv4EvictArg
                 }
                 int above = before + s - own;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
+                for (int e = 0; e < 2; ++e) {
                     if (above < left && left <= above + c[e]) {
-                        pick[pass][0] = d0 + 3 - e;
+                        pick[pass][0] = d0 + 1 - e;
                         pick[pass][1] = left - above;
                     }
                     above += c[e];
@@ -176,28 +176,25 @@ __global__ void __launch_bounds__(SEL_NT, 2) kv4_select_kernel(const Kv4EvictArg
             left = pick[pass][1];
         }
     }
-    // A warp takes consecutive positions, 32 at a time, and ranks the kept ones by votes: its lanes read neighbouring
-    // keys and write neighbouring indices.
+    // The kept positions ranked by votes: positions that stay for certain, and those that equal the threshold.
     const unsigned below = (1u << lane) - 1u;
-    const int span = ((slice + SEL_W - 1) / SEL_W + 31) & ~31, w0 = min(j1, j0 + warp * span), w1 = min(j1, w0 + span);
-    auto votes = [&](int j, unsigned& above, unsigned& equal) {  // positions that stay for certain; that equal the threshold
-        const bool in = j < w1, low = in && j < jo;
-        const uint32_t k = low && want > 0 ? key(j) : 0u;
-        above = __ballot_sync(0xffffffffu, (in && j >= jo) || (low && want > 0 && k > prefix));
-        equal = __ballot_sync(0xffffffffu, low && want > 0 && k == prefix);
+    auto votes = [&](int j, uint32_t k, unsigned& above, unsigned& equal) {
+        const bool in = j < w1, low = in && j < jo && want > 0;
+        above = __ballot_sync(0xffffffffu, (in && j >= jo) || (low && k > prefix));
+        equal = __ballot_sync(0xffffffffu, low && k == prefix);
     };
     int2 mine = make_int2(0, 0);
-    for (int j = w0; j < w1; j += 32) {
+    each([&](int j, uint32_t k) {
         unsigned above, equal;
-        votes(j + lane, above, equal);
+        votes(j, k, above, equal);
         mine.x += __popc(above);
         mine.y += __popc(equal);
-    }
+    });
     if (lane == 0) red[warp] = mine;
     __syncthreads();
-    const int2 p = lane < SEL_W ? red[lane] : make_int2(0, 0);
+    const int2 p = red[lane];
     int a_before = __reduce_add_sync(0xffffffffu, lane < warp ? p.x : 0), e_before = __reduce_add_sync(0xffffffffu, lane < warp ? p.y : 0);
-    if (cluster > 1) {
+    if (active > 1) {
         const int2 total = make_int2(__reduce_add_sync(0xffffffffu, p.x), __reduce_add_sync(0xffffffffu, p.y));
         if (tid == 0) tally = total;
         cluster_sync();
@@ -212,19 +209,19 @@ __global__ void __launch_bounds__(SEL_NT, 2) kv4_select_kernel(const Kv4EvictArg
         cluster_sync();  // a block's tally is read until here
     }
     int at = a_before + min(e_before, left);
-    for (int j = w0; j < w1; j += 32) {
+    each([&](int j, uint32_t k) {
         unsigned above, equal;
-        votes(j + lane, above, equal);
+        votes(j, k, above, equal);
         const bool tie = (equal >> lane & 1u) && e_before + __popc(equal & below) < left;  // the lowest of the equals stay
         const unsigned kept = above | __ballot_sync(0xffffffffu, tie);
         if (kept >> lane & 1u) {
             const int r = at + __popc(kept & below);
-            idx[r] = j + lane;
-            if (out) out[r] = j + lane;
+            idx[r] = j;
+            if (out) out[r] = j;
         }
         at += __popc(kept);
         e_before += __popc(equal);
-    }
+    });
 }
 
 // Out of place.  Words: one thread per 16-byte piece of MR kept rows, all loads
@@ -362,17 +359,13 @@ size_t kv4_evict_scratch_bytes(const Kv4View& src, int keep) {
 cudaError_t launch_kv4_evict(const Kv4EvictArgs& a, void* scratch, cudaStream_t st) {
     int* index = static_cast<int*>(scratch);
     int* count = index + (size_t)a.src.batch * a.src.heads * a.keep;
-    // blocks of a head: slices of about 1024 positions, as long as one round of blocks holds them all
+    // blocks of a head: as many as hold all its positions in shared memory
     int cluster = 1;
-    while (cluster < SEL_MAX_CLUSTER && a.src.max_pos > 1024 * cluster &&
-           (long long)a.src.batch * a.src.heads * cluster * 2 <= 2 * 148)
-        cluster *= 2;
-    const int keys = std::min(SEL_KEYS, (a.src.max_pos + cluster - 1) / cluster);
-    const int smem = (3 * BINS + keys) * (int)sizeof(int);
-    cudaError_t e = ensure_max_dyn_smem(kv4_select_kernel, (3 * BINS + SEL_KEYS) * (int)sizeof(int));
+    while (cluster < SEL_MAX_CLUSTER && a.src.max_pos > SLICE * cluster) cluster *= 2;
+    const int smem = (3 * BINS + std::min(SLICE, (a.src.max_pos + 31) / 32 * 32)) * (int)sizeof(int);
+    cudaError_t e = ensure_max_dyn_smem(kv4_select_kernel, (3 * BINS + SLICE) * (int)sizeof(int));
     if (e != cudaSuccess) return e;
-    e = launch(kv4_select_kernel, dim3(a.src.heads * cluster, a.src.batch), dim3(SEL_NT), smem, cluster, st, a, cluster,
-               keys, index, count);
+    e = launch(kv4_select_kernel, dim3(a.src.heads * cluster, a.src.batch), dim3(SEL_NT), smem, cluster, st, a, cluster, index, count);
     if (e != cudaSuccess) return e;
     const bool wide = a.src.D == 128;
     if (a.dst.p[0].w == a.src.p[0].w) {

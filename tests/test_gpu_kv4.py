@@ -697,6 +697,31 @@ def test_evict(H, D, lens, keep, recent, inplace):
         assert all(torch.equal(x, y) for x, y in zip(src.bits(), s0))
 
 
+@pytest.mark.parametrize("lens,cap,keep,recent", [([20000, 9000, 16384, 16385], 20480, 6000, 100), ([65000, 100, 33001], 65536, 4097, 0),
+                                                 ([150001], 150016, 70000, 3), ([131072], 131072, 10, 10)])
+def test_evict_positions_of_long_caches(lens, cap, keep, recent):
+    """Lengths that take several thread blocks, or more positions than those hold; ties across their borders."""
+    torch = _torch()
+    B = len(lens)
+    src, dst = Cache(B, 1, cap, 64), Cache(B, 1, (keep + 15) // 16 * 16, 64)
+    g = np.random.default_rng(cap)
+    m = np.exp(g.normal(size=(B, 1, cap))).astype(np.float32)
+    m[g.random(m.shape) < 0.3] = 0.5  # the threshold falls among equals
+    ms, md = torch.from_numpy(m).cuda(), torch.zeros(B, 1, dst.max_pos, device="cuda")
+    for t in src.t:
+        t.copy_(torch.arange(t[0, 0, :, 0].numel(), device="cuda").to(t.dtype)[None, None, :, None].expand_as(t))
+    index, new = _dev(np.zeros((B, 1, keep))), _dev([0] * B)
+    _evict(src, dst, ms, md, _dev(lens), new, keep, recent, index)
+    assert new.tolist() == [min(n, keep) for n in lens]
+    for b, n in enumerate(lens):
+        order = np.lexsort((np.arange(n - recent), -m[b, 0, :n - recent]))[:keep - recent] if n > keep else np.arange(n)
+        ids = np.concatenate([np.sort(order), np.arange(n - recent, n)]) if n > keep else order
+        assert index[b, 0, :len(ids)].cpu().numpy().tolist() == ids.tolist() and (index[b, 0, len(ids):] == -1).all()
+        at = torch.from_numpy(ids).cuda()
+        assert torch.equal(md[b, 0, :len(ids)], ms[b, 0, at])
+        assert all(torch.equal(d[b, 0, :len(ids)], t[b, 0, at]) for d, t in zip(dst.t, src.t))
+
+
 def test_evict_all_equal_weights_keeps_the_lowest_positions():
     torch = _torch()
     src = _filled(1, 1, 300, 64)
