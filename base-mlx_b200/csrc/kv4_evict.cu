@@ -6,7 +6,7 @@
 // with their weights; n <= keep keeps every row.
 //
 //   1. select: weights become unsigned keys of the same order.  A thread block
-//      holds the keys of a (sequence, head) in registers, 16384 of them; more
+//      holds the keys of a (sequence, head) in shared memory, 16384 of them; more
 //      positions take a cluster of blocks, a slice each.  Three histogram passes
 //      (11, 11 and 10 bits, summed over the cluster through distributed shared
 //      memory) find the threshold key and how many of its equals stay; votes rank
