@@ -607,6 +607,7 @@ __global__ void __launch_bounds__(WNT) kv4_mass_scores_kernel(const Kv4AttnArgs 
     const size_t at = ((size_t)b * a.c.heads + h) * a.c.max_pos + key;
     const bool ok = key < rw.off + rw.n;
     float v[SCORE_COLUMNS];
+    const float before = ok ? a.mass[at] : 0.f;
 #pragma unroll
     for (int c = 0; c < SCORE_COLUMNS; c += VEC)
         if (ok && c < cp) {
@@ -621,7 +622,7 @@ __global__ void __launch_bounds__(WNT) kv4_mass_scores_kernel(const Kv4AttnArgs 
 #pragma unroll
     for (int c = 0; c < SCORE_COLUMNS; ++c)
         if (c < cp) sum += base[c] == INFINITY ? 0.f : ex2(v[c] - base[c]);
-    a.mass[at] += sum;
+    a.mass[at] = before + sum;
 }
 
 // 17 to 63 columns: a warp keeps 16 keys (eight warps of 16: with 32 a chunk of 512 rows on 4096 keys left half of the
