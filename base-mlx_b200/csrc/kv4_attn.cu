@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_split_kernel(co
 
 // Short caches: a cluster of `cluster` blocks takes a whole segment, tile k by block k % cluster, and joins
 // through distributed shared memory -- one launch and no partials in memory.  32 sequences of up to 2048 keys, 2 kv
-// heads: 10.3 us; 5 rows of 32 heads on 812 keys: 10.3 us.
+// heads: 7.5 us; 5 rows of 32 heads on 812 keys: 8.6 us.
 template <int D, int NT, bool WEIGHTS>
 __global__ void __launch_bounds__(ANT, NT == 1 ? 2 : 1) kv4_attn_cluster_kernel(const Kv4AttnArgs a, int ncb, int cluster, float* scores, int cp) {
     using SM = SplitSmem<D, NT>;
@@ -590,7 +590,7 @@ QW_DEV void store_weights(float (&sum)[2 * KB], float* mass, int key0, int T, in
 
 // Up to SCORE_COLUMNS columns: the attention kernels leave their scores [batch][kv head][key][cp] (base 2; at eight
 // columns 32 bytes a key next to the 72 of its K row), so that this pass reads them from L2 and takes no products.
-// 4 sequences of up to 16000 keys, 8 columns: 30.8 us with the attention, 39.0 us with scores recomputed from K.
+// 4 sequences of up to 16000 keys, 8 columns: 29.1 us with the attention, 39.0 us with scores recomputed from K.
 // A thread adds one key's columns in their order.
 constexpr int SCORE_COLUMNS = 16, WNT = 256;
 template <int VEC>
@@ -741,7 +741,7 @@ Shape shape_of(const Kv4View& c, int S, int Hq, int num_sms) {
     const int most = (c.max_pos + TK - 1) / TK;
     int cl = 1;
     // (clusters of 8 are counted on three quarters of the SMs: what is left of a GPC holds none; 5 rows on 812 keys
-    // with clusters that did not fit at once: 16.5 us against 10.3)
+    // with clusters that did not fit at once: 1.6 times as long)
     while (cl < MAX_CLUSTER && segs * 2 * cl * (cl == 4 ? 4 : 3) <= 3ll * s.shares && most > AW * cl) cl *= 2;
     if (most <= CLUSTER_TILES * AW * cl && segs * cl <= 0x7FFFFFFF) {
         s.cluster = cl;

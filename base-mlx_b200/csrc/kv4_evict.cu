@@ -13,7 +13,7 @@
 //      the kept positions.
 //   2. move: dst row r = src row index[r].
 //
-// 8 sequences of up to 16384 positions, 8 heads, half of them kept: 43 us, of them
+// 8 sequences of up to 16384 positions, 8 heads, half of them kept: 41 us, of them
 // 24 for the move (117 MB at 4.8 TB/s, waiting on its gathers) and 14 for the
 // selection, which is bound by the latency of its passes (with clusters of four
 // blocks 16: a cluster barrier and the remote reads behind it take 1.8 us).
