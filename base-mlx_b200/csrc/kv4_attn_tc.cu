@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
                        o < 0 ? a.q : a.q + o + 8 * k, o >= 0);
         }
         cp_async_commit();
-        // largest magnitudes that the block's rows can stand for: max(|b|, |b + 15 s|) (a NaN counts as nothing here)
+        // largest magnitudes that the block's rows can stand for: max(|b|, |b + 15 s|)
         constexpr int KW = 2 / GR;  // keys of a 32-bit word of scales (rows end at a multiple of 16)
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
@@ -226,10 +226,8 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
 #pragma unroll 4
             for (int w = t0 * KT / KW + tid; w < (key_end + KW - 1) / KW; w += 256 * NB) {
                 const uint32_t us = s[w], uz = z[w];
-                const float z0 = bits_lo_f(uz), z1 = bits_hi_f(uz);
-                float m = fmaxf(fabsf(z0), fabsf(fmaf(15.f, bits_lo_f(us), z0)));
-                if (GR == 2 || w * KW + 1 < key_end) m = fmaxf(m, fmaxf(fabsf(z1), fabsf(fmaf(15.f, bits_hi_f(us), z1))));
-                mx = fmaxf(mx, m);
+                mx = fmaxf(mx, reach(bits_lo_f(us), bits_lo_f(uz)));
+                if (GR == 2 || w * KW + 1 < key_end) mx = fmaxf(mx, reach(bits_hi_f(us), bits_hi_f(uz)));
             }
             mx = warp_max(mx);
             if (lane == 0) kvmax[2 * warp + v] = mx;
@@ -339,7 +337,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
                 const int key = (t0 + i) * KT + tid;
                 if (partial(i) && key < T) {
                     const uint32_t s = group_pair<GR>(rows.s[1], key), z = group_pair<GR>(rows.b[1], key);
-                    nan = !(fabsf(bits_lo_f(s)) + fabsf(bits_lo_f(z)) < INFINITY) || !(fabsf(bits_hi_f(s)) + fabsf(bits_hi_f(z)) < INFINITY);
+                    nan = !finite(bits_lo_f(s), bits_lo_f(z)) || !finite(bits_hi_f(s), bits_hi_f(z));
                 }
                 store_offsets<GR>(dst + GR * KT * 128, tid, cs, cz, kup, nan);
             }
@@ -352,7 +350,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
 #pragma unroll
                 for (int j = 0; j < PER; ++j) {
                     float s = u16_to_f(vs.s[j]), z = u16_to_f(vs.z[j]);
-                    if (partial(i) && !(fabsf(s) + fabsf(z) < INFINITY)) s = z = 0.f;
+                    if (partial(i) && !finite(s, z)) s = z = 0.f;
                     // n 2^-18 times 2^18 s plus z, times 2^(-2 - ev): s is at most 2/15 of the largest value
                     const __half2 s2 = __float2half2_rn(s * vup), z2 = __float2half2_rn(z * vup * 0x1p-18f);
                     expand_piece<D>(vs.w[j], tid + NTH * j, dst, [&](uint32_t n) { return as_u(__hfma2(as_h2(n), s2, z2)); });

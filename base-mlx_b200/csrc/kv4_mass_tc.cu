@@ -87,9 +87,7 @@ __global__ void __launch_bounds__(MTHREADS, 1) kv4_mass_tc_kernel(const Kv4AttnA
             cs = group_pair<GR>(rows.s[0], key0 + tid);
             cz = group_pair<GR>(rows.b[0], key0 + tid);
         }
-        const float z0 = bits_lo_f(cz), z1 = bits_hi_f(cz);
-        float m = fmaxf(fmaxf(fabsf(z0), fabsf(fmaf(15.f, bits_lo_f(cs), z0))), fmaxf(fabsf(z1), fabsf(fmaf(15.f, bits_hi_f(cs), z1))));
-        m = warp_max(m);
+        const float m = warp_max(fmaxf(reach(bits_lo_f(cs), bits_lo_f(cz)), reach(bits_hi_f(cs), bits_hi_f(cz))));
         if (lane == 0) kmax[warp] = m;
     }
     __syncthreads();

@@ -146,8 +146,12 @@ QW_DEV void store_offsets(unsigned char* dst, int row, uint32_t scale, uint32_t 
         *reinterpret_cast<uint4*>(dst + at16(row, e)) = make_uint4(r[0], r[1], r[2], r[3]);
     }
 }
+// The largest magnitude that a group's scale and bias can stand for; one that is not finite counts as nothing, so that
+// it does not push the other keys' values to zero.
+QW_DEV bool finite(float s, float z) { return 0.25f * fabsf(z) + 0.25f * fabsf(fmaf(15.f, s, z)) < INFINITY; }
+QW_DEV float reach(float s, float z) { return finite(s, z) ? fmaxf(fabsf(z), fabsf(fmaf(15.f, s, z))) : 0.f; }
 // The exponent of a largest magnitude m: K enters times 2^(7 - ek), V times 2^(-2 - ev).
-QW_DEV int top_exponent(float m) { return max((int)(__float_as_uint(fminf(m, 3.0e38f)) >> 23) - 127, -100); }
+QW_DEV int top_exponent(float m) { return max((int)(__float_as_uint(m) >> 23) - 127, -100); }
 // The bf16 of every group of a key.
 template <int GR>
 QW_DEV uint32_t group_pair(const unsigned char* base, size_t key) {

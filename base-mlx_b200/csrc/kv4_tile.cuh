@@ -382,6 +382,7 @@ QW_DEV void attend_tile(State<D, NT>& st, const Cols<D, NT>& cols, const unsigne
     unpack<GR>(read_packed<D>(tile, 2, lane), vs[0]);
     smax = GR == 2 ? fmaxf(fabsf(vs[0][0]), fabsf(vs[0][GR - 1])) : fabsf(vs[0][0]);
     if (EDGE && key0 + lane >= T) smax = 0.f;
+    if (!(smax < 2.0e37f)) smax = 0.f;  // past the range times 15: must not push the values of other rows to zero
     bool raise = smax > st.sref;
     float top[NT][2];
 #pragma unroll

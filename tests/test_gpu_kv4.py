@@ -858,6 +858,28 @@ def test_weights_at_every_number_of_columns(S, Hq, Hkv, D):
     assert torch.equal(m[0], m[1]) and (m[0][1] == 0).all() and (m[0][2, :, total[2]:] == 0).all()
 
 
+INF = float("inf")
+
+
+@pytest.mark.parametrize("array,bad", [(1, INF), (1, -INF), (1, 3.0e38), (2, INF), (2, -INF), (4, INF), (4, -INF), (4, 3.0e38), (5, INF),
+                                       (5, -INF)])  # scale and bias of K, of V
+@pytest.mark.parametrize("S", [3, 20, 90])
+def test_rows_before_an_infinity(S, array, bad):
+    """Scales and biases of infinity (or past the range times 15) in a key that the last row alone sees: the other rows
+    are those of a cache without it."""
+    torch = _torch()
+    a, b = _filled(1, 1, 300, 64), _filled(1, 1, 300, 64)
+    b.t[array][0, 0, 299, 0] = int(torch.tensor(bad).bfloat16().view(torch.int16))
+    x = _rand((1, S, 2, 64), 3).cuda()
+    ma, mb = (torch.zeros(1, 1, a.max_pos, device="cuda") for _ in range(2))
+    want, lse = _attend(a, x[:, :S - 1].contiguous(), _dev([300 - S]), mass=ma)
+    got, lse_b = _attend(b, x, _dev([300 - S]), mass=mb)
+    vm = a.values64(1)[0, 0, :300].abs().max().item()
+    d = (got[:, :S - 1].double() - want.double()).abs()
+    assert (d <= 2.0 ** -7 * want.double().abs() + 2.0 ** -9 * vm).all()
+    assert ((lse_b[:, :S - 1] - lse).abs() <= 2.0 ** -16 * (1 + lse.abs())).all()
+
+
 @pytest.mark.parametrize("S", [1, 8, 20, 64, 130])
 def test_weights_beside_a_nan(S):
     """A NaN key makes the weights of the keys that its rows see NaN, and leaves those of other sequences and heads."""
