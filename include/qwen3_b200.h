@@ -378,14 +378,13 @@ QW_API int qw_kv4_attention_scratch(const qw_kv4* cache, int S, int heads, size_
  * included); a NaN among a row's visible K or V rows makes the output row NaN,
  * as a whole or in the 64 dimensions of a NaN in V, an infinite bias or a scale
  * past 2e37 leaves the row unspecified, and none of them reaches a row that
- * does not see it.
- * K enters exactly, V and the probabilities rounded to 11 bits, but for 2^-22
- * of the largest finite K or V of the sequence and kv head.  lse (fp32 [batch][S][heads], may be
- * NULL) receives the natural logarithm of each row's sum of exponentials; a
- * row without keys gives out = 0, lse = -inf.  mass (fp32 [batch][kv_heads][max_pos], may be
- * NULL) has every key's probability, summed over the sequence's rows and the
- * kv head's query heads, added to it; positions past the last key are left as
- * they are. */
+ * does not see it.  K enters exactly, V and the probabilities rounded to 11
+ * bits, but for 2^-22 of the largest finite K or V of the sequence and kv head.
+ * lse (fp32 [batch][S][heads], may be NULL) receives the natural logarithm of
+ * each row's sum of exponentials; a row without keys gives out = 0, lse = -inf.
+ * mass (fp32 [batch][kv_heads][max_pos], may be NULL) has every key's
+ * probability, summed over the sequence's rows and the kv head's query heads,
+ * added to it; positions past the last key are left as they are. */
 QW_API int qw_kv4_attention(const qw_kv4* cache, const void* q, const int64_t* q_strides, void* out,
                             const int64_t* out_strides, int S, int heads, float scale, int causal,
                             const int32_t* seq_len_dev, const int32_t* n_new_dev, float* lse, float* mass,

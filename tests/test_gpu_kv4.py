@@ -910,6 +910,44 @@ def test_attention_in_place(S, T):
     assert torch.equal(x, want)
 
 
+@pytest.mark.parametrize("S,Hq,T,D", [(1, 8, 9000, 128), (6, 8, 700, 64), (90, 4, 3000, 64), (90, 4, 700, 128)])
+def test_weights_captured_and_beside_each_other(S, Hq, T, D):
+    """A captured call replayed, and two calls on two streams with a scratch each, give what one call gives."""
+    torch, q = _torch(), _api()
+    c = _filled(2, 2, T, D)
+    lens = _dev([T - S, T // 2])
+    xs = [_rand((2, S, Hq, D), i).cuda() for i in (3, 4)]
+    want = []
+    for x in xs:
+        m = torch.zeros(2, 2, c.max_pos, device="cuda")
+        want.append((_attend(c, x, lens, mass=m), m))
+    n = q.kv4_attention_scratch_bytes(c.h, S, Hq)
+    scratch = [torch.full((n,), 0xFF, dtype=torch.uint8, device="cuda") for _ in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    ms = [torch.zeros(2, 2, c.max_pos, device="cuda") for _ in xs]
+    outs = [torch.empty_like(x) for x in xs]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for s, x, m, o, w in zip(streams, xs, ms, outs, scratch):
+            with torch.cuda.stream(s):
+                m.zero_()
+                _attend(c, x, lens, mass=m, out=o, scratch=w)
+    torch.cuda.synchronize()
+    for ((o, _), m), got, gm in zip(want, outs, ms):
+        assert torch.equal(o, got) and torch.equal(m, gm)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for x, m, o in zip(xs, ms, outs):
+            _attend(c, x, lens, mass=m, out=o, scratch=scratch[0], want_lse=False)
+    for m in ms:
+        m.zero_()
+    g.replay()
+    g.replay()
+    torch.cuda.synchronize()
+    for ((o, _), m), got, gm in zip(want, outs, ms):
+        assert torch.equal(o, got) and torch.equal(2 * m, gm)
+
+
 def test_host_memory_and_short_scratch_are_refused():
     torch, q = _torch(), _api()
     c = _filled(1, 1, 20, 64)
