@@ -396,6 +396,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
 #pragma unroll
                 for (int k = 0; k < KH; k += 2) top = max3(top, x[k], x[k + 1]);
                 if (pair_any(top > thr)) {
+                    wait_st();  // P of the round before and O of a raise there are read back below
                     xch[(2 * m + half) * CB + col] = top;
                     pair_sync();
                     top = fmaxf(top, xch[(2 * m + (half ^ 1)) * CB + col]);

@@ -1,0 +1,126 @@
+"""4-bit KV cache operators against 64 bits, with bounds that follow their arithmetic term by term.
+
+A stored row stands for s n + b per element; hat(x) = |s| n + |b| bounds what its parts sum up to.  Half steps:
+bf16 2^-8, fp16 2^-11, fp32 2^-24.
+
+* score: the integers, the queries and the key offsets enter the tensor cores exactly, or as 22 bits and more (offsets of
+  the chunk form: two fp16 terms; elements 2^-22 below the largest K are lost).  What is left are fp32 sums: at most
+  eight matrix steps of 16 terms per row, each of which may lose 17 last places of the largest partial sum, and ten
+  roundings after them, (8 * 17 + 10) 2^-24 < 2^-16.8 of the magnitudes' sum: e = 2^-16.5 |scale| (sum_d |q_d| hat(k_jd)) +
+  2^-21 |scale| max|k| sum_d |q_d|, the largest over the row's keys, and 2^-21 for the power of two itself.
+* probability: a factor exp(2 e).
+* output: p s or p, and V in the chunk form, are rounded to 11 bits: sum_j p_j hat(v_j) (2 * 2^-11 + expm1(2 e)), sums of
+  the keys in fp32 (2^-13 of the same sum covers chains of 2048 additions), 2^-21 of the largest |v|, and the
+  final rounding 2^-8 |out|.
+* log-sum-exp: e, and 2^-13 relative of the sum (2^-13 absolute of its logarithm), 2^-22 |lse|.
+* weight of a key: factors exp(2 e) of its probabilities and 2^-12 of them (the log-sum-exp's sum), fp32 sums with what
+  was there: 2^-20 (1 + |mass|).
+"""
+import pytest
+
+from test_gpu_kv4 import Cache, _append, _attend, _dev, _filled, _rand
+
+pytestmark = pytest.mark.gpu
+
+
+def _torch():
+    import torch
+    return torch
+
+
+def _parts(c, which):
+    """float64 values and hat magnitudes [B, H, max_pos, D] of the stored rows, on the GPU."""
+    torch = _torch()
+    w, s, b = c.t[3 * which:3 * which + 3]
+    s, b = (t.view(torch.bfloat16).double().repeat_interleave(64, -1) for t in (s, b))
+    n = ((w.long()[..., None] >> torch.arange(0, 32, 4, device=w.device)) & 15).reshape(s.shape).double()
+    return s * n + b, s.abs() * n + b.abs()
+
+
+def _bounds(c, x, off, n, causal=True, scale=None, leave_out=None):
+    """Per sequence b: (out, its bound [rows, Hq, D], lse, its bound [rows, Hq], weights, their bound [H, keys]) of its n[b]
+    rows behind off[b] positions.  leave_out: a range of keys that the result (not the bounds) goes without."""
+    torch = _torch()
+    B, S, Hq, D = x.shape
+    H, G = c.H, Hq // c.H
+    scale = D ** -0.5 if scale is None else scale
+    (K, Kh), (V, Vh) = _parts(c, 0), _parts(c, 1)
+    res = []
+    for b in range(B):
+        r, T = n[b], off[b] + n[b]
+        o, to, z, tz, m, tm = [], [], [], [], [], []
+        hide = torch.zeros(r, T, dtype=torch.bool, device=x.device)
+        if causal:
+            hide = torch.arange(T, device=x.device)[None] > torch.arange(off[b], T, device=x.device)[:, None]
+        gone = hide.clone()
+        if leave_out:
+            gone[:, leave_out[0]:leave_out[1]] = True
+        for h in range(H):
+            k, kh, v, vh = (t[b, h, :T] for t in (K, Kh, V, Vh))
+            q = x[b, :r, h * G:(h + 1) * G].double()
+            s = scale * torch.einsum("igd,jd->igj", q, k)
+            e = 2.0 ** -16.5 * abs(scale) * torch.einsum("igd,jd->igj", q.abs(), kh) + \
+                2.0 ** -21 * (1 + abs(scale) * k.abs().max() * q.abs().sum(-1, keepdim=True))
+            e = e.masked_fill(hide[:, None], 0).amax(-1)
+            zf = torch.logsumexp(s.masked_fill(hide[:, None], -float("inf")), -1)
+            pf = torch.exp(s.masked_fill(hide[:, None], -float("inf")) - zf[..., None])
+            s = s.masked_fill(gone[:, None], -float("inf"))
+            zz = torch.logsumexp(s, -1)
+            p = torch.exp(s - zz[..., None])
+            out = torch.einsum("igj,jd->igd", p, v)
+            o.append(out)
+            to.append(torch.einsum("igj,jd->igd", pf, vh) * (2.0 ** -10 + 2.0 ** -13 + torch.expm1(2 * e)[..., None])
+                      + 2.0 ** -21 * v.abs().max() + 2.0 ** -8 * torch.einsum("igj,jd->igd", pf, v).abs())
+            z.append(zz)
+            tz.append(e + 2.0 ** -13 + 2.0 ** -22 * zf.abs())
+            m.append(p.sum((0, 1)))
+            tm.append((pf * (torch.expm1(2 * e)[..., None] + 2.0 ** -12)).sum((0, 1)) + 2.0 ** -20 * (1 + pf.sum((0, 1))))
+        res.append((torch.cat(o, 1), torch.cat(to, 1), torch.cat(z, 1), torch.cat(tz, 1), torch.stack(m), torch.stack(tm)))
+    return res
+
+
+def _check(c, x, off, n=None, causal=True, scale=None, mass=True, **kw):
+    """The call's output, log-sum-exp and weights lie within the bounds."""
+    torch = _torch()
+    n = [x.shape[1]] * x.shape[0] if n is None else n
+    m = torch.zeros(c.B, c.H, c.max_pos, device=x.device) if mass else None
+    out, lse = _attend(c, x, _dev(off), _dev(n), causal=causal, scale=scale, mass=m, **kw)
+    for b, (o, to, z, tz, w, tw) in enumerate(_bounds(c, x, off, n, causal, scale)):
+        d = (out[b, :n[b]].double() - o).abs()
+        assert (d <= to).all(), (b, (d / to).max())
+        d = (lse[b, :n[b]].double() - z).abs()
+        assert (d <= tz).all(), (b, (d / tz).max())
+        assert (out[b, n[b]:] == 0).all() and (lse[b, n[b]:] == -float("inf")).all()
+        if mass:
+            T = off[b] + n[b]
+            d = (m[b, :, :T].double() - w).abs()
+            assert (d <= tw).all(), (b, (d / tw).max())
+            assert (m[b, :, T:] == 0).all()
+    return out, lse, m
+
+
+def _staircase(D, T, H=2):
+    """Keys whose scores (base 2) rise by 9 in every 64 positions: position 64 r + 5 is at 9 (r + 1), the others of its 64 at 9 r,
+    so that they hold a seventh of the weight.  Rows of +-7.5 s with s = m 2^-6, m <= 16, are stored exactly."""
+    torch = _torch()
+    c = Cache(1, H, (T + 15) // 16 * 16, D)
+    r = torch.arange(T) // 64
+    level = torch.where(torch.arange(T) % 64 == 5, r + 1, r).float()
+    sign = torch.where(torch.arange(D) % 2 == 0, 1.0, -1.0)
+    k = (level * 7.5 * 2.0 ** -6)[:, None, None] * sign
+    assert level.max() <= 16
+    _append(c, k[None].expand(1, T, H, D).contiguous().bfloat16().cuda(), _rand((1, T, H, D), 2).cuda(), _dev([0]))
+    beta = 9.0 / (D * 7.5 * 2.0 ** -6 * D ** -0.5 * 1.4426950408889634)
+    return c, beta * sign
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("S,G", [(1, 2), (20, 1), (70, 1), (90, 2), (64, 4)])
+def test_scores_that_rise_in_both_halves_of_every_tile(S, G, D):
+    """The running maximum moves in each 64 keys, in the first tile and in later ones: what has been summed is scaled twice a tile."""
+    torch = _torch()
+    c, u = _staircase(D, 960)
+    x = u * (1 + 0.002 * torch.arange(S * 2 * G).reshape(1, S, 2 * G, 1) / (S * 2 * G))
+    x = (x + 0.01 * _rand((1, S, 2 * G, D), 5).float()).bfloat16().cuda()
+    _check(c, x, [960 - S], mass=False)
+    _check(c, x, [960 - S], mass=False, causal=False)
