@@ -30,6 +30,10 @@ constexpr int KBLOCKS = 2;                    // key tiles of a thread block
 constexpr int PW = 16;                        // the product warp; the others: a quarter of the columns per 4 warps
 constexpr int MTHREADS = 32 * PW + 32;
 constexpr int QSTAGES = 3;
+// Column tables.  A thread arrives on s_free for tile i while it still reads table i, so that arrival only tells that it has
+// left table i - 1; table i + 2 is written behind the arrivals for tile i - 2 and must lie on table i - 3 or an older one.
+constexpr int TABLES = 8;
+static_assert(TABLES >= 5 && (TABLES & (TABLES - 1)) == 0, "tables i - 2 to i + 2 are in use at a time");
 constexpr uint32_t MASS_TMEM = 2 * KBLOCKS * CM;
 
 // Shared memory, from a 1 KB aligned base: barriers, column tables, sums, K operands, Q operands.
@@ -37,8 +41,8 @@ template <int D>
 struct MassPlan {
     static constexpr int GR = D / 64;
     static constexpr int KB = GR * KT * 128 + KT * 32, QB = q_block_bytes(D);
-    static constexpr int TAB = 1024;                   // [4][64 column pairs]{factor x 2, -log2-sum-exp x 2}
-    static constexpr int SUM = TAB + 4 * CM * 8;       // [column quarter][key tile][key]
+    static constexpr int TAB = 1024;                   // [TABLES][64 column pairs]{factor x 2, -log2-sum-exp x 2}
+    static constexpr int SUM = TAB + TABLES * CM * 8;       // [column quarter][key tile][key]
     static constexpr int K = SUM + 4 * KBLOCKS * KT * 4;   // [key tile]{[GR][128 keys][128 B] swizzled; C*}
     static constexpr int Q = K + KBLOCKS * KB;
     static constexpr int BYTES = Q + QSTAGES * QB + 1024;
@@ -140,7 +144,7 @@ __global__ void __launch_bounds__(MTHREADS, 1) kv4_mass_tc_kernel(const Kv4AttnA
     };
     auto put = [&](int i, float2 v) {
         if (tid >= CM) return;
-        float* t = tab + (i & 3) * 2 * CM + (tid >> 1) * 4 + (tid & 1);
+        float* t = tab + (i & (TABLES - 1)) * 2 * CM + (tid >> 1) * 4 + (tid & 1);
         t[0] = ldexpf(v.x, ek - 7);
         t[2] = -v.y * LOG2E;
     };
@@ -170,7 +174,7 @@ __global__ void __launch_bounds__(MTHREADS, 1) kv4_mass_tc_kernel(const Kv4AttnA
             if (ok && i > 1 && !wait_bar(s_free + buf, ((i - 2) >> 1) & 1)) ok = false;
             if (ok && !wait_bar(s_full + buf, (i >> 1) & 1)) ok = false;
             fence_after();
-            put(i + 2, ahead);  // over the table of tile i - 2, which every thread has left
+            put(i + 2, ahead);  // over the table of tile i + 2 - TABLES, which every thread has left
             ahead = fetch(i + 3);
             unsigned long long s2[KBLOCKS] = {0ull, 0ull};
 #pragma unroll 1
@@ -183,7 +187,7 @@ __global__ void __launch_bounds__(MTHREADS, 1) kv4_mass_tc_kernel(const Kv4AttnA
                     fence_before();
                     arrive(s_free + buf);
                 }
-                const ulonglong2* t = reinterpret_cast<const ulonglong2*>(tab + (i & 3) * 2 * CM) + quarter * 16 + r / 2;
+                const ulonglong2* t = reinterpret_cast<const ulonglong2*>(tab + (i & (TABLES - 1)) * 2 * CM) + quarter * 16 + r / 2;
                 if (c_first + i * CM >= c_all) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {

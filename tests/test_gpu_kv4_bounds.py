@@ -124,3 +124,21 @@ def test_scores_that_rise_in_both_halves_of_every_tile(S, G, D):
     x = (x + 0.01 * _rand((1, S, 2 * G, D), 5).float()).bfloat16().cuda()
     _check(c, x, [960 - S], mass=False)
     _check(c, x, [960 - S], mass=False, causal=False)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("S,Hq,Hkv,T", [(64, 2, 2, 700), (300, 8, 2, 300), (600, 4, 1, 1500), (1024, 4, 1, 1024)])
+def test_weights_of_long_chunks(S, Hq, Hkv, T, D):
+    """One to 32 tiles of columns, whose tables are reused, with queries of very different size from column to column; every run
+    gives the same bits."""
+    torch = _torch()
+    c = _filled(2, Hkv, T, D, outliers=False)
+    x = _rand((2, S, Hq, D), 3).float()
+    x = (x * torch.exp2(-6 * torch.rand(2, S, Hq, 1, generator=torch.Generator().manual_seed(4)))).bfloat16().cuda()
+    off, n = [T - S, 0], [S, S - S // 3]
+    _, _, m = _check(c, x, off, n)
+    _check(c, x, off, n, causal=False)
+    for _ in range(6):
+        again = torch.zeros_like(m)
+        _attend(c, x, _dev(off), _dev(n), mass=again)
+        assert torch.equal(again, m)
