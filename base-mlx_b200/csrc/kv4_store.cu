@@ -135,11 +135,12 @@ __global__ void __launch_bounds__(NT) kv4_append_kernel(const Kv4StoreArgs a) {
             scale = group_scale(hi, lo);
             if (scale != 0.f) {
                 // x - lo is exact in fp32 when no magnitude lies 2^16 below the width (or is 0: also exact,
-                // but not worth telling apart); the rest, and subnormal scales, go the long way
+                // but not worth telling apart); the rest, subnormal scales and widths past the fp32 range go the long way
                 float least = lo == 0.f ? INFINITY : fabsf(lo);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) least = fminf(least, fabsf(x[j]));
-                const bool exact = least * 65536.f >= hi - lo && scale >= 1.2e-38f;
+                const float width = hi - lo;
+                const bool exact = width <= 3.0e38f && least * 65536.f >= width && scale >= 1.2e-38f;
                 word = exact ? quantize8(x, lo, scale) : quantize8_any(u[r], lo, scale);
             }
         }

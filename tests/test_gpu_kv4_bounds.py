@@ -18,7 +18,7 @@ bf16 2^-8, fp16 2^-11, fp32 2^-24.
 """
 import pytest
 
-from test_gpu_kv4 import Cache, _append, _attend, _dev, _filled, _rand
+from test_gpu_kv4 import Cache, _append, _attend, _dev, _filled, _quantize64, _rand
 
 pytestmark = pytest.mark.gpu
 
@@ -142,3 +142,34 @@ def test_weights_of_long_chunks(S, Hq, Hkv, T, D):
         again = torch.zeros_like(m)
         _attend(c, x, _dev(off), _dev(n), mass=again)
         assert torch.equal(again, m)
+
+
+def _words(q, D):
+    """uint32 words (as int32) of 4-bit integers [..., D]."""
+    torch = _torch()
+    w = (q.long().reshape(*q.shape[:-1], D // 8, 8) << torch.arange(0, 32, 4)).sum(-1)
+    return torch.where(w >= 2 ** 31, w - 2 ** 32, w).int()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("S,shift", [(5, 0), (700, 0), (700, 3)])
+def test_append_of_groups_wider_than_fp32(S, shift, D):
+    """Groups of large magnitudes only, max - min past the fp32 range: the words of the exact quotients."""
+    torch = _torch()
+    g = torch.Generator().manual_seed(S)
+    kinds = torch.tensor([[3e38, -3e38, 1e38, -1e38, 2e38, -2e38, 5e37, -5e37], [3e38, -3e38] * 4, [2e38, -2e38, 2e38, -1.9e38] * 2,
+                          [3.38e38, -3.38e38, 1e34, -1e34] * 2]).bfloat16()
+    x = kinds[torch.randint(0, 4, (1, S, 8, D // 8), generator=g)].reshape(1, S, 8, D)  # a thread's eight values each
+    x[0, ::3, ::2] = (x[0, ::3, ::2].float() * (0.5 + torch.rand(x[0, ::3, ::2].shape, generator=g))).clamp(-3.38e38, 3.38e38).bfloat16()
+    c = Cache(1, 8, 768, D)
+    y = torch.empty(1, S, 8, D + shift, dtype=torch.bfloat16)[..., shift:]
+    y.copy_(x)
+    k = torch.empty_strided(y.shape, (S * 8 * (D + shift), 8 * (D + shift), D + shift, 1), dtype=torch.bfloat16, device="cuda")
+    k.copy_(x)
+    _append(c, k, k, _dev([0]))
+    q, s, z = _quantize64(x.double().transpose(1, 2))
+    assert torch.isfinite(s).all()
+    for which in (0, 1):
+        assert torch.equal(c.t[3 * which][:, :, :S].cpu(), _words(q, D))
+        assert torch.equal(c.t[3 * which + 1][:, :, :S].cpu().view(torch.bfloat16).double(), s)
+        assert torch.equal(c.t[3 * which + 2][:, :, :S].cpu().view(torch.bfloat16).double(), z)
