@@ -40,12 +40,23 @@ QW_DEV float group_scale(float hi, float lo) {
 // Word of the eight values' clamp(round_half_even((x - bias) / scale), 0, 15).
 // quantize8_any decides every element in fp64; quantize8 gives the same word
 // in fp32 where every x - bias is exact in it.
+//
+// x - bias may take more than fp64's 53 bits: it is d + e with d the fp64 difference
+// and e its rounding error (Knuth's two-sum).  Halves (n + 1/2) scale have 13 bits, so d's
+// neighbours among the fp64 numbers include them: a d that is not a half is farther from the
+// next one than e, its quotient does not round to one, and e decides only where d is a half.
 __device__ __noinline__ uint32_t quantize8_any(uint4 u, float bias, float scale) {
     const uint32_t X[4] = {u.x, u.y, u.z, u.w};
     uint32_t word = 0;
     for (int j = 0; j < 8; ++j) {
-        const float x = j & 1 ? bits_hi_f(X[j >> 1]) : bits_lo_f(X[j >> 1]);
-        const double r = rint(((double)x - (double)bias) / (double)scale);
+        const double x = j & 1 ? bits_hi_f(X[j >> 1]) : bits_lo_f(X[j >> 1]), b = -(double)bias, s = scale;
+        const double d = __dadd_rn(x, b);
+        double r = rint(d / s);
+        const double rem = fma(-r, s, d);  // exact
+        if (fabs(rem) == 0.5 * s) {
+            const double bv = __dadd_rn(d, -x), e = __dadd_rn(__dadd_rn(x, -__dadd_rn(d, -bv)), __dadd_rn(b, -bv));
+            if (rem * e > 0.0) r += rem > 0.0 ? 1.0 : -1.0;  // the quotient lies past the half that d fell on
+        }
         word |= (uint32_t)fmin(fmax(r, 0.0), 15.0) << (4 * j);
     }
     return word;

@@ -16,6 +16,8 @@ bf16 2^-8, fp16 2^-11, fp32 2^-24.
 * weight of a key: factors exp(2 e) of its probabilities and 2^-12 of them (the log-sum-exp's sum), fp32 sums with what
   was there: 2^-20 (1 + |mass|).
 """
+from fractions import Fraction
+
 import pytest
 
 from test_gpu_kv4 import Cache, _append, _attend, _dev, _filled, _quantize64, _rand
@@ -173,3 +175,42 @@ def test_append_of_groups_wider_than_fp32(S, shift, D):
         assert torch.equal(c.t[3 * which][:, :, :S].cpu(), _words(q, D))
         assert torch.equal(c.t[3 * which + 1][:, :, :S].cpu().view(torch.bfloat16).double(), s)
         assert torch.equal(c.t[3 * which + 2][:, :, :S].cpu().view(torch.bfloat16).double(), z)
+
+
+def _nearest(x, bias, scale):
+    """The integer nearest to the exact (x - bias) / scale, ties to even, in 0..15: rational arithmetic."""
+    f = (Fraction(float(x)) - Fraction(float(bias))) / Fraction(float(scale))
+    return max(0, min(15, round(f)))  # round() of a Fraction takes ties to even
+
+
+@pytest.mark.parametrize("tiny", [2.0 ** -30, 2.0 ** -60, 2.0 ** -110, 2.0 ** -126])
+def test_append_of_quotients_a_hair_from_a_half(tiny):
+    """(x - bias) / scale next to n + 1/2 by far less than 64 bits of floating point hold: small x beside a bias of
+    (n + 1/2) scale, and x of (n + 1/2) scale beside a small bias."""
+    torch = _torch()
+    rows = []
+    for scale in (2.0, 1.5, 2.0 ** 20, 23 * 2.0 ** -9):
+        for n in range(6):
+            r = torch.zeros(64)
+            r[0] = -(n + 0.5) * scale
+            r[1] = (15 - n - 0.5) * scale
+            r[2:22] = torch.tensor([tiny, -tiny, 2 * tiny, -3 * tiny, 0.0] * 4)
+            rows.append(r)
+        for sign in (1, -1):
+            r = torch.zeros(64)
+            r[0] = -tiny
+            r[1] = 15 * scale
+            r[2:17] = (torch.arange(15) + 0.5) * scale
+            rows.append(r * sign)
+    x = torch.stack(rows).bfloat16()[None, :, None]  # [1, rows, 1, 64]
+    S = x.shape[1]
+    c = Cache(1, 1, 64, 64)
+    _append(c, x.cuda(), x.cuda(), _dev([0]))
+    w = c.t[0][0, 0, :S].cpu().long()
+    got = ((w[..., None] >> torch.arange(0, 32, 4)) & 15).reshape(S, 64)
+    s = c.t[1][0, 0, :S, 0].cpu().view(torch.bfloat16)
+    z = c.t[2][0, 0, :S, 0].cpu().view(torch.bfloat16)
+    for i in range(S):
+        assert float(z[i]) == float(x[0, i, 0].min())
+        want = [_nearest(v, z[i], s[i]) for v in x[0, i, 0]]
+        assert got[i].tolist() == want, (i, float(s[i]))
