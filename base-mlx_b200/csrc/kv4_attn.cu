@@ -595,17 +595,21 @@ QW_DEV void store_weights(float (&sum)[2 * KB], float* mass, int key0, int T, in
 constexpr int SCORE_COLUMNS = 16, WNT = 256;
 template <int VEC>
 __global__ void __launch_bounds__(WNT) kv4_mass_scores_kernel(const Kv4AttnArgs a, const float* scores, int cp) {
-    __shared__ float base[SCORE_COLUMNS];  // the columns' log2-sum-exp; +inf for a row that is padding
+    __shared__ float base[SCORE_COLUMNS];  // the columns' log2-sum-exp
+    __shared__ int seen[SCORE_COLUMNS];    // the keys that they see (a NaN row's others have no weight from it); 0 for padding
     const int h = blockIdx.y, b = blockIdx.z, G = a.Hq / a.c.heads, C = G * a.S, key = blockIdx.x * WNT + threadIdx.x;
     const Kv4Rows rw = kv4_rows(a.seq_len, a.n_new, b, a.S, a.c.max_pos, nullptr, false);
+    const int T = rw.off + rw.n;
     pdl_wait();
-    if (blockIdx.x * WNT >= rw.off + rw.n) return;
+    if (blockIdx.x * WNT >= T) return;
     if (threadIdx.x < cp) {
         const int c = threadIdx.x, i = c / G;
-        base[c] = c < C && i < rw.n ? a.lse[((size_t)b * a.S + i) * a.Hq + h * G + c % G] * LOG2E : INFINITY;
+        const bool row = c < C && i < rw.n;
+        base[c] = row ? a.lse[((size_t)b * a.S + i) * a.Hq + h * G + c % G] * LOG2E : 0.f;
+        seen[c] = !row ? 0 : a.causal ? min(T, rw.off + i + 1) : T;
     }
     const size_t at = ((size_t)b * a.c.heads + h) * a.c.max_pos + key;
-    const bool ok = key < rw.off + rw.n;
+    const bool ok = key < T;
     float v[SCORE_COLUMNS];
     const float before = ok ? a.mass[at] : 0.f;
 #pragma unroll
@@ -621,7 +625,7 @@ __global__ void __launch_bounds__(WNT) kv4_mass_scores_kernel(const Kv4AttnArgs 
     float sum = 0.f;
 #pragma unroll
     for (int c = 0; c < SCORE_COLUMNS; ++c)
-        if (c < cp) sum += base[c] == INFINITY ? 0.f : ex2(v[c] - base[c]);
+        if (c < cp) sum += key < seen[c] ? ex2(v[c] - base[c]) : 0.f;
     a.mass[at] = before + sum;
 }
 

@@ -214,3 +214,23 @@ def test_append_of_quotients_a_hair_from_a_half(tiny):
         assert float(z[i]) == float(x[0, i, 0].min())
         want = [_nearest(v, z[i], s[i]) for v in x[0, i, 0]]
         assert got[i].tolist() == want, (i, float(s[i]))
+
+
+@pytest.mark.parametrize("T", [200, 9000])
+@pytest.mark.parametrize("S,G,row", [(2, 1, 0), (5, 2, 1), (5, 3, 3), (8, 2, 4), (20, 1, 7), (9, 6, 2), (70, 1, 3), (100, 2, 64)])
+def test_weights_beside_a_nan_query(S, G, row, T):
+    """A NaN query makes the weights of the keys that its row sees NaN; the keys behind them have the other rows' weights."""
+    torch = _torch()
+    c = _filled(1, 2, T, 64, outliers=False)
+    x = _rand((1, S, 2 * G, 64), 3)
+    off = T - S
+    _, _, _, _, want, tol = _bounds(c, x.cuda(), [off], [S])[0]
+    x[0, row, 0, 7] = float("nan")  # a head of kv head 0
+    m = torch.zeros(1, 2, c.max_pos, device="cuda")
+    out, lse = _attend(c, x.cuda(), _dev([off]), mass=m)
+    seen = off + row + 1
+    assert torch.isnan(m[0, 0, :seen]).all()
+    assert ((m[0, 0, seen:T].double() - want[0, seen:]).abs() <= tol[0, seen:]).all()
+    assert ((m[0, 1, :T].double() - want[1]).abs() <= tol[1]).all()
+    nan = torch.isnan(out).all(-1)[0]
+    assert nan[row, 0] and int(nan.sum()) == 1 and int(torch.isnan(lse).sum()) == 1
