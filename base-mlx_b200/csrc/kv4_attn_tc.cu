@@ -85,6 +85,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
     uint64_t* pv_done = p_full + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2);
     float* kvmax = reinterpret_cast<float*>(tmem_slot + 2);  // [8 NB][2] of the warps: largest |K|, |V|
+    int* left_out = reinterpret_cast<int*>(kvmax + 16 * NB);  // first key whose V is left out (see partial)
     float* xch = reinterpret_cast<float*>(sm + 1024);       // [round][half][CB]: largest scores; in the end the halves' sums
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();
@@ -121,6 +122,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
         return;
     }
     if (tid == 0) {
+        *left_out = 0x7FFFFFFF;
         for (int i = 0; i < 2; ++i) {
             mbar_init(k_full + i, 256 * NB);
             mbar_init(k_free + i, 1);
@@ -323,7 +325,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
         // ---- expansion of this thread's share of a tile --------------------------------------------------
         const float kup = __uint_as_float((uint32_t)(127 + 7 - ek) << 23), vup = __uint_as_float((uint32_t)(127 + 16 - ev) << 23);
         // A NaN in V: where every column sees the key its value is simply NaN; in a tile that some column sees in
-        // part only, the value is left out and the key's score made NaN, which reaches just the rows that see it.
+        // part only, the value is left out and the outputs of the columns that see the first such key become NaN in the end.
         auto partial = [&](int i) { return (t0 + i + 1) * KT > all; };
         auto store_k = [&](int i) {  // tile i's K operand from ks, cs, cz
             if (i >= n_tiles) return;
@@ -333,13 +335,12 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
 #pragma unroll
                 for (int j = 0; j < PER; ++j) expand_piece<D>(ks.w[j], tid + NTH * j, dst, Centred(u16_to_f(ks.s[j]) * kup));
             if (tid < KT) {
-                bool nan = false;
                 const int key = (t0 + i) * KT + tid;
                 if (partial(i) && key < T) {
                     const uint32_t s = group_pair<GR>(rows.s[1], key), z = group_pair<GR>(rows.b[1], key);
-                    nan = !finite(bits_lo_f(s), bits_lo_f(z)) || !finite(bits_hi_f(s), bits_hi_f(z));
+                    if (!finite(bits_lo_f(s), bits_lo_f(z)) || !finite(bits_hi_f(s), bits_hi_f(z))) atomicMin(left_out, key);
                 }
-                store_offsets<GR>(dst + GR * KT * 128, tid, cs, cz, kup, nan);
+                store_offsets<GR>(dst + GR * KT * 128, tid, cs, cz, kup);
             }
         };
         auto store_v = [&](int i) {
@@ -464,7 +465,9 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
         fence_after();
         // ---- output ---------------------------------------------------------------------------------
         const bool has = row && l != 0.f;
-        const float f = nsplit == 1 ? (has ? 1.f / l : 0.f) : 1.f;
+        if (ok && !wait_bar(k_full + ((n_tiles - 1) & 1), ((n_tiles - 1) >> 1) & 1)) ok = false;  // complete: it shows left_out
+        const bool spoilt = row && *left_out < (a.causal ? rw.off + i_row + 1 : T);
+        const float f = spoilt ? __int_as_float(0x7FC00000) : nsplit == 1 ? (has ? 1.f / l : 0.f) : 1.f;
         const float e0 = 4.f, e1 = __uint_as_float((uint32_t)(127 + ev) << 23);
         const size_t slot = (seg * nsplit + sp) * CB + col;
         // Through shared memory (the Q and K operands, of which every product is done), so that lanes write along

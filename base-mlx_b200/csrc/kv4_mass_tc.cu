@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(MTHREADS, 1) kv4_mass_tc_kernel(const Kv4AttnA
             expand_piece<D>(w, p, sm + P::K + kb * P::KB, Centred(in ? u16_to_f(s[key * GR + ((p % CPR) >> 1)]) * kup : 0.f));
         }
         if (tid < KBLOCKS * KT)
-            store_offsets<GR>(sm + P::K + tid / KT * P::KB + GR * KT * 128, tid % KT, cs, cz, kup, false);
+            store_offsets<GR>(sm + P::K + tid / KT * P::KB + GR * KT * 128, tid % KT, cs, cz, kup);
     }
 
     pdl_wait();  // the rows' log-sum-exp and the Q operands are the attention kernels'

@@ -126,14 +126,13 @@ struct Centred {
 };
 // C* of one key (`scale`, `bias`: its groups' bf16 pairs): 2^6 c kup in two fp16 terms, k = 5 g + {0..4}: hi, lo, hi, lo, hi.
 template <int GR>
-QW_DEV void store_offsets(unsigned char* dst, int row, uint32_t scale, uint32_t bias, float kup, bool nan) {
+QW_DEV void store_offsets(unsigned char* dst, int row, uint32_t scale, uint32_t bias, float kup) {
     __half c[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) c[e] = __float2half_rn(0.f);
 #pragma unroll
     for (int g = 0; g < GR; ++g) {
-        float x = fmaf(8.f, g ? bits_hi_f(scale) : bits_lo_f(scale), g ? bits_hi_f(bias) : bits_lo_f(bias)) * kup * 64.f;
-        if (nan) x = __int_as_float(0x7FC00000);
+        const float x = fmaf(8.f, g ? bits_hi_f(scale) : bits_lo_f(scale), g ? bits_hi_f(bias) : bits_lo_f(bias)) * kup * 64.f;
         const __half hi = __float2half_rn(x), lo = __float2half_rn(x - __half2float(hi));
         c[5 * g] = c[5 * g + 2] = c[5 * g + 4] = hi;
         c[5 * g + 1] = c[5 * g + 3] = lo;

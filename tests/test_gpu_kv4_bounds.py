@@ -234,3 +234,27 @@ def test_weights_beside_a_nan_query(S, G, row, T):
     assert ((m[0, 1, :T].double() - want[1]).abs() <= tol[1]).all()
     nan = torch.isnan(out).all(-1)[0]
     assert nan[row, 0] and int(nan.sum()) == 1 and int(torch.isnan(lse).sum()) == 1
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("S,G,T,at", [(1, 4, 300, 299), (5, 4, 300, 297), (20, 2, 300, 290), (90, 1, 300, 250), (90, 2, 300, 10),
+                                      (70, 2, 9000, 8960), (200, 2, 1500, 1301), (300, 1, 300, 0), (300, 1, 300, 260)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_value_that_is_not_finite_leaves_sums_and_weights(S, G, T, at, D, bad):
+    """Log-sum-exp and weights come from K alone: a V that is not finite changes neither, and only the outputs that see it."""
+    torch = _torch()
+    c = _filled(1, 1, T, D, outliers=False)
+    x = _rand((1, S, G, D), 3).cuda()
+    off = T - S
+    want, to, z, tz, w, tw = _bounds(c, x, [off], [S])[0]
+    c.t[4][0, 0, at, 0] = int(torch.tensor(float("nan")).bfloat16().view(torch.int16)) if bad != bad else c.t[4][0, 0, at, 0]
+    c.t[5][0, 0, at, 0] = int(torch.tensor(bad).bfloat16().view(torch.int16))
+    m = torch.zeros(1, 1, c.max_pos, device="cuda")
+    out, lse = _attend(c, x, _dev([off]), mass=m)
+    assert ((lse[0].double() - z).abs() <= tz).all()
+    assert ((m[0, :, :T].double() - w).abs() <= tw).all()
+    sees = torch.arange(S, device="cuda") + off >= at
+    assert not torch.isfinite(out[0, sees][..., :64].float()).any()
+    if bad != bad:
+        assert torch.isnan(out[0, sees][..., :64]).all()
+    assert ((out[0, ~sees].double() - want[~sees]).abs() <= to[~sees]).all()
