@@ -467,7 +467,11 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
         const bool has = row && l != 0.f;
         if (ok && !wait_bar(k_full + ((n_tiles - 1) & 1), ((n_tiles - 1) >> 1) & 1)) ok = false;  // complete: it shows left_out
         const bool spoilt = row && *left_out < (a.causal ? rw.off + i_row + 1 : T);
-        const float f = spoilt ? __int_as_float(0x7FC00000) : nsplit == 1 ? (has ? 1.f / l : 0.f) : 1.f;
+        // A split leaves its sums as they are, below 2^16 V a key: with V past 2^70 its share is taken 2^drop smaller, output and
+        // sum alike, against a base as much larger, so that they stay in range.
+        const int drop = nsplit == 1 ? 0 : max(0, ev - 70);
+        const float less = __uint_as_float((uint32_t)(127 - drop) << 23);
+        const float f = spoilt ? __int_as_float(0x7FC00000) : nsplit == 1 ? (has ? 1.f / l : 0.f) : less;
         const float e0 = 4.f, e1 = __uint_as_float((uint32_t)(127 + ev) << 23);
         const size_t slot = (seg * nsplit + sp) * CB + col;
         // Through shared memory (the Q and K operands, of which every product is done), so that lanes write along
@@ -524,7 +528,7 @@ __global__ void __launch_bounds__(THREADS<NB>, 1) kv4_attn_tc_kernel(const Kv4At
             if (nsplit == 1) {
                 if (a.lse) *lse_at() = has ? (log2f(l) - nm) * LN2 : -INFINITY;
             } else {
-                pml[slot] = make_float2(l != 0.f ? -nm : M0, l);
+                pml[slot] = make_float2(l != 0.f ? (float)drop - nm : M0, l * less);
             }
         }
     } else {

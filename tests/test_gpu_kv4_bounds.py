@@ -11,7 +11,9 @@ bf16 2^-8, fp16 2^-11, fp32 2^-24.
 * probability: a factor exp(2 e).
 * output: p s or p, and V in the chunk form, are rounded to 11 bits: sum_j p_j hat(v_j) (2 * 2^-11 + expm1(2 e)), sums of
   the keys in fp32 (2^-13 of the same sum covers chains of 2048 additions), 2^-21 of the largest |v|, and the
-  final rounding 2^-8 |out|.
+  final rounding 2^-8 |out|.  V below 2^-90 is held to 2^-111 instead: the powers of two that bring V into fp16 end at 2^98
+  (chunks: half of the last place 2^-24 is 2^-123) and p s is held against 2^-79 at least (2^-25 of 2^-79 2^-11, 15 times:
+  2^-111), and bf16 itself ends at 2^-133.
 * log-sum-exp: e, and 2^-13 relative of the sum (2^-13 absolute of its logarithm), 2^-22 |lse|.
 * weight of a key: factors exp(2 e) of its probabilities and 2^-12 of them (the log-sum-exp's sum), fp32 sums with what
   was there: 2^-20 (1 + |mass|).
@@ -72,7 +74,7 @@ def _bounds(c, x, off, n, causal=True, scale=None, leave_out=None):
             out = torch.einsum("igj,jd->igd", p, v)
             o.append(out)
             to.append(torch.einsum("igj,jd->igd", pf, vh) * (2.0 ** -10 + 2.0 ** -13 + torch.expm1(2 * e)[..., None])
-                      + 2.0 ** -21 * v.abs().max() + 2.0 ** -8 * torch.einsum("igj,jd->igd", pf, v).abs())
+                      + 2.0 ** -21 * v.abs().max().clamp(min=2.0 ** -90) + 2.0 ** -8 * torch.einsum("igj,jd->igd", pf, v).abs())
             z.append(zz)
             tz.append(e + 2.0 ** -13 + 2.0 ** -22 * zf.abs())
             m.append(p.sum((0, 1)))
@@ -258,3 +260,18 @@ def test_a_value_that_is_not_finite_leaves_sums_and_weights(S, G, T, at, D, bad)
     if bad != bad:
         assert torch.isnan(out[0, sees][..., :64]).all()
     assert ((out[0, ~sees].double() - want[~sees]).abs() <= to[~sees]).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("vmul", [1e-36, 1e-30, 1e29, 1e33, 3e36])
+@pytest.mark.parametrize("S,G,T", [(64, 1, 6000), (64, 4, 2100)])
+def test_split_chunks_of_very_large_and_small_values(S, G, T, vmul, D):
+    """Values up to the end of bf16 where a chunk's keys are split over thread blocks: their partial sums stay finite."""
+    torch = _torch()
+    c = Cache(1, 1, (T + 63) // 64 * 64, D)
+    v = (_rand((1, T, 1, D), 2).float() * vmul).bfloat16().cuda()
+    v[0, T // 2:] *= 2.0 ** -10  # shares of different magnitude
+    _append(c, _rand((1, T, 1, D), 1).cuda(), v, _dev([0]))
+    x = _rand((1, S, G, D), 3).cuda()
+    _check(c, x, [T - S])
+    _check(c, x, [T - S], causal=False)
