@@ -298,7 +298,8 @@ QW_DEV uint32_t transpose8x8(uint32_t v) {
 // columns 2 t + {0, 1} of every n-tile; l and bs are the lane's share (its
 // keys).  o, l and bs are relative to 2^-nm = 2^m sref / PSCALE with m the
 // column's running maximum and sref a power of two above the largest value
-// scale met so far, so exp2(x + nm) s <= 2^LAZY PSCALE enters fp16.
+// scale met so far, so exp2(x + nm) s <= 2^LAZY PSCALE enters fp16, and above 2^-60 of
+// the largest bias: p b <= 2^(LAZY + 71) keeps the bias sums in range where every scale is 0.
 template <int D, int NT>
 struct State {
     static constexpr int GR = D / 64;
@@ -377,10 +378,12 @@ QW_DEV void attend_tile(State<D, NT>& st, const Cols<D, NT>& cols, const unsigne
                 if (EDGE && key0 + 8 * r + g >= vis[n][e & 1]) x[kb][n][e] = -INFINITY;
             }
         }
-    // largest value scale of the tile (lane = key)
+    // largest value scale of the tile, or 2^-60 of its largest bias (lane = key)
     float vs[4][GR], vz[4][GR], smax;
     unpack<GR>(read_packed<D>(tile, 2, lane), vs[0]);
-    smax = GR == 2 ? fmaxf(fabsf(vs[0][0]), fabsf(vs[0][GR - 1])) : fabsf(vs[0][0]);
+    unpack<GR>(read_packed<D>(tile, 3, lane), vz[0]);
+    smax = fmaxf(fabsf(vs[0][0]), fabsf(vz[0][0]) * 0x1p-60f);
+    if (GR == 2) smax = fmaxf(fmaxf(smax, fabsf(vs[0][GR - 1])), fabsf(vz[0][GR - 1]) * 0x1p-60f);
     if (EDGE && key0 + lane >= T) smax = 0.f;
     if (!(smax < 2.0e37f)) smax = 0.f;  // past the range times 15: must not push the values of other rows to zero
     bool raise = smax > st.sref;

@@ -275,3 +275,19 @@ def test_split_chunks_of_very_large_and_small_values(S, G, T, vmul, D):
     x = _rand((1, S, G, D), 3).cuda()
     _check(c, x, [T - S])
     _check(c, x, [T - S], causal=False)
+
+
+@pytest.mark.parametrize("value", [3e-38, 1.0, 1e6, 1e12, 1e25, 3e38])
+@pytest.mark.parametrize("S,G,T", [(1, 4, 1), (1, 4, 40), (1, 4, 12000), (1, 16, 9000), (5, 2, 700), (20, 2, 9000), (90, 1, 700)])
+def test_values_that_are_constant_in_every_group(S, G, T, value):
+    """Scales of zero and biases of any size: the sums of biases stay in range, whichever keys come first."""
+    torch = _torch()
+    for kind in range(2):
+        c = Cache(1, 2, (T + S + 63) // 64 * 64, 128)
+        v = torch.full((1, T + S, 2, 128), value)
+        v[..., 64:] *= -0.5
+        if kind:  # zeros first, then rows of the value
+            v[:, :(T + S) // 2] = 0.0
+        _append(c, _rand((1, T + S, 2, 128), 1).cuda(), v.bfloat16().cuda(), _dev([0]))
+        assert (c.t[4][:, :, :T + S] == 0).all()
+        _check(c, _rand((1, S, 2 * G, 128), 3).cuda(), [T])
