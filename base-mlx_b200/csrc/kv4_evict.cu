@@ -39,7 +39,11 @@ QW_DEV uint32_t order_key(float v) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-QW_DEV int clamp_len(const Kv4EvictArgs& a, int b) { return max(0, min(a.seq_len[b], a.src.max_pos)); }
+// A length out of range counts as an empty sequence, as in kv4_rows.
+QW_DEV int length_of(const Kv4EvictArgs& a, int b) {
+    const int n = a.seq_len[b];
+    return n < 0 || n > a.src.max_pos ? 0 : n;
+}
 
 QW_DEV void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
@@ -67,7 +71,7 @@ __global__ void __launch_bounds__(SEL_NT, 1) kv4_select_kernel(const Kv4EvictArg
               warp = tid >> 5;
     pdl_wait();
     pdl_launch_dependents();
-    const int n = clamp_len(a, b);
+    const int n = length_of(a, b);
     const size_t bh = (size_t)b * a.src.heads + h;
     int* idx = index + bh * a.keep;
     int* out = a.index_out ? a.index_out + bh * a.keep : nullptr;

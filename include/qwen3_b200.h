@@ -399,7 +399,8 @@ QW_API int qw_kv4_evict_scratch(const qw_kv4* src, int keep, size_t* bytes);
  * accumulated weight mass_src (fp32 [batch][kv_heads][src max_pos]; equal
  * weights: the lower position stays, NaN counts as the largest).  The kept
  * rows go to positions 0.. of dst in their old order, their weights to
- * mass_dst, new_len_dev[b] = min(seq_len[b], keep).  index_out (int32
+ * mass_dst, new_len_dev[b] = min(seq_len[b], keep), or 0 for a length outside
+ * [0, src max_pos] (this operator has no error word).  index_out (int32
  * [batch][kv_heads][keep], may be NULL) receives the kept positions, -1 behind
  * them.  dst is src itself (in place; then mass_dst = mass_src, and
  * new_len_dev may be seq_len_dev) or a cache that does not overlap it, of the

@@ -22,7 +22,7 @@ from fractions import Fraction
 
 import pytest
 
-from test_gpu_kv4 import Cache, _append, _attend, _dev, _filled, _quantize64, _rand
+from test_gpu_kv4 import Cache, _append, _attend, _dev, _evict, _filled, _kept, _quantize64, _rand
 
 pytestmark = pytest.mark.gpu
 
@@ -291,3 +291,24 @@ def test_values_that_are_constant_in_every_group(S, G, T, value):
         _append(c, _rand((1, T + S, 2, 128), 1).cuda(), v.bfloat16().cuda(), _dev([0]))
         assert (c.t[4][:, :, :T + S] == 0).all()
         _check(c, _rand((1, S, 2 * G, 128), 3).cuda(), [T])
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+def test_evict_takes_a_length_out_of_range_for_an_empty_sequence(inplace):
+    """As the other operators do: nothing is moved or read, the new length is 0."""
+    torch = _torch()
+    src = _filled(6, 2, 128, 64, max_pos=128)
+    dst = src if inplace else Cache(6, 2, 48, 64)
+    ms = torch.rand(6, 2, 128, generator=torch.Generator().manual_seed(1)).cuda()
+    md = ms if inplace else torch.full((6, 2, 48), 9.0, device="cuda")
+    before, m0, source = dst.bits(), md.clone(), ms.clone()
+    lens = [-1, 129, -2 ** 31, 2 ** 31 - 1, 128, 20]
+    index, new = _dev([[[77] * 40] * 2] * 6), _dev([-5] * 6)
+    _evict(src, dst, ms, md, _dev(lens), new, 40, 8, index)
+    assert new.tolist() == [0, 0, 0, 0, 40, 20]
+    assert (index[:4] == -1).all() and (index[4] >= 0).all()
+    for t0, t1 in zip(before, dst.bits()):
+        assert torch.equal(t0[:4], t1[:4])
+    assert torch.equal(md[:4], m0[:4])
+    for h in range(2):
+        assert index[4, h].tolist() == _kept(source[4, h].cpu().double().numpy(), 128, 40, 8).tolist()
