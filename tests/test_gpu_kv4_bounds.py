@@ -22,7 +22,7 @@ from fractions import Fraction
 
 import pytest
 
-from test_gpu_kv4 import Cache, _append, _attend, _dev, _evict, _filled, _kept, _quantize64, _rand
+from test_gpu_kv4 import CASES, Cache, _append, _attend, _dev, _evict, _filled, _kept, _quantize64, _rand
 
 pytestmark = pytest.mark.gpu
 
@@ -83,7 +83,13 @@ def _bounds(c, x, off, n, causal=True, scale=None, leave_out=None):
     return res
 
 
-def _check(c, x, off, n=None, causal=True, scale=None, mass=True, **kw):
+# Euclidean norm of a row's error, relative to its output's, where V is independent of the probabilities: the roundings are
+# independent too, so those of p and v add up to at most 2 * 2^-11 sqrt(sum p^2 hat(v)^2) against sqrt(sum p^2 v^2), with hat(v)
+# at most five times v in the mean of normal rows: 5 * 2^-10, and 2^-8 for the final rounding; together below 2^-6.7.
+NORM = 2.0 ** -6
+
+
+def _check(c, x, off, n=None, causal=True, scale=None, mass=True, norm=None, **kw):
     """The call's output, log-sum-exp and weights lie within the bounds."""
     torch = _torch()
     n = [x.shape[1]] * x.shape[0] if n is None else n
@@ -92,6 +98,7 @@ def _check(c, x, off, n=None, causal=True, scale=None, mass=True, **kw):
     for b, (o, to, z, tz, w, tw) in enumerate(_bounds(c, x, off, n, causal, scale)):
         d = (out[b, :n[b]].double() - o).abs()
         assert (d <= to).all(), (b, (d / to).max())
+        assert norm is None or (d.norm(dim=-1) <= norm * o.norm(dim=-1)).all(), (b, (d.norm(dim=-1) / o.norm(dim=-1)).max())
         d = (lse[b, :n[b]].double() - z).abs()
         assert (d <= tz).all(), (b, (d / tz).max())
         assert (out[b, n[b]:] == 0).all() and (lse[b, n[b]:] == -float("inf")).all()
@@ -312,3 +319,24 @@ def test_evict_takes_a_length_out_of_range_for_an_empty_sequence(inplace):
     assert torch.equal(md[:4], m0[:4])
     for h in range(2):
         assert index[4, h].tolist() == _kept(source[4, h].cpu().double().numpy(), 128, 40, 8).tolist()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("B,Hq,Hkv,D,S,total", CASES)
+def test_attention_within_its_arithmetic(B, Hq, Hkv, D, S, total, causal):
+    c = _filled(B, Hkv, max(total), D, seed=S)
+    x = _rand((B, S, Hq, D), 77 + S, 1.5).cuda()
+    _check(c, x, [t - S for t in total], causal=causal)
+
+
+@pytest.mark.parametrize("S,Hq,Hkv,T,B,D", [
+    (1, 32, 8, 20000, 1, 128), (1, 8, 1, 9000, 2, 128), (1, 16, 4, 700, 40, 128), (16, 16, 1, 4000, 1, 128), (300, 4, 1, 3000, 1, 128),
+    (1, 16, 1, 9000, 2, 128), (5, 8, 2, 9001, 1, 128), (5, 8, 2, 5000, 3, 64), (1, 6, 1, 12345, 1, 64), (1, 64, 1, 3001, 2, 128),
+    (130, 2, 1, 4111, 2, 64), (40, 8, 2, 2500, 3, 128), (700, 2, 1, 701, 1, 128), (5, 32, 8, 9000, 2, 64), (15, 3, 1, 6001, 2, 128)])
+def test_long_attention_within_its_arithmetic(S, Hq, Hkv, T, B, D):
+    """Keys split over thread blocks, clusters and column blocks: a share that is lost, scaled or joined wrongly is outside the
+    bounds (see test_kv4_bounds_cpu.py)."""
+    c = _filled(B, Hkv, T, D, outliers=False)
+    total = [T] + [max(S, T * (i + 1) // (B + 1) + i % 7) for i in range(B - 1)]
+    x = _rand((B, S, Hq, D), 12, 1.5).cuda()
+    _check(c, x, [t - S for t in total], norm=NORM if min(total) - S > 64 else None)
