@@ -363,7 +363,7 @@ QW_DEV void write_out(const Kv4AttnArgs& a, const Kv4Rows& rw, int b, int h, int
     if (d == 0 && a.lse) a.lse[((size_t)b * a.S + i) * a.Hq + h * G + c % G] = has ? (M + log2f(l)) * LN2 : -INFINITY;
 }
 
-// 131071 keys, 8 kv heads, 4 columns each: 34.4 us = 4.4 TB/s (the keys themselves at 5.8 TB/s; ~10 us are the
+// 131071 keys, 8 kv heads, 4 columns each: 34.4 us of the call's 37.4 = 4.4 TB/s (the keys themselves at 5.8 TB/s; ~10 us are the
 // plan, the queries, the ring's start and the merges); the issue slots are 59 % taken, half of that by unpacking
 // nibbles.  A warp of its own for every tile, with no barrier on the way, because 16 warps in step took 39.6 us.
 template <int D, int NT, bool WEIGHTS>
@@ -574,9 +574,10 @@ QW_DEV void add_weights(float (&sum)[2 * KB], const MassKeys<D, KB>& k, const Co
         }
     }
 }
-// Sum over the lane quad of a key; lane t of the quad adds row r = t (and t + 4 ...) to mass.
+// Sum over the lane quad of a key; lane t of the quad adds row r = t to mass.
 template <int KB>
 QW_DEV void store_weights(float (&sum)[2 * KB], float* mass, int key0, int T, int lane) {
+    static_assert(2 * KB <= 4, "a lane of the quad for every row");
 #pragma unroll
     for (int r = 0; r < 2 * KB; ++r) {
         sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
@@ -590,7 +591,7 @@ QW_DEV void store_weights(float (&sum)[2 * KB], float* mass, int key0, int T, in
 
 // Up to SCORE_COLUMNS columns: the attention kernels leave their scores [batch][kv head][key][cp] (base 2; at eight
 // columns 32 bytes a key next to the 72 of its K row), so that this pass reads them from L2 and takes no products.
-// 4 sequences of up to 16000 keys, 8 columns: 29.1 us with the attention, 39.0 us with scores recomputed from K.
+// 4 sequences of up to 16000 keys, 8 columns: 28.9 us with the attention, 39.0 us with scores recomputed from K.
 // A thread adds one key's columns in their order.
 constexpr int SCORE_COLUMNS = 16, WNT = 256;
 template <int VEC>
@@ -711,7 +712,8 @@ __global__ void __launch_bounds__(ANT, 2) kv4_mass_kernel(const Kv4AttnArgs a) {
 }
 
 // Form of a call: from TC_COLUMNS columns per kv head the tcgen05 kernel, below it the split kernel
-// with column blocks of 8 (two blocks of threads per SM) or 16.
+// with column blocks of 8 (two blocks of threads per SM) or 16.  32768 keys, 8 kv heads: 43.0 us at 48 columns, 53.9 at 60
+// (four column blocks unpack the keys four times), 52.5 at 64 and 52.8 at 128 by the tcgen05 kernel.
 constexpr int TC_COLUMNS = 64;
 constexpr int CLUSTER_TILES = 4;
 struct Shape {

@@ -19,7 +19,7 @@
 // scales and biases alone) where fp16 holds it; the running maximum moves only
 // when a score passes it by 2^8 (P <= 2^15), and then O is rescaled in TMEM.
 //
-// 1024 rows of 32 heads on 8192 keys (8 kv heads): 187 us = 0.41 of the tensor
+// 1024 rows of 32 heads on 8192 keys (8 kv heads): 188 us = 0.41 of the tensor
 // rate.  A tile of 128 keys takes 5900 cycles for 256 columns, of which the
 // products need 2200 and the powers 2050; the softmax threads are busy
 // throughout: 2700 cycles in the softmax, 1500 expanding, 650 issuing loads.

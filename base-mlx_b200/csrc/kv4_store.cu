@@ -85,10 +85,11 @@ QW_DEV uint32_t quantize8(const float (&x)[8], float bias, float scale) {
 
 // Block = one (sequence, K or V, head) and R * NT / TPR consecutive new rows,
 // each thread one word of R of them.  Every input is loaded before the first
-// is used and before the lengths arrive: the blocks are short, so the kernel
-// is bound by the latency of its loads, not by their bytes.  4099 rows of 8
-// heads (42 MB with the read): 16 us, the integer units at 64 % of their rate (the
-// exact rounding); one row of 8 sequences with its read 3.8 us, latency alone.
+// is used and before the lengths arrive: the blocks are short, and the latency of
+// the loads counts more than their bytes.  4099 rows of 8 heads: 12.7 us (21.5 MB), issue
+// slots taken to 71 % and integer units to 64 % by the exact rounding; a warp with an element
+// 2^16 below its group's width takes fp64 quotients (18.8 us with 1 % zeros among the keys).
+// One row of 8 sequences with its read 3.8 us, latency alone.
 template <int D, bool VEC, int R>
 __global__ void __launch_bounds__(NT) kv4_append_kernel(const Kv4StoreArgs a) {
     constexpr int T = TPR<D>, RB = NT / T;

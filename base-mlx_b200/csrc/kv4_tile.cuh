@@ -300,6 +300,8 @@ QW_DEV uint32_t transpose8x8(uint32_t v) {
 // column's running maximum and sref a power of two above the largest value
 // scale met so far, so exp2(x + nm) s <= 2^LAZY PSCALE enters fp16, and above 2^-60 of
 // the largest bias: p b <= 2^(LAZY + 71) keeps the bias sums in range where every scale is 0.
+// (p ends at 2^-126, which is 2^-136 s of the largest p: 2^-36 at a scale s of 2^100.  Taking scales
+// and biases times a power of two from there on was measured: 1 to 4 % of every decode.)
 template <int D, int NT>
 struct State {
     static constexpr int GR = D / 64;

@@ -340,3 +340,33 @@ def test_long_attention_within_its_arithmetic(S, Hq, Hkv, T, B, D):
     total = [T] + [max(S, T * (i + 1) // (B + 1) + i % 7) for i in range(B - 1)]
     x = _rand((B, S, Hq, D), 12, 1.5).cuda()
     _check(c, x, [t - S for t in total], norm=NORM if min(total) - S > 64 else None)
+
+
+@pytest.mark.parametrize("scale", [1e25, 1e31, 1.0e36])  # probabilities below 2^-136 scale of the largest may be lost: 2^-16
+@pytest.mark.parametrize("S,G,T,D", [(1, 4, 200, 128), (1, 4, 9000, 128), (1, 16, 200, 64), (5, 2, 230, 64), (20, 1, 260, 128), (90, 1, 1200, 128)])
+def test_a_very_large_value_scale_leaves_sums_and_weights(S, G, T, D, scale):
+    """One key at 2^14 times the weight of each other, which together weigh half of it or less, and one very large
+    value scale: log-sum-exp and weights come from K alone; the rows that do not see that key keep their outputs
+    where it is the last one (but for 2^-22 of its values)."""
+    torch = _torch()
+    c = Cache(1, 1, (T + 15) // 16 * 16, D)
+    sign = torch.where(torch.arange(D) % 2 == 0, 1.0, -1.0)
+    k = torch.zeros(1, T, 1, D)
+    k[0, 3, 0] = 7.5 * 2.0 ** -3 * sign
+    _append(c, k.bfloat16().cuda(), _rand((1, T, 1, D), 2).cuda(), _dev([0]))
+    beta = 14.0 / (D * 7.5 * 2.0 ** -3 * D ** -0.5 * 1.4426950408889634)
+    x = (beta * sign).expand(1, S, G, D).bfloat16().cuda()
+    _, _, z, tz, w, tw = _bounds(c, x, [T - S], [S])[0]
+    for at in (T - 1, 20):
+        d = Cache(1, 1, c.max_pos, D)
+        for t, u in zip(d.t, c.t):
+            t.copy_(u)
+        d.t[4][0, 0, at, 0] = int(torch.tensor(scale).bfloat16().view(torch.int16))
+        m = torch.zeros(1, 1, c.max_pos, device="cuda")
+        out, lse = _attend(d, x, _dev([T - S]), mass=m)
+        assert ((lse[0].double() - z).abs() <= tz).all(), (at, (lse[0].double() - z).abs().max())
+        assert ((m[0, :, :T].double() - w).abs() <= tw).all(), at
+        _, to, _, _, _, _ = _bounds(d, x, [T - S], [S])[0]
+        o = _bounds(d, x, [T - S], [S])[0][0]
+        vmax = 2.0 ** -21 * 31 * scale  # the chunk form's and the hidden key's part
+        assert ((out[0].double() - o).abs() <= to + vmax).all(), at
