@@ -808,6 +808,8 @@ qw::Kv4View kv4_view(const qw_kv4* c) {
     if (c->head_dim != 64 && c->head_dim != 128)
         throw qw::Error(QW_ERR_UNSUPPORTED, "kv4: head_dim must be 64 or 128, got " + std::to_string(c->head_dim));
     need(c->max_pos >= 16 && c->max_pos % 16 == 0, "kv4: max_pos must be a positive multiple of 16");
+    // positions of the tile behind the last one, and of the next ones of a warp's turn, are counted in 32 bits
+    need(c->max_pos <= 1 << 30, "kv4: max_pos must not exceed 2^30");
     need(c->batch >= 1 && c->batch <= 65535, "kv4: batch must be 1..65535");
     need(c->kv_heads >= 1 && c->kv_heads <= 4096, "kv4: kv_heads must be 1..4096");
     qw::Kv4View v;

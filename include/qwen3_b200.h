@@ -320,8 +320,8 @@ QW_API int qw_quantized_matmul_argmax_static(const void* x, const void* w, const
  * weights (the arrays an MLX quantized KV cache holds at 64 / 4):
  *   k_w, v_w            uint32 [batch][kv_heads][max_pos][head_dim / 8], element e at bits 4 (e % 8) of word e / 8
  *   k_s, k_b, v_s, v_b  bf16   [batch][kv_heads][max_pos][head_dim / 64], value = scale * q + bias
- * head_dim is 64 or 128, max_pos a multiple of 16, every pointer 16-byte
- * aligned device memory of one GPU.  The struct is read during the call only.
+ * head_dim is 64 or 128, max_pos a multiple of 16 and at most 2^30, every pointer
+ * 16-byte aligned device memory of one GPU.  The struct is read during the call only.
  *
  * Common to the operators below (no reference counterpart: the reference
  * caches bf16 rows):

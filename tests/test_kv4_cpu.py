@@ -114,3 +114,17 @@ def test_evict_refusals():
     _refused(call(d=_cache(k_w=BASE + 16)), text="overlap")
     _refused(call(d=_cache(max_pos=32), md=m0), text="overlap")  # the same arrays under another layout
     _refused(lambda: q.kv4_evict_scratch_bytes(src, 0))
+
+
+@pytest.mark.parametrize("max_pos", [(1 << 30) + 16, (1 << 31) - 32, (1 << 31) - 16])
+def test_caches_whose_positions_do_not_fit_tile_counts_are_refused(max_pos):
+    """The tile behind the last position would be counted past 2^31 - 1, and read past the arrays."""
+    import qwen3_b200 as q
+    c, ok = _cache(batch=1, kv_heads=1, head_dim=64, max_pos=max_pos), _cache(batch=1, kv_heads=1, head_dim=64)
+    _refused(lambda: q.kv4_append(c, BASE, BASE, 1, BASE), text="2^30")
+    _refused(lambda: q.kv4_read(c, BASE, BASE, 1), text="2^30")
+    _refused(lambda: q.kv4_attention_scratch_bytes(c, 1, 4), text="2^30")
+    _refused(lambda: q.kv4_attention(c, BASE, BASE, 1, 4, 1.0, BASE, BASE, 1 << 30), text="2^30")
+    _refused(lambda: q.kv4_evict_scratch_bytes(c, 8), text="2^30")
+    _refused(lambda: q.kv4_evict(c, ok, BASE, BASE, BASE, BASE, 8, 0, BASE, 1 << 30), text="2^30")
+    _refused(lambda: q.kv4_evict(ok, c, BASE, BASE, BASE, BASE, 8, 0, BASE, 1 << 30), text="2^30")
