@@ -379,10 +379,11 @@ QW_API int qw_kv4_attention_scratch(const qw_kv4* cache, int S, int heads, size_
  * as a whole or in the 64 dimensions of a NaN in V, an infinite bias or a scale
  * past 2e37 leaves the row unspecified, and none of them reaches a row that
  * does not see it; V has no part in lse and mass.  K enters exactly, V and the
- * probabilities rounded to 11 bits, but for 2^-22 of the largest finite K or V of the sequence and kv head
- * (of 2^-80 where it is less); where a V scale s of them is past 1e30,
- * probabilities below 2^-136 s of a row's largest may count as nothing.  Scores
- * are fp32 sums: a query with |q| or |scale q| past 1e34 leaves its row unspecified.
+ * probabilities rounded to 11 bits, but for 2^-22 of the largest finite K or V
+ * of the sequence and kv head (of 2^-80 where it is less); where a V scale s of
+ * them is past 1e30, probabilities below 2^-136 s of a row's largest may count
+ * as nothing.  Scores are fp32 sums: a query with |q| or |scale q| past 1e34
+ * leaves its row unspecified.
  * lse (fp32 [batch][S][heads], may be NULL) receives the natural logarithm of
  * each row's sum of exponentials; a row without keys gives out = 0, lse = -inf.
  * mass (fp32 [batch][kv_heads][max_pos], may be NULL) has every key's
